@@ -1,4 +1,5 @@
-"""Python binding of libq4k_gemv.so (the C ABI in include/q4k_gemv.h).
+"""Python binding of libq4k_gemv.so (the C ABI in include/q4k_gemv.h,
+include/q4k_batch.h and include/q4k_gguf.h).
 
 The product is the C ABI; this module is plumbing for tests and the
 benchmark: it passes torch device tensors and torch's current HIP stream to
@@ -21,6 +22,7 @@ LIB_PATH = os.path.join(PKG_DIR, "libq4k_gemv.so")
 Q4K_OK, Q4K_EUNSUPPORTED, Q4K_EINVAL, Q4K_EHIP, Q4K_ENOMEM, Q4K_EIO, Q4K_EFORMAT, Q4K_ESCRATCH = 0, 1, 2, 3, 4, 5, 6, 7
 NOALLOC_SCRATCH_BYTES = 1 << 20
 GGML_TYPE_F32, GGML_TYPE_Q8_1, GGML_TYPE_Q4_K, GGML_TYPE_Q6_K = 0, 9, 12, 14
+GGML_TYPE_F16, GGML_TYPE_BF16 = 1, 30
 QK_K = 256
 BLOCK_Q4_K_BYTES = 144
 BLOCK_Q6_K_BYTES = 210
@@ -34,10 +36,47 @@ class q4k_gguf_tensor_info(ctypes.Structure):
                 ("data", ctypes.c_void_p)]
 
 
-# Every symbol include/q4k_gemv.h and include/q4k_gguf.h declare: (restype, argtypes)
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
+
+
+class q4k_lora(ctypes.Structure):
+    """The adapters of one projection (include/q4k_batch.h)."""
+    _fields_ = [("type", ctypes.c_int32), ("rank", ctypes.c_int32), ("n_adapters", _I64),
+                ("a", _P), ("nb_a", _I64), ("nb_a_adapter", _I64),
+                ("b", _P), ("nb_b", _I64), ("nb_b_adapter", _I64),
+                ("scale", _P), ("ranks", _P)]
+
+
+class q4k_kv_pages(ctypes.Structure):
+    """Keys and values in pages (include/q4k_batch.h)."""
+    _fields_ = [("k", _P), ("v", _P), ("n_pages", _I64), ("page_size", _I64),
+                ("nb_k_page", _I64), ("nb_k_token", _I64), ("nb_k_head", _I64),
+                ("nb_v_page", _I64), ("nb_v_token", _I64), ("nb_v_head", _I64),
+                ("table", _P), ("table_stride", _I64), ("table_len", _I64)]
+
+
+class q4k_prefix_attn_args(ctypes.Structure):
+    """Arguments of q4k_prefix_attn (include/q4k_batch.h)."""
+    _fields_ = [("q_type", ctypes.c_int32), ("kv_type", ctypes.c_int32), ("n_head", ctypes.c_int32),
+                ("n_head_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("n_tokens", _I64), ("n_requests", _I64), ("n_q", _I64), ("q_start", _P),
+                ("q", _P), ("nb_q_token", _I64), ("nb_q_head", _I64),
+                ("prefix", ctypes.POINTER(q4k_kv_pages)), ("n_prefix", _I64),
+                ("suffix", ctypes.POINTER(q4k_kv_pages)), ("suffix_len", _P), ("max_suffix", _I64),
+                ("dst", _P), ("nb_dst_token", _I64), ("nb_dst_head", _I64), ("lse", _P)]
+
+
+class q4k_logits_rules(ctypes.Structure):
+    """What changes the logits of each row (include/q4k_batch.h)."""
+    _fields_ = [("repeat", _P), ("frequency", _P), ("presence", _P),
+                ("history", _P), ("history_start", _P), ("n_history", _I64),
+                ("bias_ids", _P), ("bias", _P), ("bias_start", _P), ("n_bias", _I64),
+                ("mask", _P), ("n_masks", _I64), ("nb_mask", _I64), ("mask_rows", _P)]
+
+
+# Every symbol the headers of include/ declare: (restype, argtypes)
 SIGNATURES = {
     "q4k_version": (ctypes.c_int32, []),
     "q4k_strerror": (ctypes.c_char_p, [_I]),
@@ -69,6 +108,12 @@ SIGNATURES = {
     "q6k_gemv_geometry": (_I, [_I64, _I64, _I64, _P]),
     "q6k_gemv_geometry_q8_1": (_I, [_I64, _I64, _I64, _P]),
     "q4k_quantize_rows_q6_K": (_I, [_P, _P, _I64, _I64, _I]),
+    # include/q4k_batch.h
+    "q4k_lora_workspace_bytes": (ctypes.c_size_t, [_P, _I64, _I64, _I64]),
+    "q4k_lora_add": (_I, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _I64, _P, ctypes.c_size_t, _P]),
+    "q4k_prefix_attn_workspace_bytes": (ctypes.c_size_t, [_P]),
+    "q4k_prefix_attn": (_I, [_P, _P, ctypes.c_size_t, _P]),
+    "q4k_logits_adjust": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _P]),
     # include/q4k_gguf.h
     "q4k_gguf_open": (_I, [ctypes.c_char_p, ctypes.POINTER(_P)]),
     "q4k_gguf_close": (None, [_P]),
@@ -365,6 +410,233 @@ def geometry(K: int, M: int, N: int, wtype: int = GGML_TYPE_Q4_K, route: str = "
     keys = ("rows_per_tile", "waves_per_wg", "workgroups", "lds_bytes", "cols_per_launch", "fused",
             "kernel", "rows_per_step")
     return dict(zip(keys, list(out)))
+
+
+# ----------------------------------------------------- operators of a batch ----
+def _new(shape, dtype, device, stream):
+    """An uninitialised tensor that the allocator ties to the stream of the call."""
+    import torch
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _need(ok, what):
+    """The binding's own checks: what the C ABI cannot see of a tensor."""
+    if not ok:
+        raise ValueError(what)
+
+
+def _type16(t):
+    import torch
+    if t.dtype == torch.float16:
+        return GGML_TYPE_F16
+    if t.dtype == torch.bfloat16:
+        return GGML_TYPE_BF16
+    raise ValueError(f"{t.dtype}: float16 or bfloat16 expected")
+
+
+def _vector(t, dtype, n, device, what):
+    """A device vector of n values (n None: any number), or None."""
+    if t is not None:
+        _need(t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and t.device == device and (n is None or t.numel() == n),
+              f"{what}: contiguous {dtype} of {'any length' if n is None else n} on {device} expected")
+    return t
+
+
+def _ws(workspace):
+    return (_ptr(workspace), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
+
+
+class LoraAdapters:
+    """The low-rank adapters of one projection: a [adapters, rank, K] and
+    b [adapters, M, rank] of float16 or bfloat16 (rows contiguous), scale F32
+    [adapters] or None (1), ranks int32 [adapters] or None (all of rank).
+    Described once, used by every lora_add; the tensors are kept alive."""
+
+    def __init__(self, a, b, scale=None, ranks=None):
+        import torch
+        _need(a.dim() == 3 and b.dim() == 3 and a.dtype == b.dtype and a.device == b.device and
+              a.shape[0] == b.shape[0] and a.shape[1] == b.shape[2], "a [adapters, rank, K], b [adapters, M, rank] of one type")
+        _need(a.numel() == 0 or (a.stride(2) == 1 or a.shape[2] == 1), "rows of a are not contiguous")
+        _need(b.numel() == 0 or (b.stride(2) == 1 or b.shape[2] == 1), "rows of b are not contiguous")
+        n = a.shape[0]
+        self.tensors = (a, b, _vector(scale, torch.float32, n, a.device, "scale"),
+                        _vector(ranks, torch.int32, n, a.device, "ranks"))
+        self.K, self.M, self.rank, self.device = a.shape[2], b.shape[1], a.shape[1], a.device
+        self.desc = q4k_lora(_type16(a), self.rank, n, a.data_ptr(), a.stride(1) * 2, a.stride(0) * 2, b.data_ptr(),
+                             b.stride(1) * 2, b.stride(0) * 2, *(t.data_ptr() if t is not None else None for t in self.tensors[2:]))
+        self._ref = ctypes.byref(self.desc)
+
+
+def lora_workspace(adapters: LoraAdapters, n_tokens: int):
+    """A workspace for lora_add of up to n_tokens tokens."""
+    import torch
+    n = int(lib().q4k_lora_workspace_bytes(adapters._ref, adapters.K, adapters.M, n_tokens))
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=adapters.device)
+
+
+def lora_add(adapters: LoraAdapters, x, ids, base=None, out=None, workspace=None, stream=None):
+    """base + the tokens' adapters' products: F32 x [N, K], int32 ids [N]
+    (outside [0, adapters): none), base F32 [N, M] or None (zeros) -> F32
+    [N, M].  out may be base: the shared projection's result is then added to
+    in place."""
+    import torch
+    N = x.shape[0]
+    f32 = torch.float32
+    _need(x.dim() == 2 and x.dtype == f32 and x.shape[1] == adapters.K and x.device == adapters.device and
+          (x.stride(1) == 1 or x.shape[1] == 1), f"x: float32 [N, {adapters.K}] with contiguous rows expected")
+    _vector(ids, torch.int32, N, x.device, "ids")
+    if out is None:
+        out = _new((N, adapters.M), f32, x.device, stream)
+    for t in (out, base):
+        _need(t is None or (t.dtype == f32 and t.shape == (N, adapters.M) and t.device == x.device and
+                            (t.stride(1) == 1 or adapters.M == 1)), f"base, out: float32 [{N}, {adapters.M}] with contiguous rows expected")
+    ws, ws_bytes = _ws(workspace)
+    st = lib().q4k_lora_add(adapters._ref, adapters.K, adapters.M, x.data_ptr(), N, x.stride(0) * 4, ids.data_ptr(),
+                            base.data_ptr() if base is not None else None, base.stride(0) * 4 if base is not None else 0,
+                            out.data_ptr(), out.stride(0) * 4, ws, ws_bytes, _stream(stream))
+    if st != Q4K_OK:
+        raise Q4KError(st, "q4k_lora_add")
+    return out
+
+
+class KVPages:
+    """Keys and values k, v [pages, page_size, heads_kv, head_dim] of float16 or
+    bfloat16 (any strides, the last dimension contiguous) and the page numbers:
+    table int32 [requests, pages per request] (a prefix: [pages of it] or None
+    for the pages in order).  A contiguous prefix [tokens, heads_kv, head_dim] is
+    k[None], v[None].  The tensors are kept alive; their contents and the table's
+    may change between calls."""
+
+    def __init__(self, k, v, table=None):
+        import torch
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device and k.numel() > 0,
+              "k, v: [pages, page_size, heads_kv, head_dim] of one type and shape expected")
+        _need(k.stride(3) == 1 and v.stride(3) == 1, "head_dim of k, v is not contiguous")
+        self.tensors = (k, v, table)
+        self.type, self.heads, self.dim, self.device = _type16(k), k.shape[2], k.shape[3], k.device
+        self.rows, stride, length = None, 0, k.shape[0]
+        if table is not None:
+            _need(table.dtype == torch.int32 and table.dim() in (1, 2) and table.device == k.device and
+                  (table.stride(-1) == 1 or table.shape[-1] <= 1), "table: int32 with contiguous rows expected")
+            length = table.shape[-1]
+            if table.dim() == 2:
+                self.rows, stride = table.shape[0], table.stride(0)
+        self.desc = q4k_kv_pages(k.data_ptr(), v.data_ptr(), k.shape[0], k.shape[1], *(k.stride(i) * 2 for i in range(3)),
+                                 *(v.stride(i) * 2 for i in range(3)), table.data_ptr() if table is not None else None,
+                                 stride, length)
+        self._p = ctypes.pointer(self.desc)
+
+
+def _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, q_start, scale, out, lse):
+    import torch
+    _need(q.dim() == 3 and (q.stride(2) == 1 or q.shape[2] == 1), "q: [tokens, heads, head_dim] with contiguous dimensions expected")
+    n, heads, dim = q.shape
+    caches = [c for c in (prefix, suffix) if c is not None]
+    _need(caches and all(c.heads == caches[0].heads and c.dim == dim and c.type == caches[0].type and c.device == q.device for c in caches),
+          "prefix, suffix: at least one, of q's head_dim and device and of one type and number of heads")
+    kv = caches[0].type
+    qt = GGML_TYPE_F32 if q.dtype == torch.float32 else _type16(q)
+    if q_start is not None:
+        requests = q_start.numel() - 1
+        _vector(q_start, torch.int32, None, q.device, "q_start")
+        _need(requests >= 0, "q_start: requests + 1 entries expected")
+    else:
+        requests = n // n_q if n_q else 0
+    if max_suffix:
+        _need(suffix is not None and suffix_len is not None, "max_suffix without suffix and suffix_len")
+        _vector(suffix_len, torch.int32, requests, q.device, "suffix_len")
+        _need(suffix.rows in (None, requests) and (suffix.rows is not None or suffix.tensors[2] is None or requests == 1),
+              "suffix: a table row for each request expected")
+        if suffix.tensors[2] is None and requests:
+            suffix.desc.table_len = suffix.desc.n_pages // requests
+    _need(n_prefix == 0 or (prefix is not None and prefix.rows in (None, 1)), "n_prefix without a prefix of one table row")
+    if out is not None:
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and (out.stride(2) == 1 or dim == 1),
+              "out: shape and type of q expected")
+    if lse is not None:
+        _need(lse.shape == (n, heads) and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == q.device,
+              "lse: contiguous float32 [tokens, heads] expected")
+    es = 4 if qt == GGML_TYPE_F32 else 2
+    o = out if out is not None else q
+    return q4k_prefix_attn_args(
+        qt, kv, heads, caches[0].heads, dim, dim ** -0.5 if scale is None else scale, n, requests, n_q,
+        q_start.data_ptr() if q_start is not None else None, q.data_ptr(), q.stride(0) * es, q.stride(1) * es,
+        prefix._p if n_prefix else None, n_prefix, suffix._p if max_suffix else None,
+        suffix_len.data_ptr() if max_suffix else None, max_suffix, o.data_ptr(), o.stride(0) * es, o.stride(1) * es,
+        lse.data_ptr() if lse is not None else None)
+
+
+def prefix_attention_workspace(q, prefix, n_prefix, suffix=None, suffix_len=None, max_suffix=0, n_q=1, q_start=None):
+    """A workspace for prefix_attention calls of these sizes."""
+    import torch
+    args = _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, q_start, None, None, None)
+    n = int(lib().q4k_prefix_attn_workspace_bytes(ctypes.byref(args)))
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
+
+
+def prefix_attention(q, prefix, n_prefix, suffix=None, suffix_len=None, max_suffix=0, n_q=1, q_start=None, scale=None,
+                     out=None, lse=None, workspace=None, stream=None):
+    """Attention of a batch over n_prefix tokens that all requests share
+    (prefix, read once for all) and each request's own suffix_len[r] <=
+    max_suffix tokens (suffix), the last of which are the queries' own.
+    q [tokens, heads, head_dim], float32 or the caches' type: n_q tokens a
+    request, or q_start int32 [requests + 1] with at most n_q each.  Returns out
+    of q's type; lse F32 [tokens, heads] receives the rows' log-sum-exp."""
+    if out is None:
+        out = _new(q.shape, q.dtype, q.device, stream)
+    args = _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, q_start, scale, out, lse)
+    ws, ws_bytes = _ws(workspace)
+    st = lib().q4k_prefix_attn(ctypes.byref(args), ws, ws_bytes, _stream(stream))
+    if st != Q4K_OK:
+        raise Q4KError(st, "q4k_prefix_attn")
+    return out
+
+
+def logits_adjust(logits, repeat=None, frequency=None, presence=None, history=None, history_start=None, bias_ids=None,
+                  bias=None, bias_start=None, mask=None, mask_rows=None, out=None, stream=None):
+    """Penalties for repeated tokens, biases and grammar masks on F32 logits
+    [N, V] (q4k_logits_adjust).  repeat, frequency, presence F32 [N]; history
+    int32 with history_start int64 [N + 1]; bias_ids int32 and bias F32 with
+    bias_start int64 [N + 1]; mask int32 [masks, ceil(V / 32)] with mask_rows
+    int32 [N] (outside [0, masks): none).  out may be logits."""
+    import torch
+    f32, i32, i64 = torch.float32, torch.int32, torch.int64
+    _need(logits.dim() == 2 and logits.dtype == f32 and (logits.stride(1) == 1 or logits.shape[1] == 1), "logits: float32 [N, V] with contiguous rows expected")
+    N, V = logits.shape
+    dev = logits.device
+    if out is None:
+        out = _new((N, V), f32, dev, stream)
+    _need(out.dtype == f32 and out.shape == (N, V) and out.device == dev and (out.stride(1) == 1 or V == 1), "out: float32 [N, V] with contiguous rows expected")
+    p = [t.data_ptr() if _vector(t, f32, N, dev, "penalties") is not None else None for t in (repeat, frequency, presence)]
+    _need((history is None) == (history_start is None), "history without history_start")
+    _need((bias_ids is None) == (bias is None) == (bias_start is None), "bias_ids, bias and bias_start go together")
+    _need(mask is not None or mask_rows is None, "mask_rows without mask")
+    r = q4k_logits_rules(*p)
+    if history is not None:
+        r.history, r.history_start = _vector(history, i32, None, dev, "history").data_ptr(), _vector(history_start, i64, N + 1, dev, "history_start").data_ptr()
+        r.n_history = history.numel()
+        if not r.n_history:
+            r.history = r.history_start = None
+    if bias_ids is not None and bias_ids.numel():
+        r.n_bias = bias_ids.numel()
+        r.bias_ids, r.bias = _vector(bias_ids, i32, None, dev, "bias_ids").data_ptr(), _vector(bias, f32, r.n_bias, dev, "bias").data_ptr()
+        r.bias_start = _vector(bias_start, i64, N + 1, dev, "bias_start").data_ptr()
+    if mask is not None:
+        words = -(-V // 32)
+        _need(mask.dim() == 2 and mask.dtype == i32 and mask.shape[1] >= words and mask.device == dev and (mask.stride(1) == 1 or words <= 1),
+              f"mask: int32 [masks, {words}] with contiguous rows expected")
+        _need(mask_rows is not None or mask.shape[0] >= N, "mask: a row for each row of logits, or mask_rows, expected")
+        if mask.shape[0]:
+            r.mask, r.n_masks, r.nb_mask = mask.data_ptr(), mask.shape[0], mask.stride(0) * 4
+            r.mask_rows = _vector(mask_rows, i32, N, dev, "mask_rows").data_ptr() if mask_rows is not None else None
+    st = lib().q4k_logits_adjust(logits.data_ptr(), V, N, logits.stride(0) * 4, ctypes.byref(r), out.data_ptr(),
+                                 out.stride(0) * 4, _stream(stream))
+    if st != Q4K_OK:
+        raise Q4KError(st, "q4k_logits_adjust")
+    return out
 
 
 # ------------------------------------------------------------------ GGUF ----
