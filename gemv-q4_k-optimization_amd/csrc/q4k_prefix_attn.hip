@@ -1,104 +1,10 @@
 // q4k_prefix_attn.hip -- q4k_prefix_attn (include/q4k_batch.h): attention of a
 // batch of requests over a prefix that they share and over their own tokens.
-//
-// For a query row (token t, head h) with scores s_j = scale * q.k_j over the
-// positions j that it sees: m = max s_j, l = sum exp(s_j - m),
-// out = sum exp(s_j - m) v_j / l, lse = m + ln l, in one pass over the keys with
-// a running maximum and sum.
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
-#include <hip/hip_runtime.h>
-
-#include "q4k_batch_host.h"
-#include "q4k_device.h"
+// The kernels are in q4k_attn.h; here are the argument checks, the split of the
+// work and the launches.
+#include "q4k_attn.h"
 
 namespace q4k {
-
-struct AttnParams {
-    q4k_prefix_attn_args a;
-    q4k_kv_pages pre, suf;
-};
-
-// The element offset in bytes of token t, or -1 where its page is out of range.
-__device__ __forceinline__ int64_t page_of(const q4k_kv_pages &c, int64_t r, int64_t t, int64_t &slot) {
-    const int64_t e = t / c.page_size;
-    slot = t - e * c.page_size;
-    const int64_t pg = c.table ? (int64_t)c.table[r * c.table_stride + e] : r * c.table_len + e;
-    return pg >= 0 && pg < c.n_pages ? pg : -1;
-}
-
-// One wave per query row: 64 positions at a time, a lane's dot product each,
-// then their values one after the other with the head's dimensions over the
-// lanes.
-template <class T, class QT>
-__global__ __launch_bounds__(64) void prefix_attn_kernel(AttnParams p) {
-    __shared__ float qs[Q4K_ATTN_MAX_HEAD_DIM];
-    const q4k_prefix_attn_args &a = p.a;
-    const int lane = threadIdx.x;
-    const int64_t r = blockIdx.x / a.n_q, t = blockIdx.x % a.n_q;
-    const int head = blockIdx.y, hkv = head / (a.n_head / a.n_head_kv);
-    int64_t tok0 = r * a.n_q, tok1 = tok0 + a.n_q;
-    if (a.q_start) {
-        tok0 = a.q_start[r];
-        tok1 = a.q_start[r + 1];
-        if (tok0 < 0) tok0 = 0;
-        if (tok1 > a.n_tokens) tok1 = a.n_tokens;
-        if (tok1 > tok0 + a.n_q) tok1 = tok0 + a.n_q;
-    }
-    const int64_t tok = tok0 + t;
-    if (tok >= tok1) return;
-    const QT *q = reinterpret_cast<const QT *>((const char *)a.q + tok * a.nb_q_token + head * a.nb_q_head);
-    for (int d = lane; d < a.head_dim; d += 64) qs[d] = (float)q[d];
-    __syncthreads();
-    float m = -__builtin_inff(), l = 0.0f;
-    float o[Q4K_ATTN_MAX_HEAD_DIM / 64] = {};
-    for (int part = 0; part < 2; ++part) {
-        const q4k_kv_pages &c = part ? p.suf : p.pre;
-        int64_t len = a.n_prefix;
-        if (part) {
-            len = a.max_suffix > 0 ? a.suffix_len[r] : 0;
-            if (len > a.max_suffix) len = a.max_suffix;
-            len = len - (tok1 - tok0) + t + 1;
-        }
-        for (int64_t j0 = 0; j0 < len; j0 += 64) {
-            const int64_t j = j0 + lane;
-            int64_t slot = 0, pg = -1;
-            if (j < len) pg = page_of(c, part ? r : 0, j, slot);
-            float s = -__builtin_inff();
-            if (pg >= 0) {
-                const T *k = reinterpret_cast<const T *>((const char *)c.k + pg * c.nb_k_page + slot * c.nb_k_token +
-                                                         hkv * c.nb_k_head);
-                s = 0.0f;
-                for (int d = 0; d < a.head_dim; ++d) s += qs[d] * (float)k[d];
-                s *= a.scale;
-            }
-            float top = s;
-            for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-            const float mn = fmaxf(m, top);
-            if (mn == -__builtin_inff()) continue;
-            const float w = s == -__builtin_inff() ? 0.0f : __expf(s - mn), f = __expf(m - mn);
-            float sum = w;
-            for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
-            l = l * f + sum;
-            m = mn;
-            for (int e = 0; e < Q4K_ATTN_MAX_HEAD_DIM / 64; ++e) o[e] *= f;
-            for (int y = 0; y < 64; ++y) {
-                const int64_t pgy = __shfl((int)pg, y);
-                if (pgy < 0) continue;
-                const int64_t sy = __shfl((int)slot, y);
-                const float wy = __shfl(w, y);
-                const T *v = reinterpret_cast<const T *>((const char *)c.v + pgy * c.nb_v_page + sy * c.nb_v_token +
-                                                         hkv * c.nb_v_head);
-                for (int e = 0; e < Q4K_ATTN_MAX_HEAD_DIM / 64; ++e)
-                    if (e * 64 + lane < a.head_dim) o[e] += wy * (float)v[e * 64 + lane];
-            }
-        }
-    }
-    QT *out = reinterpret_cast<QT *>((char *)a.dst + tok * a.nb_dst_token + head * a.nb_dst_head);
-    for (int e = 0; e < Q4K_ATTN_MAX_HEAD_DIM / 64; ++e)
-        if (e * 64 + lane < a.head_dim) out[e * 64 + lane] = (QT)(l == 0.0f ? 0.0f : o[e] / l);
-    if (a.lse && lane == 0) a.lse[tok * a.n_head + head] = l == 0.0f ? -__builtin_inff() : m + logf(l);
-}
 
 static bool pages_ok(const q4k_kv_pages &c, int64_t tokens, int64_t rows) {
     if (!c.k || !c.v || c.n_pages < 1 || c.n_pages > INT32_MAX || c.page_size < 1 || c.page_size > INT32_MAX) return false;
@@ -145,13 +51,148 @@ static int attn_check(const q4k_prefix_attn_args *args, bool &empty) {
     return Q4K_OK;
 }
 
+
+// Workgroups' shapes: row tiles of 16 per wave, waves over rows.  Rows of 256
+// dimensions leave LDS for tiles of 64 positions only, two waves' worth.
+template <class T, int D, int SIZE>
+struct AttnShape;
+template <class T, int D>
+struct AttnShape<T, D, 0> {
+    using cfg = AttnCfg<T, D, 1, D == 256 ? 2 : 1>;
+};
+template <class T, int D>
+struct AttnShape<T, D, 1> {
+    using cfg = AttnCfg<T, D, 1, 4>;
+};
+template <class T, int D>
+struct AttnShape<T, D, 2> {
+    using cfg = AttnCfg<T, D, D == 256 ? 1 : 2, 4>;
+};
+
+struct AttnPlan {
+    int dim, pre_size, suf_size;  // padded head dimension, shapes
+    AttnParams p;
+    size_t bytes;
+    int lds;
+    const void *kernel;
+};
+
+template <class T, class QT, int TERMS, int D, int PS, int SS>
+void attn_kernel(AttnPlan &pl) {
+    using CP = typename AttnShape<T, D, PS>::cfg;
+    using CS = typename AttnShape<T, D, SS>::cfg;
+    pl.kernel = reinterpret_cast<const void *>(&prefix_attn_kernel<CP, CS, QT, TERMS>);
+    pl.lds = (CP::LDS > CS::LDS ? CP::LDS : CS::LDS) + 16 + 1024;
+}
+template <class T, class QT, int TERMS, int D>
+void attn_kernel_of(AttnPlan &pl) {
+    switch (pl.pre_size * 4 + pl.suf_size) {
+        case 0: return attn_kernel<T, QT, TERMS, D, 0, 0>(pl);
+        case 4: return attn_kernel<T, QT, TERMS, D, 1, 0>(pl);
+        case 8: return attn_kernel<T, QT, TERMS, D, 2, 0>(pl);
+        default: return attn_kernel<T, QT, TERMS, D, 2, 2>(pl);
+    }
+}
+template <class T, class QT, int TERMS>
+void attn_kernel_of(AttnPlan &pl) {
+    if (pl.dim == 64) attn_kernel_of<T, QT, TERMS, 64>(pl);
+    else if (pl.dim == 128) attn_kernel_of<T, QT, TERMS, 128>(pl);
+    else attn_kernel_of<T, QT, TERMS, 256>(pl);
+}
+
+static AttnCache attn_cache(const q4k_kv_pages &c, int64_t tokens) {
+    AttnCache k{};
+    k.k = (const char *)c.k;
+    k.v = (const char *)c.v;
+    k.k_page = c.nb_k_page; k.k_token = c.nb_k_token; k.k_head = c.nb_k_head;
+    k.v_page = c.nb_v_page; k.v_token = c.nb_v_token; k.v_head = c.nb_v_head;
+    k.table = c.table;
+    k.table_stride = c.table_stride;
+    k.n_pages = (int)c.n_pages;
+    k.table_len = (int)c.table_len;
+    k.one_page = !c.table && tokens <= c.page_size;
+    k.page = fastdiv_init((uint32_t)c.page_size);
+    return k;
+}
+
+static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
+    pl = AttnPlan{};
+    AttnParams &p = pl.p;
+    if (a.n_prefix > 0) p.pre = attn_cache(*a.prefix, a.n_prefix);
+    if (a.max_suffix > 0) p.suf = attn_cache(*a.suffix, a.max_suffix);
+    p.q = (const char *)a.q;
+    p.dst = (char *)a.dst;
+    p.lse = a.lse;
+    p.q_token = a.nb_q_token; p.q_head = a.nb_q_head; p.dst_token = a.nb_dst_token; p.dst_head = a.nb_dst_head;
+    p.q_start = a.q_start;
+    p.suffix_len = a.suffix_len;
+    p.n_tokens = (int)a.n_tokens; p.n_requests = (int)a.n_requests; p.n_q = (int)a.n_q;
+    p.n_prefix = (int)a.n_prefix; p.max_suffix = (int)a.max_suffix;
+    p.n_head = a.n_head; p.n_head_kv = a.n_head_kv; p.group = a.n_head / a.n_head_kv; p.head_dim = a.head_dim;
+    p.group_div = fastdiv_init((uint32_t)p.group);
+    p.scale = a.scale;
+    pl.dim = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
+    if (a.n_tokens > INT32_MAX / p.group - 256) return Q4K_EUNSUPPORTED;
+    const int64_t pre_rows = a.n_prefix > 0 ? a.n_tokens * p.group : 0, suf_rows = a.n_q * p.group;
+    const int rows_of[3] = {pl.dim == 256 ? 32 : 16, 64, pl.dim == 256 ? 64 : 128};
+    auto size_of = [&](int64_t rows) { return rows <= 16 ? 0 : rows <= 64 ? 1 : 2; };
+    pl.suf_size = suf_rows <= 64 ? 0 : 2;
+    pl.pre_size = pl.suf_size == 2 ? 2 : size_of(pre_rows);
+    const int pr = rows_of[pl.pre_size], sr = rows_of[pl.suf_size];
+    // splits: about two workgroups per CU, in whole tiles of 128 positions
+    const int64_t target = 2 * (int64_t)cus;
+    if (a.n_prefix > 0) {
+        const int64_t tiles = cdiv(pre_rows, pr), per = tiles * a.n_head_kv;
+        int64_t splits = target / per;
+        splits = splits < 1 ? 1 : splits;
+        const int64_t len = cdiv(cdiv(a.n_prefix, splits), 128) * 128;
+        p.pre_tiles = (int)tiles;
+        p.pre_len = (int)len;
+        p.pre_splits = (int)cdiv(a.n_prefix, len);
+        if (per * p.pre_splits > INT32_MAX / 2) return Q4K_EUNSUPPORTED;
+        p.pre_items = (int)(per * p.pre_splits);
+    }
+    if (a.max_suffix > 0 || a.n_prefix == 0) {
+        const int64_t tiles = cdiv(suf_rows, sr), per = tiles * a.n_head_kv * a.n_requests;
+        int64_t splits = target / per;
+        splits = splits < 1 ? 1 : splits;
+        int64_t len = cdiv(cdiv(a.max_suffix, splits), 128) * 128;
+        if (len < 128) len = 128;
+        p.suf_tiles = (int)tiles;
+        p.suf_len = (int)len;
+        p.suf_splits = a.max_suffix > 0 ? (int)cdiv(a.max_suffix, len) : 1;
+        if (per > INT32_MAX / 2 / p.suf_splits) return Q4K_EUNSUPPORTED;
+        p.suf_items = (int)(per * p.suf_splits);
+    }
+    p.slots = p.pre_splits + p.suf_splits;
+    if (p.slots > 1) {
+        const int64_t rows = a.n_tokens * a.n_head;
+        if (rows > ((int64_t)1 << 50) / p.slots / (a.head_dim + 2)) return Q4K_EUNSUPPORTED;
+        pl.bytes = (size_t)(rows * p.slots * (a.head_dim + 2) * 4);
+    }
+    if (a.n_requests * a.n_q > INT32_MAX / a.n_head) return Q4K_EUNSUPPORTED;
+    const bool f32 = a.q_type == Q4K_GGML_TYPE_F32;
+    if (a.kv_type == Q4K_GGML_TYPE_F16) f32 ? attn_kernel_of<_Float16, float, 2>(pl) : attn_kernel_of<_Float16, _Float16, 1>(pl);
+    else f32 ? attn_kernel_of<__bf16, float, 3>(pl) : attn_kernel_of<__bf16, __bf16, 1>(pl);
+    return Q4K_OK;
+}
+
 }  // namespace q4k
 
 using namespace q4k;
 
 extern "C" {
 
-size_t q4k_prefix_attn_workspace_bytes(const q4k_prefix_attn_args *) { return 0; }
+size_t q4k_prefix_attn_workspace_bytes(const q4k_prefix_attn_args *args) {
+    bool empty;
+    if (attn_check(args, empty) != Q4K_OK || empty) return 0;
+    DeviceInfo *di;
+    AttnPlan pl;
+    if (device_info(&di) != Q4K_OK || attn_plan(*args, di->cus, pl) != Q4K_OK) return 0;
+    return pl.bytes;
+}
 
 int q4k_prefix_attn(const q4k_prefix_attn_args *args, void *workspace, size_t workspace_bytes, void *stream) {
     bool empty;
@@ -160,16 +201,25 @@ int q4k_prefix_attn(const q4k_prefix_attn_args *args, void *workspace, size_t wo
     DeviceInfo *di;
     st = device_info(&di);
     if (st != Q4K_OK) return st;
-    (void)workspace;
-    (void)workspace_bytes;
-    AttnParams p{*args, {}, {}};
-    if (p.a.n_prefix > 0) p.pre = *p.a.prefix;
-    if (p.a.max_suffix > 0) p.suf = *p.a.suffix;
-    const bool f32 = p.a.q_type == Q4K_GGML_TYPE_F32;
-    auto *fn = p.a.kv_type == Q4K_GGML_TYPE_F16
-                   ? (f32 ? prefix_attn_kernel<_Float16, float> : prefix_attn_kernel<_Float16, _Float16>)
-                   : (f32 ? prefix_attn_kernel<__hip_bfloat16, float> : prefix_attn_kernel<__hip_bfloat16, __hip_bfloat16>);
-    return launch(fn, dim3((unsigned)(p.a.n_requests * p.a.n_q), (unsigned)p.a.n_head), 64, 0, stream, p);
+    AttnPlan pl;
+    st = attn_plan(*args, di->cus, pl);
+    if (st != Q4K_OK) return st;
+    st = ensure_lds(di, pl.kernel, pl.lds);
+    if (st != Q4K_OK) return st;
+    Workspace ws;
+    st = ws.begin(workspace, workspace_bytes, pl.bytes, stream);
+    if (st != Q4K_OK) return st;
+    AttnParams &p = pl.p;
+    p.part_o = (float *)ws.ptr;
+    p.part_ml = (float2 *)(p.part_o + (int64_t)p.n_tokens * p.n_head * p.slots * p.head_dim);
+    using Fn = void (*)(AttnParams);
+    st = launch((Fn)pl.kernel, dim3((unsigned)(p.pre_items + p.suf_items)), 256, pl.lds, stream, p);
+    if (st == Q4K_OK && p.slots > 1) {
+        const bool f32 = args->q_type == Q4K_GGML_TYPE_F32, f16 = args->kv_type == Q4K_GGML_TYPE_F16;
+        Fn join = f32 ? prefix_attn_join_kernel<float> : f16 ? prefix_attn_join_kernel<_Float16> : prefix_attn_join_kernel<__bf16>;
+        st = launch(join, dim3((unsigned)(p.n_requests * p.n_q * p.n_head)), 256, 0, stream, p);
+    }
+    return ws.end(st, stream);
 }
 
 }  // extern "C"
