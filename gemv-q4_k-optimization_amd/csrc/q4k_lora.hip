@@ -1,11 +1,22 @@
 // q4k_lora.hip -- q4k_lora_add (include/q4k_batch.h): low-rank adapters, one
 // per token, beside a projection that all tokens share.
 //
-//   h[n][j]   = sum_k x[n][k] a[i][j][k]           (shrink), i = ids[n]
-//   dst[n][m] = base[n][m] + scale[i] sum_j h[n][j] b[i][m][j]   (expand)
-// h is F32 in the workspace: rank values a token.
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
+//   h[n][j]   = sum_k x[n][k] a[i][j][k]                          (shrink), i = ids[n]
+//   dst[n][m] = base[n][m] + sum_j (scale[i] h[n][j]) b[i][m][j]   (expand)
+//
+// Both products run on v_mfma_f32_16x16x32_bf16 over tiles of up to 64 tokens
+// of one adapter: in the shrink the adapter's rows are the A operand and the
+// tokens the columns of B, in the expand the rows of b and the tokens' h.  A lane
+// of the result then holds four consecutive ranks (outputs) of one token.
+//
+// The F32 activations and h keep F32's precision: they enter as sums of three
+// BF16 values (24 bits), F16 adapters as sums of two (11 bits, exact), and the
+// products of all but the smallest terms are added: three matrix instructions for
+// BF16 adapters, five for F16.  BF16 has F32's exponents, so nothing overflows.
+//
+// Each column of a product depends on its token alone, so a token's result does
+// not depend on which tokens share its tile, nor on the order in which they
+// were put there.
 #include <hip/hip_runtime.h>
 
 #include "q4k_batch_host.h"
@@ -13,62 +24,472 @@
 
 namespace q4k {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kTile = 64;        // tokens of a tile
+constexpr int kSliceBallots = 8; // tokens that every workgroup looks through by itself: 8 x 64
+constexpr int kSlice = 64 * kSliceBallots;
+
 struct LoraParams {
     const char *a, *b;
-    int64_t nb_a, nb_a_adapter, nb_b, nb_b_adapter, n_adapters;
+    int64_t nb_a, nb_a_adapter, nb_b, nb_b_adapter;
     const float *scale;
     const int32_t *ranks;
     const char *x, *base;
     char *dst;
     int64_t nb_x, nb_base, nb_dst;
     const int32_t *ids;
-    float *h;
-    int64_t K, M, N;
-    int rank;
+    float *h;             // [ksplits][N][rp]
+    const int32_t *order; // grouped: tokens by adapter, and the tiles (first, count, adapter) of them
+    const int4 *tiles;
+    const int32_t *n_tiles;
+    int n_adapters, K, M, N, rank, rp;
+    int ksplits, kchunk, mchunk;
+    int copy;             // tokens without an adapter are copied (dst is not base)
 };
 
-__device__ __forceinline__ int adapter_rank(const LoraParams &p, int64_t i) {
+struct LoraTile {
+    int adapter;  // -1: tokens without one
+    int count;
+};
+
+// A tile's tokens into tok[0..63] (LDS), the same for all waves; false: nothing to do.
+// Grouped: tile blockIdx.z.  Else blockIdx.y is a token of the slice blockIdx.z,
+// and the workgroup of the first, 65th, ... token of an adapter takes the 64 from there.
+__device__ __forceinline__ bool lora_tile(const LoraParams &p, int *tok, LoraTile &t) {
+    const int lane = threadIdx.x & 63;
+    if (p.tiles) {
+        if ((int)blockIdx.z >= *p.n_tiles) return false;
+        const int4 d = p.tiles[blockIdx.z];
+        t.adapter = d.z;
+        t.count = d.y;
+        if (threadIdx.x < 64) tok[lane] = p.order[d.x + (lane < d.y ? lane : 0)];
+        __syncthreads();
+        return true;
+    }
+    const int base = blockIdx.z * kSlice, n = p.N - base < kSlice ? p.N - base : kSlice;
+    const int me = blockIdx.y;
+    if (me >= n) return false;
+    auto key_of = [&](int i) {
+        const int id = p.ids[base + i];
+        return id >= 0 && id < p.n_adapters ? id : -1;
+    };
+    const int key = __builtin_amdgcn_readfirstlane(key_of(me));
+    t.adapter = key;
+    uint64_t same[kSliceBallots];
+    int before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kSliceBallots; ++i) {
+        same[i] = 0;
+        if (i * 64 < n) {
+            const int at = i * 64 + lane;
+            same[i] = __ballot(at < n && key_of(at < n ? at : 0) == key);
+        }
+        const int d = me - i * 64;
+        before += __popcll(d >= 64 ? same[i] : d > 0 ? same[i] & ((1ull << d) - 1) : 0);
+        all += __popcll(same[i]);
+    }
+    if (before % kTile != 0) return false;
+    t.count = all - before < kTile ? all - before : kTile;
+    if (threadIdx.x < 64) {
+        tok[lane] = base + me;
+        int seen = 0;
+#pragma unroll
+        for (int i = 0; i < kSliceBallots; ++i) {
+            const int pos = seen + __popcll(same[i] & ((1ull << lane) - 1)) - before;
+            if ((same[i] >> lane & 1) && pos >= 0 && pos < kTile) tok[pos] = base + i * 64 + lane;
+            seen += __popcll(same[i]);
+        }
+    }
+    __syncthreads();
+    return true;
+}
+
+// Eight F32 as three BF16 vectors
+__device__ __forceinline__ void bf16_terms(const float (&x)[8], bf16x8 (&t)[3]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float r = x[j];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            t[i][j] = (__bf16)r;
+            r -= (float)t[i][j];
+        }
+    }
+}
+
+// Eight adapter values as BF16 terms, and the sum of products with three activation terms
+template <class T>
+struct Weights;
+template <>
+struct Weights<__bf16> {
+    bf16x8 w;
+    __device__ __forceinline__ void set(u32x4 v) { w = __builtin_bit_cast(bf16x8, v); }
+    __device__ __forceinline__ f32x4 mul(const bf16x8 (&x)[3], f32x4 c) const {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[2], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[1], c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[0], c, 0, 0, 0);
+    }
+};
+template <>
+struct Weights<_Float16> {
+    bf16x8 w, w2;
+    __device__ __forceinline__ void set(u32x4 v) {
+        const f16x8 h = __builtin_bit_cast(f16x8, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float f = (float)h[j];
+            w[j] = (__bf16)f;
+            w2[j] = (__bf16)(f - (float)w[j]);
+        }
+    }
+    __device__ __forceinline__ f32x4 mul(const bf16x8 (&x)[3], f32x4 c) const {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w2, x[1], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[2], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w2, x[0], c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[1], c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[0], c, 0, 0, 0);
+    }
+};
+
+// Values [k, k + 8) of a row of n 16-bit values, zeros past its end
+template <bool VEC>
+__device__ __forceinline__ u32x4 load_w(const char *row, int k, int n) {
+    u32x4 v = {0, 0, 0, 0};
+    if (VEC) {
+        if (k < n) v = *reinterpret_cast<const u32x4 *>(row + 2 * k);
+        return v;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint16_t *s = reinterpret_cast<const uint16_t *>(row) + k + 2 * j;
+        v[j] = (k + 2 * j < n ? s[0] : 0u) | (k + 2 * j + 1 < n ? (uint32_t)s[1] << 16 : 0u);
+    }
+    return v;
+}
+template <bool VEC>
+__device__ __forceinline__ void load_x(const float *row, int k, int n, float (&x)[8]) {
+    if (VEC) {
+        f32x4 v[2] = {};
+        if (k < n) {
+            v[0] = *reinterpret_cast<const f32x4 *>(row + k);
+            v[1] = *reinterpret_cast<const f32x4 *>(row + k + 4);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = v[j >> 2][j & 3];
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = k + j < n ? row[k + j] : 0.0f;
+}
+
+// the first n of eight values, zeros for the others
+__device__ __forceinline__ u32x4 first_w(u32x4 v, int n) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] &= (2 * j < n ? 0xffffu : 0u) | (2 * j + 1 < n ? 0xffff0000u : 0u);
+    return v;
+}
+
+__device__ __forceinline__ int adapter_rank(const LoraParams &p, int i) {
+    if (i < 0) return 0;
     const int r = p.ranks ? p.ranks[i] : p.rank;
     return r < 0 ? 0 : r > p.rank ? p.rank : r;
 }
 
-template <class T>
+// How the four waves share a tile: waves over its tiles of 16 tokens, the
+// others over the length (shrink: K, expand: M).
+struct WaveSplit {
+    int nt, part, parts;
+    __device__ __forceinline__ WaveSplit(int count, int wave) {
+        const int tiles = (count + 15) / 16;
+        const int w = tiles <= 1 ? 1 : tiles == 2 ? 2 : 4;
+        nt = wave % w;
+        part = wave / w;
+        parts = 4 / w;
+    }
+};
+
+constexpr int kRankTiles = 4;  // rank tiles of 16 per wave: 64 ranks
+
+// blockIdx.x: K split and group of 64 ranks
+template <class T, int NR, bool VEC>
 __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t n = blockIdx.x;
-    const int64_t i = p.ids[n];
-    if (i < 0 || i >= p.n_adapters) return;
-    const int r = adapter_rank(p, i);
-    const float *x = reinterpret_cast<const float *>(p.x + n * p.nb_x);
-    for (int j = wave; j < r; j += 4) {
-        const T *a = reinterpret_cast<const T *>(p.a + i * p.nb_a_adapter + j * p.nb_a);
-        float s = 0.0f;
-        for (int64_t k = lane; k < p.K; k += 64) s += x[k] * (float)a[k];
-        s = wave_sum(s);
-        if (lane == 63) p.h[n * p.rank + j] = s;
+    __shared__ int tok[kTile];
+    __shared__ f32x4 red[4][NR][64];
+    LoraTile t;
+    if (!lora_tile(p, tok, t) || t.adapter < 0) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int ks = blockIdx.x % p.ksplits, j0 = blockIdx.x / p.ksplits * (16 * NR);
+    const int r = adapter_rank(p, t.adapter);
+    const WaveSplit ws(t.count, wave);
+    const int token = tok[ws.nt * 16 + n];
+    const float *x = reinterpret_cast<const float *>(p.x + (int64_t)token * p.nb_x);
+    const char *a[NR];
+    bool row[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const int j = j0 + i * 16 + n;
+        row[i] = j < r;
+        a[i] = p.a + t.adapter * p.nb_a_adapter + (row[i] ? j : 0) * p.nb_a;
+    }
+    f32x4 acc[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // the parts of a split take its steps of 32 in turn
+    const int kend = (ks + 1) * p.kchunk < p.K ? (ks + 1) * p.kchunk : p.K;
+    if (ws.nt * 16 < t.count) {
+        constexpr int U = NR == 4 ? 2 : 4;  // steps in flight
+        const int step = ws.parts * 32;
+        for (int k0 = ks * p.kchunk + ws.part * 32; k0 < kend; k0 += step * U) {
+            float xv[U][8];
+            u32x4 av[U][NR];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k = k0 + u * step + g * 8, n_k = k0 + u * step < kend ? p.K : 0;
+                load_x<VEC>(x, k, n_k, xv[u]);
+#pragma unroll
+                for (int i = 0; i < NR; ++i) av[u][i] = load_w<VEC>(a[i], k, row[i] ? n_k : 0);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                bf16x8 xt[3];
+                bf16_terms(xv[u], xt);
+#pragma unroll
+                for (int i = 0; i < NR; ++i) {
+                    Weights<T> w;
+                    w.set(av[u][i]);
+                    acc[i] = w.mul(xt, acc[i]);
+                }
+            }
+        }
+    }
+    if (ws.parts > 1) {
+#pragma unroll
+        for (int i = 0; i < NR; ++i) red[wave][i][lane] = acc[i];
+        __syncthreads();
+        if (ws.part != 0) return;
+        for (int w = 1; w < ws.parts; ++w)
+#pragma unroll
+            for (int i = 0; i < NR; ++i) acc[i] += red[wave + w * (4 / ws.parts)][i][lane];
+    }
+    if (ws.nt * 16 + n >= t.count) return;
+    float *h = p.h + ((int64_t)ks * p.N + token) * p.rp + j0 + g * 4;
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+        if (j0 + i * 16 < p.rp) *reinterpret_cast<f32x4 *>(h + i * 16) = acc[i];
+}
+
+// KR: steps of 32 ranks; VB: rows of b in 16-byte loads; VD: base and dst in 16-byte accesses
+template <class T, int KR, bool VB, bool VD>
+__global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
+    __shared__ int tok[kTile];
+    LoraTile t;
+    if (!lora_tile(p, tok, t) || (t.adapter < 0 && !p.copy)) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int r = adapter_rank(p, t.adapter);
+    const WaveSplit ws(t.count, wave);
+    if (ws.nt * 16 >= t.count) return;
+    const bool live = ws.nt * 16 + n < t.count;
+    const int token = tok[ws.nt * 16 + n];
+    const float *base = reinterpret_cast<const float *>(p.base ? p.base + (int64_t)token * p.nb_base : nullptr);
+    float *dst = reinterpret_cast<float *>(p.dst + (int64_t)token * p.nb_dst);
+    bf16x8 ht[KR][3];
+    const float scale = p.scale && t.adapter >= 0 ? p.scale[t.adapter] : 1.0f;
+#pragma unroll
+    for (int kk = 0; kk < KR; ++kk) {
+        float hv[8] = {};
+        const int j = kk * 32 + g * 8;
+        if (j < r)  // (rp is a multiple of 16, so eight ranks are there or not)
+            for (int s = 0; s < p.ksplits; ++s) {
+                const float *h = p.h + ((int64_t)s * p.N + token) * p.rp + j;
+                const f32x4 h0 = *reinterpret_cast<const f32x4 *>(h), h1 = *reinterpret_cast<const f32x4 *>(h + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    hv[e] += h0[e];
+                    hv[e + 4] += h1[e];
+                }
+            }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hv[e] *= scale;
+        bf16_terms(hv, ht[kk]);
+    }
+    const char *b = p.b + (t.adapter < 0 ? 0 : t.adapter) * p.nb_b_adapter;
+    const int m0 = blockIdx.x * p.mchunk, m1 = m0 + p.mchunk < p.M ? m0 + p.mchunk : p.M;
+    constexpr int U = 2;  // row tiles in flight
+    for (int mb = m0 + ws.part * 16; mb < m1; mb += ws.parts * 16 * U) {
+        u32x4 bv[U][KR];
+        f32x4 y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int m = mb + u * ws.parts * 16;
+            const bool ok = m + n < m1;
+#pragma unroll
+            for (int kk = 0; kk < KR; ++kk)
+                bv[u][kk] = load_w<VB>(b + (ok ? m + n : 0) * p.nb_b, kk * 32 + g * 8, ok ? r : 0);
+            const int mm = m + g * 4;
+            y[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (base && live) {
+                if (VD) {
+                    if (mm < m1) y[u] = *reinterpret_cast<const f32x4 *>(base + mm);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (mm + j < m1) y[u][j] = base[mm + j];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int kk = 0; kk < KR; ++kk) {
+                Weights<T> w;
+                if (VB && (r & 7)) bv[u][kk] = first_w(bv[u][kk], r - kk * 32 - g * 8);
+                w.set(bv[u][kk]);
+                acc = w.mul(ht[kk], acc);
+            }
+            const int mm = mb + u * ws.parts * 16 + g * 4;
+            acc += y[u];
+            if (!live) continue;
+            if (VD) {
+                if (mm < m1) *reinterpret_cast<f32x4 *>(dst + mm) = acc;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (mm + j < m1) dst[mm + j] = acc[j];
+            }
+        }
     }
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
-    const int64_t n = blockIdx.y, m = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (m >= p.M) return;
-    const int64_t i = p.ids[n];
-    float y = p.base ? reinterpret_cast<const float *>(p.base + n * p.nb_base)[m] : 0.0f;
-    if (i >= 0 && i < p.n_adapters) {
-        const int r = adapter_rank(p, i);
-        const T *b = reinterpret_cast<const T *>(p.b + i * p.nb_b_adapter + m * p.nb_b);
-        float s = 0.0f;
-        for (int j = 0; j < r; ++j) s += p.h[n * p.rank + j] * (float)b[j];
-        y += (p.scale ? p.scale[i] : 1.0f) * s;
+// Tokens by adapter (counting sort in LDS, one workgroup) and the tiles of up to
+// 64 of them.  Atomics order the tokens within an adapter, on which no result
+// depends.
+__global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p) {
+    extern __shared__ int lds[];
+    const int keys = p.n_adapters + 1, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int *start = lds;                  // counts, then where each adapter's tokens go next
+    int *wsum = lds + keys;            // [2][16]
+    int32_t *order = const_cast<int32_t *>(p.order);
+    int4 *tiles = const_cast<int4 *>(p.tiles);
+    for (int i = tid; i < keys; i += 1024) start[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < p.N; i += 1024) {
+        const int id = p.ids[i];
+        atomicAdd(&start[id >= 0 && id < p.n_adapters ? id : p.n_adapters], 1);
     }
-    reinterpret_cast<float *>(p.dst + n * p.nb_dst)[m] = y;
+    __syncthreads();
+    // scan of the counts and of the numbers of tiles, 1024 keys at a time
+    int tokens = 0, ntiles = 0;
+    for (int k0 = 0; k0 < keys; k0 += 1024) {
+        const int k = k0 + tid;
+        const int c = k < keys ? start[k] : 0, q = (c + kTile - 1) / kTile;
+        int sc = c, sq = q;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int a = __shfl_up(sc, d), b = __shfl_up(sq, d);
+            if (lane >= d) {
+                sc += a;
+                sq += b;
+            }
+        }
+        if (lane == 63) {
+            wsum[wave] = sc;
+            wsum[16 + wave] = sq;
+        }
+        __syncthreads();
+        int bc = tokens, bq = ntiles, tc = 0, tq = 0;
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) {
+                bc += wsum[w];
+                bq += wsum[16 + w];
+            }
+            tc += wsum[w];
+            tq += wsum[16 + w];
+        }
+        const int first = bc + sc - c;
+        for (int i = 0; i < q; ++i)
+            tiles[bq + sq - q + i] = make_int4(first + i * kTile, c - i * kTile < kTile ? c - i * kTile : kTile,
+                                               k < p.n_adapters ? k : -1, 0);
+        if (k < keys) start[k] = first;
+        tokens += tc;
+        ntiles += tq;
+        __syncthreads();
+    }
+    if (tid == 0) *const_cast<int32_t *>(p.n_tiles) = ntiles;
+    for (int i = tid; i < p.N; i += 1024) {
+        const int id = p.ids[i];
+        order[atomicAdd(&start[id >= 0 && id < p.n_adapters ? id : p.n_adapters], 1)] = i;
+    }
+}
+
+// ---------------------------------------------------------------- host ----
+
+struct LoraPlan {
+    bool grouped;
+    int max_tiles;      // tiles there can be, grouped
+    int rp, nr, ksplits, kchunk, mchunk;
+    size_t h_bytes, bytes;
+};
+
+constexpr int kGroupKeys = 32000;  // counters in the group kernel's LDS
+
+static int lora_plan(const q4k_lora &l, int64_t K, int64_t M, int64_t N, LoraPlan &pl) {
+    constexpr int64_t cus = 256;
+    pl.grouped = N > kSlice && l.n_adapters < kGroupKeys;
+    const int64_t kinds = l.n_adapters + 1 < N ? l.n_adapters + 1 : N;
+    const int64_t tiles = N / kTile + kinds;  // at most
+    pl.max_tiles = (int)tiles;
+    pl.rp = (l.rank + 15) / 16 * 16;
+    pl.nr = pl.rp / 16 < kRankTiles ? pl.rp / 16 : kRankTiles;
+    if (pl.nr == 3) pl.nr = 4;
+    const int64_t groups = (pl.rp + 16 * pl.nr - 1) / (16 * pl.nr);
+    // two workgroups per CU, but at least 512 values (four steps of 32 per wave)
+    // and at most 8 splits, which every workgroup of the expand reads again
+    int64_t ks = 2 * cus / (tiles * groups);
+    const int64_t most = K / 512 < 8 ? K / 512 : 8;
+    ks = ks > most ? most : ks;
+    ks = ks < 1 ? 1 : ks;
+    pl.kchunk = (int)(((K + ks - 1) / ks + 127) / 128 * 128);
+    if (pl.kchunk < 128) pl.kchunk = 128;
+    pl.ksplits = K > 0 ? (int)((K + pl.kchunk - 1) / pl.kchunk) : 0;
+    // four workgroups per CU, at least one row tile per wave
+    int64_t mc = (M * tiles / (4 * cus) + 63) / 64 * 64;
+    mc = mc < 64 ? 64 : mc > 1024 ? 1024 : mc;
+    pl.mchunk = (int)mc;
+    if (N > ((int64_t)1 << 50) / (pl.rp * 4 * 8)) return Q4K_EUNSUPPORTED;
+    pl.h_bytes = (size_t)((int64_t)pl.ksplits * N * pl.rp * 4 + 15) / 16 * 16;
+    pl.bytes = pl.h_bytes + (pl.grouped ? (size_t)tiles * 16 + (size_t)N * 4 + 16 : 0);
+    return Q4K_OK;
 }
 
 static bool lora_sizes_ok(const q4k_lora *l, int64_t ne00, int64_t ne01, int64_t ne11) {
     return l && (l->type == Q4K_GGML_TYPE_F16 || l->type == Q4K_GGML_TYPE_BF16) && l->rank >= 1 &&
-           l->rank <= Q4K_LORA_MAX_RANK && l->n_adapters >= 0 && l->n_adapters <= INT32_MAX && ne00 >= 0 && ne01 >= 0 &&
-           ne11 >= 0 && ne00 <= INT32_MAX && ne01 <= INT32_MAX && ne11 <= INT32_MAX;
+           l->rank <= Q4K_LORA_MAX_RANK && l->n_adapters >= 0 && l->n_adapters <= INT32_MAX - 2 && ne00 >= 0 && ne01 >= 0 &&
+           ne11 >= 0 && ne00 <= INT32_MAX - 4096 && ne01 <= INT32_MAX - 4096 && ne11 <= INT32_MAX - 4096;
+}
+
+using LoraFn = void (*)(LoraParams);
+
+template <class T, bool VEC>
+LoraFn shrink_of(int nr) {
+    return nr == 1 ? lora_shrink_kernel<T, 1, VEC> : nr == 2 ? lora_shrink_kernel<T, 2, VEC> : lora_shrink_kernel<T, 4, VEC>;
+}
+template <class T, bool VB, bool VD>
+LoraFn expand_of(int kr) {
+    return kr <= 1   ? lora_expand_kernel<T, 1, VB, VD>
+           : kr <= 2 ? lora_expand_kernel<T, 2, VB, VD>
+           : kr <= 4 ? lora_expand_kernel<T, 4, VB, VD>
+                     : lora_expand_kernel<T, 8, VB, VD>;
+}
+template <class T>
+LoraFn expand_of(int kr, bool vb, bool vd) {
+    return vb ? (vd ? expand_of<T, true, true>(kr) : expand_of<T, true, false>(kr))
+              : (vd ? expand_of<T, false, true>(kr) : expand_of<T, false, false>(kr));
 }
 
 }  // namespace q4k
@@ -78,8 +499,9 @@ using namespace q4k;
 extern "C" {
 
 size_t q4k_lora_workspace_bytes(const q4k_lora *lora, int64_t ne00, int64_t ne01, int64_t ne11) {
-    if (!lora_sizes_ok(lora, ne00, ne01, ne11)) return 0;
-    return (size_t)ne11 * lora->rank * 4;
+    LoraPlan pl;
+    if (!lora_sizes_ok(lora, ne00, ne01, ne11) || ne11 == 0 || lora_plan(*lora, ne00, ne01, ne11, pl) != Q4K_OK) return 0;
+    return pl.bytes;
 }
 
 int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *src1, int64_t ne11, int64_t nb11,
@@ -103,23 +525,51 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
     DeviceInfo *di;
     int st = device_info(&di);
     if (st != Q4K_OK) return st;
-    if (ne11 > 65535) return Q4K_EUNSUPPORTED;
+    LoraPlan pl;
+    st = lora_plan(l, ne00, ne01, ne11, pl);
+    if (st != Q4K_OK) return st;
+    const int64_t slices = (ne11 + kSlice - 1) / kSlice;
+    if ((pl.grouped ? pl.max_tiles : slices) > 65535) return Q4K_EUNSUPPORTED;
     Workspace ws;
-    st = ws.begin(workspace, workspace_bytes, q4k_lora_workspace_bytes(lora, ne00, ne01, ne11), stream);
+    st = ws.begin(workspace, workspace_bytes, pl.bytes, stream);
     if (st != Q4K_OK) return st;
     LoraParams p{};
     p.a = (const char *)l.a; p.b = (const char *)l.b;
     p.nb_a = l.nb_a; p.nb_a_adapter = l.nb_a_adapter; p.nb_b = l.nb_b; p.nb_b_adapter = l.nb_b_adapter;
-    p.n_adapters = l.n_adapters; p.scale = l.scale; p.ranks = l.ranks;
+    p.n_adapters = (int)l.n_adapters; p.scale = l.scale; p.ranks = l.ranks;
     p.x = (const char *)src1; p.base = (const char *)src2; p.dst = (char *)dst;
     p.nb_x = nb11; p.nb_base = nb21; p.nb_dst = nb1;
-    p.ids = ids; p.h = (float *)ws.ptr; p.K = ne00; p.M = ne01; p.N = ne11; p.rank = l.rank;
+    p.ids = ids; p.h = (float *)ws.ptr; p.K = (int)ne00; p.M = (int)ne01; p.N = (int)ne11;
+    p.rank = l.rank; p.rp = pl.rp; p.ksplits = pl.ksplits; p.kchunk = pl.kchunk; p.mchunk = pl.mchunk;
+    p.copy = src2 != dst;
+    dim3 grid(1, (unsigned)(ne11 < kSlice ? ne11 : kSlice), (unsigned)slices);
+    if (pl.grouped) {
+        char *w = (char *)ws.ptr + pl.h_bytes;
+        p.tiles = (const int4 *)w;
+        p.order = (const int32_t *)(w + (size_t)pl.max_tiles * 16);
+        p.n_tiles = p.order + ne11;
+        grid = dim3(1, 1, (unsigned)pl.max_tiles);
+        const int lds = (int)(l.n_adapters + 1 + 32) * 4;
+        st = ensure_lds(di, (const void *)&lora_group_kernel, lds);
+        if (st == Q4K_OK) st = launch(lora_group_kernel, dim3(1), 1024, lds, stream, p);
+    }
     const bool f16 = l.type == Q4K_GGML_TYPE_F16;
-    st = launch(f16 ? lora_shrink_kernel<_Float16> : lora_shrink_kernel<__hip_bfloat16>, dim3((unsigned)ne11), 256, 0,
-                stream, p);
-    if (st == Q4K_OK)
-        st = launch(f16 ? lora_expand_kernel<_Float16> : lora_expand_kernel<__hip_bfloat16>,
-                    dim3((unsigned)((ne01 + 255) / 256), (unsigned)ne11), 256, 0, stream, p);
+    if (st == Q4K_OK && pl.ksplits > 0 && l.n_adapters > 0) {
+        const bool vec = ne00 % 8 == 0 && aligned(l.a, 16) && (l.nb_a | l.nb_a_adapter) % 16 == 0 && aligned(src1, 16) &&
+                         nb11 % 16 == 0;
+        const int groups = (pl.rp + 16 * pl.nr - 1) / (16 * pl.nr);
+        grid.x = (unsigned)(pl.ksplits * groups);
+        st = launch(f16 ? (vec ? shrink_of<_Float16, true>(pl.nr) : shrink_of<_Float16, false>(pl.nr))
+                        : (vec ? shrink_of<__bf16, true>(pl.nr) : shrink_of<__bf16, false>(pl.nr)),
+                    grid, 256, 0, stream, p);
+    }
+    if (st == Q4K_OK) {
+        const bool vb = l.rank % 8 == 0 && aligned(l.b, 16) && (l.nb_b | l.nb_b_adapter) % 16 == 0;
+        const bool vd = ne01 % 4 == 0 && aligned(dst, 16) && nb1 % 16 == 0 && aligned(src2, 16) && nb21 % 16 == 0;
+        grid.x = (unsigned)((ne01 + pl.mchunk - 1) / pl.mchunk);
+        st = launch(f16 ? expand_of<_Float16>((l.rank + 31) / 32, vb, vd) : expand_of<__bf16>((l.rank + 31) / 32, vb, vd), grid,
+                    256, 0, stream, p);
+    }
     return ws.end(st, stream);
 }
 
