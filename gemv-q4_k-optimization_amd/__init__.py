@@ -428,6 +428,20 @@ def _need(ok, what):
         raise ValueError(what)
 
 
+def _stream_of(stream, device):
+    """The stream of a call on `device`: torch's current one unless given.
+    (Without torch.cuda.current_stream, which costs as much as a launch.)"""
+    if stream is not None:
+        return stream.cuda_stream
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device) if device >= 0 else None
+
+
+def _rows(t, dtype, n, m, device):
+    """Whether t is [n, m] of dtype on device (its number) with contiguous rows."""
+    return t.dtype is dtype and t.shape == (n, m) and t.get_device() == device and (m == 1 or t.stride(1) == 1)
+
+
 def _type16(t):
     import torch
     if t.dtype == torch.float16:
@@ -438,15 +452,16 @@ def _type16(t):
 
 
 def _vector(t, dtype, n, device, what):
-    """A device vector of n values (n None: any number), or None."""
-    if t is not None:
-        _need(t.dtype == dtype and t.dim() == 1 and t.is_contiguous() and t.device == device and (n is None or t.numel() == n),
-              f"{what}: contiguous {dtype} of {'any length' if n is None else n} on {device} expected")
-    return t
+    """The address of a contiguous device vector of n values (n None: any number), or None for None."""
+    if t is None:
+        return None
+    if not (t.dtype is dtype and t.shape == (t.numel() if n is None else n,) and t.get_device() == device and t.is_contiguous()):
+        raise ValueError(f"{what}: contiguous {dtype} of {'any length' if n is None else n} on device {device} expected")
+    return t.data_ptr()
 
 
 def _ws(workspace):
-    return (_ptr(workspace), workspace.numel() * workspace.element_size()) if workspace is not None else (None, 0)
+    return (workspace.data_ptr(), workspace.nbytes) if workspace is not None else (None, 0)
 
 
 class LoraAdapters:
@@ -462,11 +477,11 @@ class LoraAdapters:
         _need(a.numel() == 0 or (a.stride(2) == 1 or a.shape[2] == 1), "rows of a are not contiguous")
         _need(b.numel() == 0 or (b.stride(2) == 1 or b.shape[2] == 1), "rows of b are not contiguous")
         n = a.shape[0]
-        self.tensors = (a, b, _vector(scale, torch.float32, n, a.device, "scale"),
-                        _vector(ranks, torch.int32, n, a.device, "ranks"))
-        self.K, self.M, self.rank, self.device = a.shape[2], b.shape[1], a.shape[1], a.device
+        self.tensors = (a, b, scale, ranks)
+        self.K, self.M, self.rank, self.device, self.index = a.shape[2], b.shape[1], a.shape[1], a.device, a.get_device()
         self.desc = q4k_lora(_type16(a), self.rank, n, a.data_ptr(), a.stride(1) * 2, a.stride(0) * 2, b.data_ptr(),
-                             b.stride(1) * 2, b.stride(0) * 2, *(t.data_ptr() if t is not None else None for t in self.tensors[2:]))
+                             b.stride(1) * 2, b.stride(0) * 2, _vector(scale, torch.float32, n, a.get_device(), "scale"),
+                             _vector(ranks, torch.int32, n, a.get_device(), "ranks"))
         self._ref = ctypes.byref(self.desc)
 
 
@@ -483,20 +498,19 @@ def lora_add(adapters: LoraAdapters, x, ids, base=None, out=None, workspace=None
     [N, M].  out may be base: the shared projection's result is then added to
     in place."""
     import torch
-    N = x.shape[0]
-    f32 = torch.float32
-    _need(x.dim() == 2 and x.dtype == f32 and x.shape[1] == adapters.K and x.device == adapters.device and
-          (x.stride(1) == 1 or x.shape[1] == 1), f"x: float32 [N, {adapters.K}] with contiguous rows expected")
-    _vector(ids, torch.int32, N, x.device, "ids")
+    f32, dev, K, M, N = torch.float32, adapters.index, adapters.K, adapters.M, x.shape[0]
+    if not _rows(x, f32, N, K, dev):
+        raise ValueError(f"x: float32 [N, {K}] with contiguous rows on {adapters.device} expected")
     if out is None:
-        out = _new((N, adapters.M), f32, x.device, stream)
-    for t in (out, base):
-        _need(t is None or (t.dtype == f32 and t.shape == (N, adapters.M) and t.device == x.device and
-                            (t.stride(1) == 1 or adapters.M == 1)), f"base, out: float32 [{N}, {adapters.M}] with contiguous rows expected")
+        out = _new((N, M), f32, adapters.device, stream)
+    elif not _rows(out, f32, N, M, dev):
+        raise ValueError(f"out: float32 [{N}, {M}] with contiguous rows on {adapters.device} expected")
+    if base is not None and not _rows(base, f32, N, M, dev):
+        raise ValueError(f"base: float32 [{N}, {M}] with contiguous rows on {adapters.device} expected")
     ws, ws_bytes = _ws(workspace)
-    st = lib().q4k_lora_add(adapters._ref, adapters.K, adapters.M, x.data_ptr(), N, x.stride(0) * 4, ids.data_ptr(),
+    st = lib().q4k_lora_add(adapters._ref, K, M, x.data_ptr(), N, x.stride(0) * 4, _vector(ids, torch.int32, N, dev, "ids"),
                             base.data_ptr() if base is not None else None, base.stride(0) * 4 if base is not None else 0,
-                            out.data_ptr(), out.stride(0) * 4, ws, ws_bytes, _stream(stream))
+                            out.data_ptr(), out.stride(0) * 4, ws, ws_bytes, _stream_of(stream, dev))
     if st != Q4K_OK:
         raise Q4KError(st, "q4k_lora_add")
     return out
@@ -516,7 +530,7 @@ class KVPages:
               "k, v: [pages, page_size, heads_kv, head_dim] of one type and shape expected")
         _need(k.stride(3) == 1 and v.stride(3) == 1, "head_dim of k, v is not contiguous")
         self.tensors = (k, v, table)
-        self.type, self.heads, self.dim, self.device = _type16(k), k.shape[2], k.shape[3], k.device
+        self.type, self.heads, self.dim, self.device = _type16(k), k.shape[2], k.shape[3], k.get_device()
         self.rows, stride, length = None, 0, k.shape[0]
         if table is not None:
             _need(table.dtype == torch.int32 and table.dim() in (1, 2) and table.device == k.device and
@@ -532,41 +546,44 @@ class KVPages:
 
 def _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, q_start, scale, out, lse):
     import torch
-    _need(q.dim() == 3 and (q.stride(2) == 1 or q.shape[2] == 1), "q: [tokens, heads, head_dim] with contiguous dimensions expected")
     n, heads, dim = q.shape
-    caches = [c for c in (prefix, suffix) if c is not None]
-    _need(caches and all(c.heads == caches[0].heads and c.dim == dim and c.type == caches[0].type and c.device == q.device for c in caches),
-          "prefix, suffix: at least one, of q's head_dim and device and of one type and number of heads")
-    kv = caches[0].type
-    qt = GGML_TYPE_F32 if q.dtype == torch.float32 else _type16(q)
+    dev, dtype = q.get_device(), q.dtype
+    cache = suffix if prefix is None else prefix
+    if cache is None or cache.dim != dim or cache.device != dev or (q.stride(2) != 1 and dim > 1):
+        raise ValueError("q: [tokens, heads, head_dim] with contiguous dimensions, of the caches' head_dim and device expected")
+    if suffix is not None and cache is not suffix and (suffix.heads, suffix.dim, suffix.type, suffix.device) != (cache.heads, dim, cache.type, dev):
+        raise ValueError("prefix, suffix: one type, number of heads, head_dim and device expected")
+    qt, es = (GGML_TYPE_F32, 4) if dtype is torch.float32 else (_type16(q), 2)
+    start = None
     if q_start is not None:
-        requests = q_start.numel() - 1
-        _vector(q_start, torch.int32, None, q.device, "q_start")
+        start = _vector(q_start, torch.int32, None, dev, "q_start")
+        requests = q_start.shape[0] - 1
         _need(requests >= 0, "q_start: requests + 1 entries expected")
     else:
         requests = n // n_q if n_q else 0
+    lens = None
     if max_suffix:
         _need(suffix is not None and suffix_len is not None, "max_suffix without suffix and suffix_len")
-        _vector(suffix_len, torch.int32, requests, q.device, "suffix_len")
-        _need(suffix.rows in (None, requests) and (suffix.rows is not None or suffix.tensors[2] is None or requests == 1),
-              "suffix: a table row for each request expected")
-        if suffix.tensors[2] is None and requests:
-            suffix.desc.table_len = suffix.desc.n_pages // requests
-    _need(n_prefix == 0 or (prefix is not None and prefix.rows in (None, 1)), "n_prefix without a prefix of one table row")
-    if out is not None:
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and (out.stride(2) == 1 or dim == 1),
-              "out: shape and type of q expected")
+        lens = _vector(suffix_len, torch.int32, requests, dev, "suffix_len")
+        if suffix.tensors[2] is None:
+            if requests:
+                suffix.desc.table_len = suffix.desc.n_pages // requests
+        elif suffix.rows != requests and requests != 1:
+            raise ValueError("suffix: a table row for each request expected")
+    if n_prefix and (prefix is None or prefix.rows not in (None, 1)):
+        raise ValueError("n_prefix without a prefix of one table row")
+    if out is None:
+        out = q
+    elif out.shape != q.shape or out.dtype is not dtype or out.get_device() != dev or (out.stride(2) != 1 and dim > 1):
+        raise ValueError("out: shape, type and device of q with contiguous dimensions expected")
     if lse is not None:
-        _need(lse.shape == (n, heads) and lse.dtype == torch.float32 and lse.is_contiguous() and lse.device == q.device,
-              "lse: contiguous float32 [tokens, heads] expected")
-    es = 4 if qt == GGML_TYPE_F32 else 2
-    o = out if out is not None else q
+        if lse.shape != (n, heads) or lse.dtype is not torch.float32 or lse.get_device() != dev or not lse.is_contiguous():
+            raise ValueError("lse: contiguous float32 [tokens, heads] expected")
+        lse = lse.data_ptr()
     return q4k_prefix_attn_args(
-        qt, kv, heads, caches[0].heads, dim, dim ** -0.5 if scale is None else scale, n, requests, n_q,
-        q_start.data_ptr() if q_start is not None else None, q.data_ptr(), q.stride(0) * es, q.stride(1) * es,
-        prefix._p if n_prefix else None, n_prefix, suffix._p if max_suffix else None,
-        suffix_len.data_ptr() if max_suffix else None, max_suffix, o.data_ptr(), o.stride(0) * es, o.stride(1) * es,
-        lse.data_ptr() if lse is not None else None)
+        qt, cache.type, heads, cache.heads, dim, dim ** -0.5 if scale is None else scale, n, requests, n_q,
+        start, q.data_ptr(), q.stride(0) * es, q.stride(1) * es, prefix._p if n_prefix else None, n_prefix,
+        suffix._p if max_suffix else None, lens, max_suffix, out.data_ptr(), out.stride(0) * es, out.stride(1) * es, lse)
 
 
 def prefix_attention_workspace(q, prefix, n_prefix, suffix=None, suffix_len=None, max_suffix=0, n_q=1, q_start=None):
@@ -589,7 +606,7 @@ def prefix_attention(q, prefix, n_prefix, suffix=None, suffix_len=None, max_suff
         out = _new(q.shape, q.dtype, q.device, stream)
     args = _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, q_start, scale, out, lse)
     ws, ws_bytes = _ws(workspace)
-    st = lib().q4k_prefix_attn(ctypes.byref(args), ws, ws_bytes, _stream(stream))
+    st = lib().q4k_prefix_attn(ctypes.byref(args), ws, ws_bytes, _stream_of(stream, q.get_device()))
     if st != Q4K_OK:
         raise Q4KError(st, "q4k_prefix_attn")
     return out
@@ -604,36 +621,47 @@ def logits_adjust(logits, repeat=None, frequency=None, presence=None, history=No
     int32 [N] (outside [0, masks): none).  out may be logits."""
     import torch
     f32, i32, i64 = torch.float32, torch.int32, torch.int64
-    _need(logits.dim() == 2 and logits.dtype == f32 and (logits.stride(1) == 1 or logits.shape[1] == 1), "logits: float32 [N, V] with contiguous rows expected")
     N, V = logits.shape
-    dev = logits.device
+    dev = logits.get_device()
+    if not _rows(logits, f32, N, V, dev):
+        raise ValueError("logits: float32 [N, V] with contiguous rows expected")
     if out is None:
-        out = _new((N, V), f32, dev, stream)
-    _need(out.dtype == f32 and out.shape == (N, V) and out.device == dev and (out.stride(1) == 1 or V == 1), "out: float32 [N, V] with contiguous rows expected")
-    p = [t.data_ptr() if _vector(t, f32, N, dev, "penalties") is not None else None for t in (repeat, frequency, presence)]
-    _need((history is None) == (history_start is None), "history without history_start")
-    _need((bias_ids is None) == (bias is None) == (bias_start is None), "bias_ids, bias and bias_start go together")
-    _need(mask is not None or mask_rows is None, "mask_rows without mask")
-    r = q4k_logits_rules(*p)
+        out = _new((N, V), f32, logits.device, stream)
+    elif not _rows(out, f32, N, V, dev):
+        raise ValueError("out: float32 [N, V] with contiguous rows expected")
+    if (history is None) != (history_start is None):
+        raise ValueError("history without history_start")
+    if (bias_ids is None) != (bias is None) or (bias_ids is None) != (bias_start is None):
+        raise ValueError("bias_ids, bias and bias_start go together")
+    h = hs = bi = bv = bs = m = mr = None
+    nh = nb = masks = nbm = 0
     if history is not None:
-        r.history, r.history_start = _vector(history, i32, None, dev, "history").data_ptr(), _vector(history_start, i64, N + 1, dev, "history_start").data_ptr()
-        r.n_history = history.numel()
-        if not r.n_history:
-            r.history = r.history_start = None
-    if bias_ids is not None and bias_ids.numel():
-        r.n_bias = bias_ids.numel()
-        r.bias_ids, r.bias = _vector(bias_ids, i32, None, dev, "bias_ids").data_ptr(), _vector(bias, f32, r.n_bias, dev, "bias").data_ptr()
-        r.bias_start = _vector(bias_start, i64, N + 1, dev, "bias_start").data_ptr()
+        h, hs, nh = _vector(history, i32, None, dev, "history"), _vector(history_start, i64, N + 1, dev, "history_start"), history.shape[0]
+        if nh == 0:
+            h = hs = None
+    if bias_ids is not None:
+        nb = bias_ids.shape[0]
+        bi, bv = _vector(bias_ids, i32, None, dev, "bias_ids"), _vector(bias, f32, nb, dev, "bias")
+        bs = _vector(bias_start, i64, N + 1, dev, "bias_start")
+        if nb == 0:
+            bi = bv = bs = None
     if mask is not None:
-        words = -(-V // 32)
-        _need(mask.dim() == 2 and mask.dtype == i32 and mask.shape[1] >= words and mask.device == dev and (mask.stride(1) == 1 or words <= 1),
-              f"mask: int32 [masks, {words}] with contiguous rows expected")
-        _need(mask_rows is not None or mask.shape[0] >= N, "mask: a row for each row of logits, or mask_rows, expected")
-        if mask.shape[0]:
-            r.mask, r.n_masks, r.nb_mask = mask.data_ptr(), mask.shape[0], mask.stride(0) * 4
-            r.mask_rows = _vector(mask_rows, i32, N, dev, "mask_rows").data_ptr() if mask_rows is not None else None
+        masks, words = mask.shape
+        if words < -(-V // 32) or not _rows(mask, i32, masks, words, dev):
+            raise ValueError(f"mask: int32 [masks, {-(-V // 32)}] with contiguous rows expected")
+        if mask_rows is None and masks < N:
+            raise ValueError("mask: a row for each row of logits, or mask_rows, expected")
+        mr = _vector(mask_rows, i32, N, dev, "mask_rows")
+        if masks:
+            m, nbm = mask.data_ptr(), mask.stride(0) * 4
+        else:
+            mr = None
+    elif mask_rows is not None:
+        raise ValueError("mask_rows without mask")
+    r = q4k_logits_rules(_vector(repeat, f32, N, dev, "repeat"), _vector(frequency, f32, N, dev, "frequency"),
+                         _vector(presence, f32, N, dev, "presence"), h, hs, nh, bi, bv, bs, nb, m, masks, nbm, mr)
     st = lib().q4k_logits_adjust(logits.data_ptr(), V, N, logits.stride(0) * 4, ctypes.byref(r), out.data_ptr(),
-                                 out.stride(0) * 4, _stream(stream))
+                                 out.stride(0) * 4, _stream_of(stream, dev))
     if st != Q4K_OK:
         raise Q4KError(st, "q4k_logits_adjust")
     return out
