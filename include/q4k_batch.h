@@ -139,7 +139,8 @@ typedef struct q4k_logits_rules {
     const float *frequency; /* subtracted once per occurrence in the history */
     const float *presence;  /* subtracted once from every token in the history */
     /* the rows' histories one after the other: row i has the entries
-     * [history_start[i], history_start[i+1]), clamped to n_history */
+     * [history_start[i], history_start[i+1]), clamped to n_history (and to less
+     * than 2^31 of them) */
     const int32_t *history;
     const int64_t *history_start;
     int64_t n_history;
