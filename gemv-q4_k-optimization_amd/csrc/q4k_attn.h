@@ -130,17 +130,16 @@ __device__ __forceinline__ float xor_sum(float v) {
 }
 
 // D: head dimension rounded up to 64, 128 or 256; RT: tiles of 16 rows per
-// wave; WR: waves over rows, the others of the four over positions; TERMS:
-// values of T per F32 query or probability.
-template <class T, int D_, int RT_, int WR_>
-struct AttnCfg {
+// wave; TERMS: values of T per F32 query or probability.
+template <class T, int D_, int RT_, int TERMS>
+struct SharedCfg {
     using Elem = T;
-    static constexpr int D = D_, RT = RT_, WR = WR_, WT = 4 / WR_;
+    static constexpr int D = D_, RT = RT_;
     static constexpr int CH = D / 8;        // 16-byte chunks of a row of K or V
     static constexpr int RP = 256 / CH;     // rows staged per pass of the workgroup
-    static constexpr int TB = D == 256 ? 64 : WT == 1 ? 64 : 128;  // positions of a tile in LDS
+    static constexpr int TB = 64;           // positions of a tile in LDS
     static constexpr int NP = TB / RP;      // passes
-    static constexpr int ROWS = 16 * RT * WR;
+    static constexpr int ROWS = 64 * RT;
     static constexpr int LDS = 2 * TB * D * 2;
 };
 
@@ -155,27 +154,25 @@ __device__ __forceinline__ int swz_v(int t, int c) {
     return D == 64 ? c ^ (((t >> 1) & 3) * 2) : c ^ ((t & 7) * 2);
 }
 
-template <class C, class QT, int TERMS>
-__device__ __forceinline__ void attn_span(const AttnParams &p, const AttnCache &kv, const AttnSpan &s, int hk, int tile0,
-                                          char *lds, int *flags) {
-    using T = typename C::Elem;
-    using V8 = typename Vec8<T>::type;
-    constexpr int D = C::D, RT = C::RT, WT = C::WT, CH = C::CH, RP = C::RP, TB = C::TB, NP = C::NP;
-    constexpr int KK = D / 32, DT = D / 16;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = lane & 15, g = lane >> 4;
-    const int wr = wave / WT, wt = wave % WT;
-    const char *ldk = lds;
-    const char *ldv = lds + TB * D * 2;
-    uint8_t *seen = reinterpret_cast<uint8_t *>(flags + 4);  // one byte per position of the tile
+// What a wave holds of its RT tiles of 16 query rows: lane n of a tile has row
+// n's limit, factor, running reference and its part of the sum.
+template <int RT, int D>
+struct AttnRows {
+    float c[RT];     // log2(e) * |scale| * 2^e of the row's own factor
+    int limit[RT];   // positions the row sees end here
+    float m[RT];     // reference in units of S
+    float l[RT];     // this lane's part of the sum of exp2(c s - c m + kBias)
+    f32x4 o[RT][D / 16];
+};
 
-    // ---- queries: lane n of a tile's rows, eight dimensions each ----
-    V8 q[RT][TERMS][KK];
-    float c[RT];       // log2(e) * scale, and 2^e of the row's own factor
-    int limit[RT];     // positions the row sees end here
+// Rows row0.. of the span: eight dimensions kk * 32 + g * 8 .. per lane, as TERMS
+// values of T, handed to put(rt, term, kk, vector).
+template <class T, int D, int RT, class QT, int TERMS, class PUT>
+__device__ __forceinline__ void attn_queries(const AttnParams &p, const AttnSpan &s, int hk, int row0, AttnRows<RT, D> &w, PUT put) {
+    using V8 = typename Vec8<T>::type;
+    constexpr int KK = D / 32;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const float sgn = p.scale < 0.0f ? -1.0f : 1.0f;
-    const int row0 = tile0 * C::ROWS + wr * RT * 16;
-    int lim_min = s.end;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int row = row0 + rt * 16 + n;
@@ -184,8 +181,7 @@ __device__ __forceinline__ void attn_span(const AttnParams &p, const AttnCache &
         const int h = hk * p.group + (ok ? row : 0) - t * p.group;
         const QT *src = reinterpret_cast<const QT *>(p.q + (int64_t)(s.tok0 + t) * p.q_token + h * p.q_head);
         const int64_t lim = (int64_t)s.causal + t + 1;
-        limit[rt] = lim < s.end ? (int)lim : s.end;
-        if (!ok) limit[rt] = s.end;
+        w.limit[rt] = ok && lim < s.end ? (int)lim : s.end;
         float x[KK][8];
         float top = 0.0f;
 #pragma unroll
@@ -193,10 +189,11 @@ __device__ __forceinline__ void attn_span(const AttnParams &p, const AttnCache &
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int d = kk * 32 + g * 8 + j;
-                x[kk][j] = ok && d < p.head_dim ? (float)src[d] * sgn : 0.0f;
+                const float y = (float)src[d < p.head_dim ? d : 0] * sgn;  // (loads without branches)
+                x[kk][j] = ok && d < p.head_dim ? y : 0.0f;
                 top = fmaxf(top, fabsf(x[kk][j]));
             }
-        c[rt] = fabsf(p.scale) * kLog2e;
+        w.c[rt] = fabsf(p.scale) * kLog2e;
         float f = 1.0f;
         if (TERMS > 1) {
             // an F32 row of any magnitude: a power of two brings its largest value to 1..2
@@ -204,82 +201,409 @@ __device__ __forceinline__ void attn_span(const AttnParams &p, const AttnCache &
             int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
             e = e < -126 || e > 127 ? 0 : e > 126 ? 126 : e;
             f = __uint_as_float((uint32_t)(127 - e) << 23);
-            c[rt] *= __uint_as_float((uint32_t)(127 + e) << 23);
+            w.c[rt] *= __uint_as_float((uint32_t)(127 + e) << 23);
         }
         // (above zero, so that c * -inf of an unseen position stays -inf at a scale of 0)
-        c[rt] = fmaxf(c[rt], 1e-37f);
+        w.c[rt] = fmaxf(w.c[rt], 1e-37f);
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
+        for (int kk = 0; kk < KK; ++kk) {
+            V8 v[TERMS];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 T t8[TERMS];
                 split_terms<T, TERMS>(x[kk][j] * f, t8);
 #pragma unroll
-                for (int i = 0; i < TERMS; ++i) q[rt][i][kk][j] = t8[i];
+                for (int i = 0; i < TERMS; ++i) v[i][j] = t8[i];
             }
+#pragma unroll
+            for (int i = 0; i < TERMS; ++i) put(rt, i, kk, v[i]);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // one row tile's registers at a time
+        w.m[rt] = -__builtin_inff();
+        w.l[rt] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) w.o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    {
-        // the first row of the workgroup sees the least
-        const int t = (int)fastdiv((uint32_t)(tile0 * C::ROWS), p.group_div);
-        const int64_t lim = (int64_t)s.causal + t + 1;
-        if (lim < lim_min) lim_min = (int)lim;
-    }
+}
 
-    f32x4 o[RT][DT];
-    float m[RT], l[RT];  // m: reference in units of S; l: this lane's part of the sum
+// The page of position t of the span (clamped to its last, so that nothing past a
+// table is read), and the position in it.
+__device__ __forceinline__ int attn_page(const AttnCache &kv, const AttnSpan &s, int t) {
+    const int first = (int)s.table_row * kv.table_len;
+    if (kv.one_page) return first;
+    const int e = (int)fastdiv((uint32_t)(t < s.end ? t : s.end - 1), kv.page);
+    return kv.table ? kv.table[s.table_row * kv.table_stride + e] : first + e;
+}
+__device__ __forceinline__ int attn_slot(const AttnCache &kv, int t) {
+    return kv.one_page ? t : t - (int)(fastdiv((uint32_t)t, kv.page) * kv.page.d);
+}
+
+// The first row of the item, which sees the least, sees positions below this.
+template <int ROWS>
+__device__ __forceinline__ int attn_least(const AttnParams &p, const AttnSpan &s, int tile) {
+    const int64_t lim = (int64_t)s.causal + (int)fastdiv((uint32_t)(tile * ROWS), p.group_div) + 1;
+    return lim < s.end ? (int)lim : s.end;
+}
+
+// 32 positions' scores sx[rt][tile of 16] to probabilities, in place of the next
+// product's B operand.
+template <class T, int D, int RT, int TERMS>
+__device__ __forceinline__ void attn_softmax(AttnRows<RT, D> &w, const f32x4 (&sx)[RT][2],
+                                             typename Vec8<T>::type (&pf)[RT][TERMS]) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -__builtin_inff();
-        l[rt] = 0.0f;
+        float top = sx[rt][0][0];
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, sx[rt][j >> 2][j & 3]);
+        // a new reference when some row passes the old one by 2^kLazy (-inf: always)
+        if (__any((top - w.m[rt]) * w.c[rt] > kLazy || w.m[rt] == -__builtin_inff())) {
+            const float mn = fmaxf(w.m[rt], xor_max(top));
+            // (nothing was summed yet, or nothing changes: also keeps inf - inf and 0 * inf out)
+            const float f = w.m[rt] == -__builtin_inff() || w.m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f((w.m[rt] - mn) * w.c[rt]);
+            w.m[rt] = mn;
+            w.l[rt] *= f;
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) w.o[rt][dt] *= f;
+        }
+        const float ref = w.m[rt] == -__builtin_inff() ? kBias : kBias - w.m[rt] * w.c[rt];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sx[rt][j >> 2][j & 3], w.c[rt], ref));
+            w.l[rt] += x;
+            T t8[TERMS];
+            split_terms<T, TERMS>(x, t8);
+#pragma unroll
+            for (int i = 0; i < TERMS; ++i) pf[rt][i][j] = t8[i];
+        }
     }
+}
 
-    // ---- staging: thread -> chunk tid % CH of positions tid / CH + RP * i ----
-    const int sc = tid % CH, sr = tid / CH;
-    const bool cok = sc * 8 < p.head_dim;
-    const char *kb = kv.k + hk * kv.k_head + sc * 16, *vb = kv.v + hk * kv.v_head + sc * 16;
-    u32x4 kr[NP], vr[NP];
-    int page[NP];   // of the tile that is loaded next; -1: not seen
+// O^T += V^T P^T over 32 positions of V in LDS from row b of ldv (swizzled rows of
+// D values).
+template <class T, int D, int RT, int TERMS>
+__device__ __forceinline__ void attn_values(AttnRows<RT, D> &w, const typename Vec8<T>::type (&pf)[RT][TERMS], const char *ldv, int b) {
+    using V8 = typename Vec8<T>::type;
+    constexpr int CH = D / 8;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int tr = b + g * 4 + (n >> 2);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+        union {
+            s16x4 h[2];
+            V8 v;
+        } va;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+            const int t = tr + tt * 16;
+            va.h[tt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4 *)(ldv + (t * CH + swz_v<D>(t, dt * 2 + ((n & 3) >> 1))) * 16 + (n & 1) * 8));
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int i = 0; i < TERMS; ++i) w.o[rt][dt] = mfma(va.v, pf[rt][i], w.o[rt][dt]);
+    }
+}
+
+// Where rows see different positions, a value of inf or NaN must not reach, as
+// 0 * inf, the rows that do not see it.  There (from the first step that ends past
+// `least`) such values are zeros in the products, attn_finite() says whether there
+// were any, and attn_rest() adds them in the end to the rows that see them: with a
+// probability above zero the sum is inf or NaN whatever the probability is.
+template <class T>
+__device__ __forceinline__ bool attn_finite(u32x4 &v) {
+    constexpr uint32_t e = sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = (v[i] & e) == e ? 0xffffu : 0u, hi = (v[i] >> 16 & e) == e ? 0xffff0000u : 0u;
+        fine = fine && (lo | hi) == 0;
+        v[i] &= ~(lo | hi);
+    }
+    return fine;
+}
+template <class T, int RT, int D>
+__device__ __forceinline__ void attn_rest(const AttnParams &p, const AttnCache &kv, const AttnSpan &s, int hk, AttnRows<RT, D> &w,
+                                          int beg, int end) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll 1
+    for (int t = beg; t < end; ++t) {
+        const int page = attn_page(kv, s, t);
+        if ((uint32_t)page >= (uint32_t)kv.n_pages) continue;
+        const T *v = reinterpret_cast<const T *>(kv.v + hk * kv.v_head + page * kv.v_page + attn_slot(kv, t) * kv.v_token);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+            const int d = dt * 16 + g * 4;
+            if (d >= p.head_dim) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float y = (float)v[d + j];
+                if (__builtin_isfinite(y)) continue;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    if (t < w.limit[rt]) w.o[rt][dt][j] += y;
+            }
+        }
+    }
+}
+
+// A row's reference in log2 units: its terms are exp2(log2(e) scale s - M).
+__device__ __forceinline__ float attn_ref(float m, float c) { return m == -__builtin_inff() ? m : m * c - kBias; }
+
+// Four dimensions of a row's result: to the partial results, or finished to dst
+template <class QT>
+__device__ __forceinline__ void attn_emit(const AttnParams &p, const AttnSpan &s, int hk, int row, int d, f32x4 x, float M, float sum) {
+    if (row >= s.rows || d >= p.head_dim) return;
+    const int t = (int)fastdiv((uint32_t)row, p.group_div);
+    const int h = hk * p.group + row - t * p.group;
+    const int64_t out = (int64_t)(s.tok0 + t) * p.n_head + h;
+    if (p.slots > 1) {
+        const int64_t at = (int64_t)s.slot * p.n_tokens * p.n_head + out;
+        if (d == 0) p.part_ml[at] = make_float2(M, sum);
+        *reinterpret_cast<f32x4 *>(p.part_o + at * p.head_dim + d) = x;
+        return;
+    }
+    if (d == 0 && p.lse) p.lse[out] = sum == 0.0f ? -__builtin_inff() : (M + log2f(sum)) * kLn2;
+    QT *dst = reinterpret_cast<QT *>(p.dst + (int64_t)(s.tok0 + t) * p.dst_token + h * p.dst_head) + d;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dst[j] = (QT)(sum == 0.0f ? 0.0f : x[j] / sum);
+}
+
+// ---- few rows: every wave takes all of them over positions of its own ----
+// K goes from memory to the registers it is multiplied from (a lane of the A
+// operand holds eight dimensions of one position), V through 32 rows of LDS that
+// belong to the wave, so waves never wait for each other before the end.  Memory
+// bound: each wave keeps the next 32 positions' K and V on their way.
+template <class T, int D_, int RT_, int TERMS>
+struct StreamCfg {
+    using Elem = T;
+    static constexpr int D = D_, RT = RT_, ROWS = 16 * RT_;
+    static constexpr bool QLDS = D_ / 32 * RT_ * TERMS > 8;  // queries in LDS: over 32 registers of them
+    static constexpr int VBYTES = 4 * 32 * D * 2;             // also one tile's outputs of two waves at the end
+    static constexpr int QBYTES = QLDS ? RT * TERMS * (D / 32) * 1024 : 0;
+    static constexpr int LDS = VBYTES * 2 > 64 * D * 4 ? VBYTES + QBYTES : 64 * D * 4 + QBYTES;
+};
+
+template <class C, class QT, int TERMS>
+__device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache &kv, const AttnSpan &s, int hk, int tile,
+                                            char *lds, int *flags) {
+    using T = typename C::Elem;
+    using V8 = typename Vec8<T>::type;
+    constexpr int D = C::D, RT = C::RT, KK = D / 32, CH = D / 8;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int row0 = tile * C::ROWS;
+    char *ldv = lds + wave * 32 * D * 2;
+    char *ldq = lds + C::LDS - C::QBYTES;
+    AttnRows<RT, D> w;
+    V8 q[C::QLDS ? 1 : RT][TERMS][KK];
+    attn_queries<T, D, RT, QT, TERMS>(p, s, hk, row0, w, [&](int rt, int i, int kk, V8 v) {
+        if (!C::QLDS) {
+            q[C::QLDS ? 0 : rt][i][kk] = v;
+        } else {
+            const int f = (rt * TERMS + i) * KK + kk;
+            if ((f & 3) == wave) *reinterpret_cast<V8 *>(ldq + f * 1024 + lane * 16) = v;
+        }
+    });
+    if (C::QLDS) __syncthreads();
+    const int least = attn_least<C::ROWS>(p, s, tile);
+
+    // lane (n, g): positions n and 16 + n of a step, chunks g, 4 + g, ... of K and V
+    u32x4 kf[2][KK], vf[2][KK];
+    uint32_t there = 0;  // bit 16 * tile + n: the position has a page
+    int page[2];
+    const char *kb = kv.k + hk * kv.k_head + g * 16, *vb = kv.v + hk * kv.v_head + g * 16;
+    const bool full = p.head_dim == D;
     auto get_pages = [&](int t0) {
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int t = t0 + sr + RP * i;
-            page[i] = -1;
-            if (t < s.end) {
-                if (kv.one_page) {
-                    page[i] = (int)s.table_row * kv.table_len;
-                } else {
-                    const int e = (int)fastdiv((uint32_t)t, kv.page);
-                    page[i] = kv.table ? kv.table[s.table_row * kv.table_stride + e] : (int)s.table_row * kv.table_len + e;
-                }
-            }
-        }
+        for (int tt = 0; tt < 2; ++tt) page[tt] = attn_page(kv, s, t0 + tt * 16 + n);
     };
     auto load = [&](int t0) {
+        uint32_t all = 0;
+        const char *ks[2], *vs[2];
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            kr[i] = u32x4{0, 0, 0, 0};
-            vr[i] = u32x4{0, 0, 0, 0};
-            const int t = t0 + sr + RP * i;
-            if ((uint32_t)page[i] < (uint32_t)kv.n_pages && cok) {
-                const int slot = kv.one_page ? t : t - (int)(fastdiv((uint32_t)t, kv.page) * kv.page.d);
-                kr[i] = *reinterpret_cast<const u32x4 *>(kb + page[i] * kv.k_page + slot * kv.k_token);
-                vr[i] = *reinterpret_cast<const u32x4 *>(vb + page[i] * kv.v_page + slot * kv.v_token);
-            }
+        for (int tt = 0; tt < 2; ++tt) {
+            const int t = t0 + tt * 16 + n;
+            const bool ok = t < s.end && (uint32_t)page[tt] < (uint32_t)kv.n_pages;
+            all |= ((uint32_t)__ballot(ok) & 0xffffu) << (16 * tt);
+            const int pg = ok ? page[tt] : 0, slot = ok ? attn_slot(kv, t) : 0;
+            ks[tt] = kb + pg * kv.k_page + slot * kv.k_token;
+            vs[tt] = vb + pg * kv.v_page + slot * kv.v_token;
+        }
+        there = all;
+        if (full) {
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    kf[tt][kk] = *reinterpret_cast<const u32x4 *>(ks[tt] + kk * 64);
+                    vf[tt][kk] = *reinterpret_cast<const u32x4 *>(vs[tt] + kk * 64);
+                }
+        } else {
+            // past the head: chunk 0 again, which the queries' zeros meet as zeros and
+            // whose values are not stored
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) {
+                    const bool in = kk * 32 + g * 8 < p.head_dim;
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(ks[tt] + (in ? kk * 64 : -g * 16));
+                    kf[tt][kk] = in ? x : u32x4{0, 0, 0, 0};
+                    vf[tt][kk] = *reinterpret_cast<const u32x4 *>(vs[tt] + (in ? kk * 64 : -g * 16));
+                }
         }
     };
-    uint32_t okbits = 0;  // which of this thread's positions have a page
-    auto get_okbits = [&]() {
+    int t0 = s.beg + wave * 32;
+    if (t0 < s.end) {
+        get_pages(t0);
+        load(t0);
+        get_pages(t0 + 128);
+    }
+    bool fine = true;  // of the values at and after the first step that ends past `least`
+    for (; t0 < s.end; t0 += 128) {
+        const uint32_t ok = there;
+        const bool careful = least < s.end && t0 + 32 > least;
+        if (careful) {
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) fine = attn_finite<T>(vf[tt][kk]) && fine;
+        }
+        if (ok != 0xffffffffu) {
+            // positions that are not there: values of zero, whatever was read
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+                if (!((ok >> (16 * tt + n)) & 1))
+#pragma unroll
+                    for (int kk = 0; kk < KK; ++kk) vf[tt][kk] = u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                const int t = tt * 16 + n;
+                *reinterpret_cast<u32x4 *>(ldv + (t * CH + swz_v<D>(t, kk * 4 + g)) * 16) = vf[tt][kk];
+            }
+        f32x4 sx[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sx[rt][0] = sx[rt][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int i = 0; i < TERMS; ++i) {
+                    const V8 qv = C::QLDS ? *reinterpret_cast<const V8 *>(ldq + ((rt * TERMS + i) * KK + kk) * 1024 + lane * 16)
+                                          : q[C::QLDS ? 0 : rt][i][kk];
+#pragma unroll
+                    for (int tt = 0; tt < 2; ++tt) sx[rt][tt] = mfma(__builtin_bit_cast(V8, kf[tt][kk]), qv, sx[rt][tt]);
+                }
+        if (t0 + 128 < s.end) {
+            load(t0 + 128);
+            get_pages(t0 + 256);
+        }
+        if (careful || ok != 0xffffffffu) {
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int u = tt * 16 + g * 4 + j;
+                        if (!((ok >> u) & 1) || t0 + u >= w.limit[rt]) sx[rt][tt][j] = -__builtin_inff();
+                    }
+        }
+        V8 pf[RT][TERMS];
+        attn_softmax<T, D, RT, TERMS>(w, sx, pf);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // V's rows are written before lanes read each other's
+        attn_values<T, D, RT, TERMS>(w, pf, ldv, 0);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    if (!__all(fine))
+        for (t0 = s.beg + wave * 32; t0 < s.end; t0 += 128)
+            if (t0 + 32 > least) attn_rest<T>(p, kv, s, hk, w, t0, t0 + 32 < s.end ? t0 + 32 : s.end);
+
+    // the four waves' parts of each row tile join in LDS
+    float *ol = reinterpret_cast<float *>(lds);        // [wave][16][D]
+    float2 *ml = reinterpret_cast<float2 *>(flags);    // [wave][16]
+    constexpr int Q4 = D / 4;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float sum = xor_sum(w.l[rt]);
+        __syncthreads();
+        if (g == 0) ml[wave * 16 + n] = make_float2(attn_ref(w.m[rt], w.c[rt]), sum);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt)
+            *reinterpret_cast<f32x4 *>(ol + (wave * 16 + n) * D + (((dt * 4 + g) ^ n) * 4)) = w.o[rt][dt];
+        __syncthreads();
+        for (int x = tid; x < 16 * Q4; x += 256) {
+            const int r = x / Q4, d4 = x % Q4;
+            float M = -__builtin_inff();
+#pragma unroll
+            for (int v = 0; v < 4; ++v) M = fmaxf(M, ml[v * 16 + r].x);
+            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            float ls = 0.0f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float2 e = ml[v * 16 + r];
+                if (e.y == 0.0f) continue;  // the row sees nothing of this wave's part
+                const float f = __builtin_amdgcn_exp2f(e.x == M ? 0.0f : e.x - M);
+                ls += e.y * f;
+                acc += *reinterpret_cast<const f32x4 *>(ol + (v * 16 + r) * D + ((d4 ^ r) * 4)) * f;
+            }
+            attn_emit<QT>(p, s, hk, row0 + rt * 16 + r, d4 * 4, acc, M, ls);
+        }
+    }
+}
+
+// ---- many rows: the waves take rows of their own and share K and V in LDS ----
+template <class C, class QT, int TERMS>
+__device__ __forceinline__ void attn_shared(const AttnParams &p, const AttnCache &kv, const AttnSpan &s, int hk, int tile,
+                                            char *lds, int *flags) {
+    using T = typename C::Elem;
+    using V8 = typename Vec8<T>::type;
+    constexpr int D = C::D, RT = C::RT, CH = C::CH, RP = C::RP, TB = C::TB, NP = C::NP;
+    constexpr int KK = D / 32;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const char *ldk = lds;
+    const char *ldv = lds + TB * D * 2;
+    uint8_t *seen = reinterpret_cast<uint8_t *>(flags + 4);  // one byte per position of the tile
+    AttnRows<RT, D> w;
+    V8 q[RT][TERMS][KK];
+    const int row0 = tile * C::ROWS + wave * RT * 16;
+    attn_queries<T, D, RT, QT, TERMS>(p, s, hk, row0, w, [&](int rt, int i, int kk, V8 v) { q[rt][i][kk] = v; });
+    const int least = attn_least<C::ROWS>(p, s, tile);
+
+    // staging: thread -> chunk tid % CH of positions tid / CH + RP * i
+    const int sc = tid % CH, sr = tid / CH;
+    const bool cok = sc * 8 < p.head_dim;
+    const char *kb = kv.k + hk * kv.k_head + (cok ? sc * 16 : 0), *vb = kv.v + hk * kv.v_head + (cok ? sc * 16 : 0);
+    u32x4 kr[NP], vr[NP];
+    int page[NP];        // of the tile that is loaded next
+    uint32_t okbits = 0; // which of this thread's positions have a page
+    auto get_pages = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) page[i] = attn_page(kv, s, t0 + sr + RP * i);
+    };
+    auto load = [&](int t0) {
         okbits = 0;
 #pragma unroll
-        for (int i = 0; i < NP; ++i) okbits |= (uint32_t)((uint32_t)page[i] < (uint32_t)kv.n_pages) << i;
+        for (int i = 0; i < NP; ++i) {
+            const int t = t0 + sr + RP * i;
+            const bool ok = t < s.end && (uint32_t)page[i] < (uint32_t)kv.n_pages;
+            const int pg = ok ? page[i] : 0, slot = ok ? attn_slot(kv, t) : 0;
+            kr[i] = *reinterpret_cast<const u32x4 *>(kb + pg * kv.k_page + slot * kv.k_token);
+            vr[i] = *reinterpret_cast<const u32x4 *>(vb + pg * kv.v_page + slot * kv.v_token);
+            okbits |= (uint32_t)ok << i;
+        }
     };
-    get_pages(s.beg);
-    load(s.beg);
-    get_okbits();
-    get_pages(s.beg + TB);
-    if (tid == 0) flags[0] = 0;
+    if (s.beg < s.end) {
+        get_pages(s.beg);
+        load(s.beg);
+        get_pages(s.beg + TB);
+    }
+    if (tid == 0) flags[0] = flags[2] = 0;
 
     int par = 0;
     for (int t0 = s.beg; t0 < s.end; t0 += TB, par ^= 1) {
@@ -287,9 +611,13 @@ __device__ __forceinline__ void attn_span(const AttnParams &p, const AttnCache &
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             const int t = sr + RP * i;
-            *reinterpret_cast<u32x4 *>(lds + (t * CH + swz_k<D>(t, sc)) * 16) = kr[i];
-            *reinterpret_cast<u32x4 *>(lds + TB * D * 2 + (t * CH + swz_v<D>(t, sc)) * 16) = vr[i];
-            if (sc == 0) seen[t] = (okbits >> i) & 1;
+            const bool ok = (okbits >> i) & 1;
+            if (least < s.end && t0 + TB > least && ok && !attn_finite<T>(vr[i])) flags[2] = 1;  // (stays for the end)
+            const u32x4 zero = {0, 0, 0, 0};
+            // (past the head: zeros for the queries' zeros; a position that is not there: values of zero)
+            *reinterpret_cast<u32x4 *>(lds + (t * CH + swz_k<D>(t, sc)) * 16) = cok ? kr[i] : zero;
+            *reinterpret_cast<u32x4 *>(lds + TB * D * 2 + (t * CH + swz_v<D>(t, sc)) * 16) = ok ? vr[i] : zero;
+            if (sc == 0) seen[t] = ok;
         }
         // flags[par]: some position of this tile is not seen.  The other word, read
         // before the barrier above, is cleared for the next tile.
@@ -298,15 +626,13 @@ __device__ __forceinline__ void attn_span(const AttnParams &p, const AttnCache &
         const int tn = t0 + TB;
         if (tn < s.end) {
             load(tn);
-            get_okbits();
             get_pages(tn + TB);
         }
         __syncthreads();
-        const bool masked = flags[par] != 0 || t0 + TB > lim_min;
+        const bool masked = flags[par] != 0 || t0 + TB > least;
 
 #pragma unroll 1
-        for (int st = wt; st < TB / 32; st += WT) {
-            const int b = st * 32;
+        for (int b = 0; b < TB; b += 32) {
             if (t0 + b >= s.end) break;
             f32x4 sx[RT][2];
 #pragma unroll
@@ -332,173 +658,37 @@ __device__ __forceinline__ void attn_span(const AttnParams &p, const AttnCache &
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            if (!((ok4 >> (8 * j)) & 1) || t0 + t + j >= limit[rt]) sx[rt][tt][j] = -__builtin_inff();
+                            if (!((ok4 >> (8 * j)) & 1) || t0 + t + j >= w.limit[rt]) sx[rt][tt][j] = -__builtin_inff();
                 }
             }
             V8 pf[RT][TERMS];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                float top = sx[rt][0][0];
-#pragma unroll
-                for (int j = 1; j < 8; ++j) top = fmaxf(top, sx[rt][j >> 2][j & 3]);
-                // a new reference when some row passes the old one by 2^kLazy (-inf: always)
-                if (__any((top - m[rt]) * c[rt] > kLazy || m[rt] == -__builtin_inff())) {
-                    const float mn = fmaxf(m[rt], xor_max(top));
-                    // (nothing was summed yet, or nothing changes: also keeps inf - inf and 0 * inf out)
-                    const float f = m[rt] == -__builtin_inff() || m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f((m[rt] - mn) * c[rt]);
-                    m[rt] = mn;
-                    l[rt] *= f;
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= f;
-                }
-                const float ref = m[rt] == -__builtin_inff() ? kBias : kBias - m[rt] * c[rt];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sx[rt][j >> 2][j & 3], c[rt], ref));
-                    l[rt] += x;
-                    T t8[TERMS];
-                    split_terms<T, TERMS>(x, t8);
-#pragma unroll
-                    for (int i = 0; i < TERMS; ++i) pf[rt][i][j] = t8[i];
-                }
-            }
-            const int tr = b + g * 4 + (n >> 2);
-            auto load_v = [&](int dt) {
-                union {
-                    s16x4 h[2];
-                    V8 v;
-                } va;
-#pragma unroll
-                for (int tt = 0; tt < 2; ++tt) {
-                    const int t = tr + tt * 16;
-                    va.h[tt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s16x4 *)(ldv + (t * CH + swz_v<D>(t, dt * 2 + ((n & 3) >> 1))) * 16 +
-                                                                    (n & 1) * 8));
-                }
-                return va.v;
-            };
-            // Where rows see different positions, a value of inf or NaN must not
-            // reach (as 0 * inf) the rows that do not see it.
-            bool odd = false;
-            if (t0 + b + 32 > lim_min) {
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    const V8 va = load_v(dt);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) odd |= !__builtin_isfinite((float)va[j]);
-                }
-            }
-            if (__any(odd)) {
-                // the finite values for all rows, then the others one position at a
-                // time, kept only by the rows that see it
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    V8 va = load_v(dt);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) va[j] = __builtin_isfinite((float)va[j]) ? va[j] : (T)0.0f;
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int i = 0; i < TERMS; ++i) o[rt][dt] = mfma(va, pf[rt][i], o[rt][dt]);
-                }
-#pragma unroll 1
-                for (int u = 0; u < 32; ++u) {
-                    const bool mine = g == ((u & 15) >> 2);
-                    const int ju = (u >> 4) * 4 + (u & 3);
-                    const bool there = seen[b + u] != 0;
-#pragma unroll
-                    for (int dt = 0; dt < DT; ++dt) {
-                        V8 va = load_v(dt);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            va[j] = mine && j == ju && !__builtin_isfinite((float)va[j]) ? va[j] : (T)0.0f;
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) {
-                            f32x4 x = o[rt][dt];
-#pragma unroll
-                            for (int i = 0; i < TERMS; ++i) {
-                                V8 pu = pf[rt][i];
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) pu[j] = mine && j == ju ? pu[j] : (T)0.0f;
-                                x = mfma(va, pu, x);
-                            }
-                            if (there && t0 + b + u < limit[rt]) o[rt][dt] = x;
-                        }
-                    }
-                }
-                continue;
-            }
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const V8 va = load_v(dt);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int i = 0; i < TERMS; ++i) o[rt][dt] = mfma(va, pf[rt][i], o[rt][dt]);
-            }
+            attn_softmax<T, D, RT, TERMS>(w, sx, pf);
+            attn_values<T, D, RT, TERMS>(w, pf, ldv, b);
         }
-    }
-
-    // ---- the row's sum over its four lane groups; waves over positions join in LDS ----
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) l[rt] = xor_sum(l[rt]);
-    // M in log2 units: the row's terms are exp2(log2(e) scale s - M)
-    auto emit = [&](int row, int d, f32x4 x, float M, float sum) {
-        if (row >= s.rows || d >= p.head_dim) return;
-        const int t = (int)fastdiv((uint32_t)row, p.group_div);
-        const int h = hk * p.group + row - t * p.group;
-        const int64_t out = (int64_t)(s.tok0 + t) * p.n_head + h;
-        if (p.slots > 1) {
-            const int64_t at = (int64_t)s.slot * p.n_tokens * p.n_head + out;
-            if (d == 0) p.part_ml[at] = make_float2(M, sum);
-            *reinterpret_cast<f32x4 *>(p.part_o + at * p.head_dim + d) = x;
-            return;
-        }
-        if (d == 0 && p.lse) p.lse[out] = sum == 0.0f ? -__builtin_inff() : (M + log2f(sum)) * kLn2;
-        QT *dst = reinterpret_cast<QT *>(p.dst + (int64_t)(s.tok0 + t) * p.dst_token + h * p.dst_head) + d;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dst[j] = (QT)(sum == 0.0f ? 0.0f : x[j] / sum);
-    };
-    if (WT == 1) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const float M = m[rt] == -__builtin_inff() ? m[rt] : m[rt] * c[rt] - kBias;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) emit(row0 + rt * 16 + n, dt * 16 + g * 4, o[rt][dt], M, l[rt]);
-        }
-        return;
     }
     __syncthreads();
-    float *ol = reinterpret_cast<float *>(lds);                 // [wave][RT * 16][D]
-    float2 *ml = reinterpret_cast<float2 *>(flags + 4);         // [wave][RT * 16]
+    if (flags[2] != 0) {
+        int t = s.beg;
+        while (t + TB <= least) t += TB;
+        attn_rest<T>(p, kv, s, hk, w, t, s.end);
+    }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int r = wave * RT * 16 + rt * 16 + n;
-        if (g == 0) ml[r] = make_float2(m[rt] == -__builtin_inff() ? m[rt] : m[rt] * c[rt] - kBias, l[rt]);
+        const float sum = xor_sum(w.l[rt]), M = attn_ref(w.m[rt], w.c[rt]);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-            *reinterpret_cast<f32x4 *>(ol + r * D + (((dt * 4 + g) ^ n) * 4)) = o[rt][dt];
+        for (int dt = 0; dt < D / 16; ++dt) attn_emit<QT>(p, s, hk, row0 + rt * 16 + n, dt * 16 + g * 4, w.o[rt][dt], M, sum);
     }
-    __syncthreads();
-    constexpr int Q4 = D / 4;
-    for (int x = tid; x < C::ROWS * Q4; x += 256) {
-        const int r = x / Q4, d4 = x % Q4;
-        const int w0 = r / (RT * 16) * WT, rr = r % (RT * 16);
-        float M = -__builtin_inff();
-#pragma unroll
-        for (int w = 0; w < WT; ++w) M = fmaxf(M, ml[(w0 + w) * RT * 16 + rr].x);
-        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        float ls = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WT; ++w) {
-            const float2 e = ml[(w0 + w) * RT * 16 + rr];
-            if (e.y == 0.0f) continue;  // no position of the row in this wave's part
-            const float f = __builtin_amdgcn_exp2f(e.x == M ? 0.0f : e.x - M);
-            ls += e.y * f;
-            sum += *reinterpret_cast<const f32x4 *>(ol + ((w0 + w) * RT * 16 + rr) * D + ((d4 ^ (rr & 15)) * 4)) * f;
-        }
-        emit(tile0 * C::ROWS + r, d4 * 4, sum, M, ls);
-    }
+}
+
+template <class T, int D, int RT, int TERMS, class QT>
+__device__ __forceinline__ void attn_item(StreamCfg<T, D, RT, TERMS>, const AttnParams &p, const AttnCache &kv, const AttnSpan &s,
+                                          int hk, int tile, char *lds, int *flags, QT) {
+    attn_stream<StreamCfg<T, D, RT, TERMS>, QT, TERMS>(p, kv, s, hk, tile, lds, flags);
+}
+template <class T, int D, int RT, int TERMS, class QT>
+__device__ __forceinline__ void attn_item(SharedCfg<T, D, RT, TERMS>, const AttnParams &p, const AttnCache &kv, const AttnSpan &s,
+                                          int hk, int tile, char *lds, int *flags, QT) {
+    attn_shared<SharedCfg<T, D, RT, TERMS>, QT, TERMS>(p, kv, s, hk, tile, lds, flags);
 }
 
 // Consecutive items to one XCD (workgroups go to the 8 XCDs in turn), so that the
@@ -508,9 +698,11 @@ __device__ __forceinline__ int xcd_item(int b, int total) {
     return x * per + (x < more ? x : more) + b / 8;
 }
 
-// CP: rows and waves of the prefix's items, CS of the suffixes'.
+constexpr int kAttnFlags = 1024;  // bytes after the tiles: flags, or (M, l) of four waves' rows
+
+// CP: how the prefix's rows are taken, CS the suffixes'.
 template <class CP, class CS, class QT, int TERMS>
-__global__ __launch_bounds__(256) void prefix_attn_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, CP::D == 256 ? 1 : 2) void prefix_attn_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int buf = CP::LDS > CS::LDS ? CP::LDS : CS::LDS;
     int *flags = reinterpret_cast<int *>(lds + buf);
@@ -526,7 +718,7 @@ __global__ __launch_bounds__(256) void prefix_attn_kernel(AttnParams p) {
         s.causal = p.n_prefix;
         s.table_row = 0;
         s.slot = sp;
-        attn_span<CP, QT, TERMS>(p, p.pre, s, hk, tile, lds, flags);
+        attn_item(CP(), p, p.pre, s, hk, tile, lds, flags, QT());
         return;
     }
     const int item = xcd_item(blockIdx.x - p.pre_items, p.suf_items);
@@ -548,7 +740,7 @@ __global__ __launch_bounds__(256) void prefix_attn_kernel(AttnParams p) {
     s.table_row = r;
     s.slot = p.pre_splits + sp;
     if (tile * CS::ROWS >= s.rows) return;
-    attn_span<CS, QT, TERMS>(p, p.suf, s, hk, tile, lds, flags);
+    attn_item(CS(), p, p.suf, s, hk, tile, lds, flags, QT());
 }
 
 // Joins a row's partial results: one workgroup of 256 per row, groups of
@@ -601,6 +793,58 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(AttnParams p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) dst[j] = (QT)(l == 0.0f ? 0.0f : o[j] / l);
     if (threadIdx.x == 0 && p.lse) p.lse[row] = l == 0.0f ? -__builtin_inff() : (M + log2f(l)) * kLn2;
+}
+
+// ---- which kernel runs a call ----
+struct AttnPlan {
+    int dim, pre_size, suf_size;  // padded head dimension, shapes
+    AttnParams p;
+    size_t bytes;
+    int lds;
+    const void *kernel;
+};
+
+// (an instantiation of attn_kernel_of per pair of types, each in a file of its own)
+void attn_kernel_f16(AttnPlan &pl);
+void attn_kernel_f16_f32(AttnPlan &pl);
+void attn_kernel_bf16(AttnPlan &pl);
+void attn_kernel_bf16_f32(AttnPlan &pl);
+
+// How rows are taken: 0 and 1 streaming 16 and 32 rows, 2 sharing K and V
+// among four waves of RT tiles of 16 rows.
+template <class T, int D, int TERMS, int SIZE>
+struct AttnShape {
+    using cfg = StreamCfg<T, D, SIZE == 1 && D < 256 ? 2 : 1, TERMS>;
+};
+template <class T, int D, int TERMS>
+struct AttnShape<T, D, TERMS, 2> {
+    using cfg = SharedCfg<T, D, D < 256 ? 2 : 1, TERMS>;
+};
+
+
+template <class T, class QT, int TERMS, int D, int PS, int SS>
+void attn_kernel(AttnPlan &pl) {
+    using CP = typename AttnShape<T, D, TERMS, PS>::cfg;
+    using CS = typename AttnShape<T, D, TERMS, SS>::cfg;
+    pl.kernel = reinterpret_cast<const void *>(&prefix_attn_kernel<CP, CS, QT, TERMS>);
+    pl.lds = (CP::LDS > CS::LDS ? CP::LDS : CS::LDS) + kAttnFlags;
+}
+template <class T, class QT, int TERMS, int D>
+void attn_kernel_of(AttnPlan &pl) {
+    switch (pl.pre_size * 4 + pl.suf_size) {
+        case 0: return attn_kernel<T, QT, TERMS, D, 0, 0>(pl);
+        case 4: return attn_kernel<T, QT, TERMS, D, 1, 0>(pl);
+        case 5: return attn_kernel<T, QT, TERMS, D, 1, 1>(pl);
+        case 8: return attn_kernel<T, QT, TERMS, D, 2, 0>(pl);
+        case 9: return attn_kernel<T, QT, TERMS, D, 2, 1>(pl);
+        default: return attn_kernel<T, QT, TERMS, D, 2, 2>(pl);
+    }
+}
+template <class T, class QT, int TERMS>
+void attn_kernel_of(AttnPlan &pl) {
+    if (pl.dim == 64) attn_kernel_of<T, QT, TERMS, 64>(pl);
+    else if (pl.dim == 128) attn_kernel_of<T, QT, TERMS, 128>(pl);
+    else attn_kernel_of<T, QT, TERMS, 256>(pl);
 }
 
 }  // namespace q4k

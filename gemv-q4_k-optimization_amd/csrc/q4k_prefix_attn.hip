@@ -52,54 +52,6 @@ static int attn_check(const q4k_prefix_attn_args *args, bool &empty) {
 }
 
 
-// Workgroups' shapes: row tiles of 16 per wave, waves over rows.  Rows of 256
-// dimensions leave LDS for tiles of 64 positions only, two waves' worth.
-template <class T, int D, int SIZE>
-struct AttnShape;
-template <class T, int D>
-struct AttnShape<T, D, 0> {
-    using cfg = AttnCfg<T, D, 1, D == 256 ? 2 : 1>;
-};
-template <class T, int D>
-struct AttnShape<T, D, 1> {
-    using cfg = AttnCfg<T, D, 1, 4>;
-};
-template <class T, int D>
-struct AttnShape<T, D, 2> {
-    using cfg = AttnCfg<T, D, D == 256 ? 1 : 2, 4>;
-};
-
-struct AttnPlan {
-    int dim, pre_size, suf_size;  // padded head dimension, shapes
-    AttnParams p;
-    size_t bytes;
-    int lds;
-    const void *kernel;
-};
-
-template <class T, class QT, int TERMS, int D, int PS, int SS>
-void attn_kernel(AttnPlan &pl) {
-    using CP = typename AttnShape<T, D, PS>::cfg;
-    using CS = typename AttnShape<T, D, SS>::cfg;
-    pl.kernel = reinterpret_cast<const void *>(&prefix_attn_kernel<CP, CS, QT, TERMS>);
-    pl.lds = (CP::LDS > CS::LDS ? CP::LDS : CS::LDS) + 16 + 1024;
-}
-template <class T, class QT, int TERMS, int D>
-void attn_kernel_of(AttnPlan &pl) {
-    switch (pl.pre_size * 4 + pl.suf_size) {
-        case 0: return attn_kernel<T, QT, TERMS, D, 0, 0>(pl);
-        case 4: return attn_kernel<T, QT, TERMS, D, 1, 0>(pl);
-        case 8: return attn_kernel<T, QT, TERMS, D, 2, 0>(pl);
-        default: return attn_kernel<T, QT, TERMS, D, 2, 2>(pl);
-    }
-}
-template <class T, class QT, int TERMS>
-void attn_kernel_of(AttnPlan &pl) {
-    if (pl.dim == 64) attn_kernel_of<T, QT, TERMS, 64>(pl);
-    else if (pl.dim == 128) attn_kernel_of<T, QT, TERMS, 128>(pl);
-    else attn_kernel_of<T, QT, TERMS, 256>(pl);
-}
-
 static AttnCache attn_cache(const q4k_kv_pages &c, int64_t tokens) {
     AttnCache k{};
     k.k = (const char *)c.k;
@@ -136,10 +88,11 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
     pl.dim = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
     if (a.n_tokens > INT32_MAX / p.group - 256) return Q4K_EUNSUPPORTED;
     const int64_t pre_rows = a.n_prefix > 0 ? a.n_tokens * p.group : 0, suf_rows = a.n_q * p.group;
-    const int rows_of[3] = {pl.dim == 256 ? 32 : 16, 64, pl.dim == 256 ? 64 : 128};
-    auto size_of = [&](int64_t rows) { return rows <= 16 ? 0 : rows <= 64 ? 1 : 2; };
-    pl.suf_size = suf_rows <= 64 ? 0 : 2;
-    pl.pre_size = pl.suf_size == 2 ? 2 : size_of(pre_rows);
+    const int rows_of[3] = {16, pl.dim == 256 ? 16 : 32, pl.dim == 256 ? 64 : 128};
+    auto size_of = [&](int64_t rows) { return rows <= 16 ? 0 : rows <= 96 ? 1 : 2; };
+    pl.suf_size = size_of(suf_rows);
+    pl.pre_size = a.n_prefix > 0 ? size_of(pre_rows) : pl.suf_size;
+    if (pl.suf_size > pl.pre_size) pl.suf_size = pl.pre_size;  // (with q_start n_q may exceed the tokens there are)
     const int pr = rows_of[pl.pre_size], sr = rows_of[pl.suf_size];
     // splits: about two workgroups per CU, in whole tiles of 128 positions
     const int64_t target = 2 * (int64_t)cus;
@@ -174,8 +127,8 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
     }
     if (a.n_requests * a.n_q > INT32_MAX / a.n_head) return Q4K_EUNSUPPORTED;
     const bool f32 = a.q_type == Q4K_GGML_TYPE_F32;
-    if (a.kv_type == Q4K_GGML_TYPE_F16) f32 ? attn_kernel_of<_Float16, float, 2>(pl) : attn_kernel_of<_Float16, _Float16, 1>(pl);
-    else f32 ? attn_kernel_of<__bf16, float, 3>(pl) : attn_kernel_of<__bf16, __bf16, 1>(pl);
+    if (a.kv_type == Q4K_GGML_TYPE_F16) f32 ? attn_kernel_f16_f32(pl) : attn_kernel_f16(pl);
+    else f32 ? attn_kernel_bf16_f32(pl) : attn_kernel_bf16(pl);
     return Q4K_OK;
 }
 
