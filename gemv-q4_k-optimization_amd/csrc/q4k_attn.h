@@ -66,6 +66,7 @@ struct AttnParams {
     int n_head, n_head_kv, group, head_dim;
     FastDiv group_div;
     float scale;
+    int q_vec;  // rows of q in 16-byte loads
     // prefix items: split, KV head, row tile (fastest); then the suffixes' items:
     // split, request, KV head, row tile
     int pre_items, pre_tiles, pre_splits, pre_len;  // pre_len, suf_len: positions of a split
@@ -165,65 +166,89 @@ struct AttnRows {
     f32x4 o[RT][D / 16];
 };
 
-// Rows row0.. of the span: eight dimensions kk * 32 + g * 8 .. per lane, as TERMS
-// values of T, handed to put(rt, term, kk, vector).
-template <class T, int D, int RT, class QT, int TERMS, class PUT>
-__device__ __forceinline__ void attn_queries(const AttnParams &p, const AttnSpan &s, int hk, int row0, AttnRows<RT, D> &w, PUT put) {
-    using V8 = typename Vec8<T>::type;
-    constexpr int KK = D / 32;
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const float sgn = p.scale < 0.0f ? -1.0f : 1.0f;
+// The limits of the wave's rows row0.. and empty sums.
+template <int RT, int D>
+__device__ __forceinline__ void attn_rows(const AttnParams &p, const AttnSpan &s, int row0, AttnRows<RT, D> &w) {
+    const int n = threadIdx.x & 15;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int row = row0 + rt * 16 + n;
-        const bool ok = row < s.rows;
-        const int t = (int)fastdiv((uint32_t)(ok ? row : 0), p.group_div);
-        const int h = hk * p.group + (ok ? row : 0) - t * p.group;
-        const QT *src = reinterpret_cast<const QT *>(p.q + (int64_t)(s.tok0 + t) * p.q_token + h * p.q_head);
-        const int64_t lim = (int64_t)s.causal + t + 1;
-        w.limit[rt] = ok && lim < s.end ? (int)lim : s.end;
-        float x[KK][8];
-        float top = 0.0f;
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int d = kk * 32 + g * 8 + j;
-                const float y = (float)src[d < p.head_dim ? d : 0] * sgn;  // (loads without branches)
-                x[kk][j] = ok && d < p.head_dim ? y : 0.0f;
-                top = fmaxf(top, fabsf(x[kk][j]));
-            }
-        w.c[rt] = fabsf(p.scale) * kLog2e;
-        float f = 1.0f;
-        if (TERMS > 1) {
-            // an F32 row of any magnitude: a power of two brings its largest value to 1..2
-            top = xor_max(top);
-            int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-            e = e < -126 || e > 127 ? 0 : e > 126 ? 126 : e;
-            f = __uint_as_float((uint32_t)(127 - e) << 23);
-            w.c[rt] *= __uint_as_float((uint32_t)(127 + e) << 23);
-        }
-        // (above zero, so that c * -inf of an unseen position stays -inf at a scale of 0)
-        w.c[rt] = fmaxf(w.c[rt], 1e-37f);
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            V8 v[TERMS];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                T t8[TERMS];
-                split_terms<T, TERMS>(x[kk][j] * f, t8);
-#pragma unroll
-                for (int i = 0; i < TERMS; ++i) v[i][j] = t8[i];
-            }
-#pragma unroll
-            for (int i = 0; i < TERMS; ++i) put(rt, i, kk, v[i]);
-        }
-        __builtin_amdgcn_sched_barrier(0);  // one row tile's registers at a time
+        const int64_t lim = (int64_t)s.causal + (int)fastdiv((uint32_t)row, p.group_div) + 1;
+        w.limit[rt] = row < s.rows && lim < s.end ? (int)lim : s.end;
         w.m[rt] = -__builtin_inff();
         w.l[rt] = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) w.o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+}
+
+// Rows row0 .. row0 + 15 of the span: dimensions kk * 32 + g * 8 .. of row n per
+// lane, as TERMS values of T, handed to put(term, kk, vector).  Returns the
+// row's factor c.
+template <class T, int D, class QT, int TERMS, class PUT>
+__device__ __forceinline__ float attn_queries(const AttnParams &p, const AttnSpan &s, int hk, int row0, PUT put) {
+    using V8 = typename Vec8<T>::type;
+    constexpr int KK = D / 32;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const float sgn = p.scale < 0.0f ? -1.0f : 1.0f;
+    const int row = row0 + n;
+    const bool ok = row < s.rows;
+    const int t = (int)fastdiv((uint32_t)(ok ? row : 0), p.group_div);
+    const int h = hk * p.group + (ok ? row : 0) - t * p.group;
+    const QT *src = reinterpret_cast<const QT *>(p.q + (int64_t)(s.tok0 + t) * p.q_token + h * p.q_head);
+    float x[KK][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+        // (clamped, so that the loads need no branches)
+        const int d = kk * 32 + g * 8;
+        const bool in = ok && d < p.head_dim;
+        const QT *at = src + (d < p.head_dim ? d : 0);
+        if (p.q_vec) {
+            constexpr int N = 8 * sizeof(QT) / 16;
+            union {
+                u32x4 v[N];
+                QT e[8];
+            } u;
+#pragma unroll
+            for (int i = 0; i < N; ++i) u.v[i] = reinterpret_cast<const u32x4 *>(at)[i];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[kk][j] = (float)u.e[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[kk][j] = (float)at[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[kk][j] = in ? x[kk][j] * sgn : 0.0f;
+            top = fmaxf(top, fabsf(x[kk][j]));
+        }
+    }
+    float c = fabsf(p.scale) * kLog2e, f = 1.0f;
+    if (TERMS > 1) {
+        // an F32 row of any magnitude: a power of two brings its largest value to 1..2
+        top = xor_max(top);
+        int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+        e = e < -126 || e > 127 ? 0 : e > 126 ? 126 : e;
+        f = __uint_as_float((uint32_t)(127 - e) << 23);
+        c *= __uint_as_float((uint32_t)(127 + e) << 23);
+    }
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+        V8 v[TERMS];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            T t8[TERMS];
+            split_terms<T, TERMS>(x[kk][j] * f, t8);
+#pragma unroll
+            for (int i = 0; i < TERMS; ++i) v[i][j] = t8[i];
+        }
+#pragma unroll
+        for (int i = 0; i < TERMS; ++i) put(i, kk, v[i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // one row tile's registers at a time
+    // (above zero, so that c * -inf of an unseen position stays -inf at a scale of 0)
+    return fmaxf(c, 1e-37f);
 }
 
 // The page of position t of the span (clamped to its last, so that nothing past a
@@ -380,7 +405,7 @@ struct StreamCfg {
     static constexpr int D = D_, RT = RT_, ROWS = 16 * RT_;
     static constexpr bool QLDS = D_ / 32 * RT_ * TERMS > 8;  // queries in LDS: over 32 registers of them
     static constexpr int VBYTES = 4 * 32 * D * 2;             // also one tile's outputs of two waves at the end
-    static constexpr int QBYTES = QLDS ? RT * TERMS * (D / 32) * 1024 : 0;
+    static constexpr int QBYTES = QLDS ? RT * TERMS * (D / 32) * 1024 : 0;  // (else they pass through V's place)
     static constexpr int LDS = VBYTES * 2 > 64 * D * 4 ? VBYTES + QBYTES : 64 * D * 4 + QBYTES;
 };
 
@@ -394,18 +419,26 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
     const int n = lane & 15, g = lane >> 4;
     const int row0 = tile * C::ROWS;
     char *ldv = lds + wave * 32 * D * 2;
-    char *ldq = lds + C::LDS - C::QBYTES;
+    char *ldq = lds + (C::QLDS ? C::LDS - C::QBYTES : 0);
     AttnRows<RT, D> w;
     V8 q[C::QLDS ? 1 : RT][TERMS][KK];
-    attn_queries<T, D, RT, QT, TERMS>(p, s, hk, row0, w, [&](int rt, int i, int kk, V8 v) {
-        if (!C::QLDS) {
-            q[C::QLDS ? 0 : rt][i][kk] = v;
-        } else {
-            const int f = (rt * TERMS + i) * KK + kk;
-            if ((f & 3) == wave) *reinterpret_cast<V8 *>(ldq + f * 1024 + lane * 16) = v;
-        }
-    });
-    if (C::QLDS) __syncthreads();
+    attn_rows<RT, D>(p, s, row0, w);
+    float *cs = reinterpret_cast<float *>(flags);
+    if (wave < RT) {
+        const float c = attn_queries<T, D, QT, TERMS>(p, s, hk, row0 + wave * 16, [&](int i, int kk, V8 v) {
+            *reinterpret_cast<V8 *>(ldq + ((wave * TERMS + i) * KK + kk) * 1024 + lane * 16) = v;
+        });
+        if (g == 0) cs[wave * 16 + n] = c;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) w.c[rt] = cs[rt * 16 + n];
+    if (!C::QLDS) {
+#pragma unroll
+        for (int f = 0; f < RT * TERMS * KK; ++f)
+            q[C::QLDS ? 0 : f / (TERMS * KK)][f / KK % TERMS][f % KK] = *reinterpret_cast<const V8 *>(ldq + f * 1024 + lane * 16);
+        __syncthreads();
+    }
     const int least = attn_least<C::ROWS>(p, s, tile);
 
     // lane (n, g): positions n and 16 + n of a step, chunks g, 4 + g, ... of K and V
@@ -572,7 +605,10 @@ __device__ __forceinline__ void attn_shared(const AttnParams &p, const AttnCache
     AttnRows<RT, D> w;
     V8 q[RT][TERMS][KK];
     const int row0 = tile * C::ROWS + wave * RT * 16;
-    attn_queries<T, D, RT, QT, TERMS>(p, s, hk, row0, w, [&](int rt, int i, int kk, V8 v) { q[rt][i][kk] = v; });
+    attn_rows<RT, D>(p, s, row0, w);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+        w.c[rt] = attn_queries<T, D, QT, TERMS>(p, s, hk, row0 + rt * 16, [&](int i, int kk, V8 v) { q[rt][i][kk] = v; });
     const int least = attn_least<C::ROWS>(p, s, tile);
 
     // staging: thread -> chunk tid % CH of positions tid / CH + RP * i

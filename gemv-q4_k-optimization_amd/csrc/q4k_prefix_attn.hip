@@ -85,6 +85,7 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
     p.n_head = a.n_head; p.n_head_kv = a.n_head_kv; p.group = a.n_head / a.n_head_kv; p.head_dim = a.head_dim;
     p.group_div = fastdiv_init((uint32_t)p.group);
     p.scale = a.scale;
+    p.q_vec = aligned(a.q, 16) && (a.nb_q_token | a.nb_q_head) % 16 == 0;
     pl.dim = a.head_dim <= 64 ? 64 : a.head_dim <= 128 ? 128 : 256;
     if (a.n_tokens > INT32_MAX / p.group - 256) return Q4K_EUNSUPPORTED;
     const int64_t pre_rows = a.n_prefix > 0 ? a.n_tokens * p.group : 0, suf_rows = a.n_q * p.group;
@@ -94,30 +95,28 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
     pl.pre_size = a.n_prefix > 0 ? size_of(pre_rows) : pl.suf_size;
     if (pl.suf_size > pl.pre_size) pl.suf_size = pl.pre_size;  // (with q_start n_q may exceed the tokens there are)
     const int pr = rows_of[pl.pre_size], sr = rows_of[pl.suf_size];
-    // splits: about two workgroups per CU, in whole tiles of 128 positions
-    const int64_t target = 2 * (int64_t)cus;
+    // Splits of one length for both parts, in whole steps of 128 positions: about
+    // two workgroups per CU in all, however the positions are shared out.
+    const int64_t pt = a.n_prefix > 0 ? cdiv(pre_rows, pr) : 0, st = cdiv(suf_rows, sr);
+    const bool own = a.max_suffix > 0 || a.n_prefix == 0;
+    const int64_t per_pre = pt * a.n_head_kv, per_suf = own ? st * a.n_head_kv * a.n_requests : 0;
+    if (per_pre > INT32_MAX / 4 || per_suf > INT32_MAX / 4) return Q4K_EUNSUPPORTED;
+    const int64_t work = a.n_prefix * per_pre + a.max_suffix * per_suf;
+    int64_t len = cdiv(cdiv(work, 2 * (int64_t)cus), 128) * 128;
+    if (len < 128) len = 128;
+    if (len > (1 << 30)) len = 1 << 30;
+    p.pre_len = p.suf_len = (int)len;
     if (a.n_prefix > 0) {
-        const int64_t tiles = cdiv(pre_rows, pr), per = tiles * a.n_head_kv;
-        int64_t splits = target / per;
-        splits = splits < 1 ? 1 : splits;
-        const int64_t len = cdiv(cdiv(a.n_prefix, splits), 128) * 128;
-        p.pre_tiles = (int)tiles;
-        p.pre_len = (int)len;
+        p.pre_tiles = (int)pt;
         p.pre_splits = (int)cdiv(a.n_prefix, len);
-        if (per * p.pre_splits > INT32_MAX / 2) return Q4K_EUNSUPPORTED;
-        p.pre_items = (int)(per * p.pre_splits);
+        if (per_pre * p.pre_splits > INT32_MAX / 2) return Q4K_EUNSUPPORTED;
+        p.pre_items = (int)(per_pre * p.pre_splits);
     }
-    if (a.max_suffix > 0 || a.n_prefix == 0) {
-        const int64_t tiles = cdiv(suf_rows, sr), per = tiles * a.n_head_kv * a.n_requests;
-        int64_t splits = target / per;
-        splits = splits < 1 ? 1 : splits;
-        int64_t len = cdiv(cdiv(a.max_suffix, splits), 128) * 128;
-        if (len < 128) len = 128;
-        p.suf_tiles = (int)tiles;
-        p.suf_len = (int)len;
+    if (own) {
+        p.suf_tiles = (int)st;
         p.suf_splits = a.max_suffix > 0 ? (int)cdiv(a.max_suffix, len) : 1;
-        if (per > INT32_MAX / 2 / p.suf_splits) return Q4K_EUNSUPPORTED;
-        p.suf_items = (int)(per * p.suf_splits);
+        if (per_suf * p.suf_splits > INT32_MAX / 2) return Q4K_EUNSUPPORTED;
+        p.suf_items = (int)(per_suf * p.suf_splits);
     }
     p.slots = p.pre_splits + p.suf_splits;
     if (p.slots > 1) {
