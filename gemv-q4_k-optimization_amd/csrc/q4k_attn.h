@@ -422,23 +422,6 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
     char *ldq = lds + (C::QLDS ? C::LDS - C::QBYTES : 0);
     AttnRows<RT, D> w;
     V8 q[C::QLDS ? 1 : RT][TERMS][KK];
-    attn_rows<RT, D>(p, s, row0, w);
-    float *cs = reinterpret_cast<float *>(flags);
-    if (wave < RT) {
-        const float c = attn_queries<T, D, QT, TERMS>(p, s, hk, row0 + wave * 16, [&](int i, int kk, V8 v) {
-            *reinterpret_cast<V8 *>(ldq + ((wave * TERMS + i) * KK + kk) * 1024 + lane * 16) = v;
-        });
-        if (g == 0) cs[wave * 16 + n] = c;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) w.c[rt] = cs[rt * 16 + n];
-    if (!C::QLDS) {
-#pragma unroll
-        for (int f = 0; f < RT * TERMS * KK; ++f)
-            q[C::QLDS ? 0 : f / (TERMS * KK)][f / KK % TERMS][f % KK] = *reinterpret_cast<const V8 *>(ldq + f * 1024 + lane * 16);
-        __syncthreads();
-    }
     const int least = attn_least<C::ROWS>(p, s, tile);
 
     // lane (n, g): positions n and 16 + n of a step, chunks g, 4 + g, ... of K and V
@@ -491,6 +474,25 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
         get_pages(t0);
         load(t0);
         get_pages(t0 + 128);
+    }
+
+    // the queries, one row tile per wave, while the first positions are on their way
+    attn_rows<RT, D>(p, s, row0, w);
+    float *cs = reinterpret_cast<float *>(flags);
+    if (wave < RT) {
+        const float c = attn_queries<T, D, QT, TERMS>(p, s, hk, row0 + wave * 16, [&](int i, int kk, V8 v) {
+            *reinterpret_cast<V8 *>(ldq + ((wave * TERMS + i) * KK + kk) * 1024 + lane * 16) = v;
+        });
+        if (g == 0) cs[wave * 16 + n] = c;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) w.c[rt] = cs[rt * 16 + n];
+    if (!C::QLDS) {
+#pragma unroll
+        for (int f = 0; f < RT * TERMS * KK; ++f)
+            q[C::QLDS ? 0 : f / (TERMS * KK)][f / KK % TERMS][f % KK] = *reinterpret_cast<const V8 *>(ldq + f * 1024 + lane * 16);
+        __syncthreads();
     }
     bool fine = true;  // of the values at and after the first step that ends past `least`
     for (; t0 < s.end; t0 += 128) {
@@ -780,10 +782,12 @@ __global__ __launch_bounds__(256, CP::D == 256 ? 1 : 2) void prefix_attn_kernel(
 }
 
 // Joins a row's partial results: one workgroup of 256 per row, groups of
-// head_dim / 4 lanes taking every 256 / (head_dim / 4)-th split.
+// head_dim / 4 lanes taking every 256 / (head_dim / 4)-th split with a running
+// reference, so that nothing waits for a first pass over the references.
 template <class QT>
 __global__ __launch_bounds__(256) void prefix_attn_join_kernel(AttnParams p) {
     __shared__ f32x4 acc[256];
+    __shared__ float2 mls[256];
     const int head = blockIdx.x % p.n_head;
     const int rt = blockIdx.x / p.n_head;
     const int r = rt / p.n_q, t = rt - r * p.n_q;
@@ -794,37 +798,41 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(AttnParams p) {
     const int len = attn_suffix(p, r);
     const int n = p.pre_splits + (p.suf_len > 0 ? (len + p.suf_len - 1) / p.suf_len : 0);
     const int64_t row = (int64_t)tok * p.n_head + head, step = (int64_t)p.n_tokens * p.n_head;
-    const int lane = threadIdx.x & 63;
-    float M = -__builtin_inff();
-    for (int i = lane; i < n; i += 64) M = fmaxf(M, p.part_ml[i * step + row].x);
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) M = fmaxf(M, __shfl_xor(M, x));
     const int q4 = p.head_dim / 4, per = 256 / q4;
     const int grp = threadIdx.x / q4, d4 = threadIdx.x % q4;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
+    float l = 0.0f, M = -__builtin_inff();
+    // A split in which the row sees nothing (l of 0) adds nothing, whatever its values.
+    auto add = [&](float2 e, f32x4 x) {
+        if (e.y == 0.0f) return;
+        const float mn = fmaxf(M, e.x);
+        const float f = M == mn || l == 0.0f ? 1.0f : __builtin_amdgcn_exp2f(M - mn);
+        const float g = e.x == mn ? 1.0f : __builtin_amdgcn_exp2f(e.x - mn);
+        l = l * f + e.y * g;
+        o = o * f + x * g;
+        M = mn;
+    };
     if (grp < per) {
-#pragma unroll 4
-        for (int i = grp; i < n; i += per) {
-            const float2 e = p.part_ml[i * step + row];
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(p.part_o + (i * step + row) * p.head_dim + d4 * 4);
-            // (a split in which the row sees nothing adds nothing, whatever its values)
-            const float f = __builtin_amdgcn_exp2f(e.x == M ? 0.0f : e.x - M);
-            if (e.y != 0.0f) {
-                l += e.y * f;
-                o += x * f;
+        constexpr int U = 4;
+        for (int i0 = grp; i0 < n; i0 += per * U) {
+            float2 e[U];
+            f32x4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t at = (i0 + u * per < n ? i0 + u * per : i0) * step + row;
+                e[u] = p.part_ml[at];
+                x[u] = *reinterpret_cast<const f32x4 *>(p.part_o + at * p.head_dim + d4 * 4);
             }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i0 + u * per < n) add(e[u], x[u]);
         }
     }
-    __shared__ float ls[256];
     acc[threadIdx.x] = o;
-    ls[threadIdx.x] = l;
+    mls[threadIdx.x] = make_float2(M, l);
     __syncthreads();
     if (threadIdx.x >= q4) return;
-    for (int i = 1; i < per; ++i) {
-        o += acc[i * q4 + d4];
-        l += ls[i * q4 + d4];
-    }
+    for (int i = 1; i < per; ++i) add(mls[i * q4 + d4], acc[i * q4 + d4]);
     QT *dst = reinterpret_cast<QT *>(p.dst + tok * p.dst_token + head * p.dst_head) + d4 * 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) dst[j] = (QT)(l == 0.0f ? 0.0f : o[j] / l);

@@ -96,7 +96,10 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
     if (pl.suf_size > pl.pre_size) pl.suf_size = pl.pre_size;  // (with q_start n_q may exceed the tokens there are)
     const int pr = rows_of[pl.pre_size], sr = rows_of[pl.suf_size];
     // Splits of one length for both parts, in whole steps of 128 positions: about
-    // two workgroups per CU in all, however the positions are shared out.
+    // two workgroups per CU in all, however the positions are shared out.  Where
+    // every workgroup streams, whose registers let two run on a CU, up to half as
+    // much again if that makes them all run at once (16 requests of 32 heads behind
+    // 8192 tokens: 26 us against 32 with 608 workgroups).
     const int64_t pt = a.n_prefix > 0 ? cdiv(pre_rows, pr) : 0, st = cdiv(suf_rows, sr);
     const bool own = a.max_suffix > 0 || a.n_prefix == 0;
     const int64_t per_pre = pt * a.n_head_kv, per_suf = own ? st * a.n_head_kv * a.n_requests : 0;
@@ -104,6 +107,12 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
     const int64_t work = a.n_prefix * per_pre + a.max_suffix * per_suf;
     int64_t len = cdiv(cdiv(work, 2 * (int64_t)cus), 128) * 128;
     if (len < 128) len = 128;
+    if (pl.pre_size < 2)
+        for (int64_t l = len; l <= len * 3 / 2; l += cdiv(len, 16 * 128) * 128)
+            if (per_pre * cdiv(a.n_prefix, l) + per_suf * cdiv(a.max_suffix, l) <= 2 * cus) {
+                len = l;
+                break;
+            }
     if (len > (1 << 30)) len = 1 << 30;
     p.pre_len = p.suf_len = (int)len;
     if (a.n_prefix > 0) {
