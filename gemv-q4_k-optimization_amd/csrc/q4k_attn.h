@@ -155,13 +155,32 @@ __device__ __forceinline__ int swz_v(int t, int c) {
     return D == 64 ? c ^ (((t >> 1) & 3) * 2) : c ^ ((t & 7) * 2);
 }
 
-// What a wave holds of its RT tiles of 16 query rows: lane n of a tile has row
-// n's limit, factor, running reference and its part of the sum.
+// Where a lane reads: the swizzles repeat every 16 rows, so the offsets of one
+// tile of 16 positions serve all, at immediate distances.
+template <int D>
+struct AttnReads {
+    static constexpr int NK = D / 32 < 4 ? D / 32 : 4, NV = D / 16 < 8 ? D / 16 : 8;
+    int k[NK], v[NV];
+    __device__ __forceinline__ AttnReads() {
+        constexpr int CH = D / 8;
+        const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4, t = g * 4 + (n >> 2);
+#pragma unroll
+        for (int i = 0; i < NK; ++i) k[i] = (n * CH + swz_k<D>(n, i * 4 + g)) * 16;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = (t * CH + swz_v<D>(t, i * 2 + ((n & 3) >> 1))) * 16 + (n & 1) * 8;
+    }
+    // chunk kk * 4 + g of row n of the tile at row b
+    __device__ __forceinline__ int at_k(int b, int kk) const { return k[kk % NK] + kk / NK * NK * 64 + b * D * 2; }
+    // dimensions dt * 16 .. of rows g * 4 .. g * 4 + 3 of the tile at row b
+    __device__ __forceinline__ int at_v(int b, int dt) const { return v[dt % NV] + dt / NV * NV * 32 + b * D * 2; }
+};
+
 template <int RT, int D>
 struct AttnRows {
     float c[RT];     // log2(e) * |scale| * 2^e of the row's own factor
     int limit[RT];   // positions the row sees end here
-    float m[RT];     // reference in units of S
+    float m[RT];     // reference in units of S; scores above `over` renew it
+    float over[RT], ref[RT];  // ref: kBias - m c
     float l[RT];     // this lane's part of the sum of exp2(c s - c m + kBias)
     f32x4 o[RT][D / 16];
 };
@@ -175,7 +194,8 @@ __device__ __forceinline__ void attn_rows(const AttnParams &p, const AttnSpan &s
         const int row = row0 + rt * 16 + n;
         const int64_t lim = (int64_t)s.causal + (int)fastdiv((uint32_t)row, p.group_div) + 1;
         w.limit[rt] = row < s.rows && lim < s.end ? (int)lim : s.end;
-        w.m[rt] = -__builtin_inff();
+        w.m[rt] = w.over[rt] = -__builtin_inff();
+        w.ref[rt] = kBias;
         w.l[rt] = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) w.o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -275,42 +295,49 @@ __device__ __forceinline__ int attn_least(const AttnParams &p, const AttnSpan &s
 template <class T, int D, int RT, int TERMS>
 __device__ __forceinline__ void attn_softmax(AttnRows<RT, D> &w, const f32x4 (&sx)[RT][2],
                                              typename Vec8<T>::type (&pf)[RT][TERMS]) {
+    float top[RT];
+    bool over = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        float top = sx[rt][0][0];
+        top[rt] = fmaxf(fmaxf(sx[rt][0][0], sx[rt][0][1]), sx[rt][0][2]);
+        top[rt] = fmaxf(fmaxf(top[rt], sx[rt][0][3]), sx[rt][1][0]);
+        top[rt] = fmaxf(fmaxf(top[rt], sx[rt][1][1]), sx[rt][1][2]);
+        top[rt] = fmaxf(top[rt], sx[rt][1][3]);
+        over |= top[rt] > w.over[rt];
+    }
+    // new references when some row passes its old one by 2^kLazy (-inf: always)
+    if (__any(over)) {
 #pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, sx[rt][j >> 2][j & 3]);
-        // a new reference when some row passes the old one by 2^kLazy (-inf: always)
-        if (__any((top - w.m[rt]) * w.c[rt] > kLazy || w.m[rt] == -__builtin_inff())) {
-            const float mn = fmaxf(w.m[rt], xor_max(top));
+        for (int rt = 0; rt < RT; ++rt) {
+            const float mn = fmaxf(w.m[rt], xor_max(top[rt]));
             // (nothing was summed yet, or nothing changes: also keeps inf - inf and 0 * inf out)
             const float f = w.m[rt] == -__builtin_inff() || w.m[rt] == mn ? 1.0f : __builtin_amdgcn_exp2f((w.m[rt] - mn) * w.c[rt]);
             w.m[rt] = mn;
+            w.over[rt] = mn + kLazy / w.c[rt];
+            w.ref[rt] = mn == -__builtin_inff() ? kBias : kBias - mn * w.c[rt];
             w.l[rt] *= f;
 #pragma unroll
             for (int dt = 0; dt < D / 16; ++dt) w.o[rt][dt] *= f;
         }
-        const float ref = w.m[rt] == -__builtin_inff() ? kBias : kBias - w.m[rt] * w.c[rt];
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sx[rt][j >> 2][j & 3], w.c[rt], ref));
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sx[rt][j >> 2][j & 3], w.c[rt], w.ref[rt]));
             w.l[rt] += x;
             T t8[TERMS];
             split_terms<T, TERMS>(x, t8);
 #pragma unroll
             for (int i = 0; i < TERMS; ++i) pf[rt][i][j] = t8[i];
         }
-    }
 }
 
-// O^T += V^T P^T over 32 positions of V in LDS from row b of ldv (swizzled rows of
-// D values).
+// O^T += V^T P^T over 32 positions of V in LDS from row b of ldv.
 template <class T, int D, int RT, int TERMS>
-__device__ __forceinline__ void attn_values(AttnRows<RT, D> &w, const typename Vec8<T>::type (&pf)[RT][TERMS], const char *ldv, int b) {
+__device__ __forceinline__ void attn_values(AttnRows<RT, D> &w, const AttnReads<D> &rd, const typename Vec8<T>::type (&pf)[RT][TERMS],
+                                            const char *ldv, int b) {
     using V8 = typename Vec8<T>::type;
-    constexpr int CH = D / 8;
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int tr = b + g * 4 + (n >> 2);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
         union {
@@ -318,11 +345,9 @@ __device__ __forceinline__ void attn_values(AttnRows<RT, D> &w, const typename V
             V8 v;
         } va;
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-            const int t = tr + tt * 16;
+        for (int tt = 0; tt < 2; ++tt)
             va.h[tt] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4 *)(ldv + (t * CH + swz_v<D>(t, dt * 2 + ((n & 3) >> 1))) * 16 + (n & 1) * 8));
-        }
+                (__attribute__((address_space(3))) s16x4 *)(ldv + rd.at_v(b + tt * 16, dt)));
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -494,6 +519,7 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
             q[C::QLDS ? 0 : f / (TERMS * KK)][f / KK % TERMS][f % KK] = *reinterpret_cast<const V8 *>(ldq + f * 1024 + lane * 16);
         __syncthreads();
     }
+    const AttnReads<D> rd;
     bool fine = true;  // of the values at and after the first step that ends past `least`
     for (; t0 < s.end; t0 += 128) {
         const uint32_t ok = there;
@@ -551,7 +577,7 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
         V8 pf[RT][TERMS];
         attn_softmax<T, D, RT, TERMS>(w, sx, pf);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // V's rows are written before lanes read each other's
-        attn_values<T, D, RT, TERMS>(w, pf, ldv, 0);
+        attn_values<T, D, RT, TERMS>(w, rd, pf, ldv, 0);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     if (!__all(fine))
@@ -643,6 +669,7 @@ __device__ __forceinline__ void attn_shared(const AttnParams &p, const AttnCache
     }
     if (tid == 0) flags[0] = flags[2] = 0;
 
+    const AttnReads<D> rd;
     int par = 0;
     for (int t0 = s.beg; t0 < s.end; t0 += TB, par ^= 1) {
         __syncthreads();  // the last tile is no longer read
@@ -669,18 +696,16 @@ __device__ __forceinline__ void attn_shared(const AttnParams &p, const AttnCache
         __syncthreads();
         const bool masked = flags[par] != 0 || t0 + TB > least;
 
-#pragma unroll 1
+#pragma unroll
         for (int b = 0; b < TB; b += 32) {
-            if (t0 + b >= s.end) break;
             f32x4 sx[RT][2];
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) sx[rt][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                const int t = b + tt * 16 + n;
 #pragma unroll
                 for (int kk = 0; kk < KK; ++kk) {
-                    const V8 ka = *reinterpret_cast<const V8 *>(ldk + (t * CH + swz_k<D>(t, kk * 4 + g)) * 16);
+                    const V8 ka = *reinterpret_cast<const V8 *>(ldk + rd.at_k(b + tt * 16, kk));
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -701,7 +726,7 @@ __device__ __forceinline__ void attn_shared(const AttnParams &p, const AttnCache
             }
             V8 pf[RT][TERMS];
             attn_softmax<T, D, RT, TERMS>(w, sx, pf);
-            attn_values<T, D, RT, TERMS>(w, pf, ldv, b);
+            attn_values<T, D, RT, TERMS>(w, rd, pf, ldv, b);
         }
     }
     __syncthreads();
