@@ -420,16 +420,17 @@ __device__ __forceinline__ void attn_emit(const AttnParams &p, const AttnSpan &s
 }
 
 // ---- few rows: every wave takes all of them over positions of its own ----
-// K goes from memory to the registers it is multiplied from (a lane of the A
-// operand holds eight dimensions of one position), V through 32 rows of LDS that
-// belong to the wave, so waves never wait for each other before the end.  Memory
-// bound: each wave keeps the next 32 positions' K and V on their way.
+// A wave's 32 rows of K, then of V, pass through LDS that belongs to it: whole
+// rows come from memory in 16-byte pieces that neighbouring lanes read side by
+// side (read in the operand's layout they would be 64 separate pieces a load), and
+// waves never wait for each other before the end.  Memory bound: each wave keeps
+// the next 32 positions' K and V on their way.
 template <class T, int D_, int RT_, int TERMS>
 struct StreamCfg {
     using Elem = T;
     static constexpr int D = D_, RT = RT_, ROWS = 16 * RT_;
     static constexpr bool QLDS = D_ / 32 * RT_ * TERMS > 8;  // queries in LDS: over 32 registers of them
-    static constexpr int VBYTES = 4 * 32 * D * 2;             // also one tile's outputs of two waves at the end
+    static constexpr int VBYTES = 4 * 32 * D * 2;             // (and a row tile's outputs of four waves at the end)
     static constexpr int QBYTES = QLDS ? RT * TERMS * (D / 32) * 1024 : 0;  // (else they pass through V's place)
     static constexpr int LDS = VBYTES * 2 > 64 * D * 4 ? VBYTES + QBYTES : 64 * D * 4 + QBYTES;
 };
@@ -440,67 +441,45 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
     using T = typename C::Elem;
     using V8 = typename Vec8<T>::type;
     constexpr int D = C::D, RT = C::RT, KK = D / 32, CH = D / 8;
+    constexpr int RI = 64 / CH, NI = 32 / RI;  // rows of a load, loads of 32 rows
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int row0 = tile * C::ROWS;
-    char *ldv = lds + wave * 32 * D * 2;
+    char *ldw = lds + wave * 32 * D * 2;
     char *ldq = lds + (C::QLDS ? C::LDS - C::QBYTES : 0);
     AttnRows<RT, D> w;
     V8 q[C::QLDS ? 1 : RT][TERMS][KK];
     const int least = attn_least<C::ROWS>(p, s, tile);
 
-    // lane (n, g): positions n and 16 + n of a step, chunks g, 4 + g, ... of K and V
-    u32x4 kf[2][KK], vf[2][KK];
-    uint32_t there = 0;  // bit 16 * tile + n: the position has a page
-    int page[2];
-    const char *kb = kv.k + hk * kv.k_head + g * 16, *vb = kv.v + hk * kv.v_head + g * 16;
-    const bool full = p.head_dim == D;
-    auto get_pages = [&](int t0) {
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt) page[tt] = attn_page(kv, s, t0 + tt * 16 + n);
-    };
+    // lane: chunk lane % CH of rows i * RI + lane / CH
+    const int sc = lane % CH, sr = lane / CH;
+    const bool cok = sc * 8 < p.head_dim;  // (past the head: chunk 0 again, as zeros in K; V's are not stored)
+    const char *kb = kv.k + hk * kv.k_head + (cok ? sc * 16 : 0), *vb = kv.v + hk * kv.v_head + (cok ? sc * 16 : 0);
+    // where each of the 32 rows begins, in K and V: lane r works out row r, all read it
+    longlong2 *rows = reinterpret_cast<longlong2 *>(reinterpret_cast<char *>(flags) + 1024) + wave * 32;
+    u32x4 kf[NI], vf[NI];
+    uint32_t there = 0;  // bit r: position r of the step that was loaded has a page
+    int page;
     auto load = [&](int t0) {
-        uint32_t all = 0;
-        const char *ks[2], *vs[2];
+        const int t = t0 + (lane & 31);
+        const bool ok = t < s.end && (uint32_t)page < (uint32_t)kv.n_pages;
+        there = (uint32_t)__ballot(ok);
+        const int pg = ok ? page : 0, slot = ok ? attn_slot(kv, t) : 0;
+        if (lane < 32) rows[lane] = make_longlong2(pg * kv.k_page + slot * kv.k_token, pg * kv.v_page + slot * kv.v_token);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-            const int t = t0 + tt * 16 + n;
-            const bool ok = t < s.end && (uint32_t)page[tt] < (uint32_t)kv.n_pages;
-            all |= ((uint32_t)__ballot(ok) & 0xffffu) << (16 * tt);
-            const int pg = ok ? page[tt] : 0, slot = ok ? attn_slot(kv, t) : 0;
-            ks[tt] = kb + pg * kv.k_page + slot * kv.k_token;
-            vs[tt] = vb + pg * kv.v_page + slot * kv.v_token;
-        }
-        there = all;
-        if (full) {
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
-                    kf[tt][kk] = *reinterpret_cast<const u32x4 *>(ks[tt] + kk * 64);
-                    vf[tt][kk] = *reinterpret_cast<const u32x4 *>(vs[tt] + kk * 64);
-                }
-        } else {
-            // past the head: chunk 0 again, which the queries' zeros meet as zeros and
-            // whose values are not stored
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
-                    const bool in = kk * 32 + g * 8 < p.head_dim;
-                    const u32x4 x = *reinterpret_cast<const u32x4 *>(ks[tt] + (in ? kk * 64 : -g * 16));
-                    kf[tt][kk] = in ? x : u32x4{0, 0, 0, 0};
-                    vf[tt][kk] = *reinterpret_cast<const u32x4 *>(vs[tt] + (in ? kk * 64 : -g * 16));
-                }
+        for (int i = 0; i < NI; ++i) {
+            const longlong2 at = rows[i * RI + sr];
+            kf[i] = *reinterpret_cast<const u32x4 *>(kb + at.x);
+            vf[i] = *reinterpret_cast<const u32x4 *>(vb + at.y);
         }
     };
     int t0 = s.beg + wave * 32;
     if (t0 < s.end) {
-        get_pages(t0);
+        page = attn_page(kv, s, t0 + (lane & 31));
         load(t0);
-        get_pages(t0 + 128);
+        page = attn_page(kv, s, t0 + 128 + (lane & 31));
     }
-
     // the queries, one row tile per wave, while the first positions are on their way
     attn_rows<RT, D>(p, s, row0, w);
     float *cs = reinterpret_cast<float *>(flags);
@@ -520,36 +499,25 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
         __syncthreads();
     }
     const AttnReads<D> rd;
+    const u32x4 zero = {0, 0, 0, 0};
     bool fine = true;  // of the values at and after the first step that ends past `least`
     for (; t0 < s.end; t0 += 128) {
         const uint32_t ok = there;
         const bool careful = least < s.end && t0 + 32 > least;
-        if (careful) {
 #pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) fine = attn_finite<T>(vf[tt][kk]) && fine;
+        for (int i = 0; i < NI; ++i) {
+            const int r = i * RI + sr;
+            *reinterpret_cast<u32x4 *>(ldw + (r * CH + swz_k<D>(r, sc)) * 16) = cok ? kf[i] : zero;
         }
-        if (ok != 0xffffffffu) {
-            // positions that are not there: values of zero, whatever was read
-#pragma unroll
-            for (int tt = 0; tt < 2; ++tt)
-                if (!((ok >> (16 * tt + n)) & 1))
-#pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) vf[tt][kk] = u32x4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt)
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                const int t = tt * 16 + n;
-                *reinterpret_cast<u32x4 *>(ldv + (t * CH + swz_v<D>(t, kk * 4 + g)) * 16) = vf[tt][kk];
-            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // rows are written before lanes read each other's
         f32x4 sx[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) sx[rt][0] = sx[rt][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
+        for (int kk = 0; kk < KK; ++kk) {
+            V8 ka[2];
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) ka[tt] = *reinterpret_cast<const V8 *>(ldw + rd.at_k(tt * 16, kk));
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -557,11 +525,26 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
                     const V8 qv = C::QLDS ? *reinterpret_cast<const V8 *>(ldq + ((rt * TERMS + i) * KK + kk) * 1024 + lane * 16)
                                           : q[C::QLDS ? 0 : rt][i][kk];
 #pragma unroll
-                    for (int tt = 0; tt < 2; ++tt) sx[rt][tt] = mfma(__builtin_bit_cast(V8, kf[tt][kk]), qv, sx[rt][tt]);
+                    for (int tt = 0; tt < 2; ++tt) sx[rt][tt] = mfma(ka[tt], qv, sx[rt][tt]);
                 }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (careful) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const bool here = (ok >> (i * RI + sr)) & 1;
+                fine = (attn_finite<T>(vf[i]) || !here) && fine;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int r = i * RI + sr;
+            // (a position that is not there: values of zero, whatever was read)
+            *reinterpret_cast<u32x4 *>(ldw + (r * CH + swz_v<D>(r, sc)) * 16) = (ok >> r) & 1 ? vf[i] : zero;
+        }
         if (t0 + 128 < s.end) {
             load(t0 + 128);
-            get_pages(t0 + 256);
+            page = attn_page(kv, s, t0 + 256 + (lane & 31));
         }
         if (careful || ok != 0xffffffffu) {
 #pragma unroll
@@ -576,8 +559,8 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
         }
         V8 pf[RT][TERMS];
         attn_softmax<T, D, RT, TERMS>(w, sx, pf);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // V's rows are written before lanes read each other's
-        attn_values<T, D, RT, TERMS>(w, rd, pf, ldv, 0);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        attn_values<T, D, RT, TERMS>(w, rd, pf, ldw, 0);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     if (!__all(fine))
@@ -761,7 +744,8 @@ __device__ __forceinline__ int xcd_item(int b, int total) {
     return x * per + (x < more ? x : more) + b / 8;
 }
 
-constexpr int kAttnFlags = 1024;  // bytes after the tiles: flags, or (M, l) of four waves' rows
+// bytes after the tiles: flags, or (M, l) of four waves' rows; where the rows of four waves begin
+constexpr int kAttnFlags = 1024 + 2048;
 
 // CP: how the prefix's rows are taken, CS the suffixes'.
 template <class CP, class CS, class QT, int TERMS>
