@@ -120,17 +120,22 @@ __device__ __forceinline__ void bf16_terms(const float (&x)[8], bf16x8 (&t)[3]) 
     }
 }
 
-// Eight adapter values as BF16 terms, and the sum of products with three activation terms
+// Eight adapter values as BF16 terms, and the sum of products with three
+// activation terms: mul with the adapter as the A operand, mul_left as B
 template <class T>
 struct Weights;
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 template <>
 struct Weights<__bf16> {
     bf16x8 w;
     __device__ __forceinline__ void set(u32x4 v) { w = __builtin_bit_cast(bf16x8, v); }
+    __device__ __forceinline__ void set_terms(bf16x8 a, bf16x8) { w = a; }
+    __device__ __forceinline__ bf16x8 second() const { return w; }
     __device__ __forceinline__ f32x4 mul(const bf16x8 (&x)[3], f32x4 c) const {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[2], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[1], c, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[0], c, 0, 0, 0);
+        return mfma(w, x[0], mfma(w, x[1], mfma(w, x[2], c)));
+    }
+    __device__ __forceinline__ f32x4 mul_left(const bf16x8 (&x)[3], f32x4 c) const {
+        return mfma(x[0], w, mfma(x[1], w, mfma(x[2], w, c)));
     }
 };
 template <>
@@ -145,12 +150,16 @@ struct Weights<_Float16> {
             w2[j] = (__bf16)(f - (float)w[j]);
         }
     }
+    __device__ __forceinline__ void set_terms(bf16x8 a, bf16x8 b) {
+        w = a;
+        w2 = b;
+    }
+    __device__ __forceinline__ bf16x8 second() const { return w2; }
     __device__ __forceinline__ f32x4 mul(const bf16x8 (&x)[3], f32x4 c) const {
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w2, x[1], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[2], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w2, x[0], c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[1], c, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, x[0], c, 0, 0, 0);
+        return mfma(w, x[0], mfma(w, x[1], mfma(w2, x[0], mfma(w, x[2], mfma(w2, x[1], c)))));
+    }
+    __device__ __forceinline__ f32x4 mul_left(const bf16x8 (&x)[3], f32x4 c) const {
+        return mfma(x[0], w, mfma(x[1], w, mfma(x[0], w2, mfma(x[2], w, mfma(x[1], w2, c)))));
     }
 };
 
@@ -282,8 +291,122 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p) {
         if (j0 + i * 16 < p.rp) *reinterpret_cast<f32x4 *>(h + i * 16) = acc[i];
 }
 
-// KR: steps of 32 ranks; VB: rows of b in 16-byte loads; VD: base and dst in 16-byte accesses
-template <class T, int KR, bool VB, bool VD>
+// The same for tiles of many tokens: activations and adapter rows come from
+// memory side by side, 64 values of K at a time, and pass through LDS -- the
+// activations as their three BF16 terms, F16 adapter rows as their two -- so each
+// value is converted once and the waves, one per 16 tokens, share the adapter.
+template <class T>
+struct LdsTerms {
+    static constexpr int n = __is_same(T, _Float16) ? 2 : 1;  // BF16 values of an adapter's value
+};
+template <class T, int NR>
+__global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
+    constexpr int KT = 64, CH = KT / 8, WT = LdsTerms<T>::n, NA = NR * 16 * CH;  // NA: 16-byte pieces of the adapter's tile
+    __shared__ int tok[kTile];
+    __shared__ __attribute__((aligned(16))) __bf16 xs[3][kTile * KT], as[WT][NR * 16 * KT];
+    LoraTile t;
+    if (!lora_tile(p, tok, t) || t.adapter < 0) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int ks = blockIdx.x % p.ksplits, j0 = blockIdx.x / p.ksplits * (16 * NR);
+    const int r = adapter_rank(p, t.adapter);
+    const int kend = (ks + 1) * p.kchunk < p.K ? (ks + 1) * p.kchunk : p.K;
+    // chunk c of row t at c ^ (t / 2 % 8): 16 lanes that read the same chunk of 16 rows meet no bank twice
+    auto at = [](int row, int c) { return (row * CH + (c ^ ((row >> 1) & 7))) * 8; };
+    // thread: activations xk.. of the tile's rows tid / 16 + 16 i, 8 values ac of adapter rows tid / 8 + 32 i
+    constexpr int XI = 4, AI = (NA + 255) / 256;
+    const int xk = tid % 16 * 4, ac = tid % CH;
+    const float *xp[XI];
+    const char *ap[AI];
+    bool arow[AI];
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+        const int row = tid / 16 + 16 * i;
+        xp[i] = reinterpret_cast<const float *>(p.x + (int64_t)tok[row < t.count ? row : 0] * p.nb_x);
+    }
+#pragma unroll
+    for (int i = 0; i < AI; ++i) {
+        const int j = j0 + tid / CH + 32 * i;
+        arow[i] = j < r && tid / CH + 32 * i < 16 * NR;
+        ap[i] = p.a + t.adapter * p.nb_a_adapter + (arow[i] ? j : 0) * p.nb_a;
+    }
+    f32x4 xv[XI];
+    u32x4 av[AI];
+    // (clamped to the row's start, zeros where there is nothing: loads without branches)
+    auto load = [&](int k0) {
+        const bool xin = k0 + xk < p.K, ain = k0 + ac * 8 < p.K;
+#pragma unroll
+        for (int i = 0; i < XI; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(xp[i] + (xin ? k0 + xk : 0));
+            xv[i] = xin ? v : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int i = 0; i < AI; ++i) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(ap[i] + (ain ? 2 * (k0 + ac * 8) : 0));
+            av[i] = ain && arow[i] ? v : u32x4{0, 0, 0, 0};
+        }
+    };
+    f32x4 acc[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    load(ks * p.kchunk);
+    for (int k0 = ks * p.kchunk; k0 < kend; k0 += KT) {
+        __syncthreads();  // the last tile is no longer read
+#pragma unroll
+        for (int i = 0; i < XI; ++i) {
+            typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+            bf16x4 tm[3];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float y = xv[i][j];
+#pragma unroll
+                for (int e = 0; e < 3; ++e) {
+                    tm[e][j] = (__bf16)y;
+                    y -= (float)tm[e][j];
+                }
+            }
+            const int o = at(tid / 16 + 16 * i, xk / 8) + (xk & 4);
+#pragma unroll
+            for (int e = 0; e < 3; ++e) *reinterpret_cast<bf16x4 *>(xs[e] + o) = tm[e];
+        }
+#pragma unroll
+        for (int i = 0; i < AI; ++i) {
+            const int row = tid / CH + 32 * i;
+            if (NA % 256 != 0 && row >= 16 * NR) continue;
+            Weights<T> w;
+            w.set(av[i]);
+            *reinterpret_cast<bf16x8 *>(as[0] + at(row, ac)) = w.w;
+            if (WT > 1) *reinterpret_cast<bf16x8 *>(as[WT - 1] + at(row, ac)) = w.second();
+        }
+        if (k0 + KT < kend) load(k0 + KT);
+        __syncthreads();
+        if (wave * 16 < t.count) {
+#pragma unroll
+            for (int kk = 0; kk < KT / 32; ++kk) {
+                bf16x8 xt[3];
+#pragma unroll
+                for (int e = 0; e < 3; ++e) xt[e] = *reinterpret_cast<const bf16x8 *>(xs[e] + at(wave * 16 + n, kk * 4 + g));
+#pragma unroll
+                for (int i = 0; i < NR; ++i) {
+                    Weights<T> w;
+                    w.set_terms(*reinterpret_cast<const bf16x8 *>(as[0] + at(i * 16 + n, kk * 4 + g)),
+                                *reinterpret_cast<const bf16x8 *>(as[WT - 1] + at(i * 16 + n, kk * 4 + g)));
+                    acc[i] = w.mul(xt, acc[i]);
+                }
+            }
+        }
+    }
+    if (wave * 16 + n >= t.count) return;
+    float *h = p.h + ((int64_t)ks * p.N + tok[wave * 16 + n]) * p.rp + j0 + g * 4;
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+        if (j0 + i * 16 < p.rp) *reinterpret_cast<f32x4 *>(h + i * 16) = acc[i];
+}
+
+// KR: steps of 32 ranks; VB: rows of b in 16-byte loads.  The tokens are the A
+// operand here: a lane holds one output of four tokens, and 16 lanes side by side
+// 16 consecutive ones, whatever the alignment of the rows.
+template <class T, int KR, bool VB>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
     __shared__ int tok[kTile];
     LoraTile t;
@@ -293,19 +416,16 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
     const int r = adapter_rank(p, t.adapter);
     const WaveSplit ws(t.count, wave);
     if (ws.nt * 16 >= t.count) return;
-    const bool live = ws.nt * 16 + n < t.count;
-    const int token = tok[ws.nt * 16 + n];
-    const float *base = reinterpret_cast<const float *>(p.base ? p.base + (int64_t)token * p.nb_base : nullptr);
-    float *dst = reinterpret_cast<float *>(p.dst + (int64_t)token * p.nb_dst);
     bf16x8 ht[KR][3];
     const float scale = p.scale && t.adapter >= 0 ? p.scale[t.adapter] : 1.0f;
+    const int mine = tok[ws.nt * 16 + n];
 #pragma unroll
     for (int kk = 0; kk < KR; ++kk) {
         float hv[8] = {};
         const int j = kk * 32 + g * 8;
         if (j < r)  // (rp is a multiple of 16, so eight ranks are there or not)
             for (int s = 0; s < p.ksplits; ++s) {
-                const float *h = p.h + ((int64_t)s * p.N + token) * p.rp + j;
+                const float *h = p.h + ((int64_t)s * p.N + mine) * p.rp + j;
                 const f32x4 h0 = *reinterpret_cast<const f32x4 *>(h), h1 = *reinterpret_cast<const f32x4 *>(h + 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -317,29 +437,32 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
         for (int e = 0; e < 8; ++e) hv[e] *= scale;
         bf16_terms(hv, ht[kk]);
     }
+    const float *base[4];
+    float *dst[4];
+    bool live[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        live[j] = ws.nt * 16 + g * 4 + j < t.count;
+        const int64_t token = tok[ws.nt * 16 + g * 4 + j];
+        base[j] = reinterpret_cast<const float *>(p.base + token * p.nb_base);
+        dst[j] = reinterpret_cast<float *>(p.dst + token * p.nb_dst);
+    }
     const char *b = p.b + (t.adapter < 0 ? 0 : t.adapter) * p.nb_b_adapter;
     const int m0 = blockIdx.x * p.mchunk, m1 = m0 + p.mchunk < p.M ? m0 + p.mchunk : p.M;
-    constexpr int U = 2;  // row tiles in flight
-    for (int mb = m0 + ws.part * 16; mb < m1; mb += ws.parts * 16 * U) {
+    constexpr int U = KR <= 2 ? 4 : 2;  // tiles of 16 outputs in flight, side by side
+    for (int mb = m0 + ws.part * 16 * U; mb < m1; mb += ws.parts * 16 * U) {
         u32x4 bv[U][KR];
-        f32x4 y[U];
+        float y[U][4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int m = mb + u * ws.parts * 16;
-            const bool ok = m + n < m1;
+            const int m = mb + u * 16 + n;
+            const bool ok = m < m1;
 #pragma unroll
-            for (int kk = 0; kk < KR; ++kk)
-                bv[u][kk] = load_w<VB>(b + (ok ? m + n : 0) * p.nb_b, kk * 32 + g * 8, ok ? r : 0);
-            const int mm = m + g * 4;
-            y[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (base && live) {
-                if (VD) {
-                    if (mm < m1) y[u] = *reinterpret_cast<const f32x4 *>(base + mm);
-                } else {
+            for (int kk = 0; kk < KR; ++kk) bv[u][kk] = load_w<VB>(b + (ok ? m : 0) * p.nb_b, kk * 32 + g * 8, ok ? r : 0);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (mm + j < m1) y[u][j] = base[mm + j];
-                }
+            for (int j = 0; j < 4; ++j) {
+                y[u][j] = 0.0f;
+                if (p.base && ok && live[j]) y[u][j] = base[j][m];
             }
         }
 #pragma unroll
@@ -350,18 +473,12 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
                 Weights<T> w;
                 if (VB && (r & 7)) bv[u][kk] = first_w(bv[u][kk], r - kk * 32 - g * 8);
                 w.set(bv[u][kk]);
-                acc = w.mul(ht[kk], acc);
+                acc = w.mul_left(ht[kk], acc);
             }
-            const int mm = mb + u * ws.parts * 16 + g * 4;
-            acc += y[u];
-            if (!live) continue;
-            if (VD) {
-                if (mm < m1) *reinterpret_cast<f32x4 *>(dst + mm) = acc;
-            } else {
+            const int m = mb + u * 16 + n;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (mm + j < m1) dst[mm + j] = acc[j];
-            }
+            for (int j = 0; j < 4; ++j)
+                if (m < m1 && live[j]) dst[j][m] = y[u][j] + acc[j];
         }
     }
 }
@@ -376,12 +493,19 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p) {
     int *wsum = lds + keys;            // [2][16]
     int32_t *order = const_cast<int32_t *>(p.order);
     int4 *tiles = const_cast<int4 *>(p.tiles);
+    auto key_of = [&](int i) {
+        const int id = i < p.N ? p.ids[i] : -1;
+        return id >= 0 && id < p.n_adapters ? id : p.n_adapters;
+    };
+    int key[4];  // the first 4096 tokens' keys stay in registers
+#pragma unroll
+    for (int u = 0; u < 4; ++u) key[u] = key_of(u * 1024 + tid);
     for (int i = tid; i < keys; i += 1024) start[i] = 0;
     __syncthreads();
-    for (int i = tid; i < p.N; i += 1024) {
-        const int id = p.ids[i];
-        atomicAdd(&start[id >= 0 && id < p.n_adapters ? id : p.n_adapters], 1);
-    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if (u * 1024 + tid < p.N) atomicAdd(&start[key[u]], 1);
+    for (int i = 4096 + tid; i < p.N; i += 1024) atomicAdd(&start[key_of(i)], 1);
     __syncthreads();
     // scan of the counts and of the numbers of tiles, 1024 keys at a time
     int tokens = 0, ntiles = 0;
@@ -421,16 +545,16 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p) {
         __syncthreads();
     }
     if (tid == 0) *const_cast<int32_t *>(p.n_tiles) = ntiles;
-    for (int i = tid; i < p.N; i += 1024) {
-        const int id = p.ids[i];
-        order[atomicAdd(&start[id >= 0 && id < p.n_adapters ? id : p.n_adapters], 1)] = i;
-    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if (u * 1024 + tid < p.N) order[atomicAdd(&start[key[u]], 1)] = u * 1024 + tid;
+    for (int i = 4096 + tid; i < p.N; i += 1024) order[atomicAdd(&start[key_of(i)], 1)] = i;
 }
 
 // ---------------------------------------------------------------- host ----
 
 struct LoraPlan {
-    bool grouped;
+    bool grouped, tiled;
     int max_tiles;      // tiles there can be, grouped
     int rp, nr, ksplits, kchunk, mchunk;
     size_t h_bytes, bytes;
@@ -444,6 +568,7 @@ static int lora_plan(const q4k_lora &l, int64_t K, int64_t M, int64_t N, LoraPla
     const int64_t kinds = l.n_adapters + 1 < N ? l.n_adapters + 1 : N;
     const int64_t tiles = N / kTile + kinds;  // at most
     pl.max_tiles = (int)tiles;
+    pl.tiled = N >= 16 * kinds;
     pl.rp = (l.rank + 15) / 16 * 16;
     pl.nr = pl.rp / 16 < kRankTiles ? pl.rp / 16 : kRankTiles;
     if (pl.nr == 3) pl.nr = 4;
@@ -479,17 +604,20 @@ template <class T, bool VEC>
 LoraFn shrink_of(int nr) {
     return nr == 1 ? lora_shrink_kernel<T, 1, VEC> : nr == 2 ? lora_shrink_kernel<T, 2, VEC> : lora_shrink_kernel<T, 4, VEC>;
 }
-template <class T, bool VB, bool VD>
+template <class T>
+LoraFn tiled_of(int nr) {
+    return nr == 1 ? lora_shrink_tiled_kernel<T, 1> : nr == 2 ? lora_shrink_tiled_kernel<T, 2> : lora_shrink_tiled_kernel<T, 4>;
+}
+template <class T, bool VB>
 LoraFn expand_of(int kr) {
-    return kr <= 1   ? lora_expand_kernel<T, 1, VB, VD>
-           : kr <= 2 ? lora_expand_kernel<T, 2, VB, VD>
-           : kr <= 4 ? lora_expand_kernel<T, 4, VB, VD>
-                     : lora_expand_kernel<T, 8, VB, VD>;
+    return kr <= 1   ? lora_expand_kernel<T, 1, VB>
+           : kr <= 2 ? lora_expand_kernel<T, 2, VB>
+           : kr <= 4 ? lora_expand_kernel<T, 4, VB>
+                     : lora_expand_kernel<T, 8, VB>;
 }
 template <class T>
-LoraFn expand_of(int kr, bool vb, bool vd) {
-    return vb ? (vd ? expand_of<T, true, true>(kr) : expand_of<T, true, false>(kr))
-              : (vd ? expand_of<T, false, true>(kr) : expand_of<T, false, false>(kr));
+LoraFn expand_of(int kr, bool vb) {
+    return vb ? expand_of<T, true>(kr) : expand_of<T, false>(kr);
 }
 
 }  // namespace q4k
@@ -559,16 +687,17 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
                          nb11 % 16 == 0;
         const int groups = (pl.rp + 16 * pl.nr - 1) / (16 * pl.nr);
         grid.x = (unsigned)(pl.ksplits * groups);
-        st = launch(f16 ? (vec ? shrink_of<_Float16, true>(pl.nr) : shrink_of<_Float16, false>(pl.nr))
-                        : (vec ? shrink_of<__bf16, true>(pl.nr) : shrink_of<__bf16, false>(pl.nr)),
-                    grid, 256, 0, stream, p);
+        // many tokens of an adapter to a tile: through LDS, else straight to the operands
+        const LoraFn fn = vec && pl.tiled ? (f16 ? tiled_of<_Float16>(pl.nr) : tiled_of<__bf16>(pl.nr))
+                          : vec           ? (f16 ? shrink_of<_Float16, true>(pl.nr) : shrink_of<__bf16, true>(pl.nr))
+                                          : (f16 ? shrink_of<_Float16, false>(pl.nr) : shrink_of<__bf16, false>(pl.nr));
+        st = launch(fn, grid, 256, 0, stream, p);
     }
     if (st == Q4K_OK) {
         const bool vb = l.rank % 8 == 0 && aligned(l.b, 16) && (l.nb_b | l.nb_b_adapter) % 16 == 0;
-        const bool vd = ne01 % 4 == 0 && aligned(dst, 16) && nb1 % 16 == 0 && aligned(src2, 16) && nb21 % 16 == 0;
         grid.x = (unsigned)((ne01 + pl.mchunk - 1) / pl.mchunk);
-        st = launch(f16 ? expand_of<_Float16>((l.rank + 31) / 32, vb, vd) : expand_of<__bf16>((l.rank + 31) / 32, vb, vd), grid,
-                    256, 0, stream, p);
+        const int kr = (l.rank + 31) / 32;
+        st = launch(f16 ? expand_of<_Float16>(kr, vb) : expand_of<__bf16>(kr, vb), grid, 256, 0, stream, p);
     }
     return ws.end(st, stream);
 }
