@@ -79,14 +79,13 @@ __device__ __forceinline__ bool lora_tile(const LoraParams &p, int *tok, LoraTil
     const int key = __builtin_amdgcn_readfirstlane(key_of(me));
     t.adapter = key;
     uint64_t same[kSliceBallots];
-    int before = 0, all = 0;
+    int before = 0, all = 0, keys[kSliceBallots];
+    // (all on their way at once; past the end the last one again)
+#pragma unroll
+    for (int i = 0; i < kSliceBallots; ++i) keys[i] = key_of(i * 64 + lane < n ? i * 64 + lane : n - 1);
 #pragma unroll
     for (int i = 0; i < kSliceBallots; ++i) {
-        same[i] = 0;
-        if (i * 64 < n) {
-            const int at = i * 64 + lane;
-            same[i] = __ballot(at < n && key_of(at < n ? at : 0) == key);
-        }
+        same[i] = __ballot(i * 64 + lane < n && keys[i] == key);
         const int d = me - i * 64;
         before += __popcll(d >= 64 ? same[i] : d > 0 ? same[i] & ((1ull << d) - 1) : 0);
         all += __popcll(same[i]);
@@ -330,27 +329,20 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
         arow[i] = j < r && tid / CH + 32 * i < 16 * NR;
         ap[i] = p.a + t.adapter * p.nb_a_adapter + (arow[i] ? j : 0) * p.nb_a;
     }
-    f32x4 xv[XI];
-    u32x4 av[AI];
-    // (clamped to the row's start, zeros where there is nothing: loads without branches)
-    auto load = [&](int k0) {
-        const bool xin = k0 + xk < p.K, ain = k0 + ac * 8 < p.K;
+    f32x4 xb[2][XI];  // two tiles on their way
+    u32x4 ab[2][AI];
+    // (clamped to the row's start: loads without branches, zeros for what is not there when it is used)
+    auto load = [&](int k0, f32x4 (&xv)[XI], u32x4 (&av)[AI]) {
+        const int xo = k0 + xk < p.K ? k0 + xk : 0, ao = k0 + ac * 8 < p.K ? 2 * (k0 + ac * 8) : 0;
 #pragma unroll
-        for (int i = 0; i < XI; ++i) {
-            const f32x4 v = *reinterpret_cast<const f32x4 *>(xp[i] + (xin ? k0 + xk : 0));
-            xv[i] = xin ? v : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
+        for (int i = 0; i < XI; ++i) xv[i] = *reinterpret_cast<const f32x4 *>(xp[i] + xo);
 #pragma unroll
-        for (int i = 0; i < AI; ++i) {
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(ap[i] + (ain ? 2 * (k0 + ac * 8) : 0));
-            av[i] = ain && arow[i] ? v : u32x4{0, 0, 0, 0};
-        }
+        for (int i = 0; i < AI; ++i) av[i] = *reinterpret_cast<const u32x4 *>(ap[i] + ao);
     };
     f32x4 acc[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    load(ks * p.kchunk);
-    for (int k0 = ks * p.kchunk; k0 < kend; k0 += KT) {
+    auto step = [&](int k0, f32x4 (&xv)[XI], u32x4 (&av)[AI]) {
         __syncthreads();  // the last tile is no longer read
 #pragma unroll
         for (int i = 0; i < XI; ++i) {
@@ -358,7 +350,7 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
             bf16x4 tm[3];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float y = xv[i][j];
+                float y = k0 + xk < p.K ? xv[i][j] : 0.0f;
 #pragma unroll
                 for (int e = 0; e < 3; ++e) {
                     tm[e][j] = (__bf16)y;
@@ -374,11 +366,11 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
             const int row = tid / CH + 32 * i;
             if (NA % 256 != 0 && row >= 16 * NR) continue;
             Weights<T> w;
-            w.set(av[i]);
+            w.set(k0 + ac * 8 < p.K && arow[i] ? av[i] : u32x4{0, 0, 0, 0});
             *reinterpret_cast<bf16x8 *>(as[0] + at(row, ac)) = w.w;
             if (WT > 1) *reinterpret_cast<bf16x8 *>(as[WT - 1] + at(row, ac)) = w.second();
         }
-        if (k0 + KT < kend) load(k0 + KT);
+        if (k0 + 2 * KT < kend) load(k0 + 2 * KT, xv, av);
         __syncthreads();
         if (wave * 16 < t.count) {
 #pragma unroll
@@ -395,6 +387,13 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
                 }
             }
         }
+    };
+    const int k_first = ks * p.kchunk;
+    load(k_first, xb[0], ab[0]);
+    if (k_first + KT < kend) load(k_first + KT, xb[1], ab[1]);
+    for (int k0 = k_first; k0 < kend; k0 += 2 * KT) {
+        step(k0, xb[0], ab[0]);
+        if (k0 + KT < kend) step(k0 + KT, xb[1], ab[1]);
     }
     if (wave * 16 + n >= t.count) return;
     float *h = p.h + ((int64_t)ks * p.N + tok[wave * 16 + n]) * p.rp + j0 + g * 4;
@@ -415,27 +414,63 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
     const int n = lane & 15, g = lane >> 4;
     const int r = adapter_rank(p, t.adapter);
     const WaveSplit ws(t.count, wave);
-    if (ws.nt * 16 >= t.count) return;
+    constexpr bool SH = KR <= 2;  // h's terms in LDS (24 KB at 64 ranks)
+    __shared__ bf16x8 hs[3][SH ? kTile * KR * 4 : 1];
     bf16x8 ht[KR][3];
     const float scale = p.scale && t.adapter >= 0 ? p.scale[t.adapter] : 1.0f;
-    const int mine = tok[ws.nt * 16 + n];
+    if (SH) {
+        // whole rows of h side by side, summed over the splits and turned into terms once per workgroup
+        constexpr int CH = KR * 4;  // pieces of eight ranks
+        const int tiles = (t.count + 15) / 16;
+        for (int x = threadIdx.x; x < tiles * 16 * CH; x += 256) {
+            const int row = x / CH, c = x % CH;
+            float hv[8] = {};
+            if (row < t.count && c * 8 < r) {  // (rp is a multiple of 16, so eight ranks are there or not)
+#pragma unroll 4
+                for (int s = 0; s < p.ksplits; ++s) {
+                    const f32x4 *h = reinterpret_cast<const f32x4 *>(p.h + ((int64_t)s * p.N + tok[row]) * p.rp + c * 8);
+                    const f32x4 h0 = h[0], h1 = h[1];
 #pragma unroll
-    for (int kk = 0; kk < KR; ++kk) {
-        float hv[8] = {};
-        const int j = kk * 32 + g * 8;
-        if (j < r)  // (rp is a multiple of 16, so eight ranks are there or not)
-            for (int s = 0; s < p.ksplits; ++s) {
-                const float *h = p.h + ((int64_t)s * p.N + mine) * p.rp + j;
-                const f32x4 h0 = *reinterpret_cast<const f32x4 *>(h), h1 = *reinterpret_cast<const f32x4 *>(h + 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    hv[e] += h0[e];
-                    hv[e + 4] += h1[e];
+                    for (int e = 0; e < 4; ++e) {
+                        hv[e] += h0[e];
+                        hv[e + 4] += h1[e];
+                    }
                 }
             }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) hv[e] *= scale;
-        bf16_terms(hv, ht[kk]);
+            for (int e = 0; e < 8; ++e) hv[e] *= scale;
+            bf16x8 tm[3];
+            bf16_terms(hv, tm);
+#pragma unroll
+            for (int e = 0; e < 3; ++e) hs[e][row * CH + (c ^ (row & (CH - 1)))] = tm[e];
+        }
+        __syncthreads();
+        if (ws.nt * 16 >= t.count) return;
+#pragma unroll
+        for (int kk = 0; kk < KR; ++kk)
+#pragma unroll
+            for (int e = 0; e < 3; ++e) ht[kk][e] = hs[e][(ws.nt * 16 + n) * CH + ((kk * 4 + g) ^ (n & (CH - 1)))];
+    } else {
+        if (ws.nt * 16 >= t.count) return;
+        const int mine = tok[ws.nt * 16 + n];
+#pragma unroll
+        for (int kk = 0; kk < KR; ++kk) {
+            float hv[8] = {};
+            const int j = kk * 32 + g * 8;
+            if (j < r)
+                for (int s = 0; s < p.ksplits; ++s) {
+                    const float *h = p.h + ((int64_t)s * p.N + mine) * p.rp + j;
+                    const f32x4 h0 = *reinterpret_cast<const f32x4 *>(h), h1 = *reinterpret_cast<const f32x4 *>(h + 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        hv[e] += h0[e];
+                        hv[e + 4] += h1[e];
+                    }
+                }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) hv[e] *= scale;
+            bf16_terms(hv, ht[kk]);
+        }
     }
     const float *base[4];
     float *dst[4];
@@ -443,28 +478,32 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         live[j] = ws.nt * 16 + g * 4 + j < t.count;
-        const int64_t token = tok[ws.nt * 16 + g * 4 + j];
+        const int64_t token = tok[live[j] ? ws.nt * 16 + g * 4 + j : 0];
         base[j] = reinterpret_cast<const float *>(p.base + token * p.nb_base);
         dst[j] = reinterpret_cast<float *>(p.dst + token * p.nb_dst);
     }
     const char *b = p.b + (t.adapter < 0 ? 0 : t.adapter) * p.nb_b_adapter;
     const int m0 = blockIdx.x * p.mchunk, m1 = m0 + p.mchunk < p.M ? m0 + p.mchunk : p.M;
     constexpr int U = KR <= 2 ? 4 : 2;  // tiles of 16 outputs in flight, side by side
-    for (int mb = m0 + ws.part * 16 * U; mb < m1; mb += ws.parts * 16 * U) {
-        u32x4 bv[U][KR];
-        float y[U][4];
+    const int step = ws.parts * 16 * U;
+    u32x4 bv[U][KR];
+    float y[U][4];
+    auto load = [&](int mb) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int m = mb + u * 16 + n;
             const bool ok = m < m1;
+            // (clamped: loads without branches)
 #pragma unroll
-            for (int kk = 0; kk < KR; ++kk) bv[u][kk] = load_w<VB>(b + (ok ? m : 0) * p.nb_b, kk * 32 + g * 8, ok ? r : 0);
+            for (int kk = 0; kk < KR; ++kk) bv[u][kk] = load_w<VB>(b + (ok ? m : m0) * p.nb_b, kk * 32 + g * 8, r);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                y[u][j] = 0.0f;
-                if (p.base && ok && live[j]) y[u][j] = base[j][m];
-            }
+            for (int j = 0; j < 4; ++j) y[u][j] = p.base ? base[j][ok ? m : m0] : 0.0f;
         }
+    };
+    int mb = m0 + ws.part * 16 * U;
+    if (mb < m1) load(mb);
+    for (; mb < m1; mb += step) {
+        float out[U][4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -475,10 +514,16 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
                 w.set(bv[u][kk]);
                 acc = w.mul_left(ht[kk], acc);
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[u][j] = y[u][j] + acc[j];
+        }
+        if (mb + step < m1) load(mb + step);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
             const int m = mb + u * 16 + n;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (m < m1 && live[j]) dst[j][m] = y[u][j] + acc[j];
+                if (m < m1 && live[j]) dst[j][m] = out[u][j];
         }
     }
 }
@@ -500,12 +545,28 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p) {
     int key[4];  // the first 4096 tokens' keys stay in registers
 #pragma unroll
     for (int u = 0; u < 4; ++u) key[u] = key_of(u * 1024 + tid);
+    // One atomic per key of a wave: in prompts the 64 lanes hold the same one.  The
+    // lane's place after what was counted before.
+    auto count = [&](int k, bool in) {
+        uint64_t rest = __ballot(in);
+        int place = 0;
+        while (rest) {
+            const int k0 = __builtin_amdgcn_readlane(k, (int)__builtin_ctzll(rest));
+            const uint64_t same = __ballot(in && k == k0);
+            int old = 0;
+            if (lane == 0) old = atomicAdd(&start[k0], (int)__popcll(same));
+            old = __builtin_amdgcn_readfirstlane(old);
+            if (k == k0) place = old + (int)__popcll(same & ((1ull << lane) - 1));
+            rest &= ~same;
+        }
+        return place;
+    };
+    const int upto = (p.N + 1023) / 1024 * 1024;
     for (int i = tid; i < keys; i += 1024) start[i] = 0;
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-        if (u * 1024 + tid < p.N) atomicAdd(&start[key[u]], 1);
-    for (int i = 4096 + tid; i < p.N; i += 1024) atomicAdd(&start[key_of(i)], 1);
+    for (int u = 0; u < 4; ++u) count(key[u], u * 1024 + tid < p.N);
+    for (int i = 4096 + tid; i < upto; i += 1024) count(key_of(i), i < p.N);
     __syncthreads();
     // scan of the counts and of the numbers of tiles, 1024 keys at a time
     int tokens = 0, ntiles = 0;
@@ -546,9 +607,14 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p) {
     }
     if (tid == 0) *const_cast<int32_t *>(p.n_tiles) = ntiles;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-        if (u * 1024 + tid < p.N) order[atomicAdd(&start[key[u]], 1)] = u * 1024 + tid;
-    for (int i = 4096 + tid; i < p.N; i += 1024) order[atomicAdd(&start[key_of(i)], 1)] = i;
+    for (int u = 0; u < 4; ++u) {
+        const int i = u * 1024 + tid, at = count(key[u], i < p.N);
+        if (i < p.N) order[at] = i;
+    }
+    for (int i = 4096 + tid; i < upto; i += 1024) {
+        const int at = count(key_of(i), i < p.N);
+        if (i < p.N) order[at] = i;
+    }
 }
 
 // ---------------------------------------------------------------- host ----
