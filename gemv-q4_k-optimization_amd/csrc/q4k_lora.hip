@@ -302,7 +302,8 @@ template <class T, int NR>
 __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
     constexpr int KT = 64, CH = KT / 8, WT = LdsTerms<T>::n, NA = NR * 16 * CH;  // NA: 16-byte pieces of the adapter's tile
     __shared__ int tok[kTile];
-    __shared__ __attribute__((aligned(16))) __bf16 xs[3][kTile * KT], as[WT][NR * 16 * KT];
+    // two tiles: one is multiplied while the next one is written
+    __shared__ __attribute__((aligned(16))) __bf16 xs2[2][3][kTile * KT], as2[2][WT][NR * 16 * KT];
     LoraTile t;
     if (!lora_tile(p, tok, t) || t.adapter < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -342,8 +343,7 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
     f32x4 acc[NR];
 #pragma unroll
     for (int i = 0; i < NR; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    auto step = [&](int k0, f32x4 (&xv)[XI], u32x4 (&av)[AI]) {
-        __syncthreads();  // the last tile is no longer read
+    auto write = [&](int k0, const f32x4 (&xv)[XI], const u32x4 (&av)[AI], __bf16 (&xs)[3][kTile * KT], __bf16 (&as)[WT][NR * 16 * KT]) {
 #pragma unroll
         for (int i = 0; i < XI; ++i) {
             typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -370,8 +370,8 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
             *reinterpret_cast<bf16x8 *>(as[0] + at(row, ac)) = w.w;
             if (WT > 1) *reinterpret_cast<bf16x8 *>(as[WT - 1] + at(row, ac)) = w.second();
         }
-        if (k0 + 2 * KT < kend) load(k0 + 2 * KT, xv, av);
-        __syncthreads();
+    };
+    auto multiply = [&](const __bf16 (&xs)[3][kTile * KT], const __bf16 (&as)[WT][NR * 16 * KT]) {
         if (wave * 16 < t.count) {
 #pragma unroll
             for (int kk = 0; kk < KT / 32; ++kk) {
@@ -390,10 +390,21 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
     };
     const int k_first = ks * p.kchunk;
     load(k_first, xb[0], ab[0]);
-    if (k_first + KT < kend) load(k_first + KT, xb[1], ab[1]);
+    load(k_first + KT, xb[1], ab[1]);  // (past the end: what is there, unused)
+    write(k_first, xb[0], ab[0], xs2[0], as2[0]);
+    load(k_first + 2 * KT, xb[0], ab[0]);
+    __syncthreads();
     for (int k0 = k_first; k0 < kend; k0 += 2 * KT) {
-        step(k0, xb[0], ab[0]);
-        if (k0 + KT < kend) step(k0 + KT, xb[1], ab[1]);
+        // tile k0 is in LDS 0; k0 + KT in registers 1, k0 + 2 KT in registers 0
+        if (k0 + KT < kend) write(k0 + KT, xb[1], ab[1], xs2[1], as2[1]);
+        if (k0 + 3 * KT < kend) load(k0 + 3 * KT, xb[1], ab[1]);
+        multiply(xs2[0], as2[0]);
+        __syncthreads();
+        if (k0 + KT >= kend) break;
+        if (k0 + 2 * KT < kend) write(k0 + 2 * KT, xb[0], ab[0], xs2[0], as2[0]);
+        if (k0 + 4 * KT < kend) load(k0 + 4 * KT, xb[0], ab[0]);
+        multiply(xs2[1], as2[1]);
+        __syncthreads();
     }
     if (wave * 16 + n >= t.count) return;
     float *h = p.h + ((int64_t)ks * p.N + tok[wave * 16 + n]) * p.rp + j0 + g * 4;
@@ -402,10 +413,12 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
         if (j0 + i * 16 < p.rp) *reinterpret_cast<f32x4 *>(h + i * 16) = acc[i];
 }
 
-// KR: steps of 32 ranks; VB: rows of b in 16-byte loads.  The tokens are the A
-// operand here: a lane holds one output of four tokens, and 16 lanes side by side
-// 16 consecutive ones, whatever the alignment of the rows.
-template <class T, int KR, bool VB>
+// KR: steps of 32 ranks; VB: rows of b in 16-byte loads; VD: base and dst in
+// 16-byte accesses.  The tokens are the A operand here: a lane of a result has one
+// output of four tokens.  Of the four tiles that are in flight, lane n's outputs
+// are 4 n .. 4 n + 3 (VD), so that 16 lanes store 256 bytes of a token side by
+// side; rows that are not aligned take outputs n of each tile and single floats.
+template <class T, int KR, bool VB, bool VD>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
     __shared__ int tok[kTile];
     LoraTile t;
@@ -484,26 +497,36 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
     }
     const char *b = p.b + (t.adapter < 0 ? 0 : t.adapter) * p.nb_b_adapter;
     const int m0 = blockIdx.x * p.mchunk, m1 = m0 + p.mchunk < p.M ? m0 + p.mchunk : p.M;
-    constexpr int U = KR <= 2 ? 4 : 2;  // tiles of 16 outputs in flight, side by side
+    constexpr int U = 4;  // tiles of 16 outputs in flight
     const int step = ws.parts * 16 * U;
+    auto out_of = [&](int u) { return VD ? n * U + u : u * 16 + n; };
     u32x4 bv[U][KR];
-    float y[U][4];
+    float y[4][U];
     auto load = [&](int mb) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int m = mb + u * 16 + n;
-            const bool ok = m < m1;
             // (clamped: loads without branches)
+            const int m = mb + out_of(u) < m1 ? mb + out_of(u) : m0;
 #pragma unroll
-            for (int kk = 0; kk < KR; ++kk) bv[u][kk] = load_w<VB>(b + (ok ? m : m0) * p.nb_b, kk * 32 + g * 8, r);
+            for (int kk = 0; kk < KR; ++kk) bv[u][kk] = load_w<VB>(b + m * p.nb_b, kk * 32 + g * 8, r);
+        }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) y[u][j] = p.base ? base[j][ok ? m : m0] : 0.0f;
+        for (int j = 0; j < 4; ++j) {
+            if (VD) {
+                const int m = mb + n * U < m1 ? mb + n * U : m0;
+                const f32x4 v = p.base ? *reinterpret_cast<const f32x4 *>(base[j] + m) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int u = 0; u < U; ++u) y[j][u] = v[u];
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u) y[j][u] = p.base ? base[j][mb + out_of(u) < m1 ? mb + out_of(u) : m0] : 0.0f;
+            }
         }
     };
     int mb = m0 + ws.part * 16 * U;
     if (mb < m1) load(mb);
     for (; mb < m1; mb += step) {
-        float out[U][4];
+        f32x4 out[4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -515,15 +538,19 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
                 acc = w.mul_left(ht[kk], acc);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) out[u][j] = y[u][j] + acc[j];
+            for (int j = 0; j < 4; ++j) out[j][u] = y[j][u] + acc[j];
         }
         if (mb + step < m1) load(mb + step);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int m = mb + u * 16 + n;
+        for (int j = 0; j < 4; ++j) {
+            if (!live[j]) continue;
+            if (VD) {
+                if (mb + n * U < m1) *reinterpret_cast<f32x4 *>(dst[j] + mb + n * U) = out[j];
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (m < m1 && live[j]) dst[j][m] = out[u][j];
+                for (int u = 0; u < U; ++u)
+                    if (mb + out_of(u) < m1) dst[j][mb + out_of(u)] = out[j][u];
+            }
         }
     }
 }
@@ -674,16 +701,17 @@ template <class T>
 LoraFn tiled_of(int nr) {
     return nr == 1 ? lora_shrink_tiled_kernel<T, 1> : nr == 2 ? lora_shrink_tiled_kernel<T, 2> : lora_shrink_tiled_kernel<T, 4>;
 }
-template <class T, bool VB>
+template <class T, bool VB, bool VD>
 LoraFn expand_of(int kr) {
-    return kr <= 1   ? lora_expand_kernel<T, 1, VB>
-           : kr <= 2 ? lora_expand_kernel<T, 2, VB>
-           : kr <= 4 ? lora_expand_kernel<T, 4, VB>
-                     : lora_expand_kernel<T, 8, VB>;
+    return kr <= 1   ? lora_expand_kernel<T, 1, VB, VD>
+           : kr <= 2 ? lora_expand_kernel<T, 2, VB, VD>
+           : kr <= 4 ? lora_expand_kernel<T, 4, VB, VD>
+                     : lora_expand_kernel<T, 8, VB, VD>;
 }
 template <class T>
-LoraFn expand_of(int kr, bool vb) {
-    return vb ? expand_of<T, true>(kr) : expand_of<T, false>(kr);
+LoraFn expand_of(int kr, bool vb, bool vd) {
+    return vb ? (vd ? expand_of<T, true, true>(kr) : expand_of<T, true, false>(kr))
+              : (vd ? expand_of<T, false, true>(kr) : expand_of<T, false, false>(kr));
 }
 
 }  // namespace q4k
@@ -763,7 +791,8 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
         const bool vb = l.rank % 8 == 0 && aligned(l.b, 16) && (l.nb_b | l.nb_b_adapter) % 16 == 0;
         grid.x = (unsigned)((ne01 + pl.mchunk - 1) / pl.mchunk);
         const int kr = (l.rank + 31) / 32;
-        st = launch(f16 ? expand_of<_Float16>(kr, vb) : expand_of<__bf16>(kr, vb), grid, 256, 0, stream, p);
+        const bool vd = ne01 % 4 == 0 && aligned(dst, 16) && nb1 % 16 == 0 && aligned(src2, 16) && nb21 % 16 == 0;
+        st = launch(f16 ? expand_of<_Float16>(kr, vb, vd) : expand_of<__bf16>(kr, vb, vd), grid, 256, 0, stream, p);
     }
     return ws.end(st, stream);
 }
