@@ -55,20 +55,30 @@ struct LoraTile {
     int count;
 };
 
-// A tile's tokens into tok[0..63] (LDS), the same for all waves; false: nothing to do.
-// Grouped: tile blockIdx.z.  Else blockIdx.y is a token of the slice blockIdx.z,
-// and the workgroup of the first, 65th, ... token of an adapter takes the 64 from there.
-__device__ __forceinline__ bool lora_tile(const LoraParams &p, int *tok, LoraTile &t) {
+// A tile's tokens into tok[0..63] (LDS), the same for all waves, and the
+// workgroup's part x of `parts` of the tile's work; false: nothing to do.
+// Grouped: the workgroups of an XCD (they go to the 8 XCDs in turn) take part
+// after part of tiles that follow each other, so that an adapter's tiles read the
+// same piece of it through one L2 (4096 tokens of 16 adapters of rank 64 and K
+// 14336: 147 MB that would come from beyond it).
+// Else blockIdx.y is a token of the slice blockIdx.z, and the workgroup of the
+// first, 65th, ... token of an adapter takes the 64 from there.
+__device__ __forceinline__ bool lora_tile(const LoraParams &p, int parts, int *tok, LoraTile &t, int &x) {
     const int lane = threadIdx.x & 63;
     if (p.tiles) {
-        if ((int)blockIdx.z >= *p.n_tiles) return false;
-        const int4 d = p.tiles[blockIdx.z];
+        const int tiles = *p.n_tiles, total = tiles * parts, id = blockIdx.x;
+        if (id >= total) return false;
+        const int per = total / 8, more = total % 8, xcd = id % 8;
+        const int item = xcd * per + (xcd < more ? xcd : more) + id / 8;
+        x = item / tiles;
+        const int4 d = p.tiles[item - x * tiles];
         t.adapter = d.z;
         t.count = d.y;
         if (threadIdx.x < 64) tok[lane] = p.order[d.x + (lane < d.y ? lane : 0)];
         __syncthreads();
         return true;
     }
+    x = blockIdx.x;
     const int base = blockIdx.z * kSlice, n = p.N - base < kSlice ? p.N - base : kSlice;
     const int me = blockIdx.y;
     if (me >= n) return false;
@@ -227,10 +237,11 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p) {
     __shared__ int tok[kTile];
     __shared__ f32x4 red[4][NR][64];
     LoraTile t;
-    if (!lora_tile(p, tok, t) || t.adapter < 0) return;
+    int part;
+    if (!lora_tile(p, p.ksplits * ((p.rp + 16 * NR - 1) / (16 * NR)), tok, t, part) || t.adapter < 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int ks = blockIdx.x % p.ksplits, j0 = blockIdx.x / p.ksplits * (16 * NR);
+    const int ks = part % p.ksplits, j0 = part / p.ksplits * (16 * NR);
     const int r = adapter_rank(p, t.adapter);
     const WaveSplit ws(t.count, wave);
     const int token = tok[ws.nt * 16 + n];
@@ -305,10 +316,11 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
     // two tiles: one is multiplied while the next one is written
     __shared__ __attribute__((aligned(16))) __bf16 xs2[2][3][kTile * KT], as2[2][WT][NR * 16 * KT];
     LoraTile t;
-    if (!lora_tile(p, tok, t) || t.adapter < 0) return;
+    int part;
+    if (!lora_tile(p, p.ksplits * ((p.rp + 16 * NR - 1) / (16 * NR)), tok, t, part) || t.adapter < 0) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int ks = blockIdx.x % p.ksplits, j0 = blockIdx.x / p.ksplits * (16 * NR);
+    const int ks = part % p.ksplits, j0 = part / p.ksplits * (16 * NR);
     const int r = adapter_rank(p, t.adapter);
     const int kend = (ks + 1) * p.kchunk < p.K ? (ks + 1) * p.kchunk : p.K;
     // chunk c of row t at c ^ (t / 2 % 8): 16 lanes that read the same chunk of 16 rows meet no bank twice
@@ -332,9 +344,11 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
     }
     f32x4 xb[2][XI];  // two tiles on their way
     u32x4 ab[2][AI];
-    // (clamped to the row's start: loads without branches, zeros for what is not there when it is used)
+    // (No branches, or the waits for these loads would be for all of them: past the
+    // end the split's first values again, taken for zeros when they are used.)
+    const int k_first = ks * p.kchunk;
     auto load = [&](int k0, f32x4 (&xv)[XI], u32x4 (&av)[AI]) {
-        const int xo = k0 + xk < p.K ? k0 + xk : 0, ao = k0 + ac * 8 < p.K ? 2 * (k0 + ac * 8) : 0;
+        const int xo = k0 + xk < kend ? k0 + xk : k_first, ao = 2 * (k0 + ac * 8 < kend ? k0 + ac * 8 : k_first);
 #pragma unroll
         for (int i = 0; i < XI; ++i) xv[i] = *reinterpret_cast<const f32x4 *>(xp[i] + xo);
 #pragma unroll
@@ -350,7 +364,7 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
             bf16x4 tm[3];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                float y = k0 + xk < p.K ? xv[i][j] : 0.0f;
+                float y = k0 + xk < kend ? xv[i][j] : 0.0f;
 #pragma unroll
                 for (int e = 0; e < 3; ++e) {
                     tm[e][j] = (__bf16)y;
@@ -366,7 +380,7 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
             const int row = tid / CH + 32 * i;
             if (NA % 256 != 0 && row >= 16 * NR) continue;
             Weights<T> w;
-            w.set(k0 + ac * 8 < p.K && arow[i] ? av[i] : u32x4{0, 0, 0, 0});
+            w.set(k0 + ac * 8 < kend && arow[i] ? av[i] : u32x4{0, 0, 0, 0});
             *reinterpret_cast<bf16x8 *>(as[0] + at(row, ac)) = w.w;
             if (WT > 1) *reinterpret_cast<bf16x8 *>(as[WT - 1] + at(row, ac)) = w.second();
         }
@@ -388,21 +402,19 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
             }
         }
     };
-    const int k_first = ks * p.kchunk;
     load(k_first, xb[0], ab[0]);
-    load(k_first + KT, xb[1], ab[1]);  // (past the end: what is there, unused)
+    load(k_first + KT, xb[1], ab[1]);
     write(k_first, xb[0], ab[0], xs2[0], as2[0]);
     load(k_first + 2 * KT, xb[0], ab[0]);
     __syncthreads();
     for (int k0 = k_first; k0 < kend; k0 += 2 * KT) {
         // tile k0 is in LDS 0; k0 + KT in registers 1, k0 + 2 KT in registers 0
-        if (k0 + KT < kend) write(k0 + KT, xb[1], ab[1], xs2[1], as2[1]);
-        if (k0 + 3 * KT < kend) load(k0 + 3 * KT, xb[1], ab[1]);
+        write(k0 + KT, xb[1], ab[1], xs2[1], as2[1]);
+        load(k0 + 3 * KT, xb[1], ab[1]);
         multiply(xs2[0], as2[0]);
         __syncthreads();
-        if (k0 + KT >= kend) break;
-        if (k0 + 2 * KT < kend) write(k0 + 2 * KT, xb[0], ab[0], xs2[0], as2[0]);
-        if (k0 + 4 * KT < kend) load(k0 + 4 * KT, xb[0], ab[0]);
+        write(k0 + 2 * KT, xb[0], ab[0], xs2[0], as2[0]);
+        load(k0 + 4 * KT, xb[0], ab[0]);
         multiply(xs2[1], as2[1]);
         __syncthreads();
     }
@@ -422,7 +434,8 @@ template <class T, int KR, bool VB, bool VD>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
     __shared__ int tok[kTile];
     LoraTile t;
-    if (!lora_tile(p, tok, t) || (t.adapter < 0 && !p.copy)) return;
+    int part;
+    if (!lora_tile(p, (p.M + p.mchunk - 1) / p.mchunk, tok, t, part) || (t.adapter < 0 && !p.copy)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int r = adapter_rank(p, t.adapter);
@@ -496,7 +509,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
         dst[j] = reinterpret_cast<float *>(p.dst + token * p.nb_dst);
     }
     const char *b = p.b + (t.adapter < 0 ? 0 : t.adapter) * p.nb_b_adapter;
-    const int m0 = blockIdx.x * p.mchunk, m1 = m0 + p.mchunk < p.M ? m0 + p.mchunk : p.M;
+    const int m0 = part * p.mchunk, m1 = m0 + p.mchunk < p.M ? m0 + p.mchunk : p.M;
     constexpr int U = 4;  // tiles of 16 outputs in flight
     const int step = ws.parts * 16 * U;
     auto out_of = [&](int u) { return VD ? n * U + u : u * 16 + n; };
@@ -751,7 +764,9 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
     st = lora_plan(l, ne00, ne01, ne11, pl);
     if (st != Q4K_OK) return st;
     const int64_t slices = (ne11 + kSlice - 1) / kSlice;
-    if ((pl.grouped ? pl.max_tiles : slices) > 65535) return Q4K_EUNSUPPORTED;
+    const int64_t parts1 = (int64_t)pl.ksplits * ((pl.rp + 16 * pl.nr - 1) / (16 * pl.nr)), parts2 = (ne01 + pl.mchunk - 1) / pl.mchunk;
+    const int64_t most = parts1 > parts2 ? parts1 : parts2;
+    if (pl.grouped ? pl.max_tiles > INT32_MAX / most : slices > 65535) return Q4K_EUNSUPPORTED;
     Workspace ws;
     st = ws.begin(workspace, workspace_bytes, pl.bytes, stream);
     if (st != Q4K_OK) return st;
@@ -764,13 +779,16 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
     p.ids = ids; p.h = (float *)ws.ptr; p.K = (int)ne00; p.M = (int)ne01; p.N = (int)ne11;
     p.rank = l.rank; p.rp = pl.rp; p.ksplits = pl.ksplits; p.kchunk = pl.kchunk; p.mchunk = pl.mchunk;
     p.copy = src2 != dst;
-    dim3 grid(1, (unsigned)(ne11 < kSlice ? ne11 : kSlice), (unsigned)slices);
+    dim3 grid;
+    auto grid_of = [&](int64_t parts) {
+        return pl.grouped ? dim3((unsigned)(parts * pl.max_tiles))
+                          : dim3((unsigned)parts, (unsigned)(ne11 < kSlice ? ne11 : kSlice), (unsigned)slices);
+    };
     if (pl.grouped) {
         char *w = (char *)ws.ptr + pl.h_bytes;
         p.tiles = (const int4 *)w;
         p.order = (const int32_t *)(w + (size_t)pl.max_tiles * 16);
         p.n_tiles = p.order + ne11;
-        grid = dim3(1, 1, (unsigned)pl.max_tiles);
         const int lds = (int)(l.n_adapters + 1 + 32) * 4;
         st = ensure_lds(di, (const void *)&lora_group_kernel, lds);
         if (st == Q4K_OK) st = launch(lora_group_kernel, dim3(1), 1024, lds, stream, p);
@@ -779,8 +797,7 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
     if (st == Q4K_OK && pl.ksplits > 0 && l.n_adapters > 0) {
         const bool vec = ne00 % 8 == 0 && aligned(l.a, 16) && (l.nb_a | l.nb_a_adapter) % 16 == 0 && aligned(src1, 16) &&
                          nb11 % 16 == 0;
-        const int groups = (pl.rp + 16 * pl.nr - 1) / (16 * pl.nr);
-        grid.x = (unsigned)(pl.ksplits * groups);
+        grid = grid_of(parts1);
         // many tokens of an adapter to a tile: through LDS, else straight to the operands
         const LoraFn fn = vec && pl.tiled ? (f16 ? tiled_of<_Float16>(pl.nr) : tiled_of<__bf16>(pl.nr))
                           : vec           ? (f16 ? shrink_of<_Float16, true>(pl.nr) : shrink_of<__bf16, true>(pl.nr))
@@ -789,7 +806,7 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
     }
     if (st == Q4K_OK) {
         const bool vb = l.rank % 8 == 0 && aligned(l.b, 16) && (l.nb_b | l.nb_b_adapter) % 16 == 0;
-        grid.x = (unsigned)((ne01 + pl.mchunk - 1) / pl.mchunk);
+        grid = grid_of(parts2);
         const int kr = (l.rank + 31) / 32;
         const bool vd = ne01 % 4 == 0 && aligned(dst, 16) && nb1 % 16 == 0 && aligned(src2, 16) && nb21 % 16 == 0;
         st = launch(f16 ? expand_of<_Float16>(kr, vb, vd) : expand_of<__bf16>(kr, vb, vd), grid, 256, 0, stream, p);
