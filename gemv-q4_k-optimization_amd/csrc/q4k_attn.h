@@ -17,12 +17,11 @@
 
 #include <hip/hip_runtime.h>
 
-#include "q4k_batch_host.h"
+#include "q4k_batch.h"
 #include "q4k_device.h"
 
 namespace q4k {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 

@@ -9,12 +9,10 @@
 #include <hip/hip_runtime.h>
 
 #include "../../include/q4k_batch.h"
-#include "q4k_batch_host.h"
+#include "q4k_batch.h"
 #include "q4k_device.h"
 
 namespace q4k {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct LogitsParams {
     const char *src;
@@ -86,7 +84,7 @@ struct ListRegs {
 // slices begin at 16-byte boundaries of the row of src, whatever its start.  The
 // slice's occurrences are counted in LDS with integer atomics, and the last bias
 // entry of each token is the maximum of their numbers: neither depends on the order.
-template <int THREADS, int H>
+template <int THREADS, int H, bool NT>
 __global__ __launch_bounds__(THREADS, 8) void logits_kernel(LogitsParams p) {
     constexpr int SLICE = THREADS * kLogitsPer;
     __shared__ __attribute__((aligned(16))) uint32_t cnt[SLICE], last[SLICE];
@@ -129,7 +127,7 @@ __global__ __launch_bounds__(THREADS, 8) void logits_kernel(LogitsParams p) {
             x[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             m[k] = 0;
             if (v >= 0 && v + 4 <= V) {
-                x[k] = *reinterpret_cast<const f32x4 *>(src + v);
+                x[k] = load4<NT>(src + v);
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -219,7 +217,7 @@ __global__ __launch_bounds__(THREADS, 8) void logits_kernel(LogitsParams p) {
                 }
             }
             if (wide_out && v >= 0 && v + 4 <= V) {
-                *reinterpret_cast<f32x4 *>(dst + v) = l[k];
+                store4<NT>(dst + v, l[k]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -276,6 +274,7 @@ extern "C" int q4k_logits_adjust(const float *src, int64_t n_vocab, int64_t n_ro
     const LogitsParams p{reinterpret_cast<const char *>(src), reinterpret_cast<char *>(dst), nb_src, nb_dst, (int)n_vocab,
                          (int)n_rows, (int)runs, (int)run, r};
     const dim3 grid((unsigned)(rows * runs));
-    return big ? launch(logits_kernel<1024, 2>, grid, 1024, 0, stream, p)
-               : launch(logits_kernel<256, 4>, grid, 256, 0, stream, p);
+    return !big                                ? launch(logits_kernel<256, 4, false>, grid, 256, 0, stream, p)
+           : n_rows * n_vocab < kStreamFloats ? launch(logits_kernel<1024, 2, false>, grid, 1024, 0, stream, p)
+                                               : launch(logits_kernel<1024, 2, true>, grid, 1024, 0, stream, p);
 }

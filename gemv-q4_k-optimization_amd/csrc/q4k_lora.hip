@@ -19,12 +19,11 @@
 // were put there.
 #include <hip/hip_runtime.h>
 
-#include "q4k_batch_host.h"
+#include "q4k_batch.h"
 #include "q4k_device.h"
 
 namespace q4k {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -350,7 +349,7 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
     auto load = [&](int k0, f32x4 (&xv)[XI], u32x4 (&av)[AI]) {
         const int xo = k0 + xk < kend ? k0 + xk : k_first, ao = 2 * (k0 + ac * 8 < kend ? k0 + ac * 8 : k_first);
 #pragma unroll
-        for (int i = 0; i < XI; ++i) xv[i] = *reinterpret_cast<const f32x4 *>(xp[i] + xo);
+        for (int i = 0; i < XI; ++i) xv[i] = load4<true>(xp[i] + xo);
 #pragma unroll
         for (int i = 0; i < AI; ++i) av[i] = *reinterpret_cast<const u32x4 *>(ap[i] + ao);
     };
@@ -430,7 +429,8 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
 // output of four tokens.  Of the four tiles that are in flight, lane n's outputs
 // are 4 n .. 4 n + 3 (VD), so that 16 lanes store 256 bytes of a token side by
 // side; rows that are not aligned take outputs n of each tile and single floats.
-template <class T, int KR, bool VB, bool VD>
+// NT: base and dst past the caches, where they are larger than the L2s.
+template <class T, int KR, bool VB, bool VD, bool NT>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
     __shared__ int tok[kTile];
     LoraTile t;
@@ -527,7 +527,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
         for (int j = 0; j < 4; ++j) {
             if (VD) {
                 const int m = mb + n * U < m1 ? mb + n * U : m0;
-                const f32x4 v = p.base ? *reinterpret_cast<const f32x4 *>(base[j] + m) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                const f32x4 v = p.base ? load4<NT>(base[j] + m) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int u = 0; u < U; ++u) y[j][u] = v[u];
             } else {
@@ -558,7 +558,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
         for (int j = 0; j < 4; ++j) {
             if (!live[j]) continue;
             if (VD) {
-                if (mb + n * U < m1) *reinterpret_cast<f32x4 *>(dst[j] + mb + n * U) = out[j];
+                if (mb + n * U < m1) store4<NT>(dst[j] + mb + n * U, out[j]);
             } else {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
@@ -714,17 +714,18 @@ template <class T>
 LoraFn tiled_of(int nr) {
     return nr == 1 ? lora_shrink_tiled_kernel<T, 1> : nr == 2 ? lora_shrink_tiled_kernel<T, 2> : lora_shrink_tiled_kernel<T, 4>;
 }
-template <class T, bool VB, bool VD>
+template <class T, bool VB, bool VD, bool NT>
 LoraFn expand_of(int kr) {
-    return kr <= 1   ? lora_expand_kernel<T, 1, VB, VD>
-           : kr <= 2 ? lora_expand_kernel<T, 2, VB, VD>
-           : kr <= 4 ? lora_expand_kernel<T, 4, VB, VD>
-                     : lora_expand_kernel<T, 8, VB, VD>;
+    return kr <= 1   ? lora_expand_kernel<T, 1, VB, VD, NT>
+           : kr <= 2 ? lora_expand_kernel<T, 2, VB, VD, NT>
+           : kr <= 4 ? lora_expand_kernel<T, 4, VB, VD, NT>
+                     : lora_expand_kernel<T, 8, VB, VD, NT>;
 }
 template <class T>
-LoraFn expand_of(int kr, bool vb, bool vd) {
-    return vb ? (vd ? expand_of<T, true, true>(kr) : expand_of<T, true, false>(kr))
-              : (vd ? expand_of<T, false, true>(kr) : expand_of<T, false, false>(kr));
+LoraFn expand_of(int kr, bool vb, bool vd, bool nt) {
+    if (nt && vd) return vb ? expand_of<T, true, true, true>(kr) : expand_of<T, false, true, true>(kr);
+    return vb ? (vd ? expand_of<T, true, true, false>(kr) : expand_of<T, true, false, false>(kr))
+              : (vd ? expand_of<T, false, true, false>(kr) : expand_of<T, false, false, false>(kr));
 }
 
 }  // namespace q4k
@@ -809,7 +810,8 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
         grid = grid_of(parts2);
         const int kr = (l.rank + 31) / 32;
         const bool vd = ne01 % 4 == 0 && aligned(dst, 16) && nb1 % 16 == 0 && aligned(src2, 16) && nb21 % 16 == 0;
-        st = launch(f16 ? expand_of<_Float16>(kr, vb, vd) : expand_of<__bf16>(kr, vb, vd), grid, 256, 0, stream, p);
+        const bool nt = ne11 * ne01 >= kStreamFloats;
+        st = launch(f16 ? expand_of<_Float16>(kr, vb, vd, nt) : expand_of<__bf16>(kr, vb, vd, nt), grid, 256, 0, stream, p);
     }
     return ws.end(st, stream);
 }
