@@ -437,9 +437,12 @@ def _stream_of(stream, device):
     return torch._C._cuda_getCurrentRawStream(device) if device >= 0 else None
 
 
-def _rows(t, dtype, n, m, device):
-    """Whether t is [n, m] of dtype on device (its number) with contiguous rows."""
-    return t.dtype is dtype and t.shape == (n, m) and t.get_device() == device and (m == 1 or t.stride(1) == 1)
+def _rows(t, dtype, shape, device, what):
+    """The row stride of t, checked to be of dtype and shape (n, m) on device (its number) with contiguous rows."""
+    strides = t.stride()
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or (strides[1] != 1 and shape[1] > 1):
+        raise ValueError(f"{what}: {dtype} {list(shape)} with contiguous rows on device {device} expected")
+    return strides[0]
 
 
 def _type16(t):
@@ -451,12 +454,12 @@ def _type16(t):
     raise ValueError(f"{t.dtype}: float16 or bfloat16 expected")
 
 
-def _vector(t, dtype, n, device, what):
-    """The address of a contiguous device vector of n values (n None: any number), or None for None."""
+def _vector(t, dtype, shape, device, what):
+    """The address of a contiguous device vector of shape (n,) (None: any n), or None for None."""
     if t is None:
         return None
-    if not (t.dtype is dtype and t.shape == (t.numel() if n is None else n,) and t.get_device() == device and t.is_contiguous()):
-        raise ValueError(f"{what}: contiguous {dtype} of {'any length' if n is None else n} on device {device} expected")
+    if t.dtype is not dtype or (t.dim() != 1 if shape is None else t.shape != shape) or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{what}: contiguous {dtype} {'vector' if shape is None else list(shape)} on device {device} expected")
     return t.data_ptr()
 
 
@@ -480,8 +483,8 @@ class LoraAdapters:
         self.tensors = (a, b, scale, ranks)
         self.K, self.M, self.rank, self.device, self.index = a.shape[2], b.shape[1], a.shape[1], a.device, a.get_device()
         self.desc = q4k_lora(_type16(a), self.rank, n, a.data_ptr(), a.stride(1) * 2, a.stride(0) * 2, b.data_ptr(),
-                             b.stride(1) * 2, b.stride(0) * 2, _vector(scale, torch.float32, n, a.get_device(), "scale"),
-                             _vector(ranks, torch.int32, n, a.get_device(), "ranks"))
+                             b.stride(1) * 2, b.stride(0) * 2, _vector(scale, torch.float32, (n,), a.get_device(), "scale"),
+                             _vector(ranks, torch.int32, (n,), a.get_device(), "ranks"))
         self._ref = ctypes.byref(self.desc)
 
 
@@ -499,18 +502,15 @@ def lora_add(adapters: LoraAdapters, x, ids, base=None, out=None, workspace=None
     in place."""
     import torch
     f32, dev, K, M, N = torch.float32, adapters.index, adapters.K, adapters.M, x.shape[0]
-    if not _rows(x, f32, N, K, dev):
-        raise ValueError(f"x: float32 [N, {K}] with contiguous rows on {adapters.device} expected")
+    shape = (N, M)
+    ldx = _rows(x, f32, (N, K), dev, "x")
     if out is None:
-        out = _new((N, M), f32, adapters.device, stream)
-    elif not _rows(out, f32, N, M, dev):
-        raise ValueError(f"out: float32 [{N}, {M}] with contiguous rows on {adapters.device} expected")
-    if base is not None and not _rows(base, f32, N, M, dev):
-        raise ValueError(f"base: float32 [{N}, {M}] with contiguous rows on {adapters.device} expected")
+        out = _new(shape, f32, adapters.device, stream)
+    ldo = _rows(out, f32, shape, dev, "out")
+    bp, ldb = (base.data_ptr(), _rows(base, f32, shape, dev, "base")) if base is not None else (None, 0)
     ws, ws_bytes = _ws(workspace)
-    st = lib().q4k_lora_add(adapters._ref, K, M, x.data_ptr(), N, x.stride(0) * 4, _vector(ids, torch.int32, N, dev, "ids"),
-                            base.data_ptr() if base is not None else None, base.stride(0) * 4 if base is not None else 0,
-                            out.data_ptr(), out.stride(0) * 4, ws, ws_bytes, _stream_of(stream, dev))
+    st = lib().q4k_lora_add(adapters._ref, K, M, x.data_ptr(), N, ldx * 4, _vector(ids, torch.int32, (N,), dev, "ids"), bp, ldb * 4,
+                            out.data_ptr(), ldo * 4, ws, ws_bytes, _stream_of(stream, dev))
     if st != Q4K_OK:
         raise Q4KError(st, "q4k_lora_add")
     return out
@@ -564,7 +564,7 @@ def _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, 
     lens = None
     if max_suffix:
         _need(suffix is not None and suffix_len is not None, "max_suffix without suffix and suffix_len")
-        lens = _vector(suffix_len, torch.int32, requests, dev, "suffix_len")
+        lens = _vector(suffix_len, torch.int32, (requests,), dev, "suffix_len")
         if suffix.tensors[2] is None:
             if requests:
                 suffix.desc.table_len = suffix.desc.n_pages // requests
@@ -623,12 +623,11 @@ def logits_adjust(logits, repeat=None, frequency=None, presence=None, history=No
     f32, i32, i64 = torch.float32, torch.int32, torch.int64
     N, V = logits.shape
     dev = logits.get_device()
-    if not _rows(logits, f32, N, V, dev):
-        raise ValueError("logits: float32 [N, V] with contiguous rows expected")
+    shape, per_row, starts = (N, V), (N,), (N + 1,)
+    ldx = _rows(logits, f32, shape, dev, "logits")
     if out is None:
-        out = _new((N, V), f32, logits.device, stream)
-    elif not _rows(out, f32, N, V, dev):
-        raise ValueError("out: float32 [N, V] with contiguous rows expected")
+        out = _new(shape, f32, logits.device, stream)
+    ldo = _rows(out, f32, shape, dev, "out")
     if (history is None) != (history_start is None):
         raise ValueError("history without history_start")
     if (bias_ids is None) != (bias is None) or (bias_ids is None) != (bias_start is None):
@@ -636,32 +635,32 @@ def logits_adjust(logits, repeat=None, frequency=None, presence=None, history=No
     h = hs = bi = bv = bs = m = mr = None
     nh = nb = masks = nbm = 0
     if history is not None:
-        h, hs, nh = _vector(history, i32, None, dev, "history"), _vector(history_start, i64, N + 1, dev, "history_start"), history.shape[0]
+        h, hs, nh = _vector(history, i32, None, dev, "history"), _vector(history_start, i64, starts, dev, "history_start"), history.shape[0]
         if nh == 0:
             h = hs = None
     if bias_ids is not None:
         nb = bias_ids.shape[0]
-        bi, bv = _vector(bias_ids, i32, None, dev, "bias_ids"), _vector(bias, f32, nb, dev, "bias")
-        bs = _vector(bias_start, i64, N + 1, dev, "bias_start")
+        bi, bv = _vector(bias_ids, i32, None, dev, "bias_ids"), _vector(bias, f32, (nb,), dev, "bias")
+        bs = _vector(bias_start, i64, starts, dev, "bias_start")
         if nb == 0:
             bi = bv = bs = None
     if mask is not None:
         masks, words = mask.shape
-        if words < -(-V // 32) or not _rows(mask, i32, masks, words, dev):
-            raise ValueError(f"mask: int32 [masks, {-(-V // 32)}] with contiguous rows expected")
+        ldm = _rows(mask, i32, (masks, words), dev, "mask")
+        if words < -(-V // 32):
+            raise ValueError(f"mask: int32 [masks, {-(-V // 32)}] expected")
         if mask_rows is None and masks < N:
             raise ValueError("mask: a row for each row of logits, or mask_rows, expected")
-        mr = _vector(mask_rows, i32, N, dev, "mask_rows")
+        mr = _vector(mask_rows, i32, per_row, dev, "mask_rows")
         if masks:
-            m, nbm = mask.data_ptr(), mask.stride(0) * 4
+            m, nbm = mask.data_ptr(), ldm * 4
         else:
             mr = None
     elif mask_rows is not None:
         raise ValueError("mask_rows without mask")
-    r = q4k_logits_rules(_vector(repeat, f32, N, dev, "repeat"), _vector(frequency, f32, N, dev, "frequency"),
-                         _vector(presence, f32, N, dev, "presence"), h, hs, nh, bi, bv, bs, nb, m, masks, nbm, mr)
-    st = lib().q4k_logits_adjust(logits.data_ptr(), V, N, logits.stride(0) * 4, ctypes.byref(r), out.data_ptr(),
-                                 out.stride(0) * 4, _stream_of(stream, dev))
+    r = q4k_logits_rules(_vector(repeat, f32, per_row, dev, "repeat"), _vector(frequency, f32, per_row, dev, "frequency"),
+                         _vector(presence, f32, per_row, dev, "presence"), h, hs, nh, bi, bv, bs, nb, m, masks, nbm, mr)
+    st = lib().q4k_logits_adjust(logits.data_ptr(), V, N, ldx * 4, ctypes.byref(r), out.data_ptr(), ldo * 4, _stream_of(stream, dev))
     if st != Q4K_OK:
         raise Q4KError(st, "q4k_logits_adjust")
     return out
