@@ -71,7 +71,7 @@ struct AttnParams {
     int pre_items, pre_tiles, pre_splits, pre_len;  // pre_len, suf_len: positions of a split
     int suf_items, suf_tiles, suf_splits, suf_len;
     // partial results of `slots` splits: (M, l) and the unscaled output of every row
-    int slots;
+    int slots, join_groups, join_rows;
     float2 *part_ml;
     float *part_o;
 };
@@ -466,12 +466,16 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
         const int pg = ok ? page : 0, slot = ok ? attn_slot(kv, t) : 0;
         if (lane < 32) rows[lane] = make_longlong2(pg * kv.k_page + slot * kv.k_token, pg * kv.v_page + slot * kv.v_token);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        // (K first: it is waited for first)
+        int64_t vo[NI];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const longlong2 at = rows[i * RI + sr];
             kf[i] = *reinterpret_cast<const u32x4 *>(kb + at.x);
-            vf[i] = *reinterpret_cast<const u32x4 *>(vb + at.y);
+            vo[i] = at.y;
         }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) vf[i] = *reinterpret_cast<const u32x4 *>(vb + vo[i]);
     };
     int t0 = s.beg + wave * 32;
     if (t0 < s.end) {
@@ -541,10 +545,10 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
             // (a position that is not there: values of zero, whatever was read)
             *reinterpret_cast<u32x4 *>(ldw + (r * CH + swz_v<D>(r, sc)) * 16) = (ok >> r) & 1 ? vf[i] : zero;
         }
-        if (t0 + 128 < s.end) {
-            load(t0 + 128);
-            page = attn_page(kv, s, t0 + 256 + (lane & 31));
-        }
+        // (No branch, or the waits for these loads would be for all of them: past the
+        // end no position is there.)
+        load(t0 + 128);
+        page = attn_page(kv, s, t0 + 256 + (lane & 31));
         if (careful || ok != 0xffffffffu) {
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
@@ -789,25 +793,20 @@ __global__ __launch_bounds__(256, CP::D == 256 ? 1 : 2) void prefix_attn_kernel(
     attn_item(CS(), p, p.suf, s, hk, tile, lds, flags, QT());
 }
 
-// Joins a row's partial results: one workgroup of 256 per row, groups of
-// head_dim / 4 lanes taking every 256 / (head_dim / 4)-th split with a running
-// reference, so that nothing waits for a first pass over the references.
+// Joins the partial results of p.join_rows rows per workgroup of 256: groups of
+// head_dim / 4 lanes, p.join_groups of them to a row, take every join_groups-th
+// split with a running reference, so that nothing waits for a first pass over the
+// references.
 template <class QT>
 __global__ __launch_bounds__(256) void prefix_attn_join_kernel(AttnParams p) {
     __shared__ f32x4 acc[256];
     __shared__ float2 mls[256];
-    const int head = blockIdx.x % p.n_head;
-    const int rt = blockIdx.x / p.n_head;
+    const int q4 = p.head_dim / 4;
+    const int grp = threadIdx.x / q4, d4 = threadIdx.x - grp * q4;
+    const int sub = grp % p.join_groups, which = grp / p.join_groups;
+    const int item = blockIdx.x * p.join_rows + which;
+    const int rt = item / p.n_head, head = item - rt * p.n_head;
     const int r = rt / p.n_q, t = rt - r * p.n_q;
-    int t0, t1;
-    attn_tokens(p, r, t0, t1);
-    const int tok = t0 + t;
-    if (tok >= t1) return;
-    const int len = attn_suffix(p, r);
-    const int n = p.pre_splits + (p.suf_len > 0 ? (len + p.suf_len - 1) / p.suf_len : 0);
-    const int64_t row = (int64_t)tok * p.n_head + head, step = (int64_t)p.n_tokens * p.n_head;
-    const int q4 = p.head_dim / 4, per = 256 / q4;
-    const int grp = threadIdx.x / q4, d4 = threadIdx.x % q4;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
     float l = 0.0f, M = -__builtin_inff();
     // A split in which the row sees nothing (l of 0) adds nothing, whatever its values.
@@ -820,31 +819,43 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(AttnParams p) {
         o = o * f + x * g;
         M = mn;
     };
-    if (grp < per) {
+    int tok = -1;
+    if (which < p.join_rows && r < p.n_requests) {
+        int t0, t1;
+        attn_tokens(p, r, t0, t1);
+        if (t0 + t < t1) tok = t0 + t;
+    }
+    const int64_t row = (int64_t)tok * p.n_head + head, step = (int64_t)p.n_tokens * p.n_head;
+    if (tok >= 0) {
+        const int len = attn_suffix(p, r);
+        const int n = p.pre_splits + (p.suf_len > 0 ? (len + p.suf_len - 1) / p.suf_len : 0);
         constexpr int U = 4;
-        for (int i0 = grp; i0 < n; i0 += per * U) {
+        for (int i0 = sub; i0 < n; i0 += p.join_groups * U) {
             float2 e[U];
             f32x4 x[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int64_t at = (i0 + u * per < n ? i0 + u * per : i0) * step + row;
+                const int64_t at = (i0 + u * p.join_groups < n ? i0 + u * p.join_groups : i0) * step + row;
                 e[u] = p.part_ml[at];
                 x[u] = *reinterpret_cast<const f32x4 *>(p.part_o + at * p.head_dim + d4 * 4);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (i0 + u * per < n) add(e[u], x[u]);
+                if (i0 + u * p.join_groups < n) add(e[u], x[u]);
         }
     }
-    acc[threadIdx.x] = o;
-    mls[threadIdx.x] = make_float2(M, l);
-    __syncthreads();
-    if (threadIdx.x >= q4) return;
-    for (int i = 1; i < per; ++i) add(mls[i * q4 + d4], acc[i * q4 + d4]);
+    if (p.join_groups > 1) {
+        acc[threadIdx.x] = o;
+        mls[threadIdx.x] = make_float2(M, l);
+        __syncthreads();
+        if (sub == 0)
+            for (int i = 1; i < p.join_groups; ++i) add(mls[threadIdx.x + i * q4], acc[threadIdx.x + i * q4]);
+    }
+    if (tok < 0 || sub != 0) return;
     QT *dst = reinterpret_cast<QT *>(p.dst + tok * p.dst_token + head * p.dst_head) + d4 * 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) dst[j] = (QT)(l == 0.0f ? 0.0f : o[j] / l);
-    if (threadIdx.x == 0 && p.lse) p.lse[row] = l == 0.0f ? -__builtin_inff() : (M + log2f(l)) * kLn2;
+    if (d4 == 0 && p.lse) p.lse[row] = l == 0.0f ? -__builtin_inff() : (M + log2f(l)) * kLn2;
 }
 
 // ---- which kernel runs a call ----

@@ -128,6 +128,12 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
         p.suf_items = (int)(per_suf * p.suf_splits);
     }
     p.slots = p.pre_splits + p.suf_splits;
+    // the join: four splits or so to a group of lanes, more rows to a workgroup where
+    // that leaves groups (4096 rows of 2 splits: 8.5 us with a workgroup each)
+    const int groups = 256 / (a.head_dim / 4);
+    p.join_groups = 1;
+    while (p.join_groups * 4 < p.slots && p.join_groups * 2 <= groups) p.join_groups *= 2;
+    p.join_rows = groups / p.join_groups;
     if (p.slots > 1) {
         const int64_t rows = a.n_tokens * a.n_head;
         if (rows > ((int64_t)1 << 50) / p.slots / (a.head_dim + 2)) return Q4K_EUNSUPPORTED;
@@ -178,7 +184,7 @@ int q4k_prefix_attn(const q4k_prefix_attn_args *args, void *workspace, size_t wo
     if (st == Q4K_OK && p.slots > 1) {
         const bool f32 = args->q_type == Q4K_GGML_TYPE_F32, f16 = args->kv_type == Q4K_GGML_TYPE_F16;
         Fn join = f32 ? prefix_attn_join_kernel<float> : f16 ? prefix_attn_join_kernel<_Float16> : prefix_attn_join_kernel<__bf16>;
-        st = launch(join, dim3((unsigned)(p.n_requests * p.n_q * p.n_head)), 256, 0, stream, p);
+        st = launch(join, dim3((unsigned)cdiv((int64_t)p.n_requests * p.n_q * p.n_head, p.join_rows)), 256, 0, stream, p);
     }
     return ws.end(st, stream);
 }
