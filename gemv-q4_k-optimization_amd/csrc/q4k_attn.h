@@ -712,7 +712,11 @@ __device__ __forceinline__ void attn_shared(const AttnParams &p, const AttnCache
             }
             V8 pf[RT][TERMS];
             attn_softmax<T, D, RT, TERMS>(w, sx, pf);
+            // (ahead of the other workgroup's softmax, which fills the gaps: 148 -> 142 us for
+            // 64 requests of 64 heads behind 32768 tokens)
+            __builtin_amdgcn_s_setprio(1);
             attn_values<T, D, RT, TERMS>(w, rd, pf, ldv, b);
+            __builtin_amdgcn_s_setprio(0);
         }
     }
     __syncthreads();
@@ -721,11 +725,26 @@ __device__ __forceinline__ void attn_shared(const AttnParams &p, const AttnCache
         while (t + TB <= least) t += TB;
         attn_rest<T>(p, kv, s, hk, w, t, s.end);
     }
+    // through LDS, so that rows are stored by lanes side by side
+    float *ol = reinterpret_cast<float *>(lds);        // [wave][16][D]
+    float2 *ml = reinterpret_cast<float2 *>(flags);    // [wave][16]
+    constexpr int Q4 = D / 4;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float sum = xor_sum(w.l[rt]), M = attn_ref(w.m[rt], w.c[rt]);
+        const float sum = xor_sum(w.l[rt]);
+        __syncthreads();
+        if (g == 0) ml[wave * 16 + n] = make_float2(attn_ref(w.m[rt], w.c[rt]), sum);
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) attn_emit<QT>(p, s, hk, row0 + rt * 16 + n, dt * 16 + g * 4, w.o[rt][dt], M, sum);
+        for (int dt = 0; dt < D / 16; ++dt)
+            *reinterpret_cast<f32x4 *>(ol + (wave * 16 + n) * D + (((dt * 4 + g) ^ n) * 4)) = w.o[rt][dt];
+        __syncthreads();
+#pragma unroll 2
+        for (int x = tid; x < 64 * Q4; x += 256) {
+            const int r = x / Q4, d4 = x % Q4;
+            const float2 e = ml[r];
+            attn_emit<QT>(p, s, hk, tile * C::ROWS + (r / 16 * RT + rt) * 16 + r % 16, d4 * 4,
+                          *reinterpret_cast<const f32x4 *>(ol + r * D + ((d4 ^ (r & 15)) * 4)), e.x, e.y);
+        }
     }
 }
 
