@@ -439,9 +439,50 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int r = adapter_rank(p, t.adapter);
-    const WaveSplit ws(t.count, wave);
+    const WaveSplit ws(t.count, wave);  // (waves without tokens take the first one along and store nothing)
     constexpr bool SH = KR <= 2;  // h's terms in LDS (24 KB at 64 ranks)
     __shared__ bf16x8 hs[3][SH ? kTile * KR * 4 : 1];
+    const float *base[4];
+    float *dst[4];
+    bool live[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        live[j] = ws.nt * 16 + g * 4 + j < t.count;
+        const int64_t token = tok[live[j] ? ws.nt * 16 + g * 4 + j : 0];
+        base[j] = reinterpret_cast<const float *>(p.base + token * p.nb_base);
+        dst[j] = reinterpret_cast<float *>(p.dst + token * p.nb_dst);
+    }
+    const char *b = p.b + (t.adapter < 0 ? 0 : t.adapter) * p.nb_b_adapter;
+    const int m0 = part * p.mchunk, m1 = m0 + p.mchunk < p.M ? m0 + p.mchunk : p.M;
+    constexpr int U = 4;  // tiles of 16 outputs in flight
+    const int step = ws.parts * 16 * U;
+    auto out_of = [&](int u) { return VD ? n * U + u : u * 16 + n; };
+    u32x4 bv[U][KR];
+    float y[4][U];
+    auto load = [&](int mb) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            // (clamped: loads without branches)
+            const int m = mb + out_of(u) < m1 ? mb + out_of(u) : m0;
+#pragma unroll
+            for (int kk = 0; kk < KR; ++kk) bv[u][kk] = load_w<VB>(b + m * p.nb_b, kk * 32 + g * 8, r);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (VD) {
+                const int m = mb + n * U < m1 ? mb + n * U : m0;
+                const f32x4 v = p.base ? load4<NT>(base[j] + m) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int u = 0; u < U; ++u) y[j][u] = v[u];
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u) y[j][u] = p.base ? base[j][mb + out_of(u) < m1 ? mb + out_of(u) : m0] : 0.0f;
+            }
+        }
+    };
+    int mb = m0 + ws.part * 16 * U;
+    if (mb < m1) load(mb);
+    // h, while the first outputs' values are on their way
     bf16x8 ht[KR][3];
     const float scale = p.scale && t.adapter >= 0 ? p.scale[t.adapter] : 1.0f;
     if (SH) {
@@ -498,46 +539,6 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
             bf16_terms(hv, ht[kk]);
         }
     }
-    const float *base[4];
-    float *dst[4];
-    bool live[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        live[j] = ws.nt * 16 + g * 4 + j < t.count;
-        const int64_t token = tok[live[j] ? ws.nt * 16 + g * 4 + j : 0];
-        base[j] = reinterpret_cast<const float *>(p.base + token * p.nb_base);
-        dst[j] = reinterpret_cast<float *>(p.dst + token * p.nb_dst);
-    }
-    const char *b = p.b + (t.adapter < 0 ? 0 : t.adapter) * p.nb_b_adapter;
-    const int m0 = part * p.mchunk, m1 = m0 + p.mchunk < p.M ? m0 + p.mchunk : p.M;
-    constexpr int U = 4;  // tiles of 16 outputs in flight
-    const int step = ws.parts * 16 * U;
-    auto out_of = [&](int u) { return VD ? n * U + u : u * 16 + n; };
-    u32x4 bv[U][KR];
-    float y[4][U];
-    auto load = [&](int mb) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            // (clamped: loads without branches)
-            const int m = mb + out_of(u) < m1 ? mb + out_of(u) : m0;
-#pragma unroll
-            for (int kk = 0; kk < KR; ++kk) bv[u][kk] = load_w<VB>(b + m * p.nb_b, kk * 32 + g * 8, r);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (VD) {
-                const int m = mb + n * U < m1 ? mb + n * U : m0;
-                const f32x4 v = p.base ? load4<NT>(base[j] + m) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int u = 0; u < U; ++u) y[j][u] = v[u];
-            } else {
-#pragma unroll
-                for (int u = 0; u < U; ++u) y[j][u] = p.base ? base[j][mb + out_of(u) < m1 ? mb + out_of(u) : m0] : 0.0f;
-            }
-        }
-    };
-    int mb = m0 + ws.part * 16 * U;
-    if (mb < m1) load(mb);
     for (; mb < m1; mb += step) {
         f32x4 out[4];
 #pragma unroll
@@ -688,8 +689,8 @@ static int lora_plan(const q4k_lora &l, int64_t K, int64_t M, int64_t N, LoraPla
     pl.kchunk = (int)(((K + ks - 1) / ks + 127) / 128 * 128);
     if (pl.kchunk < 128) pl.kchunk = 128;
     pl.ksplits = K > 0 ? (int)((K + pl.kchunk - 1) / pl.kchunk) : 0;
-    // four workgroups per CU, at least one row tile per wave
-    int64_t mc = (M * tiles / (4 * cus) + 63) / 64 * 64;
+    // two workgroups per CU, at least one row tile per wave
+    int64_t mc = (M * tiles / (2 * cus) + 63) / 64 * 64;
     mc = mc < 64 ? 64 : mc > 1024 ? 1024 : mc;
     pl.mchunk = (int)mc;
     if (N > ((int64_t)1 << 50) / (pl.rp * 4 * 8)) return Q4K_EUNSUPPORTED;
