@@ -913,13 +913,15 @@ void attn_kernel(AttnPlan &pl) {
 }
 template <class T, class QT, int TERMS, int D>
 void attn_kernel_of(AttnPlan &pl) {
+    // (three terms a query and up to 128 dimensions: streaming only)
+    constexpr int most = TERMS == 3 && D < 256 ? 1 : 2;
     switch (pl.pre_size * 4 + pl.suf_size) {
         case 0: return attn_kernel<T, QT, TERMS, D, 0, 0>(pl);
         case 4: return attn_kernel<T, QT, TERMS, D, 1, 0>(pl);
         case 5: return attn_kernel<T, QT, TERMS, D, 1, 1>(pl);
-        case 8: return attn_kernel<T, QT, TERMS, D, 2, 0>(pl);
-        case 9: return attn_kernel<T, QT, TERMS, D, 2, 1>(pl);
-        default: return attn_kernel<T, QT, TERMS, D, 2, 2>(pl);
+        case 8: return attn_kernel<T, QT, TERMS, D, most, 0>(pl);
+        case 9: return attn_kernel<T, QT, TERMS, D, most, 1>(pl);
+        default: return attn_kernel<T, QT, TERMS, D, most, most>(pl);
     }
 }
 template <class T, class QT, int TERMS>

@@ -90,7 +90,15 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
     if (a.n_tokens > INT32_MAX / p.group - 256) return Q4K_EUNSUPPORTED;
     const int64_t pre_rows = a.n_prefix > 0 ? a.n_tokens * p.group : 0, suf_rows = a.n_q * p.group;
     const int rows_of[3] = {16, pl.dim == 256 ? 16 : 32, pl.dim == 256 ? 64 : 128};
-    auto size_of = [&](int64_t rows) { return rows <= 16 ? 0 : rows <= 96 ? 1 : 2; };
+    // Streaming to this many rows of a KV head, us streaming / sharing: 128 dimensions
+    // in 16 bits 96 (16 requests of 4 rows 24.6 / -, 128 rows 30.5 / 29.2, 192 rows
+    // 47.1 / 44.5); F32 queries on F16 and 64 dimensions 256 (128 rows 32.7 / 34.4, 160
+    // rows of 64 dimensions 25.5 / 33.1; 512 rows 73.3 / 69.5 and 50.1 / 47.6); 256
+    // dimensions 96 (120 rows 64.3 / 47.2); F32 queries on BF16, whose three terms a
+    // query leave sharing waves no registers, any (256 rows 74 / 143, 1024 rows 131 / 237).
+    const int terms = a.q_type != Q4K_GGML_TYPE_F32 ? 1 : a.kv_type == Q4K_GGML_TYPE_F16 ? 2 : 3;
+    const int64_t most = pl.dim == 256 ? 96 : terms == 3 ? INT32_MAX : terms == 2 || pl.dim == 64 ? 256 : 96;
+    auto size_of = [&](int64_t rows) { return rows <= 16 ? 0 : rows <= most ? 1 : 2; };
     pl.suf_size = size_of(suf_rows);
     pl.pre_size = a.n_prefix > 0 ? size_of(pre_rows) : pl.suf_size;
     if (pl.suf_size > pl.pre_size) pl.suf_size = pl.pre_size;  // (with q_start n_q may exceed the tokens there are)
