@@ -629,6 +629,7 @@ __device__ __forceinline__ void attn_shared(const AttnParams &p, const AttnCache
     const int sc = tid % CH, sr = tid / CH;
     const bool cok = sc * 8 < p.head_dim;
     const char *kb = kv.k + hk * kv.k_head + (cok ? sc * 16 : 0), *vb = kv.v + hk * kv.v_head + (cok ? sc * 16 : 0);
+    const int64_t one = (int64_t)((int)s.table_row * kv.table_len) * kv.k_page, one_v = (int64_t)((int)s.table_row * kv.table_len) * kv.v_page;
     u32x4 kr[NP], vr[NP];
     int page[NP];        // of the tile that is loaded next
     uint32_t okbits = 0; // which of this thread's positions have a page
@@ -637,6 +638,17 @@ __device__ __forceinline__ void attn_shared(const AttnParams &p, const AttnCache
         for (int i = 0; i < NP; ++i) page[i] = attn_page(kv, s, t0 + sr + RP * i);
     };
     auto load = [&](int t0) {
+        if (kv.one_page && t0 + TB <= s.end) {
+            // one stretch of memory: a row's place is the first one's and a constant
+            const char *k0 = kb + one + (int64_t)(t0 + sr) * kv.k_token, *v0 = vb + one_v + (int64_t)(t0 + sr) * kv.v_token;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                kr[i] = *reinterpret_cast<const u32x4 *>(k0 + i * (RP * kv.k_token));
+                vr[i] = *reinterpret_cast<const u32x4 *>(v0 + i * (RP * kv.v_token));
+            }
+            okbits = (1u << NP) - 1;
+            return;
+        }
         okbits = 0;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
