@@ -82,6 +82,33 @@ def test_attention_sizes(Q, gpu, qt, kv, B, nq, H, hk, D, prefix, suffix, page):
     Case(gpu, B, nq, H, hk, D, prefix, suffix, page, qt, kv, seed=B + D).check(Q)
 
 
+@pytest.mark.parametrize("qt,kv", TYPES)
+@pytest.mark.parametrize("B,nq,H,hk,D,prefix,suffix,page", [
+    (2, 150, 2, 1, 128, 100, 260, 16), (2, 130, 4, 1, 64, 70, 200, 40), (1, 60, 4, 2, 256, 65, 90, 16), (3, 100, 3, 1, 96, 0, 130, 16)])
+def test_attention_many_queries_a_request(Q, gpu, qt, kv, B, nq, H, hk, D, prefix, suffix, page):
+    """Rows enough that waves share the suffix too, whose bound is the queries' own."""
+    c = Case(gpu, B, nq, H, hk, D, prefix, suffix, page, qt, kv, seed=D, lens=[suffix, nq + 3, nq // 2][:B])
+    want = c.run(Q)
+    c.check(Q)
+    # what only the last query sees leaves the others alone
+    k, v, t = c.suffix
+    for r, length in enumerate(c.lens):
+        j = length - 1
+        v[int(t[r, j // page]), j % page, :, ::2] = float("-inf")
+        k[int(t[r, j // page]), j % page] = float("nan")
+    got = c.run(Q)
+    for r in range(B):
+        lo, hi = r * nq, (r + 1) * nq - 1
+        assert torch.equal(got[0][lo:hi], want[0][lo:hi]) and torch.equal(got[1][lo:hi], want[1][lo:hi])
+        assert not torch.isfinite(got[0][hi].float()).any()
+    # an infinite value that several queries see, behind the bound of the others
+    c = Case(gpu, B, nq, H, hk, D, prefix, suffix, page, qt, kv, seed=D, lens=[suffix, nq + 3, nq // 2][:B])
+    k, v, t = c.suffix
+    j = c.lens[0] - 5
+    v[int(t[0, j // page]), j % page, :, 1] = float("inf")
+    c.check(Q)
+
+
 @pytest.mark.parametrize("qt,kv", TYPES[:1] + TYPES[3:])
 @pytest.mark.parametrize("prefix", [0, 1, 15, 16, 17, 63, 64, 65, 127, 128, 129])
 def test_attention_lengths_around_a_tile(Q, gpu, qt, kv, prefix):
