@@ -273,10 +273,10 @@ __device__ __forceinline__ float attn_queries(const AttnParams &p, const AttnSpa
 // The page of position t of the span (clamped to its last, so that nothing past a
 // table is read), and the position in it.
 __device__ __forceinline__ int attn_page(const AttnCache &kv, const AttnSpan &s, int t) {
-    const int first = (int)s.table_row * kv.table_len;
-    if (kv.one_page) return first;
+    // (without a table the host has checked that a request's table_len pages are there)
+    if (kv.one_page) return (int)(s.table_row * kv.table_len);
     const int e = (int)fastdiv((uint32_t)(t < s.end ? t : s.end - 1), kv.page);
-    return kv.table ? kv.table[s.table_row * kv.table_stride + e] : first + e;
+    return kv.table ? kv.table[s.table_row * kv.table_stride + e] : (int)(s.table_row * kv.table_len) + e;
 }
 __device__ __forceinline__ int attn_slot(const AttnCache &kv, int t) {
     return kv.one_page ? t : t - (int)(fastdiv((uint32_t)t, kv.page) * kv.page.d);
@@ -629,7 +629,7 @@ __device__ __forceinline__ void attn_shared(const AttnParams &p, const AttnCache
     const int sc = tid % CH, sr = tid / CH;
     const bool cok = sc * 8 < p.head_dim;
     const char *kb = kv.k + hk * kv.k_head + (cok ? sc * 16 : 0), *vb = kv.v + hk * kv.v_head + (cok ? sc * 16 : 0);
-    const int64_t one = (int64_t)((int)s.table_row * kv.table_len) * kv.k_page, one_v = (int64_t)((int)s.table_row * kv.table_len) * kv.v_page;
+    const int64_t first = kv.one_page ? s.table_row * kv.table_len : 0, one = first * kv.k_page, one_v = first * kv.v_page;
     u32x4 kr[NP], vr[NP];
     int page[NP];        // of the tile that is loaded next
     uint32_t okbits = 0; // which of this thread's positions have a page

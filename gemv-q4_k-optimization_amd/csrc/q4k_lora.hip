@@ -46,6 +46,7 @@ struct LoraParams {
     const int32_t *n_tiles;
     int n_adapters, K, M, N, rank, rp;
     int ksplits, kchunk, mchunk;
+    int enumerate;        // not grouped: blockIdx.y is a tile, not a token
     int copy;             // tokens without an adapter are copied (dst is not base)
 };
 
@@ -60,8 +61,10 @@ struct LoraTile {
 // after part of tiles that follow each other, so that an adapter's tiles read the
 // same piece of it through one L2 (4096 tokens of 16 adapters of rank 64 and K
 // 14336: 147 MB that would come from beyond it).
-// Else blockIdx.y is a token of the slice blockIdx.z, and the workgroup of the
-// first, 65th, ... token of an adapter takes the 64 from there.
+// Else, in the slice blockIdx.z of 512 tokens, blockIdx.y is a token, and the
+// workgroup of the first, 65th, ... token of an adapter takes the 64 from there;
+// or, where tiles are few against tokens, blockIdx.y is a tile that the workgroup
+// counts its way to.
 __device__ __forceinline__ bool lora_tile(const LoraParams &p, int parts, int *tok, LoraTile &t, int &x) {
     const int lane = threadIdx.x & 63;
     if (p.tiles) {
@@ -79,19 +82,62 @@ __device__ __forceinline__ bool lora_tile(const LoraParams &p, int parts, int *t
     }
     x = blockIdx.x;
     const int base = blockIdx.z * kSlice, n = p.N - base < kSlice ? p.N - base : kSlice;
-    const int me = blockIdx.y;
-    if (me >= n) return false;
+    int me = blockIdx.y;
+    if (!p.enumerate && me >= n) return false;
     auto key_of = [&](int i) {
         const int id = p.ids[base + i];
         return id >= 0 && id < p.n_adapters ? id : -1;
     };
-    const int key = __builtin_amdgcn_readfirstlane(key_of(me));
-    t.adapter = key;
     uint64_t same[kSliceBallots];
     int before = 0, all = 0, keys[kSliceBallots];
     // (all on their way at once; past the end the last one again)
 #pragma unroll
     for (int i = 0; i < kSliceBallots; ++i) keys[i] = key_of(i * 64 + lane < n ? i * 64 + lane : n - 1);
+    int key;
+    if (p.enumerate) {
+        // blockIdx.y is the number of a tile: adapters in the order of their first tokens
+        uint64_t rest[kSliceBallots];
+#pragma unroll
+        for (int i = 0; i < kSliceBallots; ++i) rest[i] = __ballot(i * 64 + lane < n);
+        for (;;) {
+            bool found = false;
+            key = 0;
+#pragma unroll
+            for (int i = 0; i < kSliceBallots; ++i)
+                if (!found && rest[i]) {
+                    key = __builtin_amdgcn_readlane(keys[i], (int)__builtin_ctzll(rest[i]));
+                    found = true;
+                }
+            if (!found) return false;
+            all = 0;
+#pragma unroll
+            for (int i = 0; i < kSliceBallots; ++i) {
+                same[i] = rest[i] & __ballot(keys[i] == key);
+                all += __popcll(same[i]);
+                rest[i] &= ~same[i];
+            }
+            const int tiles = (all + kTile - 1) / kTile;
+            if (me < tiles) break;
+            me -= tiles;
+        }
+        t.adapter = key;
+        before = me * kTile;
+        t.count = all - before < kTile ? all - before : kTile;
+        if (threadIdx.x < 64) {
+            int seen = 0;
+            tok[lane] = base;
+#pragma unroll
+            for (int i = 0; i < kSliceBallots; ++i) {
+                const int pos = seen + __popcll(same[i] & ((1ull << lane) - 1)) - before;
+                if ((same[i] >> lane & 1) && pos >= 0 && pos < kTile) tok[pos] = base + i * 64 + lane;
+                seen += __popcll(same[i]);
+            }
+        }
+        __syncthreads();
+        return true;
+    }
+    key = __builtin_amdgcn_readfirstlane(key_of(me));
+    t.adapter = key;
 #pragma unroll
     for (int i = 0; i < kSliceBallots; ++i) {
         same[i] = __ballot(i * 64 + lane < n && keys[i] == key);
@@ -171,13 +217,24 @@ struct Weights<_Float16> {
     }
 };
 
-// Values [k, k + 8) of a row of n 16-bit values, zeros past its end
+// Values [k, k + 8) of a row of n 16-bit values, zeros past its end.  VEC: n is a
+// multiple of 8 and the row 16-byte aligned; else one 16-byte load of any alignment
+// that ends with the row (the hardware takes them), moved into place, or single
+// values in rows of fewer than eight.
 template <bool VEC>
 __device__ __forceinline__ u32x4 load_w(const char *row, int k, int n) {
     u32x4 v = {0, 0, 0, 0};
     if (VEC) {
         if (k < n) v = *reinterpret_cast<const u32x4 *>(row + 2 * k);
         return v;
+    }
+    if (n >= 8) {
+        const int from = k + 8 <= n ? k : n - 8, shift = 16 * (k - from);  // shift >= 128: past the end
+        __builtin_memcpy(&v, row + 2 * from, 16);
+        const uint64_t w[2] = {v[0] | (uint64_t)v[1] << 32, v[2] | (uint64_t)v[3] << 32};
+        const uint64_t lo = shift < 64 ? w[0] >> shift | (shift ? w[1] << (64 - shift) : 0) : shift < 128 ? w[1] >> (shift - 64) : 0;
+        const uint64_t hi = shift < 64 ? w[1] >> shift : 0;
+        return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -188,11 +245,11 @@ __device__ __forceinline__ u32x4 load_w(const char *row, int k, int n) {
 }
 template <bool VEC>
 __device__ __forceinline__ void load_x(const float *row, int k, int n, float (&x)[8]) {
-    if (VEC) {
+    if (VEC || k + 8 <= n) {
         f32x4 v[2] = {};
-        if (k < n) {
-            v[0] = *reinterpret_cast<const f32x4 *>(row + k);
-            v[1] = *reinterpret_cast<const f32x4 *>(row + k + 4);
+        if (!VEC || k < n) {
+            v[0] = *reinterpret_cast<const f32x4_any *>(row + k);
+            v[1] = *reinterpret_cast<const f32x4_any *>(row + k + 4);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = v[j >> 2][j & 3];
@@ -424,13 +481,12 @@ __global__ __launch_bounds__(256) void lora_shrink_tiled_kernel(LoraParams p) {
         if (j0 + i * 16 < p.rp) *reinterpret_cast<f32x4 *>(h + i * 16) = acc[i];
 }
 
-// KR: steps of 32 ranks; VB: rows of b in 16-byte loads; VD: base and dst in
-// 16-byte accesses.  The tokens are the A operand here: a lane of a result has one
-// output of four tokens.  Of the four tiles that are in flight, lane n's outputs
-// are 4 n .. 4 n + 3 (VD), so that 16 lanes store 256 bytes of a token side by
-// side; rows that are not aligned take outputs n of each tile and single floats.
+// KR: steps of 32 ranks; VB: rows of b in aligned 16-byte loads.  The tokens are
+// the A operand here: a lane of a result has one output of four tokens.  Of the
+// four tiles that are in flight, lane n's outputs are 4 n .. 4 n + 3, so that 16
+// lanes store 256 bytes of a token side by side.
 // NT: base and dst past the caches, where they are larger than the L2s.
-template <class T, int KR, bool VB, bool VD, bool NT>
+template <class T, int KR, bool VB, bool NT>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
     __shared__ int tok[kTile];
     LoraTile t;
@@ -456,28 +512,27 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
     const int m0 = part * p.mchunk, m1 = m0 + p.mchunk < p.M ? m0 + p.mchunk : p.M;
     constexpr int U = 4;  // tiles of 16 outputs in flight
     const int step = ws.parts * 16 * U;
-    auto out_of = [&](int u) { return VD ? n * U + u : u * 16 + n; };
     u32x4 bv[U][KR];
-    float y[4][U];
+    f32x4 y[4];
     auto load = [&](int mb) {
+        // (rows of b clamped; only whole fours of a row in one access)
+        const int m = mb + n * U;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            // (clamped: loads without branches)
-            const int m = mb + out_of(u) < m1 ? mb + out_of(u) : m0;
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int kk = 0; kk < KR; ++kk) bv[u][kk] = load_w<VB>(b + m * p.nb_b, kk * 32 + g * 8, r);
-        }
+            for (int kk = 0; kk < KR; ++kk) bv[u][kk] = load_w<VB>(b + (m + u < m1 ? m + u : m0) * p.nb_b, kk * 32 + g * 8, r);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (VD) {
-                const int m = mb + n * U < m1 ? mb + n * U : m0;
-                const f32x4 v = p.base ? load4<NT>(base[j] + m) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < 4; ++j) y[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (!p.base) return;
+        if (m + U <= m1) {
 #pragma unroll
-                for (int u = 0; u < U; ++u) y[j][u] = v[u];
-            } else {
+            for (int j = 0; j < 4; ++j) y[j] = load4<NT>(base[j] + m);
+        } else {
 #pragma unroll
-                for (int u = 0; u < U; ++u) y[j][u] = p.base ? base[j][mb + out_of(u) < m1 ? mb + out_of(u) : m0] : 0.0f;
-            }
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (m + u < m1) y[j][u] = base[j][m + u];
         }
     };
     int mb = m0 + ws.part * 16 * U;
@@ -555,15 +610,16 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
             for (int j = 0; j < 4; ++j) out[j][u] = y[j][u] + acc[j];
         }
         if (mb + step < m1) load(mb + step);
+        const int m = mb + n * U;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (!live[j]) continue;
-            if (VD) {
-                if (mb + n * U < m1) store4<NT>(dst[j] + mb + n * U, out[j]);
+            if (m + U <= m1) {
+                store4<NT>(dst[j] + m, out[j]);
             } else {
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (mb + out_of(u) < m1) dst[j][mb + out_of(u)] = out[j][u];
+                    if (m + u < m1) dst[j][m + u] = out[j][u];
             }
         }
     }
@@ -662,6 +718,8 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p) {
 
 struct LoraPlan {
     bool grouped, tiled;
+    int rows;           // not grouped: workgroups in y, one per tile if enumerate
+    bool enumerate;
     int max_tiles;      // tiles there can be, grouped
     int rp, nr, ksplits, kchunk, mchunk;
     size_t h_bytes, bytes;
@@ -676,6 +734,11 @@ static int lora_plan(const q4k_lora &l, int64_t K, int64_t M, int64_t N, LoraPla
     const int64_t tiles = N / kTile + kinds;  // at most
     pl.max_tiles = (int)tiles;
     pl.tiled = N >= 16 * kinds;
+    // Counting to a tile takes about 0.1 us for each adapter before it, a workgroup
+    // for a token that leads no tile 1.5 us of its place.
+    const int64_t in_slice = N < kSlice ? N : kSlice, slice_tiles = in_slice / kTile + (kinds < in_slice ? kinds : in_slice);
+    pl.enumerate = slice_tiles * 16 <= in_slice;
+    pl.rows = (int)(pl.enumerate ? slice_tiles : in_slice);
     pl.rp = (l.rank + 15) / 16 * 16;
     pl.nr = pl.rp / 16 < kRankTiles ? pl.rp / 16 : kRankTiles;
     if (pl.nr == 3) pl.nr = 4;
@@ -715,18 +778,17 @@ template <class T>
 LoraFn tiled_of(int nr) {
     return nr == 1 ? lora_shrink_tiled_kernel<T, 1> : nr == 2 ? lora_shrink_tiled_kernel<T, 2> : lora_shrink_tiled_kernel<T, 4>;
 }
-template <class T, bool VB, bool VD, bool NT>
+template <class T, bool VB, bool NT>
 LoraFn expand_of(int kr) {
-    return kr <= 1   ? lora_expand_kernel<T, 1, VB, VD, NT>
-           : kr <= 2 ? lora_expand_kernel<T, 2, VB, VD, NT>
-           : kr <= 4 ? lora_expand_kernel<T, 4, VB, VD, NT>
-                     : lora_expand_kernel<T, 8, VB, VD, NT>;
+    return kr <= 1   ? lora_expand_kernel<T, 1, VB, NT>
+           : kr <= 2 ? lora_expand_kernel<T, 2, VB, NT>
+           : kr <= 4 ? lora_expand_kernel<T, 4, VB, NT>
+                     : lora_expand_kernel<T, 8, VB, NT>;
 }
 template <class T>
-LoraFn expand_of(int kr, bool vb, bool vd, bool nt) {
-    if (nt && vd) return vb ? expand_of<T, true, true, true>(kr) : expand_of<T, false, true, true>(kr);
-    return vb ? (vd ? expand_of<T, true, true, false>(kr) : expand_of<T, true, false, false>(kr))
-              : (vd ? expand_of<T, false, true, false>(kr) : expand_of<T, false, false, false>(kr));
+LoraFn expand_of(int kr, bool vb, bool nt) {
+    return vb ? (nt ? expand_of<T, true, true>(kr) : expand_of<T, true, false>(kr))
+              : (nt ? expand_of<T, false, true>(kr) : expand_of<T, false, false>(kr));
 }
 
 }  // namespace q4k
@@ -781,10 +843,11 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
     p.ids = ids; p.h = (float *)ws.ptr; p.K = (int)ne00; p.M = (int)ne01; p.N = (int)ne11;
     p.rank = l.rank; p.rp = pl.rp; p.ksplits = pl.ksplits; p.kchunk = pl.kchunk; p.mchunk = pl.mchunk;
     p.copy = src2 != dst;
+    p.enumerate = pl.enumerate;
     dim3 grid;
     auto grid_of = [&](int64_t parts) {
         return pl.grouped ? dim3((unsigned)(parts * pl.max_tiles))
-                          : dim3((unsigned)parts, (unsigned)(ne11 < kSlice ? ne11 : kSlice), (unsigned)slices);
+                          : dim3((unsigned)parts, (unsigned)pl.rows, (unsigned)slices);
     };
     if (pl.grouped) {
         char *w = (char *)ws.ptr + pl.h_bytes;
@@ -810,9 +873,10 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
         const bool vb = l.rank % 8 == 0 && aligned(l.b, 16) && (l.nb_b | l.nb_b_adapter) % 16 == 0;
         grid = grid_of(parts2);
         const int kr = (l.rank + 31) / 32;
-        const bool vd = ne01 % 4 == 0 && aligned(dst, 16) && nb1 % 16 == 0 && aligned(src2, 16) && nb21 % 16 == 0;
-        const bool nt = ne11 * ne01 >= kStreamFloats;
-        st = launch(f16 ? expand_of<_Float16>(kr, vb, vd, nt) : expand_of<__bf16>(kr, vb, vd, nt), grid, 256, 0, stream, p);
+        // (rows that begin inside a cache line would write their ends past the caches in
+        // parts: 4089 tokens of 13249 outputs 219 us against 187)
+        const bool nt = ne11 * ne01 >= kStreamFloats && aligned(dst, 64) && nb1 % 64 == 0;
+        st = launch(f16 ? expand_of<_Float16>(kr, vb, nt) : expand_of<__bf16>(kr, vb, nt), grid, 256, 0, stream, p);
     }
     return ws.end(st, stream);
 }

@@ -47,7 +47,7 @@ static int attn_check(const q4k_prefix_attn_args *args, bool &empty) {
         return Q4K_EINVAL;
     if (a.head_dim % 8 != 0 || a.head_dim > Q4K_ATTN_MAX_HEAD_DIM) return Q4K_EUNSUPPORTED;
     if ((a.n_prefix > 0 && !pages_vec(*a.prefix)) || (a.max_suffix > 0 && !pages_vec(*a.suffix))) return Q4K_EUNSUPPORTED;
-    if (a.n_requests * a.n_q > INT32_MAX || a.n_head > 65535) return Q4K_EUNSUPPORTED;
+    if (a.n_requests * a.n_q > INT32_MAX || a.n_prefix > (1 << 30) || a.max_suffix > (1 << 30)) return Q4K_EUNSUPPORTED;
     return Q4K_OK;
 }
 

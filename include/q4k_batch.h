@@ -63,9 +63,10 @@ size_t q4k_lora_workspace_bytes(const q4k_lora *lora, int64_t ne00, int64_t ne01
  *   ids:  ne11 adapter numbers on the device; a token whose number is outside
  *         [0, n_adapters) takes no adapter: dst[n] = src2[n]
  *   dst:  ne11 tokens of ne01 floats, stride nb1
- * Any ne00, ne01, ne11 and rank; rows of a and b that are 16-byte aligned run
- * faster.  Sums are F32; the F32 activations enter the matrix cores as sums of
- * BF16 values that hold 16 bits or more of them.  ne00 == 0 adds nothing. */
+ * Any ne00, ne01, ne11 and rank; rows of a and b that are 16-byte aligned and
+ * rows of dst that are 64-byte aligned run faster.  Sums are F32; the F32
+ * activations and a's products enter the matrix cores as sums of three BF16
+ * values, which hold F32's 24 bits.  ne00 == 0 adds nothing. */
 int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *src1, int64_t ne11,
                  int64_t nb11, const int32_t *ids, const float *src2, int64_t nb21, float *dst,
                  int64_t nb1, void *workspace, size_t workspace_bytes, void *stream);
@@ -126,7 +127,7 @@ size_t q4k_prefix_attn_workspace_bytes(const q4k_prefix_attn_args *args);
  * maximum and sum and the output sum are F32.  With q_type F32 the queries and
  * probabilities enter the matrix cores as sums of two (F16) or three (BF16)
  * values of kv_type, with q_type kv_type as one rounded value.  Tokens of no
- * request are left as they are. */
+ * request are left as they are.  Up to 2^30 positions a part. */
 int q4k_prefix_attn(const q4k_prefix_attn_args *args, void *workspace, size_t workspace_bytes,
                     void *stream);
 
@@ -158,7 +159,7 @@ typedef struct q4k_logits_rules {
     const int32_t *mask_rows;
 } q4k_logits_rules;
 
-/* dst = src (F32, n_rows rows of n_vocab logits) with, per row and in this
+/* dst = src (F32, n_rows rows of up to 2^30 n_vocab logits) with, per row and in this
  * order: the repetition factor, frequency and presence penalties, biases, the
  * mask.  Token ids outside [0, n_vocab) are ignored.  dst may be src (same
  * stride), else must not overlap it.  Takes no workspace. */
