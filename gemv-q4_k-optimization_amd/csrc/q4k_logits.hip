@@ -5,7 +5,12 @@
 //   l = c > 0 ? (l > 0 ? l / repeat : l * repeat) : l
 //   l = l - c * frequency - (c > 0 ? presence : 0)
 //   l = l + bias (the last entry of the token), -inf where the mask bit is 0
-// One pass over the logits: 8 bytes a logit, the bound.
+// One pass over the logits: 8 bytes a logit and the history once per workgroup.
+// 256 rows of 151936 logits with histories of 2048 to 8192 tokens take 73 us (4.3
+// TB/s of what has to move; 61 us without histories, 5.2 TB/s; a copy reaches 5.4):
+// memory bound, and with long histories bound by the counting in the slices of
+// frequent tokens too.  Few rows are bound by the launch and three memory round
+// trips (starts, histories, logits): 5.0 us for 32768 logits, 6.6 for 8 x 128256.
 #include <hip/hip_runtime.h>
 
 #include "../../include/q4k_batch.h"

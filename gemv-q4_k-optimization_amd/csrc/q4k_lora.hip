@@ -14,6 +14,13 @@
 // products of all but the smallest terms are added: three matrix instructions for
 // BF16 adapters, five for F16.  BF16 has F32's exponents, so nothing overflows.
 //
+// Memory bound: 4096 tokens of 16 adapters of rank 64, K 14336, 4096 outputs take
+// 103 us (group 6, shrink 62, expand 44 one by one) where their 407 MB take 75 at a
+// copy's rate.  The shrink reads its 235 MB at 3.8 TB/s; a plain read of the same
+// tiles takes 40 us, the rest is its conversions and barriers at seven waves a CU.
+// A few tokens are bound by two launches and their chains of round trips: 1 token,
+// 1024 x 4096, rank 8: 5.3 + 5.3 us; 8 tokens, 14336 x 4096, rank 16: 5.5 + 6.2.
+//
 // Each column of a product depends on its token alone, so a token's result does
 // not depend on which tokens share its tile, nor on the order in which they
 // were put there.
