@@ -425,13 +425,16 @@ __device__ __forceinline__ void attn_emit(const AttnParams &p, const AttnSpan &s
 // waves never wait for each other before the end.  Memory bound: each wave keeps
 // the next 32 positions' K and V on their way.  24 rows over 131072 positions of 8
 // heads of 128 BF16 dimensions (537 MB): 113 us, 4.8 TB/s with F32 queries as three
-// terms; 64 rows over 8192 positions: 18 us, bound by the four steps' round trips.
+// terms.  64 F16 rows over 8192 positions and 16 x 256 of their own, with the join:
+// 22.2 us, of which about 5 read memory: bound by the four steps' round trips.
 template <class T, int D_, int RT_, int TERMS>
 struct StreamCfg {
     using Elem = T;
     static constexpr int D = D_, RT = RT_, ROWS = 16 * RT_;
-    static constexpr bool QLDS = D_ / 32 * RT_ * TERMS > 8;  // queries in LDS: over 32 registers of them
-    static constexpr int VBYTES = 4 * 32 * D * 2;             // (and a row tile's outputs of four waves at the end)
+    // Queries of 32 registers and more stay in LDS: held in registers they spill
+    // beside two steps' K and V (64 F16 rows over 65536 positions: 76 / 65 us).
+    static constexpr bool QLDS = D_ / 32 * RT_ * TERMS >= 8;
+    static constexpr int VBYTES = 4 * 32 * D * 2;  // (and a row tile's outputs of four waves at the end)
     static constexpr int QBYTES = QLDS ? RT * TERMS * (D / 32) * 1024 : 0;  // (else they pass through V's place)
     static constexpr int LDS = VBYTES * 2 > 64 * D * 4 ? VBYTES + QBYTES : 64 * D * 4 + QBYTES;
 };
@@ -461,28 +464,25 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
     u32x4 kf[NI], vf[NI];
     uint32_t there = 0;  // bit r: position r of the step that was loaded has a page
     int page;
-    auto load = [&](int t0) {
+    auto load_k = [&](int t0) {
         const int t = t0 + (lane & 31);
         const bool ok = t < s.end && (uint32_t)page < (uint32_t)kv.n_pages;
         there = (uint32_t)__ballot(ok);
         const int pg = ok ? page : 0, slot = ok ? attn_slot(kv, t) : 0;
         if (lane < 32) rows[lane] = make_longlong2(pg * kv.k_page + slot * kv.k_token, pg * kv.v_page + slot * kv.v_token);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        // (K first: it is waited for first)
-        int64_t vo[NI];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const longlong2 at = rows[i * RI + sr];
-            kf[i] = *reinterpret_cast<const u32x4 *>(kb + at.x);
-            vo[i] = at.y;
-        }
+        for (int i = 0; i < NI; ++i) kf[i] = *reinterpret_cast<const u32x4 *>(kb + rows[i * RI + sr].x);
+    };
+    auto load_v = [&]() {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) vf[i] = *reinterpret_cast<const u32x4 *>(vb + vo[i]);
+        for (int i = 0; i < NI; ++i) vf[i] = *reinterpret_cast<const u32x4 *>(vb + rows[i * RI + sr].y);
     };
     int t0 = s.beg + wave * 32;
     if (t0 < s.end) {
         page = attn_page(kv, s, t0 + (lane & 31));
-        load(t0);
+        load_k(t0);
+        load_v();
         page = attn_page(kv, s, t0 + 128 + (lane & 31));
     }
     // the queries, one row tile per wave, while the first positions are on their way
@@ -514,6 +514,11 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
             const int r = i * RI + sr;
             *reinterpret_cast<u32x4 *>(ldw + (r * CH + swz_k<D>(r, sc)) * 16) = cok ? kf[i] : zero;
         }
+        // The next step's K leaves before this one's scores (own positions only: 43.5 us
+        // after them, 42.6 so).  No branch, or the waits for these loads would be for
+        // all of them: past the end no position is there.
+        load_k(t0 + 128);
+        page = attn_page(kv, s, t0 + 256 + (lane & 31));
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // rows are written before lanes read each other's
         f32x4 sx[RT][2];
 #pragma unroll
@@ -547,10 +552,7 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
             // (a position that is not there: values of zero, whatever was read)
             *reinterpret_cast<u32x4 *>(ldw + (r * CH + swz_v<D>(r, sc)) * 16) = (ok >> r) & 1 ? vf[i] : zero;
         }
-        // (No branch, or the waits for these loads would be for all of them: past the
-        // end no position is there.)
-        load(t0 + 128);
-        page = attn_page(kv, s, t0 + 256 + (lane & 31));
+        load_v();
         if (careful || ok != 0xffffffffu) {
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)

@@ -90,17 +90,26 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
     if (a.n_tokens > INT32_MAX / p.group - 256) return Q4K_EUNSUPPORTED;
     const int64_t pre_rows = a.n_prefix > 0 ? a.n_tokens * p.group : 0, suf_rows = a.n_q * p.group;
     const int rows_of[3] = {16, pl.dim == 256 ? 16 : 32, pl.dim == 256 ? 64 : 128};
-    // Streaming to this many rows of a KV head, us streaming / sharing: 128 dimensions
-    // in 16 bits 96 (16 requests of 4 rows 24.6 / -, 128 rows 30.5 / 29.2, 192 rows
-    // 47.1 / 44.5); F32 queries on F16 and 64 dimensions 256 (128 rows 32.7 / 34.4, 160
-    // rows of 64 dimensions 25.5 / 33.1; 512 rows 73.3 / 69.5 and 50.1 / 47.6); 256
-    // dimensions 96 (120 rows 64.3 / 47.2); F32 queries on BF16, whose three terms a
-    // query leave sharing waves no registers, any (256 rows 74 / 143, 1024 rows 131 / 237).
+    // Streaming to this many rows of a KV head (prefix of 8 KV heads, us streaming /
+    // sharing).  Each tile of 32 rows reads the positions again, so fewer where the
+    // prefix's K and V are more than the caches hold, from 100 MB:
+    //   128 dimensions, 16 bits: 96, then 32 (8192 positions: 64 rows 22.2 / 22.5, 128
+    //   28.2 / 27.8, 256 39.5 / 34.4; 65536: 48 rows 80.6 / 69.5, 128 102 / 79);
+    //   64 dimensions: 192, then 32 (8192: 192 rows 22.5 / 22.8, 384 33.8 / 31.3; 65536:
+    //   128 rows 67.6 / 49.4);
+    //   F32 queries on F16: 192, then 64 (8192: 192 rows 38.0 / 44.4, 512 88 / 78; 65536:
+    //   64 rows 87.6 / 92.3, 128 119 / 104);
+    //   256 dimensions, tiles of 16 rows: 32 (65536: 32 rows 131 / 152, 48 187 / 155);
+    //   F32 queries on BF16, whose three terms a query leave sharing waves no registers:
+    //   any, but for 256 dimensions (128 rows 109 / 89).
     const int terms = a.q_type != Q4K_GGML_TYPE_F32 ? 1 : a.kv_type == Q4K_GGML_TYPE_F16 ? 2 : 3;
-    const int64_t most = pl.dim == 256 ? 96 : terms == 3 ? INT32_MAX : terms == 2 || pl.dim == 64 ? 256 : 96;
-    auto size_of = [&](int64_t rows) { return rows <= 16 ? 0 : rows <= most ? 1 : 2; };
-    pl.suf_size = size_of(suf_rows);
-    pl.pre_size = a.n_prefix > 0 ? size_of(pre_rows) : pl.suf_size;
+    const bool far = (double)a.n_prefix * a.n_head_kv * pl.dim * 4 > 100e6;
+    auto size_of = [&](int64_t rows, bool far) {
+        const int64_t most = pl.dim == 256 ? 32 : terms == 3 ? INT32_MAX : far ? 32 * terms : terms == 1 && pl.dim == 128 ? 96 : 192;
+        return rows <= 16 ? 0 : rows <= most ? 1 : 2;
+    };
+    pl.suf_size = size_of(suf_rows, false);
+    pl.pre_size = a.n_prefix > 0 ? size_of(pre_rows, far) : pl.suf_size;
     if (pl.suf_size > pl.pre_size) pl.suf_size = pl.pre_size;  // (with q_start n_q may exceed the tokens there are)
     const int pr = rows_of[pl.pre_size], sr = rows_of[pl.suf_size];
     // Splits of one length for both parts, in whole steps of 128 positions: about

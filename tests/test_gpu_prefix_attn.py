@@ -109,6 +109,19 @@ def test_attention_many_queries_a_request(Q, gpu, qt, kv, B, nq, H, hk, D, prefi
     c.check(Q)
 
 
+@pytest.mark.parametrize("qt,kv", TYPES)
+@pytest.mark.parametrize("B,nq,H,hk,D,prefix,suffix,page", [(35, 1, 4, 4, 256, 33, 70, 16), (12, 6, 8, 2, 128, 300, 70, 16)])
+def test_attention_shared_prefix_streamed_suffix(Q, gpu, qt, kv, B, nq, H, hk, D, prefix, suffix, page):
+    Case(gpu, B, nq, H, hk, D, prefix, suffix, page, qt, kv, seed=B).check(Q)
+
+
+@pytest.mark.parametrize("qt,kv,B,nq,H,hk,D,prefix,suffix", [
+    (F16, F16, 1, 5, 64, 8, 128, 25100, 40), (F32, F16, 2, 1, 280, 8, 64, 50100, 20)])
+def test_attention_few_rows_over_a_large_prefix(Q, gpu, qt, kv, B, nq, H, hk, D, prefix, suffix):
+    """More than 100 MB of keys and values, whose tiles waves share from few rows on."""
+    Case(gpu, B, nq, H, hk, D, prefix, suffix, 16, qt, kv, seed=B).check(Q)
+
+
 @pytest.mark.parametrize("qt,kv", TYPES[:1] + TYPES[3:])
 @pytest.mark.parametrize("prefix", [0, 1, 15, 16, 17, 63, 64, 65, 127, 128, 129])
 def test_attention_lengths_around_a_tile(Q, gpu, qt, kv, prefix):
