@@ -294,7 +294,7 @@ struct WaveSplit {
 
 constexpr int kRankTiles = 4;  // rank tiles of 16 per wave: 64 ranks
 
-// blockIdx.x: K split and group of 64 ranks
+// A tile's parts: K splits, groups of 16 NR ranks.
 template <class T, int NR, bool VEC>
 __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p) {
     __shared__ int tok[kTile];
@@ -649,21 +649,19 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p) {
     int key[4];  // the first 4096 tokens' keys stay in registers
 #pragma unroll
     for (int u = 0; u < 4; ++u) key[u] = key_of(u * 1024 + tid);
-    // One atomic per key of a wave: in prompts the 64 lanes hold the same one.  The
-    // lane's place after what was counted before.
+    // The lane's place after what was counted before.  In prompts the 64 lanes hold
+    // one key, which the first lane counts for all that hold its own; the others count
+    // themselves (an atomic per key in turn: 2414 tokens of 37 adapters 27 us).
     auto count = [&](int k, bool in) {
-        uint64_t rest = __ballot(in);
-        int place = 0;
-        while (rest) {
-            const int k0 = __builtin_amdgcn_readlane(k, (int)__builtin_ctzll(rest));
-            const uint64_t same = __ballot(in && k == k0);
-            int old = 0;
-            if (lane == 0) old = atomicAdd(&start[k0], (int)__popcll(same));
-            old = __builtin_amdgcn_readfirstlane(old);
-            if (k == k0) place = old + (int)__popcll(same & ((1ull << lane) - 1));
-            rest &= ~same;
-        }
-        return place;
+        const uint64_t any = __ballot(in);
+        const int first = any ? (int)__builtin_ctzll(any) : 0;
+        const int k0 = __builtin_amdgcn_readlane(k, first);
+        const bool with = in && k == k0;
+        const uint64_t same = __ballot(with);
+        int old = 0;
+        if (with ? lane == first : in) old = atomicAdd(&start[k], with ? (int)__popcll(same) : 1);
+        const int old0 = __builtin_amdgcn_readlane(old, first);
+        return with ? old0 + (int)__popcll(same & ((1ull << lane) - 1)) : old;
     };
     const int upto = (p.N + 1023) / 1024 * 1024;
     for (int i = tid; i < keys; i += 1024) start[i] = 0;
@@ -750,10 +748,13 @@ static int lora_plan(const q4k_lora &l, int64_t K, int64_t M, int64_t N, LoraPla
     pl.nr = pl.rp / 16 < kRankTiles ? pl.rp / 16 : kRankTiles;
     if (pl.nr == 3) pl.nr = 4;
     const int64_t groups = (pl.rp + 16 * pl.nr - 1) / (16 * pl.nr);
-    // two workgroups per CU, but at least 512 values (four steps of 32 per wave)
-    // and at most 8 splits, which every workgroup of the expand reads again
+    // Two workgroups per CU, in splits that every workgroup of the expand reads again:
+    // of tiled loads at most 32 and at least 256 values (us at most 8 of 512 / 16 / 32:
+    // one tile of 64 tokens, K 14336, rank 16: 29.4 / 20.6 / 17.4; 8 tiles 32.6 / 23.9 /
+    // 22.5), of direct ones, whose workgroups share less work, 8 and 512 values (48
+    // tokens of 32 adapters, K 8192: 13.9 / 15.6 / 15.7).
     int64_t ks = 2 * cus / (tiles * groups);
-    const int64_t most = K / 512 < 8 ? K / 512 : 8;
+    const int64_t most = pl.tiled ? (K / 256 < 32 ? K / 256 : 32) : K / 512 < 8 ? K / 512 : 8;
     ks = ks > most ? most : ks;
     ks = ks < 1 ? 1 : ks;
     pl.kchunk = (int)(((K + ks - 1) / ks + 127) / 128 * 128);
@@ -763,7 +764,7 @@ static int lora_plan(const q4k_lora &l, int64_t K, int64_t M, int64_t N, LoraPla
     int64_t mc = (M * tiles / (2 * cus) + 63) / 64 * 64;
     mc = mc < 64 ? 64 : mc > 1024 ? 1024 : mc;
     pl.mchunk = (int)mc;
-    if (N > ((int64_t)1 << 50) / (pl.rp * 4 * 8)) return Q4K_EUNSUPPORTED;
+    if (N > ((int64_t)1 << 50) / (pl.rp * 4 * 32)) return Q4K_EUNSUPPORTED;
     pl.h_bytes = (size_t)((int64_t)pl.ksplits * N * pl.rp * 4 + 15) / 16 * 16;
     pl.bytes = pl.h_bytes + (pl.grouped ? (size_t)tiles * 16 + (size_t)N * 4 + 16 : 0);
     return Q4K_OK;

@@ -35,6 +35,12 @@ def test_lora_sizes(Q, gpu, dtype, N, K, M, r, A):
     check(Q, make(gpu, N, K, M, r, A, dtype, seed=N + K))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("N,K,M,r,A", [(64, 8448, 130, 16, 1), (90, 8200, 96, 70, 2), (200, 8197, 64, 8, 3), (5000, 264, 64, 24, 300), (4097, 96, 36, 8, 1)])
+def test_lora_long_sums_and_many_tokens(Q, gpu, dtype, N, K, M, r, A):
+    check(Q, make(gpu, N, K, M, r, A, dtype, seed=N + K))
+
+
 @pytest.mark.parametrize("N", [1, 9, 70, 200])
 def test_lora_ranks_of_their_own(Q, gpu, N):
     check(Q, make(gpu, N, 512, 260, 24, 6, torch.float16, seed=N, ragged=True))
