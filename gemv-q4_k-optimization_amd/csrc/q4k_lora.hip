@@ -740,7 +740,8 @@ static int lora_plan(const q4k_lora &l, int64_t K, int64_t M, int64_t N, LoraPla
     pl.max_tiles = (int)tiles;
     pl.tiled = N >= 16 * kinds;
     // Counting to a tile takes about 0.1 us for each adapter before it, a workgroup
-    // for a token that leads no tile 1.5 us of its place.
+    // for a token that leads no tile 1.5 us of its place: counted where there are
+    // sixteen tokens and more a tile.
     const int64_t in_slice = N < kSlice ? N : kSlice, slice_tiles = in_slice / kTile + (kinds < in_slice ? kinds : in_slice);
     pl.enumerate = slice_tiles * 16 <= in_slice;
     pl.rows = (int)(pl.enumerate ? slice_tiles : in_slice);
