@@ -31,14 +31,15 @@ struct LogitsParams {
 constexpr int kLogitsPer = 8;  // logits per thread, two 16-byte accesses
 
 // The list of row i: [start[i], start[i+1]) clamped to [0, n), empty where the
-// entries run backwards.  Its length, and where it begins.
+// entries run backwards.  Its length, and where it begins.  (Both ends are clamped
+// before they are subtracted: starts may be any 64 bits.)
 __device__ __forceinline__ int list_range(const int64_t *start, int64_t i, int64_t n, int64_t &beg) {
     beg = start[i];
     int64_t end = start[i + 1];
-    if (beg < 0) beg = 0;
-    if (end > n) end = n;
+    beg = beg < 0 ? 0 : beg > n ? n : beg;
+    end = end < beg ? beg : end > n ? n : end;
     end -= beg;
-    return end < 0 ? 0 : end > INT32_MAX - 8192 ? INT32_MAX - 8192 : (int)end;
+    return end > INT32_MAX - 8192 ? INT32_MAX - 8192 : (int)end;
 }
 
 // A list's entries in registers, H quads of them per thread of the workgroup:

@@ -146,3 +146,18 @@ def test_logits_refusals_of_the_binding(Q, gpu):
     with pytest.raises(ValueError):
         Q.logits_adjust(x, mask=torch.zeros(1, 4, dtype=torch.int32, device=gpu))
     assert Q.logits_adjust(x[:0]).shape == (0, 100)
+
+
+def test_logits_list_starts_of_any_value(Q, gpu):
+    """Starts so far apart that their difference passes 64 bits: the list is empty or ends with the entries there are."""
+    lo, hi = -2 ** 63, 2 ** 63 - 1
+    x, pen, _, _, _, _ = make(gpu, 7, 700, 10, 1, 2)
+    h = torch.arange(10, dtype=torch.int32, device=gpu)
+    bias = torch.arange(10, dtype=torch.float32, device=gpu)
+    start = [5, lo, hi, lo, 3, hi, -9, 10 ** 15]
+    lists = [list(range(10))[max(a, 0):max(b, 0)] for a, b in zip(start, start[1:])]
+    assert [len(r) for r in lists] == [0, 10, 0, 3, 7, 0, 10]
+    starts = torch.tensor(start, device=gpu)
+    got = Q.logits_adjust(x, *pen, history=h, history_start=starts, bias_ids=h, bias=bias, bias_start=starts)
+    want, tol = _batch.logits(x, *pen, lists, [[(t, float(t)) for t in r] for r in lists], None, None)
+    _batch.assert_close(got, want, tol, "lists")
