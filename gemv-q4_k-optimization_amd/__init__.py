@@ -434,7 +434,7 @@ def _stream_of(stream, device):
     if stream is not None:
         return stream.cuda_stream
     import torch
-    return torch._C._cuda_getCurrentRawStream(device) if device >= 0 else None
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _rows(t, dtype, shape, device, what):
@@ -463,8 +463,12 @@ def _vector(t, dtype, shape, device, what):
     return t.data_ptr()
 
 
-def _ws(workspace):
-    return (workspace.data_ptr(), workspace.nbytes) if workspace is not None else (None, 0)
+def _ws(workspace, device):
+    if workspace is None:
+        return None, 0
+    if workspace.get_device() != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace: contiguous on device {device} expected")
+    return workspace.data_ptr(), workspace.nbytes
 
 
 class LoraAdapters:
@@ -475,6 +479,7 @@ class LoraAdapters:
 
     def __init__(self, a, b, scale=None, ranks=None):
         import torch
+        _need(a.is_cuda, "a, b: device tensors expected")
         _need(a.dim() == 3 and b.dim() == 3 and a.dtype == b.dtype and a.device == b.device and
               a.shape[0] == b.shape[0] and a.shape[1] == b.shape[2], "a [adapters, rank, K], b [adapters, M, rank] of one type")
         _need(a.numel() == 0 or (a.stride(2) == 1 or a.shape[2] == 1), "rows of a are not contiguous")
@@ -508,7 +513,7 @@ def lora_add(adapters: LoraAdapters, x, ids, base=None, out=None, workspace=None
         out = _new(shape, f32, adapters.device, stream)
     ldo = _rows(out, f32, shape, dev, "out")
     bp, ldb = (base.data_ptr(), _rows(base, f32, shape, dev, "base")) if base is not None else (None, 0)
-    ws, ws_bytes = _ws(workspace)
+    ws, ws_bytes = _ws(workspace, dev)
     st = lib().q4k_lora_add(adapters._ref, K, M, x.data_ptr(), N, ldx * 4, _vector(ids, torch.int32, (N,), dev, "ids"), bp, ldb * 4,
                             out.data_ptr(), ldo * 4, ws, ws_bytes, _stream_of(stream, dev))
     if st != Q4K_OK:
@@ -526,6 +531,7 @@ class KVPages:
 
     def __init__(self, k, v, table=None):
         import torch
+        _need(k.is_cuda, "k, v: device tensors expected")
         _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device and k.numel() > 0,
               "k, v: [pages, page_size, heads_kv, head_dim] of one type and shape expected")
         _need(k.stride(3) == 1 and v.stride(3) == 1, "head_dim of k, v is not contiguous")
@@ -605,8 +611,9 @@ def prefix_attention(q, prefix, n_prefix, suffix=None, suffix_len=None, max_suff
     if out is None:
         out = _new(q.shape, q.dtype, q.device, stream)
     args = _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, q_start, scale, out, lse)
-    ws, ws_bytes = _ws(workspace)
-    st = lib().q4k_prefix_attn(ctypes.byref(args), ws, ws_bytes, _stream_of(stream, q.get_device()))
+    dev = q.get_device()
+    ws, ws_bytes = _ws(workspace, dev)
+    st = lib().q4k_prefix_attn(ctypes.byref(args), ws, ws_bytes, _stream_of(stream, dev))
     if st != Q4K_OK:
         raise Q4KError(st, "q4k_prefix_attn")
     return out
@@ -621,6 +628,7 @@ def logits_adjust(logits, repeat=None, frequency=None, presence=None, history=No
     int32 [N] (outside [0, masks): none).  out may be logits."""
     import torch
     f32, i32, i64 = torch.float32, torch.int32, torch.int64
+    _need(logits.is_cuda, "logits: a device tensor expected")
     N, V = logits.shape
     dev = logits.get_device()
     shape, per_row, starts = (N, V), (N,), (N + 1,)

@@ -113,3 +113,14 @@ def test_logits_empty(Q):
     assert logits(Q, N=0, src=None, dst=None) == OK
     assert logits(Q, V=0) == OK
     assert Q.lib().q4k_logits_adjust(FAKE, 100, 2, 400, None, FAKE, 400, None) == EINVAL
+
+
+def test_binding_refuses_tensors_in_host_memory(Q):
+    import torch
+    f16, f32 = torch.float16, torch.float32
+    with pytest.raises(ValueError):
+        Q.logits_adjust(torch.zeros(2, 100, dtype=f32))
+    with pytest.raises(ValueError):
+        Q.LoraAdapters(torch.zeros(2, 8, 256, dtype=f16), torch.zeros(2, 64, 8, dtype=f16))
+    with pytest.raises(ValueError):
+        Q.KVPages(torch.zeros(2, 16, 2, 64, dtype=f16), torch.zeros(2, 16, 2, 64, dtype=f16))

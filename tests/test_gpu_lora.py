@@ -177,3 +177,13 @@ def test_lora_refusals_of_the_binding(Q, gpu):
     with pytest.raises(Q.Q4KError):
         Q.lora_add(ad, x, ids, workspace=torch.empty(8, dtype=torch.uint8, device=gpu))
     assert Q.lora_add(ad, x[:0], ids[:0]).shape == (0, 64)
+
+
+def test_lora_refuses_operands_in_host_memory(Q, gpu):
+    a, b, x, ids, base, _, _ = make(gpu, 4, 256, 64, 8, 2, torch.float16, 2)
+    ad = Q.LoraAdapters(a, b)
+    size = Q.lora_workspace(ad, 4).numel()
+    for bad in (dict(workspace=torch.empty(size, dtype=torch.uint8)), dict(workspace=torch.empty(1, dtype=torch.uint8, device=gpu).expand(size)),
+                dict(base=base.cpu()), dict(out=torch.empty(4, 64))):
+        with pytest.raises(ValueError):
+            Q.lora_add(ad, x, ids, **bad)

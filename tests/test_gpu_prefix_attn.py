@@ -326,3 +326,17 @@ def test_attention_refusals_of_the_binding(Q, gpu):
             bad()
     with pytest.raises(Q.Q4KError):
         Q.prefix_attention(c.q, pre, 61)
+
+
+def test_attention_refuses_operands_in_host_memory(Q, gpu):
+    c = Case(gpu, 2, 1, 8, 2, 64, 3000, 20, 16, F16, F16)
+    pre, suf = Q.KVPages(*c.prefix[:2], table=c.prefix[2]), Q.KVPages(*c.suffix[:2], table=c.suffix[2])
+    lens = torch.tensor(c.lens, dtype=torch.int32, device=gpu)
+    ws = Q.prefix_attention_workspace(c.q, pre, 3000, suf, lens, 20)
+    for bad in (dict(workspace=ws.cpu()), dict(workspace=ws[:1].expand(ws.numel())), dict(out=torch.empty_like(c.q, device="cpu"))):
+        with pytest.raises(ValueError):
+            Q.prefix_attention(c.q, pre, 3000, suf, lens, 20, **bad)
+    with pytest.raises(ValueError):
+        Q.prefix_attention(c.q.cpu(), pre, 3000, suf, lens, 20)
+    with pytest.raises(ValueError):
+        Q.prefix_attention(c.q, pre, 3000, suf, lens.cpu(), 20)
