@@ -734,6 +734,7 @@ constexpr int kGroupKeys = 32000;  // counters in the group kernel's LDS
 
 static int lora_plan(const q4k_lora &l, int64_t K, int64_t M, int64_t N, LoraPlan &pl) {
     constexpr int64_t cus = 256;
+    if (K > 1 << 30) return Q4K_EUNSUPPORTED;  // the kernels count a 16-bit row's bytes in 31 bits
     pl.grouped = N > kSlice && l.n_adapters < kGroupKeys;
     const int64_t kinds = l.n_adapters + 1 < N ? l.n_adapters + 1 : N;
     const int64_t tiles = N / kTile + kinds;  // at most
@@ -834,11 +835,11 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
         if (l.nb_a % 2 != 0 || l.nb_b % 2 != 0 || l.nb_a_adapter % 2 != 0 || l.nb_b_adapter % 2 != 0) return Q4K_EINVAL;
         if (l.nb_a < 2 * ne00 || l.nb_b < 2 * l.rank || l.nb_a_adapter < 0 || l.nb_b_adapter < 0) return Q4K_EINVAL;
     }
-    DeviceInfo *di;
-    int st = device_info(&di);
-    if (st != Q4K_OK) return st;
     LoraPlan pl;
-    st = lora_plan(l, ne00, ne01, ne11, pl);
+    int st = lora_plan(l, ne00, ne01, ne11, pl);
+    if (st != Q4K_OK) return st;
+    DeviceInfo *di;
+    st = device_info(&di);
     if (st != Q4K_OK) return st;
     const int64_t slices = (ne11 + kSlice - 1) / kSlice;
     const int64_t parts1 = (int64_t)pl.ksplits * ((pl.rp + 16 * pl.nr - 1) / (16 * pl.nr)), parts2 = (ne01 + pl.mchunk - 1) / pl.mchunk;

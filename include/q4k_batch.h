@@ -63,9 +63,9 @@ size_t q4k_lora_workspace_bytes(const q4k_lora *lora, int64_t ne00, int64_t ne01
  *   ids:  ne11 adapter numbers on the device; a token whose number is outside
  *         [0, n_adapters) takes no adapter: dst[n] = src2[n]
  *   dst:  ne11 tokens of ne01 floats, stride nb1
- * Any ne00, ne01, ne11 and rank; rows of a and b that are 16-byte aligned and
- * rows of dst that are 64-byte aligned run faster.  Sums are F32; the F32
- * activations and a's products enter the matrix cores as sums of three BF16
+ * Any ne01, ne11 and rank, ne00 up to 2^30; rows of a and b that are 16-byte
+ * aligned and rows of dst that are 64-byte aligned run faster.  Sums are F32; the
+ * F32 activations and a's products enter the matrix cores as sums of three BF16
  * values, which hold F32's 24 bits; an activation or sum that is not finite in
  * BF16 (past 3.39e38) makes its token's results NaN.  ne00 == 0 adds nothing. */
 int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *src1, int64_t ne11,

@@ -124,3 +124,12 @@ def test_binding_refuses_tensors_in_host_memory(Q):
         Q.LoraAdapters(torch.zeros(2, 8, 256, dtype=f16), torch.zeros(2, 64, 8, dtype=f16))
     with pytest.raises(ValueError):
         Q.KVPages(torch.zeros(2, 16, 2, 64, dtype=f16), torch.zeros(2, 16, 2, 64, dtype=f16))
+
+
+def test_lora_rows_past_the_kernels_offsets(Q):
+    """Values of a row are counted in 31 bits of bytes of a 16-bit row: up to 2^30 of them."""
+    l = lora(Q, nb_a=1 << 33, nb_a_adapter=1 << 34)
+    for K in ((1 << 30) + 1, (1 << 31) - 8192):
+        assert lora_call(Q, l, ne00=K, N=1) == EUNSUPPORTED
+        assert Q.lib().q4k_lora_workspace_bytes(ctypes.byref(l), K, 64, 1) == 0
+    assert Q.lib().q4k_lora_workspace_bytes(ctypes.byref(l), 1 << 30, 64, 1) > 0
