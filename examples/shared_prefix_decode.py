@@ -69,6 +69,7 @@ class Decoder:
         self.table = torch.randperm(requests * per, device=dev, generator=g).view(requests, per).int()
         self.own = Q.KVPages(self.own_k, self.own_v, table=self.table)
         self.lens = torch.zeros(requests, dtype=torch.int32, device=dev)
+        self.steps = 0  # taken: what every request has generated, known without asking the device
         self.row = torch.arange(requests, device=dev)
         # histories: what each request has generated, one list of `most_new` places each
         self.history = torch.full((requests, most_new), -1, dtype=torch.int32, device=dev)
@@ -94,6 +95,9 @@ class Decoder:
 
     def step(self, tokens):
         """tokens int64 [requests] -> the next tokens."""
+        if self.steps == self.most:
+            raise ValueError(f"the requests' own pages hold {self.most} tokens each")
+        self.steps += 1
         Q, B = self.Q, self.B
         x = self.embed[tokens]
         q, k, v = (self.project(n, x) for n in "qkv")
@@ -123,7 +127,7 @@ def main():
     ap.add_argument("--prefix", type=int, default=4096)
     ap.add_argument("--steps", type=int, default=4)
     a = ap.parse_args()
-    d = Decoder(requests=a.requests, prefix=a.prefix)
+    d = Decoder(requests=a.requests, prefix=a.prefix, most_new=max(256, a.steps))
     tokens = torch.arange(a.requests, device=d.dev) + 5
     for i in range(a.steps):
         tokens = d.step(tokens)

@@ -46,3 +46,16 @@ def test_shared_prefix_decode_example(Q, gpu):
     for step in range(20):
         tokens = d2.step(tokens)
         assert tokens.tolist() == seen[step]
+
+
+def test_shared_prefix_decode_example_ends_with_its_pages(Q, gpu):
+    spec = importlib.util.spec_from_file_location("shared_prefix_decode", os.path.join(_common.ROOT, "examples", "shared_prefix_decode.py"))
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    d = ex.Decoder(requests=2, prefix=20, embd=512, heads=8, heads_kv=2, vocab=256, page=16, most_new=3, rank=8, seed=3)
+    tokens = torch.arange(2, device=gpu)
+    for _ in range(3):
+        tokens = d.step(tokens)
+    with pytest.raises(ValueError):
+        d.step(tokens)
+    assert d.lens.tolist() == [3, 3]
