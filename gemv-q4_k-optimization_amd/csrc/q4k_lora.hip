@@ -21,9 +21,10 @@
 // A few tokens are bound by two launches and their chains of round trips: 1 token,
 // 1024 x 4096, rank 8: 5.3 + 5.3 us; 8 tokens, 14336 x 4096, rank 16: 5.5 + 6.2.
 //
-// Each column of a product depends on its token alone, so a token's result does
-// not depend on which tokens share its tile, nor on the order in which they
-// were put there.
+// A token's sums are cut by the sizes of the call and, in the direct shrink, by how
+// many tokens its adapter has (to 64; of a slice of 512 where each workgroup looks
+// for its tile), not by its tile: its result does not depend on which tokens share
+// the tile, nor on the order in which they were put there.
 #include <hip/hip_runtime.h>
 
 #include "q4k_batch.h"
@@ -48,7 +49,7 @@ struct LoraParams {
     int64_t nb_x, nb_base, nb_dst;
     const int32_t *ids;
     float *h;             // [ksplits][N][rp]
-    const int32_t *order; // grouped: tokens by adapter, and the tiles (first, count, adapter) of them
+    const int32_t *order; // grouped: tokens by adapter, and the tiles (first, count, adapter, LoraTile::of) of them
     const int4 *tiles;
     const int32_t *n_tiles;
     int n_adapters, K, M, N, rank, rp;
@@ -60,6 +61,7 @@ struct LoraParams {
 struct LoraTile {
     int adapter;  // -1: tokens without one
     int count;
+    int of;       // tokens of the adapter, at most a tile's: the same for its short last tile
 };
 
 // A tile's tokens into tok[0..63] (LDS), the same for all waves, and the
@@ -83,6 +85,7 @@ __device__ __forceinline__ bool lora_tile(const LoraParams &p, int parts, int *t
         const int4 d = p.tiles[item - x * tiles];
         t.adapter = d.z;
         t.count = d.y;
+        t.of = d.w;
         if (threadIdx.x < 64) tok[lane] = p.order[d.x + (lane < d.y ? lane : 0)];
         __syncthreads();
         return true;
@@ -130,6 +133,7 @@ __device__ __forceinline__ bool lora_tile(const LoraParams &p, int parts, int *t
         t.adapter = key;
         before = me * kTile;
         t.count = all - before < kTile ? all - before : kTile;
+        t.of = all < kTile ? all : kTile;
         if (threadIdx.x < 64) {
             int seen = 0;
             tok[lane] = base;
@@ -154,6 +158,7 @@ __device__ __forceinline__ bool lora_tile(const LoraParams &p, int parts, int *t
     }
     if (before % kTile != 0) return false;
     t.count = all - before < kTile ? all - before : kTile;
+    t.of = all < kTile ? all : kTile;
     if (threadIdx.x < 64) {
         tok[lane] = base + me;
         int seen = 0;
@@ -280,7 +285,9 @@ __device__ __forceinline__ int adapter_rank(const LoraParams &p, int i) {
 }
 
 // How the four waves share a tile: waves over its tiles of 16 tokens, the
-// others over the length (shrink: K, expand: M).
+// others over the length (shrink: K, expand: M).  The shrink cuts its sums by it, so
+// it takes the adapter's tokens for count (LoraTile::of): a short last tile has no
+// more waves along K than the full ones beside it, and is done no later.
 struct WaveSplit {
     int nt, part, parts;
     __device__ __forceinline__ WaveSplit(int count, int wave) {
@@ -306,7 +313,7 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(LoraParams p) {
     const int n = lane & 15, g = lane >> 4;
     const int ks = part % p.ksplits, j0 = part / p.ksplits * (16 * NR);
     const int r = adapter_rank(p, t.adapter);
-    const WaveSplit ws(t.count, wave);
+    const WaveSplit ws(t.of, wave);
     const int token = tok[ws.nt * 16 + n];
     const float *x = reinterpret_cast<const float *>(p.x + (int64_t)token * p.nb_x);
     const char *a[NR];
@@ -701,7 +708,7 @@ __global__ __launch_bounds__(1024) void lora_group_kernel(LoraParams p) {
         const int first = bc + sc - c;
         for (int i = 0; i < q; ++i)
             tiles[bq + sq - q + i] = make_int4(first + i * kTile, c - i * kTile < kTile ? c - i * kTile : kTile,
-                                               k < p.n_adapters ? k : -1, 0);
+                                               k < p.n_adapters ? k : -1, c < kTile ? c : kTile);
         if (k < keys) start[k] = first;
         tokens += tc;
         ntiles += tq;

@@ -187,3 +187,20 @@ def test_lora_refuses_operands_in_host_memory(Q, gpu):
                 dict(base=base.cpu()), dict(out=torch.empty(4, 64))):
         with pytest.raises(ValueError):
             Q.lora_add(ad, x, ids, **bad)
+
+
+@pytest.mark.parametrize("N,K,A", [(90, 333, 2), (300, 512, 30), (600, 333, 3), (600, 512, 40), (1500, 1024, 120)])
+def test_lora_bits_do_not_depend_on_the_order_of_tokens(Q, gpu, N, K, A):
+    """An adapter of 70 tokens, a tile of 64 and one of 6: whichever tokens come
+    to lie in the second one have the same bits, from call to call too."""
+    g = torch.Generator(device=gpu).manual_seed(N)
+    ids = torch.randint(0, A, (N,), device=gpu, generator=g)
+    ids[ids == 1] = -1
+    ids[torch.randperm(N, device=gpu, generator=g)[:70]] = 1
+    a, b, x, ids, base, scale, _ = make(gpu, N, K, 64, 16, A, torch.float16, seed=N, ids=ids.int())
+    ad = Q.LoraAdapters(a, b, scale=scale)
+    want = Q.lora_add(ad, x, ids, base=base)
+    for _ in range(3):
+        perm = torch.randperm(N, device=gpu, generator=g)
+        assert torch.equal(Q.lora_add(ad, x[perm], ids[perm], base=base[perm]), want[perm])
+        assert torch.equal(Q.lora_add(ad, x, ids, base=base), want)
