@@ -735,6 +735,7 @@ struct LoraPlan {
     int max_tiles;      // tiles there can be, grouped
     int rp, nr, ksplits, kchunk, mchunk;
     size_t h_bytes, bytes;
+    size_t upto_bytes;  // enough for this many tokens and for any fewer
 };
 
 constexpr int kGroupKeys = 32000;  // counters in the group kernel's LDS
@@ -779,7 +780,15 @@ static int lora_plan(const q4k_lora &l, int64_t K, int64_t M, int64_t N, LoraPla
     pl.mchunk = (int)mc;
     if (N > ((int64_t)1 << 50) / (pl.rp * 4 * 32)) return Q4K_EUNSUPPORTED;
     pl.h_bytes = (size_t)((int64_t)pl.ksplits * N * pl.rp * 4 + 15) / 16 * 16;
-    pl.bytes = pl.h_bytes + (pl.grouped ? (size_t)tiles * 16 + (size_t)N * 4 + 16 : 0);
+    const size_t group_bytes = pl.grouped ? (size_t)tiles * 16 + (size_t)N * 4 + 16 : 0;
+    pl.bytes = pl.h_bytes + group_bytes;
+    // Fewer tokens take more splits of K each.  n tokens are more than n / 64 tiles, so
+    // ks n <= 2 cus n / (tiles groups) < 128 cus / groups where there is more than one
+    // split, and there are no more splits than `most` may be.
+    const int64_t max_splits = K / 256 < 1 ? 1 : K / 256 < 32 ? K / 256 : 32;
+    int64_t split_rows = max_splits * N < 128 * cus / groups ? max_splits * N : 128 * cus / groups;
+    split_rows = K == 0 ? 0 : split_rows < N ? N : split_rows;
+    pl.upto_bytes = (size_t)(split_rows * pl.rp * 4) + group_bytes;
     return Q4K_OK;
 }
 
@@ -821,7 +830,7 @@ extern "C" {
 size_t q4k_lora_workspace_bytes(const q4k_lora *lora, int64_t ne00, int64_t ne01, int64_t ne11) {
     LoraPlan pl;
     if (!lora_sizes_ok(lora, ne00, ne01, ne11) || ne11 == 0 || lora_plan(*lora, ne00, ne01, ne11, pl) != Q4K_OK) return 0;
-    return pl.bytes;
+    return pl.upto_bytes;
 }
 
 int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *src1, int64_t ne11, int64_t nb11,

@@ -52,7 +52,8 @@ typedef struct q4k_lora {
                             * and columns of b[i] count (clamped to 0..rank); NULL = rank */
 } q4k_lora;
 
-/* Bytes of workspace that q4k_lora_add takes for ne11 tokens (0: invalid sizes). */
+/* Bytes of workspace that are enough for q4k_lora_add of ne11 tokens and of any
+ * fewer (0: invalid sizes). */
 size_t q4k_lora_workspace_bytes(const q4k_lora *lora, int64_t ne00, int64_t ne01, int64_t ne11);
 
 /* dst[n] = src2[n] + scale[i] * b[i] (a[i] src1[n]),  i = ids[n], for n < ne11.

@@ -133,3 +133,12 @@ def test_lora_rows_past_the_kernels_offsets(Q):
         assert lora_call(Q, l, ne00=K, N=1) == EUNSUPPORTED
         assert Q.lib().q4k_lora_workspace_bytes(ctypes.byref(l), K, 64, 1) == 0
     assert Q.lib().q4k_lora_workspace_bytes(ctypes.byref(l), 1 << 30, 64, 1) > 0
+
+
+@pytest.mark.parametrize("K,rank,adapters,type", [(4096, 16, 256, 1), (4096, 16, 16, 1), (14336, 16, 4, 30), (4096, 8, 4, 1), (14336, 64, 16, 30),
+                                                  (256, 200, 2, 1), (0, 16, 2, 1), (2304, 24, 40000, 30)])
+def test_lora_workspace_serves_every_smaller_batch(Q, K, rank, adapters, type):
+    """The size for n tokens is enough for fewer, so it never falls as n rises."""
+    L, l = Q.lib(), lora(Q, rank=rank, n_adapters=adapters, type=type)
+    sizes = [L.q4k_lora_workspace_bytes(ctypes.byref(l), K, 64, n) for n in [*range(1, 2200), 4095, 4096, 4097, 65536, 1 << 20]]
+    assert sizes == sorted(sizes)

@@ -204,3 +204,11 @@ def test_lora_bits_do_not_depend_on_the_order_of_tokens(Q, gpu, N, K, A):
         perm = torch.randperm(N, device=gpu, generator=g)
         assert torch.equal(Q.lora_add(ad, x[perm], ids[perm], base=base[perm]), want[perm])
         assert torch.equal(Q.lora_add(ad, x, ids, base=base), want)
+
+
+@pytest.mark.parametrize("A,K,most,N", [(256, 4096, 254, 127), (16, 4096, 1024, 1023), (4, 14336, 896, 895), (3, 4096, 600, 1)])
+def test_lora_workspace_of_a_larger_batch(Q, gpu, A, K, most, N):
+    a, b, x, ids, base, scale, _ = make(gpu, N, K, 64, 16, A, torch.float16, seed=N)
+    ad = Q.LoraAdapters(a, b, scale=scale)
+    got = Q.lora_add(ad, x, ids, base=base, workspace=Q.lora_workspace(ad, most))
+    assert torch.equal(got, Q.lora_add(ad, x, ids, base=base, workspace=Q.lora_workspace(ad, N)))
