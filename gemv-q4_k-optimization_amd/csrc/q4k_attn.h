@@ -70,8 +70,9 @@ struct AttnParams {
     // split, request, KV head, row tile
     int pre_items, pre_tiles, pre_splits, pre_len;  // pre_len, suf_len: positions of a split
     int suf_items, suf_tiles, suf_splits, suf_len;
-    // partial results of `slots` splits: (M, l) and the unscaled output of every row
-    int slots, join_groups, join_rows;
+    // partial results of `slots` splits: (M, l) and the unscaled output of every row,
+    // where a second kernel joins them
+    int join, slots, join_groups, join_rows;
     float2 *part_ml;
     float *part_o;
 };
@@ -406,7 +407,7 @@ __device__ __forceinline__ void attn_emit(const AttnParams &p, const AttnSpan &s
     const int t = (int)fastdiv((uint32_t)row, p.group_div);
     const int h = hk * p.group + row - t * p.group;
     const int64_t out = (int64_t)(s.tok0 + t) * p.n_head + h;
-    if (p.slots > 1) {
+    if (p.join) {
         const int64_t at = (int64_t)s.slot * p.n_tokens * p.n_head + out;
         if (d == 0) p.part_ml[at] = make_float2(M, sum);
         *reinterpret_cast<f32x4 *>(p.part_o + at * p.head_dim + d) = x;
@@ -822,7 +823,7 @@ __global__ __launch_bounds__(256, CP::D == 256 ? 1 : 2) void prefix_attn_kernel(
     const int len = attn_suffix(p, r);
     s.beg = sp * p.suf_len;
     // (the first split of a request that sees nothing writes its empty rows when nothing else would)
-    if (s.beg >= len && (p.slots > 1 || sp > 0)) return;
+    if (s.beg >= len && (p.join || sp > 0)) return;
     s.end = s.beg + p.suf_len < len ? s.beg + p.suf_len : len;
     s.rows = (t1 - t0) * p.group;
     s.tok0 = t0;

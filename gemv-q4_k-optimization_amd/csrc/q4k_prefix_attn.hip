@@ -145,13 +145,15 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
         p.suf_items = (int)(per_suf * p.suf_splits);
     }
     p.slots = p.pre_splits + p.suf_splits;
+    // (the prefix's rows are all tokens: with q_start the join leaves those of no request out)
+    p.join = p.slots > 1 || (a.n_prefix > 0 && a.q_start);
     // the join: four splits or so to a group of lanes, more rows to a workgroup where
     // that leaves groups (4096 rows of 2 splits: 8.5 us with a workgroup each)
     const int groups = 256 / (a.head_dim / 4);
     p.join_groups = 1;
     while (p.join_groups * 4 < p.slots && p.join_groups * 2 <= groups) p.join_groups *= 2;
     p.join_rows = groups / p.join_groups;
-    if (p.slots > 1) {
+    if (p.join) {
         const int64_t rows = a.n_tokens * a.n_head;
         if (rows > ((int64_t)1 << 50) / p.slots / (a.head_dim + 2)) return Q4K_EUNSUPPORTED;
         pl.bytes = (size_t)(rows * p.slots * (a.head_dim + 2) * 4);
@@ -198,7 +200,7 @@ int q4k_prefix_attn(const q4k_prefix_attn_args *args, void *workspace, size_t wo
     p.part_ml = (float2 *)(p.part_o + (int64_t)p.n_tokens * p.n_head * p.slots * p.head_dim);
     using Fn = void (*)(AttnParams);
     st = launch((Fn)pl.kernel, dim3((unsigned)(p.pre_items + p.suf_items)), 256, pl.lds, stream, p);
-    if (st == Q4K_OK && p.slots > 1) {
+    if (st == Q4K_OK && p.join) {
         const bool f32 = args->q_type == Q4K_GGML_TYPE_F32, f16 = args->kv_type == Q4K_GGML_TYPE_F16;
         Fn join = f32 ? prefix_attn_join_kernel<float> : f16 ? prefix_attn_join_kernel<_Float16> : prefix_attn_join_kernel<__bf16>;
         st = launch(join, dim3((unsigned)cdiv((int64_t)p.n_requests * p.n_q * p.n_head, p.join_rows)), 256, 0, stream, p);

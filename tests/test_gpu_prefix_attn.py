@@ -340,3 +340,26 @@ def test_attention_refuses_operands_in_host_memory(Q, gpu):
         Q.prefix_attention(c.q.cpu(), pre, 3000, suf, lens, 20)
     with pytest.raises(ValueError):
         Q.prefix_attention(c.q, pre, 3000, suf, lens.cpu(), 20)
+
+
+@pytest.mark.parametrize("qt,kv", TYPES)
+@pytest.mark.parametrize("heads,prefix,suffix", [(4, 1, 0), (4, 100, 0), (4, 3000, 0), (64, 120, 0), (64, 3000, 0), (4, 100, 40), (64, 0, 40)])
+def test_attention_leaves_tokens_of_no_request_alone(Q, gpu, qt, kv, heads, prefix, suffix):
+    """Tokens before the first request, past the n_q of a request and behind the last one."""
+    c = Case(gpu, 4, 3, heads, 2, 64, prefix, suffix, 16, qt, kv, seed=heads)
+    spans, n = [(2, 4), (4, 4), (4, 7), (9, 10)], 13    # the third request has 5 tokens, of which 3 count
+    starts = torch.tensor([2, 4, 4, 9, 10], dtype=torch.int32, device=gpu)
+    c.q = torch.randn(n, heads, 64, device=gpu).to(qt)
+    pre = Q.KVPages(*c.prefix[:2]) if prefix else None
+    suf = Q.KVPages(*c.suffix[:2], table=c.suffix[2]) if suffix else None
+    lens = torch.tensor(c.lens, dtype=torch.int32, device=gpu) if suffix else None
+    out, lse = torch.full_like(c.q, 7.0), torch.full((n, heads), 7.0, device=gpu)
+    Q.prefix_attention(c.q, pre, prefix, suf, lens, suffix, n_q=3, q_start=starts, scale=c.scale, out=out, lse=lse)
+    # (a prefix of its own page, so that its table is the pages in order)
+    want, wl, tol, tl = _batch.attention(c.q, spans, c.prefix, c.suffix, (prefix, c.lens), c.scale)
+    mine = torch.zeros(n, dtype=torch.bool)
+    for lo, hi in spans:
+        mine[lo:hi] = True
+    _batch.assert_close(out.cpu()[mine], want[mine], tol[mine], "out")
+    _batch.assert_close(lse.cpu()[mine], wl[mine], tl[mine], "lse")
+    assert (out.cpu()[~mine] == 7).all() and (lse.cpu()[~mine] == 7).all()
