@@ -567,13 +567,15 @@ def _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, 
         _need(requests >= 0, "q_start: requests + 1 entries expected")
     else:
         requests = n // n_q if n_q else 0
-    lens = None
+    lens = own = None
     if max_suffix:
         _need(suffix is not None and suffix_len is not None, "max_suffix without suffix and suffix_len")
         lens = _vector(suffix_len, torch.int32, (requests,), dev, "suffix_len")
+        own = suffix._p
         if suffix.tensors[2] is None:
-            if requests:
-                suffix.desc.table_len = suffix.desc.n_pages // requests
+            if requests:  # the call's own description: pages in order, as many for each request
+                own = ctypes.pointer(q4k_kv_pages.from_buffer_copy(suffix.desc))
+                own.contents.table_len = suffix.desc.n_pages // requests
         elif suffix.rows != requests and requests != 1:
             raise ValueError("suffix: a table row for each request expected")
     if n_prefix and (prefix is None or prefix.rows not in (None, 1)):
@@ -589,7 +591,7 @@ def _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, 
     return q4k_prefix_attn_args(
         qt, cache.type, heads, cache.heads, dim, dim ** -0.5 if scale is None else scale, n, requests, n_q,
         start, q.data_ptr(), q.stride(0) * es, q.stride(1) * es, prefix._p if n_prefix else None, n_prefix,
-        suffix._p if max_suffix else None, lens, max_suffix, out.data_ptr(), out.stride(0) * es, out.stride(1) * es, lse)
+        own, lens, max_suffix, out.data_ptr(), out.stride(0) * es, out.stride(1) * es, lse)
 
 
 def prefix_attention_workspace(q, prefix, n_prefix, suffix=None, suffix_len=None, max_suffix=0, n_q=1, q_start=None):

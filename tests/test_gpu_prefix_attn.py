@@ -363,3 +363,24 @@ def test_attention_leaves_tokens_of_no_request_alone(Q, gpu, qt, kv, heads, pref
     _batch.assert_close(out.cpu()[mine], want[mine], tol[mine], "out")
     _batch.assert_close(lse.cpu()[mine], wl[mine], tl[mine], "lse")
     assert (out.cpu()[~mine] == 7).all() and (lse.cpu()[~mine] == 7).all()
+
+
+def test_attention_keeps_the_description_of_a_cache(Q, gpu):
+    """One KVPages without a table as the requests' pages of batches of several
+    sizes, then as a prefix, and as both in one call."""
+    g = torch.Generator(device=gpu).manual_seed(2)
+    k, v = (torch.randn(12, 16, 2, 64, device=gpu, generator=g).half() for _ in range(2))
+    q = torch.randn(4, 8, 64, device=gpu, generator=g).half()
+    lens = torch.tensor([16, 9, 3, 30], dtype=torch.int32, device=gpu)
+    pool, scale = Q.KVPages(k, v), 64 ** -0.5
+    table = lambda n: torch.arange(12 // n * n, dtype=torch.int32, device=gpu).view(n, -1)  # noqa: E731
+
+    def check(n, n_prefix, most):
+        got = Q.prefix_attention(q[:n], pool if n_prefix else None, n_prefix, pool if most else None, lens[:n] if most else None, most)
+        cache = (k, v, torch.arange(12))
+        want, _, tol, _ = _batch.attention(q[:n], [(i, i + 1) for i in range(n)], cache if n_prefix else None, (k, v, table(n)) if most else None,
+                                           (n_prefix, lens[:n].tolist() if most else None), scale)
+        _batch.assert_close(got, want, tol, f"{n} requests, {n_prefix} + {most}")
+
+    for n, n_prefix, most in ((4, 0, 40), (2, 0, 90), (3, 180, 0), (4, 180, 40), (1, 192, 16)):
+        check(n, n_prefix, most)
