@@ -561,6 +561,8 @@ def _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, 
         raise ValueError("prefix, suffix: one type, number of heads, head_dim and device expected")
     qt, es = (GGML_TYPE_F32, 4) if dtype is torch.float32 else (_type16(q), 2)
     start = None
+    if n_q is None:  # one token a request; as many as there are where q_start tells
+        n_q = 1 if q_start is None else n
     if q_start is not None:
         start = _vector(q_start, torch.int32, None, dev, "q_start")
         requests = q_start.shape[0] - 1
@@ -594,7 +596,7 @@ def _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, 
         own, lens, max_suffix, out.data_ptr(), out.stride(0) * es, out.stride(1) * es, lse)
 
 
-def prefix_attention_workspace(q, prefix, n_prefix, suffix=None, suffix_len=None, max_suffix=0, n_q=1, q_start=None):
+def prefix_attention_workspace(q, prefix, n_prefix, suffix=None, suffix_len=None, max_suffix=0, n_q=None, q_start=None):
     """A workspace for prefix_attention calls of these sizes."""
     import torch
     args = _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, q_start, None, None, None)
@@ -602,14 +604,15 @@ def prefix_attention_workspace(q, prefix, n_prefix, suffix=None, suffix_len=None
     return torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
 
 
-def prefix_attention(q, prefix, n_prefix, suffix=None, suffix_len=None, max_suffix=0, n_q=1, q_start=None, scale=None,
+def prefix_attention(q, prefix, n_prefix, suffix=None, suffix_len=None, max_suffix=0, n_q=None, q_start=None, scale=None,
                      out=None, lse=None, workspace=None, stream=None):
     """Attention of a batch over n_prefix tokens that all requests share
     (prefix, read once for all) and each request's own suffix_len[r] <=
     max_suffix tokens (suffix), the last of which are the queries' own.
     q [tokens, heads, head_dim], float32 or the caches' type: n_q tokens a
-    request, or q_start int32 [requests + 1] with at most n_q each.  Returns out
-    of q's type; lse F32 [tokens, heads] receives the rows' log-sum-exp."""
+    request (1), or q_start int32 [requests + 1] with at most n_q each (all tokens;
+    a bound near the longest request runs faster, tokens past it are left out).
+    Returns out of q's type; lse F32 [tokens, heads] receives the rows' log-sum-exp."""
     if out is None:
         out = _new(q.shape, q.dtype, q.device, stream)
     args = _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, q_start, scale, out, lse)

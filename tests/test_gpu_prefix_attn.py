@@ -384,3 +384,16 @@ def test_attention_keeps_the_description_of_a_cache(Q, gpu):
 
     for n, n_prefix, most in ((4, 0, 40), (2, 0, 90), (3, 180, 0), (4, 180, 40), (1, 192, 16)):
         check(n, n_prefix, most)
+
+
+@pytest.mark.parametrize("qt,kv", TYPES)
+def test_attention_without_a_bound_on_the_queries_takes_all(Q, gpu, qt, kv):
+    spans = [(0, 3), (3, 3), (3, 4), (4, 11), (11, 12)]
+    c = Case(gpu, 5, 7, 12, 4, 64, 77, 50, 16, qt, kv, lens=[10, 4, 0, 50, 33], spans=spans)
+    pre, suf = Q.KVPages(*c.prefix[:2], table=c.prefix[2]), Q.KVPages(*c.suffix[:2], table=c.suffix[2])
+    lens = torch.tensor(c.lens, dtype=torch.int32, device=gpu)
+    ws = Q.prefix_attention_workspace(c.q, pre, 77, suf, lens, 50, q_start=c.q_start)
+    out = torch.full_like(c.q, 7.0)
+    Q.prefix_attention(c.q, pre, 77, suf, lens, 50, q_start=c.q_start, scale=c.scale, out=out, workspace=ws)
+    want, _, tol, _ = _batch.attention(c.q, spans, c.prefix, c.suffix, (77, c.lens), c.scale)
+    _batch.assert_close(out, want, tol, "out")
