@@ -578,7 +578,7 @@ def _prefix_attn_args(q, prefix, n_prefix, suffix, suffix_len, max_suffix, n_q, 
             if requests:  # the call's own description: pages in order, as many for each request
                 own = ctypes.pointer(q4k_kv_pages.from_buffer_copy(suffix.desc))
                 own.contents.table_len = suffix.desc.n_pages // requests
-        elif suffix.rows != requests and requests != 1:
+        elif suffix.rows != requests and (requests != 1 or suffix.rows == 0):
             raise ValueError("suffix: a table row for each request expected")
     if n_prefix and (prefix is None or prefix.rows not in (None, 1)):
         raise ValueError("n_prefix without a prefix of one table row")

@@ -397,3 +397,14 @@ def test_attention_without_a_bound_on_the_queries_takes_all(Q, gpu, qt, kv):
     Q.prefix_attention(c.q, pre, 77, suf, lens, 50, q_start=c.q_start, scale=c.scale, out=out, workspace=ws)
     want, _, tol, _ = _batch.attention(c.q, spans, c.prefix, c.suffix, (77, c.lens), c.scale)
     _batch.assert_close(out, want, tol, "out")
+
+
+def test_attention_refuses_a_table_without_rows(Q, gpu):
+    """A table of no requests for one request, whose pages would be taken in order instead."""
+    c = Case(gpu, 1, 1, 8, 2, 64, 30, 20, 16, F16, F16, lens=[20])
+    pre, lens = Q.KVPages(*c.prefix[:2], table=c.prefix[2]), torch.tensor([20], dtype=torch.int32, device=gpu)
+    with pytest.raises(ValueError):
+        Q.prefix_attention(c.q, pre, 30, Q.KVPages(*c.suffix[:2], table=c.st[:0]), lens, 20)
+    with pytest.raises(ValueError):
+        Q.prefix_attention(c.q, Q.KVPages(*c.prefix[:2], table=c.st[:0]), 30)
+    assert Q.prefix_attention(c.q[:0], pre, 30, Q.KVPages(*c.suffix[:2], table=c.st[:0]), lens[:0], 20).shape == (0, 8, 64)
