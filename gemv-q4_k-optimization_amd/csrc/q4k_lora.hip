@@ -278,8 +278,9 @@ __device__ __forceinline__ u32x4 first_w(u32x4 v, int n) {
     return v;
 }
 
+// (without activations no adapter adds anything)
 __device__ __forceinline__ int adapter_rank(const LoraParams &p, int i) {
-    if (i < 0) return 0;
+    if (i < 0 || p.K == 0) return 0;
     const int r = p.ranks ? p.ranks[i] : p.rank;
     return r < 0 ? 0 : r > p.rank ? p.rank : r;
 }
@@ -553,7 +554,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraParams p) {
     if (mb < m1) load(mb);
     // h, while the first outputs' values are on their way
     bf16x8 ht[KR][3];
-    const float scale = p.scale && t.adapter >= 0 ? p.scale[t.adapter] : 1.0f;
+    const float scale = p.scale && r > 0 ? p.scale[t.adapter] : 1.0f;  // (of rank 0 it may be alpha / 0)
     if (SH) {
         // whole rows of h side by side, summed over the splits and turned into terms once per workgroup
         constexpr int CH = KR * 4;  // pieces of eight ranks
@@ -847,7 +848,7 @@ int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *
     if (ne11 > 1 && (nb11 < 4 * ne00 || nb1 < 4 * ne01 || (src2 && nb21 < 4 * ne01))) return Q4K_EINVAL;
     if (ne11 > 1 && src2 == dst && nb21 != nb1) return Q4K_EINVAL;
     if (l.n_adapters > 0) {
-        if (!l.a || !l.b) return Q4K_EINVAL;
+        if ((ne00 > 0 && !l.a) || !l.b) return Q4K_EINVAL;
         if (l.nb_a % 2 != 0 || l.nb_b % 2 != 0 || l.nb_a_adapter % 2 != 0 || l.nb_b_adapter % 2 != 0) return Q4K_EINVAL;
         if (l.nb_a < 2 * ne00 || l.nb_b < 2 * l.rank || l.nb_a_adapter < 0 || l.nb_b_adapter < 0) return Q4K_EINVAL;
     }

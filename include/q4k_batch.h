@@ -68,7 +68,8 @@ size_t q4k_lora_workspace_bytes(const q4k_lora *lora, int64_t ne00, int64_t ne01
  * aligned and rows of dst that are 64-byte aligned run faster.  Sums are F32; the
  * F32 activations and a's products enter the matrix cores as sums of three BF16
  * values, which hold F32's 24 bits; an activation or sum that is not finite in
- * BF16 (past 3.39e38) makes its token's results NaN.  ne00 == 0 adds nothing. */
+ * BF16 (past 3.39e38) makes its token's results NaN.  With ne00 == 0 or a rank of 0
+ * an adapter adds nothing, whatever its scale and values. */
 int q4k_lora_add(const q4k_lora *lora, int64_t ne00, int64_t ne01, const float *src1, int64_t ne11,
                  int64_t nb11, const int32_t *ids, const float *src2, int64_t nb21, float *dst,
                  int64_t nb1, void *workspace, size_t workspace_bytes, void *stream);

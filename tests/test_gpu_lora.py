@@ -212,3 +212,17 @@ def test_lora_workspace_of_a_larger_batch(Q, gpu, A, K, most, N):
     ad = Q.LoraAdapters(a, b, scale=scale)
     got = Q.lora_add(ad, x, ids, base=base, workspace=Q.lora_workspace(ad, most))
     assert torch.equal(got, Q.lora_add(ad, x, ids, base=base, workspace=Q.lora_workspace(ad, N)))
+
+
+@pytest.mark.parametrize("N", [1, 40, 700])
+def test_lora_adapters_that_add_nothing(Q, gpu, N):
+    """No rank or no activations: the base, whatever scale (alpha over a rank of zero) and b hold."""
+    inf, nan = float("inf"), float("nan")
+    a, b, x, _, base, _, _ = make(gpu, N, 256, 96, 8, 3, torch.float16, 1)
+    ids = torch.arange(N, dtype=torch.int32, device=gpu) % 2 * 2
+    scale, ranks = torch.tensor([inf, 1.0, nan], device=gpu), torch.tensor([0, 8, -1], dtype=torch.int32, device=gpu)
+    b[0], b[2] = inf, nan
+    assert torch.equal(Q.lora_add(Q.LoraAdapters(a, b, scale=scale, ranks=ranks), x, ids, base=base), base)
+    assert torch.equal(Q.lora_add(Q.LoraAdapters(a[:, :, :0], b, scale=scale), x[:, :0], ids, base=base), base)
+    empty = torch.empty(3, 8, 0, dtype=torch.float16, device=gpu)
+    assert torch.equal(Q.lora_add(Q.LoraAdapters(empty, b, scale=scale), torch.empty(N, 0, device=gpu), ids, base=base), base)
