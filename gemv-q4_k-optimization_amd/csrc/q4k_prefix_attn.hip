@@ -158,7 +158,8 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
         if (rows > ((int64_t)1 << 50) / p.slots / (a.head_dim + 2)) return Q4K_EUNSUPPORTED;
         pl.bytes = (size_t)(rows * p.slots * (a.head_dim + 2) * 4);
     }
-    if (a.n_requests * a.n_q > INT32_MAX / a.n_head) return Q4K_EUNSUPPORTED;
+    // (the join counts its rows in 31 bits, up to a workgroup's past the last one)
+    if (a.n_requests * a.n_q > (INT32_MAX - 256) / a.n_head) return Q4K_EUNSUPPORTED;
     const bool f32 = a.q_type == Q4K_GGML_TYPE_F32;
     if (a.kv_type == Q4K_GGML_TYPE_F16) f32 ? attn_kernel_f16_f32(pl) : attn_kernel_f16(pl);
     else f32 ? attn_kernel_bf16_f32(pl) : attn_kernel_bf16(pl);

@@ -408,3 +408,14 @@ def test_attention_refuses_a_table_without_rows(Q, gpu):
     with pytest.raises(ValueError):
         Q.prefix_attention(c.q, Q.KVPages(*c.prefix[:2], table=c.st[:0]), 30)
     assert Q.prefix_attention(c.q[:0], pre, 30, Q.KVPages(*c.suffix[:2], table=c.st[:0]), lens[:0], 20).shape == (0, 8, 64)
+
+
+def test_attention_sizes_past_the_join(Q, gpu):
+    """Rows of requests of up to n_q tokens are counted in 31 bits, with room for a workgroup's."""
+    import ctypes
+    fake = 0x10000   # sizes only: nothing is read
+    pages = Q.q4k_kv_pages(fake, fake, 8, 4096, 1 << 20, 256, 128, 1 << 20, 256, 128, None, 0, 8)
+    size = lambda requests: Q.lib().q4k_prefix_attn_workspace_bytes(ctypes.byref(Q.q4k_prefix_attn_args(  # noqa: E731
+        0, 1, 1, 1, 8, 1.0, 4, requests, 1, fake, fake, 32, 32, ctypes.pointer(pages), 30000, None, None, 0, fake, 32, 32, None)))
+    assert size(1 << 20) > 0 and size((1 << 31) - 1000) > 0
+    assert size((1 << 31) - 1) == 0 and size((1 << 31) - 100) == 0
