@@ -291,7 +291,10 @@ __device__ __forceinline__ int attn_least(const AttnParams &p, const AttnSpan &s
 }
 
 // 32 positions' scores sx[rt][tile of 16] to probabilities, in place of the next
-// product's B operand.
+// product's B operand.  With 16-bit queries (one term) a probability is rounded once
+// to T there, the sum l takes it in F32: the result is off by 1.4 times (rms) what
+// rounding it to T costs anyway (64 rows of BF16 over 32768 positions 2.3e-3 against
+// 1.7e-3, F16 2.9e-4 against 2.1e-4); a second term would double the value product.
 template <class T, int D, int RT, int TERMS>
 __device__ __forceinline__ void attn_softmax(AttnRows<RT, D> &w, const f32x4 (&sx)[RT][2],
                                              typename Vec8<T>::type (&pf)[RT][TERMS]) {
@@ -427,7 +430,8 @@ __device__ __forceinline__ void attn_emit(const AttnParams &p, const AttnSpan &s
 // the next 32 positions' K and V on their way.  24 rows over 131072 positions of 8
 // heads of 128 BF16 dimensions (537 MB): 113 us, 4.8 TB/s with F32 queries as three
 // terms.  64 F16 rows over 8192 positions and 16 x 256 of their own, with the join:
-// 22.2 us, of which about 5 read memory: bound by the four steps' round trips.
+// 22.2 us, of which about 5 read memory: bound by the four steps' round trips.  Of 256
+// dimensions they spill 20 bytes a lane, one workgroup a CU as it is.
 template <class T, int D_, int RT_, int TERMS>
 struct StreamCfg {
     using Elem = T;
@@ -609,11 +613,14 @@ __device__ __forceinline__ void attn_stream(const AttnParams &p, const AttnCache
 }
 
 // ---- many rows: the waves take rows of their own and share K and V in LDS ----
-// 512 rows over 32768 positions of 8 heads of 128 BF16 dimensions: 69 GFLOP in about
-// 95 us, 800 TFLOP/s over long prefixes (a large library product reaches 1217).  The
+// 512 rows over 32768 positions of 8 heads of 128 BF16 dimensions: 69 GFLOP in 108 us
+// with the join (635 TFLOP/s), over 131072 in 337 us (816; a large library product
+// reaches 1217).  The
 // softmax's vector work (exponentials a quarter rate) takes 30 % of the time, the
 // matrix cores 20 %, LDS 20 %; two workgroups a CU, whose registers allow no third,
-// do not overlap them fully.  Tiles of 64 rows per wave do not fit the registers.
+// do not overlap them fully.  Tiles of 64 rows per wave do not fit the registers, nor
+// do F32 queries on F16 at 128 dimensions: their two terms a query take the 256
+// registers and 36 to 48 bytes of scratch a lane.
 template <class C, class QT, int TERMS>
 __device__ __forceinline__ void attn_shared(const AttnParams &p, const AttnCache &kv, const AttnSpan &s, int hk, int tile,
                                             char *lds, int *flags) {

@@ -17,9 +17,12 @@
 // Memory bound: 4096 tokens of 16 adapters of rank 64, K 14336, 4096 outputs take
 // 103 us (group 6, shrink 62, expand 44 one by one) where their 407 MB take 75 at a
 // copy's rate.  The shrink reads its 235 MB at 3.8 TB/s; a plain read of the same
-// tiles takes 40 us, the rest is its conversions and barriers at seven waves a CU.
+// tiles takes 40 us, the rest is its conversions and barriers at the two workgroups a
+// CU that 66 KB of LDS allow (F16 adapters of ranks above 32 take 82 KB: one).  The
+// expand moves its 139 MB at 3.2 TB/s: h is summed again for each chunk of outputs,
+// and one step of outputs is on its way while another is computed.
 // A few tokens are bound by two launches and their chains of round trips: 1 token,
-// 1024 x 4096, rank 8: 5.3 + 5.3 us; 8 tokens, 14336 x 4096, rank 16: 5.5 + 6.2.
+// 1024 x 4096, rank 8: 5.3 + 5.5 us; 8 tokens, 14336 x 4096, rank 16: 5.5 + 6.3.
 //
 // A token's sums are cut by the sizes of the call and, in the direct shrink, by how
 // many tokens its adapter has (to 64; of a slice of 512 where each workgroup looks

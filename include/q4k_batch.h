@@ -130,7 +130,9 @@ size_t q4k_prefix_attn_workspace_bytes(const q4k_prefix_attn_args *args);
  * maximum and sum and the output sum are F32.  With q_type F32 the queries and
  * probabilities enter the matrix cores as sums of two (F16) or three (BF16)
  * values of kv_type, with q_type kv_type as one rounded value.  Tokens of no
- * request are left as they are.  Up to 2^30 positions a part. */
+ * request (before, between and behind those that q_start names, or past n_q of a
+ * request) are left as they are.  dst and lse must not overlap what is read.  Up
+ * to 2^30 positions a part. */
 int q4k_prefix_attn(const q4k_prefix_attn_args *args, void *workspace, size_t workspace_bytes,
                     void *stream);
 
