@@ -1,5 +1,5 @@
 """Python binding of libq4k_gemv.so (the C ABI in include/q4k_gemv.h,
-include/q4k_batch.h and include/q4k_gguf.h).
+include/q4k_batch.h, include/q4k_step.h and include/q4k_gguf.h).
 
 The product is the C ABI; this module is plumbing for tests and the
 benchmark: it passes torch device tensors and torch's current HIP stream to
@@ -76,6 +76,21 @@ class q4k_logits_rules(ctypes.Structure):
                 ("mask", _P), ("n_masks", _I64), ("nb_mask", _I64), ("mask_rows", _P)]
 
 
+class q4k_rope_rows(ctypes.Structure):
+    """Rows of queries or keys (include/q4k_step.h)."""
+    _fields_ = [("src", _P), ("dst", _P), ("src_type", ctypes.c_int32), ("dst_type", ctypes.c_int32), ("n_head", _I64),
+                ("nb_src_token", _I64), ("nb_src_head", _I64), ("nb_dst_token", _I64), ("nb_dst_head", _I64), ("norm", _P)]
+
+
+class q4k_rope_args(ctypes.Structure):
+    """Arguments of q4k_rope (include/q4k_step.h)."""
+    _fields_ = [("head_dim", ctypes.c_int32), ("n_rot", ctypes.c_int32), ("mode", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("freq_base", ctypes.c_float), ("freq_scale", ctypes.c_float), ("ext_factor", ctypes.c_float),
+                ("attn_factor", ctypes.c_float), ("beta_fast", ctypes.c_float), ("beta_slow", ctypes.c_float),
+                ("n_ctx_orig", _I64), ("freq_factors", _P), ("n_tokens", _I64), ("pos", _P),
+                ("q", ctypes.POINTER(q4k_rope_rows)), ("k", ctypes.POINTER(q4k_rope_rows))]
+
+
 # Every symbol the headers of include/ declare: (restype, argtypes)
 SIGNATURES = {
     "q4k_version": (ctypes.c_int32, []),
@@ -114,6 +129,8 @@ SIGNATURES = {
     "q4k_prefix_attn_workspace_bytes": (ctypes.c_size_t, [_P]),
     "q4k_prefix_attn": (_I, [_P, _P, ctypes.c_size_t, _P]),
     "q4k_logits_adjust": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _P]),
+    # include/q4k_step.h
+    "q4k_rope": (_I, [_P, _P]),
     # include/q4k_gguf.h
     "q4k_gguf_open": (_I, [ctypes.c_char_p, ctypes.POINTER(_P)]),
     "q4k_gguf_close": (None, [_P]),
@@ -677,6 +694,107 @@ def logits_adjust(logits, repeat=None, frequency=None, presence=None, history=No
     if st != Q4K_OK:
         raise Q4KError(st, "q4k_logits_adjust")
     return out
+
+
+# ------------------------------------------------- operators of a decode step ----
+ROPE_NORMAL, ROPE_NEOX = 0, 2
+
+
+def _types():
+    """The ggml type and bytes of a value of the float types that rows may have."""
+    import torch
+    return {torch.float32: (GGML_TYPE_F32, 4), torch.float16: (GGML_TYPE_F16, 2), torch.bfloat16: (GGML_TYPE_BF16, 2)}
+
+
+_TYPES = {}
+
+
+def _float_type(t, what):
+    if not _TYPES:
+        _TYPES.update(_types())
+    got = _TYPES.get(t.dtype)
+    if got is None:
+        raise ValueError(f"{what}: float32, float16 or bfloat16 expected, not {t.dtype}")
+    return got
+
+
+def _on_device(name, device, *args):
+    """Calls the library with `device` (its number) as the current one."""
+    import torch
+    f = getattr(lib(), name)
+    if torch._C._cuda_getDevice() == device:
+        st = f(*args)
+    else:
+        with torch.cuda.device(device):
+            st = f(*args)
+    if st != Q4K_OK:
+        raise Q4KError(st, name)
+
+
+class Rope:
+    """The norms and position rotation of a model's heads, described once for
+    every rope call (include/q4k_step.h): n_rot of head_dim dimensions (all)
+    are rotated, mode "normal" (pairs of neighbours) or "neox" (of halves);
+    freq_factors F32 [n_rot / 2]; YaRN with ext_factor not 0 and n_ctx_orig;
+    q_norm, k_norm F32 [head_dim], eps of the norms.  The tensors are kept alive."""
+
+    def __init__(self, head_dim, n_rot=None, mode="normal", freq_base=10000.0, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0,
+                 beta_fast=32.0, beta_slow=1.0, n_ctx_orig=0, freq_factors=None, q_norm=None, k_norm=None, eps=1e-6):
+        import torch
+        _need(mode in ("normal", "neox"), 'mode: "normal" or "neox" expected')
+        n_rot = head_dim if n_rot is None else n_rot
+        self.head_dim, self.device = head_dim, None
+        self.tensors = (freq_factors, q_norm, k_norm)
+        for t in self.tensors:
+            if t is not None:
+                _need(t.is_cuda, "freq_factors, q_norm, k_norm: device tensors expected")
+                _need(self.device in (None, t.get_device()), "freq_factors, q_norm, k_norm: one device expected")
+                self.device = t.get_device()
+        dev, f32 = self.device, torch.float32
+        self.q_norm, self.k_norm = _vector(q_norm, f32, (head_dim,), dev, "q_norm"), _vector(k_norm, f32, (head_dim,), dev, "k_norm")
+        self.desc = q4k_rope_args(head_dim, n_rot, ROPE_NORMAL if mode == "normal" else ROPE_NEOX, eps, freq_base, freq_scale, ext_factor,
+                                  attn_factor, beta_fast, beta_slow, n_ctx_orig, _vector(freq_factors, f32, (n_rot // 2,), dev, "freq_factors"))
+        # (what the library refuses of it, here already: a call without tokens checks the description alone)
+        st = lib().q4k_rope(ctypes.byref(self.desc), None)
+        if st != Q4K_OK:
+            raise Q4KError(st, "q4k_rope")
+
+
+def _rope_rows(x, out, norm, tokens, dim, device, what):
+    st, es = _float_type(x, what)
+    dt, ds = _float_type(out, what)
+    if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != dim or x.get_device() != device or (x.stride(2) != 1 and dim > 1):
+        raise ValueError(f"{what}: [{tokens}, heads, {dim}] with contiguous dimensions on device {device} expected")
+    if out.shape != x.shape or out.get_device() != device or (out.stride(2) != 1 and dim > 1):
+        raise ValueError(f"{what}_out: shape and device of {what} with contiguous dimensions expected")
+    return q4k_rope_rows(x.data_ptr(), out.data_ptr(), st, dt, x.shape[1], x.stride(0) * es, x.stride(1) * es, out.stride(0) * ds,
+                         out.stride(1) * ds, norm)
+
+
+def rope(r: Rope, q, k, pos, q_out=None, k_out=None, stream=None):
+    """The norms and rotation r of queries q [tokens, heads, head_dim] and keys k
+    (either may be None) at int32 positions pos [tokens]; float32, float16 or
+    bfloat16, results of the same type in new tensors, or in q_out, k_out, which
+    may be q, k themselves or, of float32 rows, of 16 bits.  Returns (q_out, k_out)."""
+    import torch
+    some = q if q is not None else k
+    if some is None:
+        raise ValueError("q or k expected")
+    dev, n = some.get_device(), some.shape[0]
+    if dev < 0 or r.device not in (None, dev):
+        raise ValueError("q, k: tensors on the description's device expected")
+    args = q4k_rope_args.from_buffer_copy(r.desc)
+    args.n_tokens, args.pos = n, _vector(pos, torch.int32, (n,), dev, "pos")
+    if q is not None:
+        if q_out is None:
+            q_out = _new(q.shape, q.dtype, q.device, stream)
+        args.q = ctypes.pointer(_rope_rows(q, q_out, r.q_norm, n, r.head_dim, dev, "q"))
+    if k is not None:
+        if k_out is None:
+            k_out = _new(k.shape, k.dtype, k.device, stream)
+        args.k = ctypes.pointer(_rope_rows(k, k_out, r.k_norm, n, r.head_dim, dev, "k"))
+    _on_device("q4k_rope", dev, ctypes.byref(args), _stream_of(stream, dev))
+    return q_out, k_out
 
 
 # ------------------------------------------------------------------ GGUF ----

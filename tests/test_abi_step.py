@@ -1,0 +1,63 @@
+"""Argument checks of the operators of a decode step (include/q4k_step.h) that need no GPU."""
+import ctypes
+
+import pytest
+import torch
+
+FAKE = 0x10000  # never dereferenced by the host checks
+OK, EUNSUPPORTED, EINVAL = 0, 1, 2
+
+
+def rows(Q, **kw):
+    d = dict(src=FAKE, dst=FAKE + 65536, src_type=0, dst_type=0, n_head=8, nb_src_token=4096, nb_src_head=512, nb_dst_token=4096,
+             nb_dst_head=512, norm=None)
+    d.update(kw)
+    return Q.q4k_rope_rows(*d.values())
+
+
+def rope(Q, q={}, k={}, **kw):
+    d = dict(head_dim=128, n_rot=128, mode=0, eps=1e-6, freq_base=1e4, freq_scale=1.0, ext_factor=0.0, attn_factor=1.0, beta_fast=32.0,
+             beta_slow=1.0, n_ctx_orig=0, freq_factors=None, n_tokens=2, pos=FAKE)
+    d.update(kw)
+    a = Q.q4k_rope_args(*d.values())
+    for name, r in (("q", q), ("k", k)):
+        if r is not None:
+            setattr(a, name, ctypes.pointer(rows(Q, **r)))
+    return Q.lib().q4k_rope(ctypes.byref(a), None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(head_dim=0), dict(n_rot=130), dict(n_rot=3), dict(n_rot=-2), dict(mode=1), dict(mode=8), dict(eps=-1.0), dict(eps=float("nan")), dict(freq_base=0.0),
+    dict(freq_base=float("nan")), dict(freq_scale=float("inf")), dict(ext_factor=1.0), dict(ext_factor=1.0, n_ctx_orig=4096, freq_scale=0.0),
+    dict(ext_factor=1.0, n_ctx_orig=4096, freq_base=1.0), dict(ext_factor=1.0, n_ctx_orig=4096, beta_slow=0.0), dict(freq_factors=FAKE + 2),
+    dict(n_tokens=-1), dict(n_tokens=1 << 31), dict(pos=None), dict(pos=FAKE + 2), dict(q=dict(src=None)), dict(k=dict(dst=None)),
+    dict(q=dict(src=FAKE + 2)), dict(q=dict(src_type=12)), dict(q=dict(src_type=1)), dict(k=dict(src_type=1, dst_type=30)), dict(q=dict(n_head=-1)),
+    dict(q=dict(nb_src_head=508)), dict(q=dict(nb_dst_head=256)), dict(q=dict(nb_src_token=4098)), dict(k=dict(norm=FAKE + 1)), dict(q=dict(nb_dst_token=256)),
+    dict(q=dict(dst=FAKE, nb_dst_token=8192)), dict(q=dict(dst=FAKE, dst_type=1))])
+def test_rope_checks(Q, kw):
+    assert rope(Q, **kw) == EINVAL
+
+
+def test_rope_unsupported_and_empty(Q):
+    assert rope(Q, head_dim=258, n_rot=2, q=dict(nb_src_head=2048, nb_dst_head=2048), k=dict(nb_src_head=2048, nb_dst_head=2048)) == EUNSUPPORTED
+    assert rope(Q, head_dim=127, n_rot=64) == EUNSUPPORTED
+    assert rope(Q, q=dict(n_head=1 << 30)) == EUNSUPPORTED
+    assert rope(Q, n_tokens=0, pos=None) == OK
+    assert rope(Q, q=None, k=None) == OK
+    assert rope(Q, q=dict(n_head=0, src=None), k=None) == OK
+    assert Q.lib().q4k_rope(None, None) == EINVAL
+
+
+def test_rope_binding(Q):
+    x, pos = torch.zeros(3, 4, 64), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        Q.rope(Q.Rope(64), x, None, pos)
+    with pytest.raises(ValueError):
+        Q.rope(Q.Rope(64), None, None, pos)
+    with pytest.raises(ValueError):
+        Q.Rope(64, mode="half")
+    with pytest.raises(ValueError):
+        Q.Rope(64, q_norm=torch.ones(64))
+    for kw in (dict(n_rot=66), dict(n_rot=5), dict(ext_factor=1.0), dict(freq_base=-1.0)):
+        with pytest.raises(Q.Q4KError):
+            Q.Rope(64, **kw)
