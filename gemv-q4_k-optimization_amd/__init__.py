@@ -91,6 +91,23 @@ class q4k_rope_args(ctypes.Structure):
                 ("q", ctypes.POINTER(q4k_rope_rows)), ("k", ctypes.POINTER(q4k_rope_rows))]
 
 
+class q4k_kv8_pages(ctypes.Structure):
+    """Keys and values in pages of 8 bits (include/q4k_step.h)."""
+    _fields_ = [("type", ctypes.c_int32), ("n_head_kv", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("block", ctypes.c_int32),
+                ("k", _P), ("v", _P), ("n_pages", _I64), ("page_size", _I64),
+                ("nb_k_page", _I64), ("nb_k_token", _I64), ("nb_k_head", _I64),
+                ("nb_v_page", _I64), ("nb_v_token", _I64), ("nb_v_head", _I64),
+                ("k_scale", _P), ("v_scale", _P), ("nb_s_page", _I64), ("nb_s_block", _I64), ("nb_s_head", _I64),
+                ("table", _P), ("table_stride", _I64), ("table_len", _I64)]
+
+
+class q4k_kv8_rows(ctypes.Structure):
+    """The last tokens of each request (include/q4k_step.h)."""
+    _fields_ = [("pages", ctypes.POINTER(q4k_kv8_pages)), ("type", ctypes.c_int32), ("n_tokens", _I64), ("n_requests", _I64),
+                ("n_q", _I64), ("q_start", _P), ("len", _P), ("max_len", _I64), ("k", _P), ("v", _P),
+                ("nb_k_token", _I64), ("nb_k_head", _I64), ("nb_v_token", _I64), ("nb_v_head", _I64)]
+
+
 # Every symbol the headers of include/ declare: (restype, argtypes)
 SIGNATURES = {
     "q4k_version": (ctypes.c_int32, []),
@@ -131,6 +148,8 @@ SIGNATURES = {
     "q4k_logits_adjust": (_I, [_P, _I64, _I64, _I64, _P, _P, _I64, _P]),
     # include/q4k_step.h
     "q4k_rope": (_I, [_P, _P]),
+    "q4k_kv8_store": (_I, [_P, _P]),
+    "q4k_kv8_load": (_I, [_P, _P]),
     # include/q4k_gguf.h
     "q4k_gguf_open": (_I, [ctypes.c_char_p, ctypes.POINTER(_P)]),
     "q4k_gguf_close": (None, [_P]),
@@ -795,6 +814,104 @@ def rope(r: Rope, q, k, pos, q_out=None, k_out=None, stream=None):
         args.k = ctypes.pointer(_rope_rows(k, k_out, r.k_norm, n, r.head_dim, dev, "k"))
     _on_device("q4k_rope", dev, ctypes.byref(args), _stream_of(stream, dev))
     return q_out, k_out
+
+
+TYPE_I8, TYPE_E4M3 = 24, 1000
+
+
+class KV8Pages:
+    """Keys and values in 8 bits: k, v [pages, page_size, heads_kv, head_dim] of
+    int8 or float8_e4m3fn (any strides of multiples of 16, the last dimension
+    contiguous), their scales F32 [pages, page_size / block, heads_kv] (of both
+    with the same strides) and the page numbers: table int32 [requests, pages per request],
+    or None for the pages in order, as many for each request.  The tensors are kept
+    alive; their contents and the table's may change between calls."""
+
+    def __init__(self, k, v, k_scale, v_scale, table=None):
+        import torch
+        _need(k.is_cuda, "k, v: device tensors expected")
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device and k.numel() > 0,
+              "k, v: [pages, page_size, heads_kv, head_dim] of one type and shape expected")
+        _need(k.dtype in (torch.int8, torch.float8_e4m3fn), "k, v: int8 or float8_e4m3fn expected")
+        _need(k.stride(3) == 1 and v.stride(3) == 1, "head_dim of k, v is not contiguous")
+        pages, page, heads, dim = k.shape
+        for s in (k_scale, v_scale):
+            _need(s.dtype == torch.float32 and s.device == k.device and s.dim() == 3 and s.shape == k_scale.shape and
+                  s.stride() == k_scale.stride() and s.shape[0] == pages and s.shape[2] == heads and s.shape[1] > 0 and page % s.shape[1] == 0,
+                  "k_scale, v_scale: float32 [pages, page_size / block, heads_kv] of one layout expected")
+        self.tensors = (k, v, k_scale, v_scale, table)
+        self.heads, self.dim, self.device, self.rows, stride, length = heads, dim, k.get_device(), None, 0, pages
+        if table is not None:
+            _need(table.dtype == torch.int32 and table.dim() == 2 and table.device == k.device and
+                  (table.stride(1) == 1 or table.shape[1] <= 1), "table: int32 [requests, pages] with contiguous rows expected")
+            self.rows, length = table.shape
+            stride = table.stride(0)
+        self.desc = q4k_kv8_pages(TYPE_I8 if k.dtype == torch.int8 else TYPE_E4M3, heads, dim, page // k_scale.shape[1], k.data_ptr(), v.data_ptr(),
+                                  pages, page, *(k.stride(i) for i in range(3)), *(v.stride(i) for i in range(3)), k_scale.data_ptr(),
+                                  v_scale.data_ptr(), *(k_scale.stride(i) * 4 for i in range(3)),
+                                  table.data_ptr() if table is not None else None, stride, length)
+        self._p = ctypes.pointer(self.desc)
+
+    def _of(self, requests):
+        """The description for a call of so many requests."""
+        if self.rows is None:
+            if not requests:
+                return self._p
+            own = q4k_kv8_pages.from_buffer_copy(self.desc)  # pages in order, as many for each request
+            own.table_len = self.desc.n_pages // requests
+            return ctypes.pointer(own)
+        _need(self.rows == requests or (requests == 1 and self.rows > 0) or not requests, "table: a row for each request expected")
+        return self._p
+
+
+def _kv8_requests(n, n_q, q_start, lens, device):
+    """Requests, the most tokens of one, and the addresses of q_start and lens."""
+    import torch
+    start = None
+    if n_q is None:  # one token a request; as many as there are where q_start tells
+        n_q = 1 if q_start is None else n
+    if q_start is not None:
+        start = _vector(q_start, torch.int32, None, device, "q_start")
+        requests = q_start.shape[0] - 1
+        _need(requests >= 0, "q_start: requests + 1 entries expected")
+    else:
+        requests = n // n_q if n_q else 0
+    return requests, n_q, start, _vector(lens, torch.int32, (requests,), device, "lens")
+
+
+def _kv8_rows(name, pages, k, v, lens, max_len, n_q, q_start, stream):
+    some = k if k is not None else v
+    _need(some is not None, "k or v expected")
+    t, es = _float_type(some, "k, v")
+    dev, n, shape = pages.device, some.shape[0], (some.shape[0], pages.heads, pages.dim)
+    requests, n_q, start, lens = _kv8_requests(n, n_q, q_start, lens, dev)
+    at = []
+    for x in (k, v):
+        if x is None:
+            at.append((None, 0, 0))
+            continue
+        if x.shape != shape or x.dtype is not some.dtype or x.get_device() != dev or x.stride(2) != 1:
+            raise ValueError(f"k, v: {some.dtype} {list(shape)} with contiguous dimensions on device {dev} expected")
+        at.append((x.data_ptr(), x.stride(0) * es, x.stride(1) * es))
+    (kp, *ks), (vp, *vs) = at
+    args = q4k_kv8_rows(pages._of(requests), t, n, requests, n_q, start, lens, max_len, kp, vp, *ks, *vs)
+    _on_device(name, dev, ctypes.byref(args), _stream_of(stream, dev))
+
+
+def kv8_store(pages: KV8Pages, k, v, lens, max_len, n_q=None, q_start=None, stream=None):
+    """Writes the requests' new keys and values k, v [tokens, heads_kv, head_dim]
+    (float32, float16 or bfloat16) into their pages: the last of each request's lens[r]
+    <= max_len tokens (int32, with the new ones), n_q each (1), or those that q_start
+    int32 [requests + 1] names, at most n_q each (all tokens)."""
+    _need(k is not None and v is not None, "k and v expected")
+    _kv8_rows("q4k_kv8_store", pages, k, v, lens, max_len, n_q, q_start, stream)
+
+
+def kv8_load(pages: KV8Pages, k, v, lens, max_len, n_q=None, q_start=None, stream=None):
+    """Reads each request's last tokens into k, v (either may be None), as the
+    values that the pages' bytes stand for; requests and tokens as in kv8_store."""
+    _kv8_rows("q4k_kv8_load", pages, k, v, lens, max_len, n_q, q_start, stream)
+    return k, v
 
 
 # ------------------------------------------------------------------ GGUF ----

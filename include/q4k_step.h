@@ -3,6 +3,9 @@
  * projections (q4k_gemv.h) and its next token (MI355X, gfx950):
  *   q4k_rope        norms of queries and keys for each head and the rotation by
  *                   their positions, in one pass
+ *   q4k_kv8_store   new keys and values into a paged cache of 8 bits with a scale
+ *                   for each block of tokens and head
+ *   q4k_kv8_load    tokens of such a cache as the values they stand for
  * No counterpart in the reference, whose path ends at the product.
  *
  * Conventions as in q4k_batch.h: strides (nb*) in bytes, a q4k_status, device
@@ -63,6 +66,66 @@ typedef struct q4k_rope_args {
  * rotations are F32, results are rounded once.  Rows of 16-byte aligned addresses
  * and strides, with n_rot / 2 and head_dim - n_rot multiples of 4 and 8, run faster. */
 int q4k_rope(const q4k_rope_args *args, void *stream);
+
+/* ------------------------------------- keys and values in 8 bits, paged */
+
+#define Q4K_TYPE_I8 24     /* GGML_TYPE_I8: -127..127 times the scale */
+#define Q4K_TYPE_E4M3 1000 /* OCP 8-bit floats of 4 exponent bits, up to 448, times the scale (no ggml type) */
+
+#define Q4K_KV8_MAX_HEAD_DIM 256
+
+/* Keys and values in pages of page_size tokens, one byte a value: token t of head
+ * h in page p is at k + p * nb_k_page + t * nb_k_token + h * nb_k_head, head_dim
+ * contiguous values (v alike), and stands for its values times the scale at
+ * k_scale + p * nb_s_page + (t / block) * nb_s_block + h * nb_s_head (v_scale
+ * alike, with the same strides).  page_size is a multiple of block.  k, v and
+ * their strides are multiples of 16 bytes, else Q4K_EUNSUPPORTED. */
+typedef struct q4k_kv8_pages {
+    int32_t type;  /* Q4K_TYPE_I8 or Q4K_TYPE_E4M3 */
+    int32_t n_head_kv, head_dim; /* head_dim: a multiple of 16 up to Q4K_KV8_MAX_HEAD_DIM */
+    int32_t block; /* tokens of a scale */
+    void *k, *v;   /* (only q4k_kv8_store writes) */
+    int64_t n_pages, page_size;
+    int64_t nb_k_page, nb_k_token, nb_k_head;
+    int64_t nb_v_page, nb_v_token, nb_v_head;
+    float *k_scale, *v_scale;
+    int64_t nb_s_page, nb_s_block, nb_s_head;
+    /* page numbers as in q4k_kv_pages; NULL: pages r * table_len, r * table_len + 1, ... */
+    const int32_t *table;
+    int64_t table_stride, table_len;
+} q4k_kv8_pages;
+
+/* The last tokens of each request: with len = len[r] and n tokens, token t of
+ * request r has position len - n + t. */
+typedef struct q4k_kv8_rows {
+    const q4k_kv8_pages *pages;
+    int32_t type;           /* of k and v here: Q4K_GGML_TYPE_F32, _F16 or _BF16 */
+    int64_t n_tokens, n_requests;
+    int64_t n_q;            /* tokens of each request, with q_start the most of any */
+    const int32_t *q_start; /* as in q4k_prefix_attn_args; NULL: r * n_q */
+    const int32_t *len;     /* device, n_requests, clamped to 0..max_len */
+    int64_t max_len;        /* up to 2^30 */
+    void *k, *v;            /* n_tokens rows of n_head_kv heads of head_dim (q4k_kv8_store: read only) */
+    int64_t nb_k_token, nb_k_head, nb_v_token, nb_v_head;
+} q4k_kv8_rows;
+
+/* Writes each request's new tokens into its pages.  A block's scale becomes the
+ * largest magnitude of its new tokens / 127 (E4M3: / 448), or stays what it is
+ * where the block holds earlier tokens of the request and their scale is larger;
+ * where it grows, the earlier tokens are rounded again from the values that they
+ * stood for (in F32).  Values are the nearest to x / scale, ties to even (worked out exactly);
+ * infinities and values that are not finite take no part in the magnitude and
+ * become the largest of their sign, NaN 0.  Tokens at positions below 0 or in
+ * pages out of range are left out, bytes of positions that no new or earlier
+ * token of the block has stay as they are.  Two requests' new tokens must not fall
+ * into one block, nor a block of one hold earlier tokens of another that is
+ * read meanwhile. */
+int q4k_kv8_store(const q4k_kv8_rows *rows, void *stream);
+
+/* Reads each request's last tokens as the values they stand for, rounded to
+ * `type`: zeros at positions below 0 and in pages out of range.  Rows of no
+ * request stay as they are.  k or v may be NULL. */
+int q4k_kv8_load(const q4k_kv8_rows *rows, void *stream);
 
 #ifdef __cplusplus
 }

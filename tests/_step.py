@@ -49,3 +49,72 @@ def rope(x, pos, n_rot, mode, base=10000.0, freq_scale=1.0, ext=0.0, attn=1.0, f
         tol = both * (10 * u + far) + abs(m) * (mag[..., a] + mag[..., b])
         mag[..., a], mag[..., b] = tol, tol
     return y, mag + UNIT[out or torch.float32] * y.abs() * (1 + 2.0 ** -8) + 1e-38 + (2.0 ** -25 if out == torch.float16 else 0)
+
+
+# ------------------------------------------------------------ caches of 8 bits ----
+TOP = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+#: every value of e4m3 from 0 up, by its code
+CODES = torch.tensor([m / 8 * 2.0 ** -6 if e == 0 else (1 + m / 8) * 2.0 ** (e - 7) for e in range(16) for m in range(8)][:127],
+                     dtype=torch.float64)
+
+
+def round8(x, scale, dtype):
+    """x / scale in 64 bits to the nearest value of dtype (as its bytes' values, float64),
+    ties to even; x F32, scale F32 of x's shape."""
+    y = x.double() / torch.where(scale > 0, scale, 1.0).double()
+    y = torch.where(scale > 0, y, 0.0)
+    y = torch.where(torch.isinf(x), x.double(), y)
+    y = torch.where(torch.isnan(x), 0.0, y).clamp(-TOP[dtype], TOP[dtype])
+    if dtype == torch.int8:
+        return torch.round(y)
+    mid = (CODES[1:] + CODES[:-1]) / 2
+    i = torch.searchsorted(mid, y.abs().contiguous())
+    i = i + ((y.abs() == mid[i.clamp(max=125)]) & (i % 2 == 1)).long()
+    return torch.sign(y) * CODES[i]
+
+
+class Cache8:
+    """A cache of 8 bits in plain steps on the CPU: bytes' values [pages, page, heads, dim] float64, scales F32."""
+
+    def __init__(self, k, v, k_scale, v_scale, table):
+        self.dtype = k.dtype
+        self.held = [t.cpu().float().double() for t in (k, v)]
+        self.scale = [t.cpu().clone() for t in (k_scale, v_scale)]
+        self.table, self.page = table.long().cpu(), k.shape[1]
+        self.block = self.page // k_scale.shape[1]
+
+    def place(self, r, t):
+        p = int(self.table[r, t // self.page])
+        return (p, t % self.page) if 0 <= p < self.held[0].shape[0] else None
+
+    def store(self, new, spans, lens):
+        """new: (k, v) rows; spans: [first, last) tokens of a request."""
+        for r, (t0, t1) in enumerate(spans):
+            first = lens[r] - (t1 - t0)
+            for b0 in sorted({t // self.block * self.block for t in range(max(first, 0), lens[r])}):
+                at = self.place(r, b0)
+                if at is None:
+                    continue
+                p, s0 = at
+                lo, hi = max(first, b0), min(lens[r], b0 + self.block)
+                for held, scale, x in zip(self.held, self.scale, new):
+                    rows = x[t0 + lo - first:t0 + hi - first].float().cpu()           # [n, heads, dim]
+                    top = torch.where(torch.isfinite(rows), rows.abs(), 0.0).amax((0, 2))
+                    s = (top.double() / TOP[self.dtype]).float()
+                    was = scale[p, s0 // self.block]
+                    if lo > b0:
+                        s = torch.maximum(s, was)
+                        old = held[p, s0:s0 + lo - b0]
+                        again = round8((old * was.double()[:, None]).float(), s[:, None].expand(old.shape), self.dtype)
+                        held[p, s0:s0 + lo - b0] = torch.where((s > was)[:, None], again, old)
+                    held[p, s0 + lo - b0:s0 + hi - b0] = round8(rows, s[:, None].expand(rows.shape), self.dtype)
+                    scale[p, s0 // self.block] = s
+
+    def values(self, r, length):
+        """Keys and values of the first tokens of a request, float64, and which have a page."""
+        at = torch.arange(length)
+        pages = self.table[r][at // self.page]
+        ok = (pages >= 0) & (pages < self.held[0].shape[0])
+        pages = torch.where(ok, pages, 0)
+        s = at % self.page
+        return [h[pages, s] * c[pages, s // self.block].double()[:, :, None] for h, c in zip(self.held, self.scale)] + [ok]

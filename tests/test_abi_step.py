@@ -61,3 +61,53 @@ def test_rope_binding(Q):
     for kw in (dict(n_rot=66), dict(n_rot=5), dict(ext_factor=1.0), dict(freq_base=-1.0)):
         with pytest.raises(Q.Q4KError):
             Q.Rope(64, **kw)
+
+
+def kv8(Q, **kw):
+    d = dict(type=24, n_head_kv=8, head_dim=128, block=16, k=FAKE, v=FAKE, n_pages=8, page_size=16, nb_k_page=16384, nb_k_token=1024,
+             nb_k_head=128, nb_v_page=16384, nb_v_token=1024, nb_v_head=128, k_scale=FAKE, v_scale=FAKE, nb_s_page=32, nb_s_block=32,
+             nb_s_head=4, table=FAKE, table_stride=4, table_len=4)
+    d.update(kw)
+    return Q.q4k_kv8_pages(*d.values())
+
+
+def kv8_rows(Q, name, pages={}, **kw):
+    d = dict(pages=ctypes.pointer(kv8(Q, **pages)) if pages is not None else None, type=0, n_tokens=2, n_requests=2, n_q=1, q_start=None, len=FAKE,
+             max_len=64, k=FAKE, v=FAKE, nb_k_token=4096, nb_k_head=512, nb_v_token=4096, nb_v_head=512)
+    d.update(kw)
+    a = Q.q4k_kv8_rows(*d.values())
+    return getattr(Q.lib(), name)(ctypes.byref(a), None)
+
+
+PAGES_INVALID = [dict(type=0), dict(type=1), dict(n_head_kv=0), dict(head_dim=0), dict(block=0), dict(block=32), dict(k=None), dict(v_scale=None),
+                 dict(n_pages=0), dict(page_size=0), dict(k_scale=FAKE + 2), dict(nb_s_head=2), dict(table=FAKE + 2), dict(table_len=-1),
+                 dict(table_len=3), dict(table_stride=-1), dict(table=None, table_len=5)]
+PAGES_UNSUPPORTED = [dict(head_dim=120), dict(head_dim=272), dict(k=FAKE + 8), dict(nb_v_token=1032), dict(nb_k_page=16392)]
+
+
+@pytest.mark.parametrize("name", ["q4k_kv8_store", "q4k_kv8_load"])
+def test_kv8_rows_checks(Q, name):
+    for pages in PAGES_INVALID:
+        assert kv8_rows(Q, name, pages) == EINVAL, pages
+    for pages in PAGES_UNSUPPORTED:
+        assert kv8_rows(Q, name, pages, nb_k_head=2048, nb_v_head=2048) == EUNSUPPORTED, pages
+    for kw in (dict(pages=None), dict(type=12), dict(n_tokens=-1), dict(n_tokens=3), dict(n_requests=-1), dict(n_q=-1), dict(n_q=2), dict(q_start=FAKE + 2),
+               dict(len=None), dict(len=FAKE + 1), dict(max_len=-1), dict(max_len=65), dict(k=FAKE + 2), dict(nb_v_head=508), dict(nb_k_token=4098)):
+        assert kv8_rows(Q, name, **kw) == EINVAL, kw
+    big = dict(page_size=1 << 30, table_len=4)
+    assert kv8_rows(Q, name, big, max_len=(1 << 30) + 1) == EUNSUPPORTED
+    assert kv8_rows(Q, name, n_tokens=5, n_requests=1 << 16, n_q=1 << 16, q_start=FAKE) == EUNSUPPORTED
+    assert kv8_rows(Q, name, n_tokens=0, n_requests=0, len=None, k=None, v=None) == OK
+    assert kv8_rows(Q, name, n_tokens=0, n_q=0) == OK
+    assert getattr(Q.lib(), name)(None, None) == EINVAL
+
+
+def test_kv8_store_needs_both(Q):
+    assert kv8_rows(Q, "q4k_kv8_store", k=None) == EINVAL and kv8_rows(Q, "q4k_kv8_store", v=None) == EINVAL
+    assert kv8_rows(Q, "q4k_kv8_load", k=None, v=None) == OK
+
+
+def test_kv8_binding_refuses_host_memory(Q):
+    k = torch.zeros(2, 16, 2, 64, dtype=torch.int8)
+    with pytest.raises(ValueError):
+        Q.KV8Pages(k, k, torch.zeros(2, 1, 2), torch.zeros(2, 1, 2))
