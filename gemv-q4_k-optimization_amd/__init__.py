@@ -108,6 +108,13 @@ class q4k_kv8_rows(ctypes.Structure):
                 ("nb_k_token", _I64), ("nb_k_head", _I64), ("nb_v_token", _I64), ("nb_v_head", _I64)]
 
 
+class q4k_kv8_attn_args(ctypes.Structure):
+    """Arguments of q4k_kv8_attn (include/q4k_step.h)."""
+    _fields_ = [("pages", ctypes.POINTER(q4k_kv8_pages)), ("q_type", ctypes.c_int32), ("n_head", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("n_tokens", _I64), ("n_requests", _I64), ("n_q", _I64), ("q_start", _P), ("len", _P), ("max_len", _I64),
+                ("q", _P), ("nb_q_token", _I64), ("nb_q_head", _I64), ("dst", _P), ("nb_dst_token", _I64), ("nb_dst_head", _I64), ("lse", _P)]
+
+
 # Every symbol the headers of include/ declare: (restype, argtypes)
 SIGNATURES = {
     "q4k_version": (ctypes.c_int32, []),
@@ -150,6 +157,8 @@ SIGNATURES = {
     "q4k_rope": (_I, [_P, _P]),
     "q4k_kv8_store": (_I, [_P, _P]),
     "q4k_kv8_load": (_I, [_P, _P]),
+    "q4k_kv8_attn_workspace_bytes": (ctypes.c_size_t, [_P]),
+    "q4k_kv8_attn": (_I, [_P, _P, ctypes.c_size_t, _P]),
     # include/q4k_gguf.h
     "q4k_gguf_open": (_I, [ctypes.c_char_p, ctypes.POINTER(_P)]),
     "q4k_gguf_close": (None, [_P]),
@@ -912,6 +921,54 @@ def kv8_load(pages: KV8Pages, k, v, lens, max_len, n_q=None, q_start=None, strea
     values that the pages' bytes stand for; requests and tokens as in kv8_store."""
     _kv8_rows("q4k_kv8_load", pages, k, v, lens, max_len, n_q, q_start, stream)
     return k, v
+
+
+def _kv8_attn_args(q, pages, lens, max_len, n_q, q_start, scale, out, lse):
+    dev = pages.device
+    if q.dim() != 3 or q.shape[2] != pages.dim or q.get_device() != dev or (q.stride(2) != 1 and pages.dim > 1):
+        raise ValueError("q: [tokens, heads, head_dim] with contiguous dimensions, of the cache's head_dim and device expected")
+    n, heads, dim = q.shape
+    t, es = _float_type(q, "q")
+    requests, n_q, start, lens = _kv8_requests(n, n_q, q_start, lens, dev)
+    if out is None:
+        out = q
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev or (out.stride(2) != 1 and dim > 1):
+        raise ValueError("out: shape, type and device of q with contiguous dimensions expected")
+    if lse is not None:
+        lse = _lse(lse, n, heads, dev)
+    return q4k_kv8_attn_args(pages._of(requests), t, heads, dim ** -0.5 if scale is None else scale, n, requests, n_q, start, lens, max_len,
+                             q.data_ptr(), q.stride(0) * es, q.stride(1) * es, out.data_ptr(), out.stride(0) * es, out.stride(1) * es, lse)
+
+
+def _lse(lse, n, heads, device):
+    import torch
+    if lse.shape != (n, heads) or lse.dtype is not torch.float32 or lse.get_device() != device or not lse.is_contiguous():
+        raise ValueError("lse: contiguous float32 [tokens, heads] expected")
+    return lse.data_ptr()
+
+
+def kv8_attention_workspace(q, pages: KV8Pages, lens, max_len, n_q=None, q_start=None):
+    """A workspace for kv8_attention calls of these sizes."""
+    import torch
+    args = _kv8_attn_args(q, pages, lens, max_len, n_q, q_start, None, None, None)
+    with torch.cuda.device(pages.device):
+        n = int(lib().q4k_kv8_attn_workspace_bytes(ctypes.byref(args)))
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
+
+
+def kv8_attention(q, pages: KV8Pages, lens, max_len, n_q=None, q_start=None, scale=None, out=None, lse=None, workspace=None, stream=None):
+    """Attention of a batch over its caches of 8 bits: q [tokens, heads, head_dim]
+    (float32, float16 or bfloat16) are the last of each request's lens[r] <= max_len
+    tokens (int32), n_q each (1), or those that q_start int32 [requests + 1] names, at
+    most n_q each (all tokens; a bound near the longest request runs faster).  Returns
+    out of q's type; lse F32 [tokens, heads] receives the rows' log-sum-exp."""
+    if out is None:
+        out = _new(q.shape, q.dtype, q.device, stream)
+    args = _kv8_attn_args(q, pages, lens, max_len, n_q, q_start, scale, out, lse)
+    dev = pages.device
+    ws, ws_bytes = _ws(workspace, dev)
+    _on_device("q4k_kv8_attn", dev, ctypes.byref(args), ws, ws_bytes, _stream_of(stream, dev))
+    return out
 
 
 # ------------------------------------------------------------------ GGUF ----

@@ -1,0 +1,124 @@
+// q4k_kv8_attn.hip -- q4k_kv8_attn (include/q4k_step.h): attention of a batch of
+// requests over their paged caches of 8 bits.  The kernel is in q4k_kv8_attn.h;
+// here are the argument checks, the split of the work and the launches.
+#include "q4k_kv8_attn.h"
+
+namespace q4k {
+
+static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+static int kv8_attn_check(const q4k_kv8_attn_args *args, bool &empty) {
+    if (!args || !args->pages) return Q4K_EINVAL;
+    const q4k_kv8_attn_args &a = *args;
+    const q4k_kv8_pages &c = *a.pages;
+    if (!kv8_kind_ok(c)) return Q4K_EINVAL;
+    if (a.q_type != Q4K_GGML_TYPE_F32 && a.q_type != Q4K_GGML_TYPE_F16 && a.q_type != Q4K_GGML_TYPE_BF16) return Q4K_EINVAL;
+    if (a.n_head < 1 || a.n_head % c.n_head_kv != 0) return Q4K_EINVAL;
+    const int st = kv8_tokens_check(a.n_tokens, a.n_requests, a.n_q, a.q_start, a.len, a.max_len, empty);
+    if (st != Q4K_OK || empty) return st;
+    const int es = a.q_type == Q4K_GGML_TYPE_F32 ? 4 : 2;
+    if (!a.q || !a.dst || !aligned(a.q, es) || !aligned(a.dst, es) || !aligned(a.lse, 4)) return Q4K_EINVAL;
+    if ((a.nb_q_token | a.nb_q_head | a.nb_dst_token | a.nb_dst_head) & (es - 1)) return Q4K_EINVAL;
+    if (a.n_head > 1 && (a.nb_q_head < es * (int64_t)c.head_dim || a.nb_dst_head < es * (int64_t)c.head_dim)) return Q4K_EINVAL;
+    if (!kv8_pages_ok(c, a.max_len, a.n_requests)) return Q4K_EINVAL;
+    return kv8_pages_vec(c) ? Q4K_OK : Q4K_EUNSUPPORTED;
+}
+
+static int kv8_attn_plan(const q4k_kv8_attn_args &a, int cus, Kv8AttnPlan &pl) {
+    pl = Kv8AttnPlan{};
+    const q4k_kv8_pages &c = *a.pages;
+    AttnParams &p = pl.p.a;
+    pl.p.c = kv8_cache(c);
+    p.q = (const char *)a.q;
+    p.dst = (char *)a.dst;
+    p.lse = a.lse;
+    p.q_token = a.nb_q_token; p.q_head = a.nb_q_head; p.dst_token = a.nb_dst_token; p.dst_head = a.nb_dst_head;
+    p.q_start = a.q_start;
+    p.suffix_len = a.len;
+    p.n_tokens = (int)a.n_tokens; p.n_requests = (int)a.n_requests; p.n_q = (int)a.n_q;
+    p.max_suffix = (int)a.max_len;
+    p.n_head = a.n_head; p.n_head_kv = c.n_head_kv; p.group = a.n_head / c.n_head_kv; p.head_dim = c.head_dim;
+    p.group_div = fastdiv_init((uint32_t)p.group);
+    p.scale = a.scale;
+    p.q_vec = aligned(a.q, 16) && ((a.nb_q_token | a.nb_q_head) & 15) == 0;
+    pl.dim = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+    pl.i8 = c.type == Q4K_TYPE_I8;
+    pl.block8 = c.block % 8 == 0;
+    if (a.n_q > INT32_MAX / p.group - 256) return Q4K_EUNSUPPORTED;
+    const int64_t rows = a.n_q * p.group;
+    pl.rt = rows <= 16 || pl.dim == 256 ? 1 : 2;
+    const int64_t tiles = cdiv(rows, 16 * pl.rt);
+    if (tiles > INT32_MAX / 4 / p.n_head_kv / a.n_requests) return Q4K_EUNSUPPORTED;
+    const int64_t per = tiles * p.n_head_kv * a.n_requests;
+    // Splits of one length in whole steps of 128 positions.
+    int64_t len = cdiv(cdiv(a.max_len * per, 3 * (int64_t)cus), 128) * 128;
+    if (len < 256) len = 256;
+    if (len > (1 << 30)) len = 1 << 30;
+    p.suf_len = (int)len;
+    p.suf_tiles = (int)tiles;
+    p.suf_splits = a.max_len > 0 ? (int)cdiv(a.max_len, len) : 1;
+    if (per * p.suf_splits > INT32_MAX / 2) return Q4K_EUNSUPPORTED;
+    p.suf_items = (int)(per * p.suf_splits);
+    p.slots = p.suf_splits;
+    p.join = p.slots > 1;
+    // (the join as in q4k_prefix_attn.hip)
+    const int groups = 256 / (p.head_dim / 4);
+    p.join_groups = 1;
+    while (p.join_groups * 4 < p.slots && p.join_groups * 2 <= groups) p.join_groups *= 2;
+    p.join_rows = groups / p.join_groups;
+    if (p.join) {
+        const int64_t all = a.n_tokens * a.n_head;
+        if (all > ((int64_t)1 << 50) / p.slots / (p.head_dim + 2)) return Q4K_EUNSUPPORTED;
+        pl.bytes = (size_t)(all * p.slots * (p.head_dim + 2) * 4);
+    }
+    // (the join counts its rows in 31 bits, up to a workgroup's past the last one)
+    if (a.n_requests * a.n_q > (INT32_MAX - 256) / a.n_head) return Q4K_EUNSUPPORTED;
+    a.q_type == Q4K_GGML_TYPE_F32 ? kv8_attn_f32(pl) : a.q_type == Q4K_GGML_TYPE_F16 ? kv8_attn_f16(pl) : kv8_attn_bf16(pl);
+    return Q4K_OK;
+}
+
+}  // namespace q4k
+
+using namespace q4k;
+
+extern "C" {
+
+size_t q4k_kv8_attn_workspace_bytes(const q4k_kv8_attn_args *args) {
+    bool empty;
+    if (kv8_attn_check(args, empty) != Q4K_OK || empty) return 0;
+    DeviceInfo *di;
+    Kv8AttnPlan pl;
+    if (device_info(&di) != Q4K_OK || kv8_attn_plan(*args, di->cus, pl) != Q4K_OK) return 0;
+    return pl.bytes;
+}
+
+int q4k_kv8_attn(const q4k_kv8_attn_args *args, void *workspace, size_t workspace_bytes, void *stream) {
+    bool empty;
+    int st = kv8_attn_check(args, empty);
+    if (st != Q4K_OK || empty) return st;
+    DeviceInfo *di;
+    st = device_info(&di);
+    if (st != Q4K_OK) return st;
+    Kv8AttnPlan pl;
+    st = kv8_attn_plan(*args, di->cus, pl);
+    if (st != Q4K_OK) return st;
+    st = ensure_lds(di, pl.kernel, pl.lds);
+    if (st != Q4K_OK) return st;
+    Workspace ws;
+    st = ws.begin(workspace, workspace_bytes, pl.bytes, stream);
+    if (st != Q4K_OK) return st;
+    AttnParams &p = pl.p.a;
+    p.part_o = (float *)ws.ptr;
+    p.part_ml = (float2 *)(p.part_o + (int64_t)p.n_tokens * p.n_head * p.slots * p.head_dim);
+    st = launch((void (*)(Kv8AttnParams))pl.kernel, dim3((unsigned)p.suf_items), 256, pl.lds, stream, pl.p);
+    if (st == Q4K_OK && p.join) {
+        using Fn = void (*)(AttnParams);
+        const Fn join = args->q_type == Q4K_GGML_TYPE_F32   ? prefix_attn_join_kernel<float>
+                        : args->q_type == Q4K_GGML_TYPE_F16 ? prefix_attn_join_kernel<_Float16>
+                                                            : prefix_attn_join_kernel<__bf16>;
+        st = launch(join, dim3((unsigned)cdiv((int64_t)p.n_requests * p.n_q * p.n_head, p.join_rows)), 256, 0, stream, p);
+    }
+    return ws.end(st, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,6 @@
+// q4k_kv8_attn_bf16.hip -- the attention kernels over caches of 8 bits for BF16 queries
+#include "q4k_kv8_attn.h"
+
+namespace q4k {
+void kv8_attn_bf16(Kv8AttnPlan &pl) { kv8_attn_kernel_of<__bf16>(pl); }
+}  // namespace q4k

@@ -6,6 +6,7 @@
  *   q4k_kv8_store   new keys and values into a paged cache of 8 bits with a scale
  *                   for each block of tokens and head
  *   q4k_kv8_load    tokens of such a cache as the values they stand for
+ *   q4k_kv8_attn    attention of a batch of requests over such a cache
  * No counterpart in the reference, whose path ends at the product.
  *
  * Conventions as in q4k_batch.h: strides (nb*) in bytes, a q4k_status, device
@@ -126,6 +127,38 @@ int q4k_kv8_store(const q4k_kv8_rows *rows, void *stream);
  * `type`: zeros at positions below 0 and in pages out of range.  Rows of no
  * request stay as they are.  k or v may be NULL. */
 int q4k_kv8_load(const q4k_kv8_rows *rows, void *stream);
+
+typedef struct q4k_kv8_attn_args {
+    const q4k_kv8_pages *pages;
+    int32_t q_type;  /* of q and dst: Q4K_GGML_TYPE_F32, _F16 or _BF16 */
+    int32_t n_head;  /* a multiple of pages->n_head_kv */
+    float scale;     /* factor of q.k, usually head_dim^-0.5 */
+    int64_t n_tokens, n_requests;
+    int64_t n_q;            /* as in q4k_kv8_rows */
+    const int32_t *q_start;
+    const int32_t *len;
+    int64_t max_len;
+    const void *q;
+    int64_t nb_q_token, nb_q_head;
+    void *dst;
+    int64_t nb_dst_token, nb_dst_head;
+    float *lse; /* n_tokens x n_head, as in q4k_prefix_attn_args; may be NULL */
+} q4k_kv8_attn_args;
+
+/* Bytes of workspace that q4k_kv8_attn takes (0 if the arguments are invalid or
+ * it takes none). */
+size_t q4k_kv8_attn_workspace_bytes(const q4k_kv8_attn_args *args);
+
+/* Attention of every request's last tokens over the request's tokens: token t of n
+ * sees positions up to len - n + t.  What a query does not see has no effect on
+ * it; one that sees nothing gives zeros and an lse of -inf; tokens of no request
+ * are left as they are.  Scores, the softmax's maximum and sum and the output sum
+ * are F32.  Bytes enter the matrix cores exactly, as F16 (keys; BF16 with BF16
+ * queries) and BF16 (values), scales are applied in F32; queries of F32 enter as
+ * two F16 values (22 bits), probabilities times their value's scale as three BF16
+ * values with F32 queries, two with F16 and one with BF16.  Scales of values below
+ * 2^100.  dst and lse must not overlap what is read. */
+int q4k_kv8_attn(const q4k_kv8_attn_args *args, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -118,3 +118,48 @@ class Cache8:
         pages = torch.where(ok, pages, 0)
         s = at % self.page
         return [h[pages, s] * c[pages, s // self.block].double()[:, :, None] for h, c in zip(self.held, self.scale)] + [ok]
+
+
+# ------------------------------------------------ attention over caches of 8 bits ----
+#: what a probability times its value's scale keeps: terms of BF16, three, two and one
+PROBABILITY = {torch.float32: 2.0 ** -23, torch.float16: 2.0 ** -15, torch.bfloat16: 2.0 ** -8}
+
+
+def attention8(q, spans, cache, lens, scale):
+    """(out, lse, bound of out, bound of lse) of queries q [tokens, heads, dim], the
+    spans' [first, last) tokens of each request, over a Cache8.
+
+    The bounds: a score is off by e, 2^-17 of sum |q k| (two F16 terms of a query
+    2^-22 of each product, F32 sums of up to 256 of them and their scale and factor
+    below 64 units of 2^-24); a probability by 2 e, the exponent's units (2^-22) and what
+    its terms keep; a sum over n positions by a unit for each step of a wave (n /
+    128) and 40 more for its lanes, waves and splits."""
+    H, D = q.shape[1], q.shape[2]
+    hk = cache.held[0].shape[2]
+    u, uo = PROBABILITY[q.dtype], UNIT[q.dtype]
+    qd = q.double().cpu()
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    lse = torch.full(q.shape[:2], -float("inf"), dtype=torch.float64)
+    tol, tol_lse = torch.zeros_like(out), torch.zeros_like(lse)
+    for r, (t0, t1) in enumerate(spans):
+        length = max(0, lens[r])
+        k, v, ok = cache.values(r, length)
+        for t in range(t0, t1):
+            seen = ok.clone()
+            seen[max(0, length - (t1 - t0) + (t - t0) + 1):] = False
+            if not seen.any():
+                continue
+            ks = k[seen].repeat_interleave(H // hk, 1)
+            vs = v[seen].repeat_interleave(H // hk, 1)
+            s = (ks * qd[t]).sum(-1) * scale                                    # [L, H]
+            e = (ks.abs() * qd[t].abs()).sum(-1).amax(0) * abs(scale) * 2.0 ** -17 + 2.0 ** -22
+            lse[t] = torch.logsumexp(s, 0)
+            p = torch.softmax(s, 0)
+            out[t] = (p[:, :, None] * vs).sum(0)
+            mass = (p[:, :, None] * vs.abs()).sum(0)
+            sums = (s.shape[0] / 128 + 40) * 2.0 ** -24
+            tol[t] = (u + 2 * e[:, None] + 2 * sums) * mass + uo * out[t].abs() * 1.01 + 1e-30
+            tol_lse[t] = 2 * e + 2 * sums + 2.0 ** -21 * lse[t].abs()
+            if q.dtype == torch.float16:
+                tol[t] += 2.0 ** -25
+    return out, lse, tol, tol_lse

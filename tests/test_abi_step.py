@@ -111,3 +111,26 @@ def test_kv8_binding_refuses_host_memory(Q):
     k = torch.zeros(2, 16, 2, 64, dtype=torch.int8)
     with pytest.raises(ValueError):
         Q.KV8Pages(k, k, torch.zeros(2, 1, 2), torch.zeros(2, 1, 2))
+
+
+def kv8_attn(Q, pages={}, **kw):
+    d = dict(pages=ctypes.pointer(kv8(Q, **pages)) if pages is not None else None, q_type=0, n_head=32, scale=1.0, n_tokens=2, n_requests=2, n_q=1,
+             q_start=None, len=FAKE, max_len=64, q=FAKE, nb_q_token=16384, nb_q_head=512, dst=FAKE, nb_dst_token=16384, nb_dst_head=512, lse=None)
+    d.update(kw)
+    a = Q.q4k_kv8_attn_args(*d.values())
+    return Q.lib().q4k_kv8_attn(ctypes.byref(a), None, 0, None), Q.lib().q4k_kv8_attn_workspace_bytes(ctypes.byref(a))
+
+
+def test_kv8_attn_checks(Q):
+    for pages in PAGES_INVALID:
+        assert kv8_attn(Q, pages) == (EINVAL, 0), pages
+    for pages in PAGES_UNSUPPORTED:
+        assert kv8_attn(Q, pages, nb_q_head=2048, nb_dst_head=2048) == (EUNSUPPORTED, 0), pages
+    for kw in (dict(pages=None), dict(q_type=24), dict(q_type=12), dict(n_head=0), dict(n_head=33), dict(n_tokens=-1), dict(n_tokens=3), dict(n_requests=-1),
+               dict(n_q=-1), dict(q_start=FAKE + 2), dict(len=None), dict(len=FAKE + 2), dict(max_len=-1), dict(max_len=65), dict(q=None), dict(dst=None),
+               dict(q=FAKE + 2), dict(dst=FAKE + 1), dict(lse=FAKE + 2), dict(nb_q_token=16386), dict(nb_q_head=508), dict(nb_dst_head=508)):
+        assert kv8_attn(Q, **kw) == (EINVAL, 0), kw
+    assert kv8_attn(Q, dict(page_size=1 << 30), max_len=(1 << 30) + 1) == (EUNSUPPORTED, 0)
+    assert kv8_attn(Q, n_tokens=0, n_requests=0, q=None, dst=None, len=None)[0] == OK
+    assert kv8_attn(Q, n_tokens=0, n_q=0)[0] == OK
+    assert Q.lib().q4k_kv8_attn(None, None, 0, None) == EINVAL and Q.lib().q4k_kv8_attn_workspace_bytes(None) == 0
