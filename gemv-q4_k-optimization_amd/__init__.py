@@ -115,6 +115,11 @@ class q4k_kv8_attn_args(ctypes.Structure):
                 ("q", _P), ("nb_q_token", _I64), ("nb_q_head", _I64), ("dst", _P), ("nb_dst_token", _I64), ("nb_dst_head", _I64), ("lse", _P)]
 
 
+class q4k_sample_rules(ctypes.Structure):
+    """How the next token of each row is drawn (include/q4k_step.h)."""
+    _fields_ = [("temperature", _P), ("top_k", _P), ("top_p", _P), ("min_p", _P), ("uniform", _P)]
+
+
 # Every symbol the headers of include/ declare: (restype, argtypes)
 SIGNATURES = {
     "q4k_version": (ctypes.c_int32, []),
@@ -159,6 +164,8 @@ SIGNATURES = {
     "q4k_kv8_load": (_I, [_P, _P]),
     "q4k_kv8_attn_workspace_bytes": (ctypes.c_size_t, [_P]),
     "q4k_kv8_attn": (_I, [_P, _P, ctypes.c_size_t, _P]),
+    "q4k_sample_workspace_bytes": (ctypes.c_size_t, [_I64, _I64]),
+    "q4k_sample": (_I, [_P, _I64, _I64, _I64, _P, _P, _P, _P, ctypes.c_size_t, _P]),
     # include/q4k_gguf.h
     "q4k_gguf_open": (_I, [ctypes.c_char_p, ctypes.POINTER(_P)]),
     "q4k_gguf_close": (None, [_P]),
@@ -969,6 +976,37 @@ def kv8_attention(q, pages: KV8Pages, lens, max_len, n_q=None, q_start=None, sca
     ws, ws_bytes = _ws(workspace, dev)
     _on_device("q4k_kv8_attn", dev, ctypes.byref(args), ws, ws_bytes, _stream_of(stream, dev))
     return out
+
+
+def sample_workspace(logits):
+    """A workspace for sample calls of up to these rows of logits [N, V]."""
+    import torch
+    N, V = logits.shape
+    with torch.cuda.device(logits.device):
+        n = int(lib().q4k_sample_workspace_bytes(V, N))
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=logits.device)
+
+
+def sample(logits, uniform=None, temperature=None, top_k=None, top_p=None, min_p=None, out=None, logprob=None, workspace=None, stream=None):
+    """The next token of each row of F32 logits [N, V]: temperature (1; 0: the
+    largest), then top_k int32 (0: all), top_p (1: all) and min_p (0: all), F32 [N] each,
+    drawn by uniform F32 [N] in [0, 1) (None: the largest logit).  Returns (tokens
+    int32 [N], logprob F32 [N] or None): the logarithm of the token's share of what
+    the cuts kept goes to logprob where one is given."""
+    import torch
+    f32 = torch.float32
+    _need(logits.is_cuda, "logits: a device tensor expected")
+    N, V = logits.shape
+    dev, n = logits.get_device(), (N,)
+    ldx = _rows(logits, f32, (N, V), dev, "logits")
+    if out is None:
+        out = _new(n, torch.int32, logits.device, stream)
+    r = q4k_sample_rules(_vector(temperature, f32, n, dev, "temperature"), _vector(top_k, torch.int32, n, dev, "top_k"),
+                         _vector(top_p, f32, n, dev, "top_p"), _vector(min_p, f32, n, dev, "min_p"), _vector(uniform, f32, n, dev, "uniform"))
+    ws, ws_bytes = _ws(workspace, dev)
+    _on_device("q4k_sample", dev, logits.data_ptr(), V, N, ldx * 4, ctypes.byref(r), _vector(out, torch.int32, n, dev, "out"),
+               _vector(logprob, f32, n, dev, "logprob"), ws, ws_bytes, _stream_of(stream, dev))
+    return out, logprob
 
 
 # ------------------------------------------------------------------ GGUF ----

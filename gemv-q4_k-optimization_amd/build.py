@@ -41,7 +41,7 @@ def build(verbose: bool = False, save_temps: bool = False) -> str:
     for src in ("q4k_gemv.hip", "q6k_gemv.hip", "q4k_sums.hip", "q6k_sums.hip", "q4k_short.hip", "q6k_short.hip",
                 "q4k_mfma.hip", "q6k_mfma.hip", "q4k_probe.hip", "q4k_lora.hip", "q4k_prefix_attn.hip",
                 "q4k_attn_f16.hip", "q4k_attn_f16_f32.hip", "q4k_attn_bf16.hip", "q4k_attn_bf16_f32.hip", "q4k_logits.hip",
-                "q4k_rope.hip", "q4k_kv8.hip", "q4k_kv8_attn.hip", "q4k_kv8_attn_f32.hip", "q4k_kv8_attn_f16.hip", "q4k_kv8_attn_bf16.hip"):
+                "q4k_rope.hip", "q4k_kv8.hip", "q4k_kv8_attn.hip", "q4k_kv8_attn_f32.hip", "q4k_kv8_attn_f16.hip", "q4k_kv8_attn_bf16.hip", "q4k_sample.hip"):
         obj = os.path.join(BUILD, src.replace(".hip", ".o"))
         cmd = [hipcc, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
                # no packed-FP32 instructions in device code

@@ -7,6 +7,8 @@
  *                   for each block of tokens and head
  *   q4k_kv8_load    tokens of such a cache as the values they stand for
  *   q4k_kv8_attn    attention of a batch of requests over such a cache
+ *   q4k_sample      the next tokens from logits: temperature, top-k, top-p, min-p
+ *                   and given random numbers
  * No counterpart in the reference, whose path ends at the product.
  *
  * Conventions as in q4k_batch.h: strides (nb*) in bytes, a q4k_status, device
@@ -159,6 +161,38 @@ size_t q4k_kv8_attn_workspace_bytes(const q4k_kv8_attn_args *args);
  * values with F32 queries, two with F16 and one with BF16.  Scales of values below
  * 2^100.  dst and lse must not overlap what is read. */
 int q4k_kv8_attn(const q4k_kv8_attn_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------- next tokens */
+
+/* Per-row rules on the device, n_rows each; absent ones are NULL. */
+typedef struct q4k_sample_rules {
+    const float *temperature; /* NULL: 1; 0 and below, or NaN: the largest logit */
+    const int32_t *top_k;     /* 0 and below: all */
+    const float *top_p;       /* 1 and above, or NaN: all */
+    const float *min_p;       /* 0 and below, or NaN: all; 1 and above: 1 */
+    const float *uniform;     /* in [0, 1) (clamped to it, NaN: 0); NULL: the largest logit of every row */
+} q4k_sample_rules;
+
+/* Bytes of workspace that are enough for q4k_sample of these sizes and of any
+ * smaller n_rows (0: invalid sizes, or none taken). */
+size_t q4k_sample_workspace_bytes(int64_t n_vocab, int64_t n_rows);
+
+/* tokens[i] = a token of row i of src (F32, n_rows rows of up to 2^30 n_vocab
+ * logits).  With m the row's largest logit, w_v = exp((l_v - m) / temperature); the
+ * cuts, one after the other:
+ *   top-k   the top_k largest logits (of equal ones the lower tokens)
+ *   top-p   of those, in descending order (of equal ones the lower tokens first), each
+ *           whose predecessors' sum of w is below top_p times the sum of all of
+ *           them, and always the first
+ *   min-p   of those, w_v >= min_p
+ * The token is the first, in the order of token numbers, up to which the kept w's
+ * sum exceeds uniform times their sum.  Logits of -inf and NaN are no candidates; a
+ * row without any gives -1; with logits of +inf those are the candidates, alike.
+ * w and its sums are 64 bits; tokens below 2^-127 of the largest w count as 0.
+ * logprob[i] (may be NULL): the logarithm of the token's share of the kept
+ * w's sum, 0 where the largest logit was taken, -inf where there is none. */
+int q4k_sample(const float *src, int64_t n_vocab, int64_t n_rows, int64_t nb_src, const q4k_sample_rules *rules,
+               int32_t *tokens, float *logprob, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

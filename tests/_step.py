@@ -163,3 +163,49 @@ def attention8(q, spans, cache, lens, scale):
             if q.dtype == torch.float16:
                 tol[t] += 2.0 ** -25
     return out, lse, tol, tol_lse
+
+
+# --------------------------------------------------------------------- next tokens ----
+def sample(logits, u, t, k, p, m):
+    """(token, log-probability, margin) of one row in 64 bits: the margin is how far, of
+    the kept or the whole sum, the nearest other choice lies (a kernel whose sums
+    are of 64 bits too decides alike beyond some 2^-40 of it)."""
+    x = logits.double().cpu()
+    x = torch.where(torch.isnan(x), -float("inf"), x)
+    top = float(x.max()) if x.numel() else -float("inf")
+    if top == -float("inf"):
+        return -1, -float("inf"), 1.0
+    if u is None or not t > 0:
+        return int((x == top).nonzero()[0, 0]), 0.0, 1.0
+    u = min(max(u, 0.0), 1 - 2.0 ** -24) if u == u else 0.0
+    if top == float("inf"):
+        w = (x == top).double()
+    else:
+        w = torch.exp((x - top) / t)
+    order = torch.argsort(torch.where(x == 0, 0.0, x), descending=True, stable=True)
+    order = order[torch.isfinite(x[order]) | (x[order] == float("inf"))]
+    margin = 1.0
+    if 0 < k < x.numel():
+        order = order[:k]
+    if p < 1:
+        before = torch.cumsum(w[order], 0) - w[order]
+        whole = float(w[order].sum())
+        keep = before < p * whole
+        keep[0] = True
+        off = (before - p * whole).abs()[1:]
+        if off.numel():
+            margin = min(margin, float(off.min()) / whole)
+        order = order[keep]
+    if m > 0:
+        m = min(m, 1.0)
+        off = (w[order] - m).abs()
+        margin = min(margin, float(off[off > 0].min()) if (off > 0).any() else 1.0)
+        order = order[w[order] >= m]
+    order = order.sort().values
+    c = torch.cumsum(w[order], 0)
+    whole = float(c[-1])
+    off = (c[:-1] - u * whole).abs()
+    if off.numel():
+        margin = min(margin, float(off.min()) / whole)
+    n = min(int((c <= u * whole).sum()), order.numel() - 1)
+    return int(order[n]), math.log(float(w[order[n]]) / whole) if w[order[n]] > 0 else -float("inf"), margin

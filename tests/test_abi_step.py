@@ -134,3 +134,30 @@ def test_kv8_attn_checks(Q):
     assert kv8_attn(Q, n_tokens=0, n_requests=0, q=None, dst=None, len=None)[0] == OK
     assert kv8_attn(Q, n_tokens=0, n_q=0)[0] == OK
     assert Q.lib().q4k_kv8_attn(None, None, 0, None) == EINVAL and Q.lib().q4k_kv8_attn_workspace_bytes(None) == 0
+
+
+def sample(Q, src=FAKE, V=100, N=2, nb=400, tokens=FAKE, logprob=None, **kw):
+    r = Q.q4k_sample_rules()
+    for k, v in kw.items():
+        setattr(r, k, v)
+    return Q.lib().q4k_sample(src, V, N, nb, ctypes.byref(r), tokens, logprob, None, 0, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(V=-1), dict(N=-1), dict(src=None), dict(tokens=None), dict(src=FAKE + 2), dict(tokens=FAKE + 2), dict(logprob=FAKE + 1), dict(nb=396), dict(nb=402),
+    dict(V=1 << 33), dict(N=1 << 33), dict(temperature=FAKE + 2), dict(top_k=FAKE + 1), dict(top_p=FAKE + 3), dict(min_p=FAKE + 2), dict(uniform=FAKE + 2)])
+def test_sample_checks(Q, kw):
+    assert sample(Q, **kw) == EINVAL
+
+
+def test_sample_empty_unsupported_and_binding(Q):
+    assert sample(Q, N=0, src=None, tokens=None) == OK
+    assert sample(Q, V=(1 << 30) + 4, N=1) == EUNSUPPORTED
+    assert Q.lib().q4k_sample(FAKE, 100, 2, 400, None, FAKE, None, None, 0, None) == EINVAL
+    size = Q.lib().q4k_sample_workspace_bytes
+    assert size(-1, 4) == 0 and size(4, -1) == 0 and size(1 << 40, 4) == 0
+    for V in (1000, 32768, 151936, 1 << 30):
+        sizes = [size(V, n) for n in [*range(1, 600), 4096]]
+        assert sizes == sorted(sizes)
+    with pytest.raises(ValueError):
+        Q.sample(torch.zeros(2, 100), torch.zeros(2))
