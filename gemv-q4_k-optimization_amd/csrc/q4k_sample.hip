@@ -5,12 +5,18 @@
 // row.  Cuts keep what is not below one token, in the order of falling logits and
 // rising numbers, so they come from sums over a histogram of the exponents and an
 // order within one of its bins:
-//   1. one pass over the row counts tokens and sums their w in bins of 2^(1/32)
-//   2. top-k, then top-p: the bin of the last token that is kept, and that token, from
-//      the bin's tokens put in order (a bin of more than kList is divided again by
-//      the logits' bits; equal logits are told apart by a count)
-//   3. the kept w of each chunk of the row, the chunk that the random number falls
-//      into, the token in it
+//   scan  parts of the rows, read once: the largest logit of each chunk of 256 and
+//         what the row's rules need, counts and sums of w in bins of 2^(1/24), or
+//         without cuts the sum of each chunk
+//   pick  a workgroup a row: the bin of the last token that is kept, and where the tokens
+//         from there up are few (kList) that token among them, the kept sum of each
+//         chunk, the chunk that the random number falls into and the token in it
+//   rest  where they are not, workgroups of all parts of the row again: the sums by
+//         chunks of what is above that bin and the bin's own tokens; the last of them
+//         finds the last token that is kept, and draws.  What is rare, one workgroup does
+//         from the row alone: rows out of the scan's reach, top-k and top-p both past
+//         kList, a bin of more than kList tokens (divided by the logits' bits until it
+//         has less or only equal ones, which are told apart by a count).
 // Sums of bins are integers (any order gives the same), all others are 64-bit floats
 // in an order of their own: equal calls give equal bits.  A chunk whose largest
 // logit is below the cut is not read again.
@@ -20,7 +26,44 @@
 #include "q4k_batch.h"
 #include "q4k_device.h"
 
+// A token's weight is compared with the same token's, worked out elsewhere: products and
+// sums are fused where fma() says so only.
+#pragma clang fp contract(off)
+
 namespace q4k {
+
+// (Eight and four waves: what is not memory is chains of scans over the workgroup, whose
+// instructions cost each SIMD the more the more waves it has.)
+constexpr int kPickThreads = 512, kRestThreads = 256, kMostWaves = 8;
+constexpr int kScanThreads = 512, kScanWaves = kScanThreads / 64, kTile = kScanThreads * 8;
+constexpr int kOctave = 24, kBins = 64 * kOctave;  // what is below the last bin is never drawn
+constexpr int kChunk = 256, kChunks = 1024, kList = 1024, kParts = 16;
+// Rows whose a l is past this (in bins) lose bits of w and are not scanned: the pick
+// takes them by the differences from their largest logit.
+constexpr double kReach = 16384.0;
+// Sums nearer to a border than this part of it count as equal to it.
+constexpr double kNear = 0x1p-40;
+
+// What a part of a row was found to hold.
+struct SamplePart {
+    double base;   // bin i is place base - kBins + i
+    float skipped; // the largest logit of tiles that were too low to be placed
+    int used;      // whether some tile was not
+    unsigned long long mass[kBins];
+    uint32_t cnt[kBins];
+};
+
+// What the pick leaves to the rest of a row.
+struct SampleRest {
+    int kind, bin, by_count;  // (bin: of the last token that is kept, for kCut)
+    int n_list, done;         // tokens of the bin; parts that are done
+    float m;
+    double most, base_cnt, base_mass;
+    float list_l[kList];
+    int list_i[kList];
+};
+// nothing; the tokens above the bin and some in it; all that min-p keeps; all of the row's work
+constexpr int kNone = 0, kCut = 1, kBound = 2, kAlone = 3;
 
 struct SampleParams {
     const char *src;
@@ -28,127 +71,247 @@ struct SampleParams {
     int n_vocab, n_rows;
     int chunk, chunks;  // tokens of a chunk (a multiple of 256), chunks of a row
     int mass_bits;      // of a token's integer weight in its bin
+    int parts, tiles;   // of a row; of a part
+    SamplePart *part;
+    float *cmax;        // [rows][kChunks]
+    double *cmass;
+    SampleRest *rest;   // null: the rest does all
+    int rest_parts;
     q4k_sample_rules r;
     int32_t *tokens;
     float *logprob;
 };
 
-constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64;
-constexpr int kBins = 4096, kOctave = 32;  // bins of the histogram, of a factor of two
-constexpr int kAnchor = kBins - 1;         // the bin of the largest logit; what is below the last bin, 2^-128 of it, is never drawn
-constexpr int kChunks = 1024, kList = 1024;
-
-struct SampleLds {
-    unsigned long long mass[kBins];
-    uint32_t cnt[kBins];
-    float cmax[kChunks];
-    double cmass[kChunks];
-    float list_l[kList], sort_l[kList];
-    int list_i[kList], sort_i[kList];
-    double scan[kSampleWaves];
-    double scan2[kSampleWaves];
-    int n_list, best;
-    int found_i;
-    double base_cnt, base_mass;
-    float found_l;
+// A row's rules.
+struct SampleRules {
+    float temperature, top_p, min_p;
+    int top_k;
+    float u;
+    bool greedy, cut;
+    __device__ __forceinline__ SampleRules(const SampleParams &p, int row) {
+        temperature = p.r.temperature ? p.r.temperature[row] : 1.0f;
+        top_p = p.r.top_p ? p.r.top_p[row] : 1.0f;
+        min_p = p.r.min_p ? p.r.min_p[row] : 0.0f;
+        top_k = p.r.top_k ? p.r.top_k[row] : 0;
+        if (top_k < 0 || top_k >= p.n_vocab) top_k = 0;
+        top_p = top_p < 1.0f ? fmaxf(top_p, 0.0f) : 1.0f;
+        min_p = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
+        u = p.r.uniform ? p.r.uniform[row] : 0.0f;
+        u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+        greedy = !p.r.uniform || !(temperature > 0.0f);
+        cut = !greedy && (top_k > 0 || top_p < 1.0f);
+    }
+    // neither cuts nor a bound: every chunk's sum is what the draw needs
+    __device__ __forceinline__ bool free() const { return !greedy && !cut && min_p == 0.0f; }
+    // bins per unit of a logit
+    __device__ __forceinline__ double rate() const { return kOctave * 1.4426950408889634074 / (double)temperature; }
 };
 
-__device__ __forceinline__ double shfl_up(double x, int d) {
+// ---- sums over a wave's lanes ----
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp64(double x) {  // 0 where no lane is
     const unsigned long long b = __double_as_longlong(x);
-    const uint32_t lo = __shfl_up((uint32_t)b, d), hi = __shfl_up((uint32_t)(b >> 32), d);
-    return __longlong_as_double(((unsigned long long)hi << 32) | lo);
-}
-__device__ __forceinline__ double shfl_xor(double x, int d) {
-    const unsigned long long b = __double_as_longlong(x);
-    const uint32_t lo = __shfl_xor((uint32_t)b, d), hi = __shfl_xor((uint32_t)(b >> 32), d);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
     return __longlong_as_double(((unsigned long long)hi << 32) | lo);
 }
 __device__ __forceinline__ double wave_scan(double x) {  // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double y = shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
+    x += dpp64<0x111, 0xf>(x);  // row_shr:1, 2, 4, 8 within 16 lanes
+    x += dpp64<0x112, 0xf>(x);
+    x += dpp64<0x114, 0xf>(x);
+    x += dpp64<0x118, 0xf>(x);
+    x += dpp64<0x142, 0xa>(x);  // the last lane of rows 0 and 2 to the next row
+    x += dpp64<0x143, 0xc>(x);  // of row 1 to rows 2 and 3
     return x;
 }
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) x += shfl_xor(x, d);
-    return x;
+__device__ __forceinline__ double lane_of(double x, int lane) {
+    const unsigned long long b = __double_as_longlong(x);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+    return __longlong_as_double(((unsigned long long)hi << 32) | lo);
+}
+__device__ __forceinline__ double last_lane(double x) { return lane_of(x, 63); }
+__device__ __forceinline__ double wave_sum(double x) { return last_lane(wave_scan(x)); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_max(float x) {
+    const int b = __float_as_int(x);
+    return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(b, b, CTRL, ROWS, 0xf, false)));
 }
 __device__ __forceinline__ float wave_max(float x) {
+    x = dpp_max<0x111, 0xf>(x);
+    x = dpp_max<0x112, 0xf>(x);
+    x = dpp_max<0x114, 0xf>(x);
+    x = dpp_max<0x118, 0xf>(x);
+    x = dpp_max<0x142, 0xa>(x);
+    x = dpp_max<0x143, 0xc>(x);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
+// Four logits of a row of n; NaN and what is past the row are no candidates.
+__device__ __forceinline__ f32x4 sample_load(const float *src, int n, int64_t i) {
+    f32x4 x;
+    if (i + 4 <= n) {
+        x = load4<false>(src + i);
+    } else {
 #pragma unroll
-    for (int d = 32; d > 0; d /= 2) x = fmaxf(x, __shfl_xor(x, d));
+        for (int j = 0; j < 4; ++j) x[j] = i + j < n ? src[i + j] : -__builtin_inff();
+    }
     return x;
 }
+// (zeros are equal whatever their sign)
+__device__ __forceinline__ float sample_clean(float l) { return l != l ? -__builtin_inff() : l + 0.0f; }
 
-// What is below x over the workgroup's threads in order, and the whole sum.
-__device__ __forceinline__ double block_scan(double x, double *scan, double &total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const double inc = wave_scan(x);
-    __syncthreads();
-    if (lane == 63) scan[wave] = inc;
-    __syncthreads();
-    double before = 0.0;
-    total = 0.0;
-#pragma unroll
-    for (int i = 0; i < kSampleWaves; ++i) {
-        if (i < wave) before += scan[i];
-        total += scan[i];
-    }
-    return before + (inc - x);
+// scale * 2^(x / 24) + plus for 0 <= x < 1: the exponential's series (the next term is
+// 2^-48 of it).
+__device__ __forceinline__ double sample_exp(double x, double scale, double plus) {
+    constexpr double k = 0.6931471805599453094 / kOctave;
+    double e = k * k * k * k * k * k / 720.0;
+    e = __builtin_fma(e, x, k * k * k * k * k / 120.0);
+    e = __builtin_fma(e, x, k * k * k * k / 24.0);
+    e = __builtin_fma(e, x, k * k * k / 6.0);
+    e = __builtin_fma(e, x, k * k / 2.0);
+    e = __builtin_fma(e, x, k);
+    return __builtin_fma(e * x, scale, scale + plus);
+}
+// 2^((b - kBins) / 24) times e, from the 24 powers of an octave.
+__device__ __forceinline__ double sample_weight(const double *octave, int b, double e) {
+    const int q = b * 2731 >> 16;  // b / 24, below 8192
+    return ldexp(octave[b - q * kOctave] * e, q - kBins / kOctave);
+}
+// as an integer of bits and one more, scale 2^bits: 2^52 more leaves it in the last bits
+__device__ __forceinline__ unsigned long long sample_mass(double x, double scale) {
+    return __double_as_longlong(sample_exp(x, scale, 0x1p52)) & 0xfffffffffffffull;
 }
 
-// A row's logits, and how they weigh.
-struct SampleRow {
-    const float *src;
-    int n, chunk, chunks;
-    float m;        // the largest logit
-    bool flat;      // only logits equal to m count, all alike
-    double a32;     // bins: a32 * (l - m) + kAnchor
-
-    __device__ __forceinline__ float4 load(int i) const {
-        float4 x;
-        if (i + 4 <= n) {
-            const f32x4 v = load4<false>(src + i);
-            x = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-            const float none = -__builtin_inff();
-            x = make_float4(i < n ? src[i] : none, i + 1 < n ? src[i + 1] : none, i + 2 < n ? src[i + 2] : none, none);
+// ---- scan: parts of the rows ----
+// Tiles of 4096 logits, eight a thread, the next one on its way.  The bins are a ring
+// about the place of the largest logit so far, in whole octaves.
+__global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams p) {
+    __shared__ unsigned long long mass[kBins];
+    __shared__ uint32_t cnt[kBins];
+    __shared__ double octave[kOctave];
+    __shared__ float tops[2][kScanWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x / p.parts, part = blockIdx.x - row * p.parts;
+    const float *src = reinterpret_cast<const float *>(p.src + row * p.nb_src);
+    const int64_t beg = (int64_t)part * p.tiles * kTile;
+    if (beg >= p.n_vocab) return;
+    const int64_t end = beg + (int64_t)p.tiles * kTile;
+    // thread: tokens wave * 512 + lane * 4 and 256 past it
+    const int at = wave * 2 * kChunk + lane * 4;
+    f32x4 next[2];
+    next[0] = sample_load(src, p.n_vocab, beg + at);
+    next[1] = sample_load(src, p.n_vocab, beg + at + kChunk);
+    const SampleRules r(p, row);
+    const bool cut = r.cut, by_mass = r.top_k == 0, free = r.free();  // (top-k needs counts alone)
+    const double rate = r.rate(), scale = (double)(1ull << p.mass_bits);
+    if (free) {
+        if (tid < kOctave) octave[tid] = exp2(tid * (1.0 / kOctave));
+        __syncthreads();
+    }
+    float *cmax = p.cmax + (int64_t)row * kChunks;
+    double *cmass = p.cmass + (int64_t)row * kChunks;
+    double base = 0.0;  // bins: places base - kBins .. base - 1
+    int off = 0;        // where bin 0 is in the ring
+    bool used = false;
+    float skipped = -__builtin_inff();
+    int par = 0;
+    for (int64_t t0 = beg; t0 < end && t0 < p.n_vocab; t0 += kTile, par ^= 1) {
+        f32x4 l[2] = {next[0], next[1]};
+        if (t0 + kTile < end && t0 + kTile < p.n_vocab) {
+            next[0] = sample_load(src, p.n_vocab, t0 + kTile + at);
+            next[1] = sample_load(src, p.n_vocab, t0 + kTile + at + kChunk);
         }
-        x.x = clean(x.x);
-        x.y = clean(x.y);
-        x.z = clean(x.z);
-        x.w = clean(x.w);
-        return x;
-    }
-    // NaN is no candidate; zeros are equal whatever their sign
-    __device__ __forceinline__ float clean(float l) const { return l != l ? -__builtin_inff() : l + 0.0f; }
-    __device__ __forceinline__ bool counts(float l) const { return flat ? l == m : l > -__builtin_inff(); }
-    __device__ __forceinline__ double place(float l) const { return flat ? kAnchor : __builtin_fma((double)l - (double)m, a32, kAnchor); }
-    // the bin, below 0 where the token is none that counts
-    __device__ __forceinline__ int bin(float l) const {
-        if (!counts(l)) return -1;
-        const double p = floor(place(l));
-        return p < 0.0 ? -1 : (int)p;
-    }
-    // 2^(x / 32), x from place() less that of the largest
-    __device__ __forceinline__ double weight(float l) const { return counts(l) ? exp2((place(l) - kAnchor) * (1.0 / kOctave)) : 0.0; }
-    // in this order lower tokens of equal logits come first
-    __device__ __forceinline__ static bool before(float l, int i, float k, int j) { return l > k || (l == k && i < j); }
-
-    // f(token, four logits) of the chunks that on() asks for, each by one wave
-    template <class ON, class F, class END>
-    __device__ __forceinline__ void each(ON on, F f, END end) const {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        for (int c = wave; c < chunks; c += kSampleWaves) {
-            if (!on(c)) continue;
-            const int64_t c0 = (int64_t)c * chunk, c1 = c0 + chunk;
-            for (int64_t i = c0; i < c1 && i < n; i += 256) f((int)i + lane * 4, load((int)i + lane * 4));
-            end(c);
+        float top[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            top[k] = wave_max(fmaxf(fmaxf(l[k][0], l[k][1]), fmaxf(l[k][2], l[k][3])));  // (NaN passed over)
+            const int64_t c = (t0 + at - lane * 4) / kChunk + k;
+            if (lane == 0 && c < p.chunks) cmax[c] = sample_clean(top[k]);
+            if (!free) continue;
+            const double cb = floor((double)top[k] * rate) + 1.0;
+            double sum = 0.0;
+            if (fabs(cb) < kReach) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const double t = (double)l[k][j] * rate, f = floor(t), i = f - cb + kBins;
+                    if (i >= 0.0) sum += sample_weight(octave, (int)i, sample_exp(t - f, 1.0, 0.0));
+                }
+                sum = wave_sum(sum);
+            }
+            if (lane == 0 && c < p.chunks) cmass[c] = sum;
         }
+        if (!cut) continue;
+        if (lane == 0) tops[par][wave] = fmaxf(top[0], top[1]);
+        __syncthreads();
+        float tile = tops[par][0];
+#pragma unroll
+        for (int i = 1; i < kScanWaves; ++i) tile = fmaxf(tile, tops[par][i]);
+        const double place = (double)tile * rate;
+        if (!(place > -kReach)) {
+            skipped = fmaxf(skipped, tile);
+            continue;
+        }
+        if (place > kReach) continue;  // (the row's largest logit tells)
+        const double up = (floor(place / kOctave) + 1.0) * kOctave;
+        if (!used || up > base) {
+            // bins that enter at the top, where the lowest ones were
+            const int by = !used || up - base >= kBins ? kBins : (int)(up - base);
+            off = by == kBins ? 0 : off + by >= kBins ? off + by - kBins : off + by;
+            for (int i = tid; i < by; i += kScanThreads) {
+                const int b = by == kBins ? i : off - 1 - i + (off - 1 - i < 0 ? kBins : 0);
+                mass[b] = 0;
+                cnt[b] = 0;
+            }
+            base = up;
+            used = true;
+            __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const double t = (double)l[k][j] * rate, f = floor(t), i = f - base + kBins;
+                if (i >= 0.0) {
+                    int b = (int)i + off;
+                    b = b >= kBins ? b - kBins : b;
+                    if (by_mass) atomicAdd(&mass[b], sample_mass(t - f, scale));
+                    atomicAdd(&cnt[b], 1u);
+                }
+            }
     }
+    if (!cut) return;
+    __syncthreads();
+    SamplePart &out = p.part[(int64_t)row * p.parts + part];
+    if (tid == 0) {
+        out.base = base;
+        out.skipped = skipped;
+        out.used = used;
+    }
+    if (!used) return;
+    for (int i = tid; i < kBins; i += kScanThreads) {
+        const int b = i + off >= kBins ? i + off - kBins : i + off;
+        if (by_mass) out.mass[i] = mass[b];
+        out.cnt[i] = cnt[b];
+    }
+}
+
+// ---- pick and rest: a row's token from what the scan found ----
+struct PickLds {
+    unsigned long long mass[kBins];
+    double octave[kOctave];  // the powers of 2^(1/24)
+    double cmass[kChunks];
+    uint32_t cnt[kBins];
+    float cmax[kChunks];
+    float list_l[kList], sort_l[kList];
+    int list_i[kList], sort_i[kList];
+    int todo[kChunks];
+    double scan[2][kMostWaves];
+    float tops[kMostWaves], lows[kMostWaves];
+    int bests[kMostWaves];
+    int n_todo, n_list, n_sort, best, found_i;
+    double base_cnt, base_mass;
+    int ahead[kParts];  // bins that a part's base lies below the row's; kBins: nothing in it
+    float low[kParts];
 };
 
 // ordered bits of a float: larger logits have larger keys
@@ -156,71 +319,467 @@ __device__ __forceinline__ uint32_t sample_key(float l) {
     const uint32_t b = __float_as_uint(l);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+// the order of the cuts: lower tokens of equal logits come first
+__device__ __forceinline__ bool sample_before(float l, int i, float k, int j) { return l > k || (l == k && i < j); }
+// A list's weights are taken in steps of 2^-42 (the row's largest is above 1/2): sums of a
+// thousand in any order are the same.
+__device__ __forceinline__ unsigned long long sample_steps(double w) { return (unsigned long long)(w * 0x1p42 + 0.5); }
+constexpr double kStep = 0x1p-42;
 
-// 2^(x / 32) for 0 <= x < 1 in units of 1 / scale: the exponential's series (the next
-// term is 2^-51 of it; exact at 0, where the largest logits are).
-__device__ __forceinline__ unsigned long long sample_mass(double x, double scale) {
-    const double y = x * (0.6931471805599453094 / kOctave);
-    double e = 1.0 / 720.0;
-    e = __builtin_fma(e, y, 1.0 / 120.0);
-    e = __builtin_fma(e, y, 1.0 / 24.0);
-    e = __builtin_fma(e, y, 1.0 / 6.0);
-    e = __builtin_fma(e, y, 0.5);
-    e = __builtin_fma(e, y, 1.0);
-    e = __builtin_fma(e, y, 1.0);
-    return (unsigned long long)(e * scale + 0.5);
-}
+// (Loops over chunks and cuts are kept rolled: the code runs once for a row, and waits
+// for its own instructions too.)
+// ALONE: by the differences from the largest logit, which any row's are fit for.
+template <int THREADS, bool ALONE>
+struct PickRow {
+    static constexpr int kPickThreads = THREADS, kPickWaves = THREADS / 64;
+    static constexpr int kEach = kChunks / THREADS;  // chunks of a thread
+    PickLds &s;
+    const SampleParams &p;
+    const float *src;
+    int n, chunk, chunks;
+    float m;            // the largest logit
+    bool flat;          // (ALONE) only logits equal to m count, all alike
+    double rate, base, min_w;
+    float last_l;       // the last token that is kept, in the order of the cuts
+    int last_i;
 
-__global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleParams p) {
-    extern __shared__ __attribute__((aligned(16))) char lds_bytes[];
-    SampleLds &s = *reinterpret_cast<SampleLds *>(lds_bytes);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int row = blockIdx.x;
-    const float inf = __builtin_inff();
-    SampleRow x;
-    x.src = reinterpret_cast<const float *>(p.src + row * p.nb_src);
-    x.n = p.n_vocab;
-    x.chunk = p.chunk;
-    x.chunks = p.chunks;
-    x.flat = false;
-    x.a32 = 0.0;
-    const float temperature = p.r.temperature ? p.r.temperature[row] : 1.0f;
-    const float top_p = p.r.top_p ? p.r.top_p[row] : 1.0f;
-    const float min_p = p.r.min_p ? p.r.min_p[row] : 0.0f;
-    const int top_k = p.r.top_k ? p.r.top_k[row] : 0;
-    float u = p.r.uniform ? p.r.uniform[row] : 0.0f;
-    u = u > 0.0f ? fminf(u, 0.99999994f) : 0.0f;
-    const bool greedy = !p.r.uniform || !(temperature > 0.0f);
-    const bool cut_k = top_k > 0 && top_k < p.n_vocab, cut_p = top_p < 1.0f;
+    __device__ __forceinline__ PickRow(PickLds &lds, const SampleParams &params, int row)
+        : s(lds), p(params), src(reinterpret_cast<const float *>(params.src + row * params.nb_src)), n(params.n_vocab), chunk(params.chunk),
+          chunks(params.chunks), m(-__builtin_inff()), flat(false), rate(0.0), base(1.0), min_w(0.0), last_l(-__builtin_inff()),
+          last_i(INT32_MAX) {}
 
-    // the largest logit of each chunk and of the row, and its first token
-    auto all = [](int) { return true; };
-    float mc = -inf;
-    x.each(all, [&](int, float4 l) { mc = fmaxf(fmaxf(fmaxf(mc, l.x), fmaxf(l.y, l.z)), l.w); },
-           [&](int c) {
-               mc = wave_max(mc);
-               if (lane == 0) s.cmax[c] = mc;
-               mc = -inf;
-           });
-    __syncthreads();
-    x.m = wave_max(tid < p.chunks ? s.cmax[tid] : -inf);
-    if (lane == 0) s.scan[wave] = x.m;
-    if (tid == 0) s.found_i = INT32_MAX;
-    __syncthreads();
-    for (int i = 0; i < kSampleWaves; ++i) x.m = fmaxf(x.m, (float)s.scan[i]);
-    if (x.m == -inf) {
-        if (tid == 0) {
-            p.tokens[row] = -1;
-            if (p.logprob) p.logprob[row] = -inf;
-        }
-        return;
+    __device__ __forceinline__ double place(float l) const { return ALONE ? flat ? 0.0 : ((double)l - (double)m) * rate : (double)l * rate; }
+    // the bin (below 0: none), and what is past its lower end
+    __device__ __forceinline__ int bin(float l, double &past) const {
+        const double t = place(l), f = floor(t), i = f - base + kBins;
+        past = t - f;
+        // (-inf: no place is, or at a rate of 0 none is a number)
+        const bool is = i >= 0.0 && (!ALONE || !flat || l == m);
+        return is ? (int)i : -1;
     }
-    auto has_max = [&](int c) { return s.cmax[c] == x.m; };
-    if (greedy) {
+    __device__ __forceinline__ int bin(float l) const {
+        double past;
+        return bin(l, past);
+    }
+    __device__ __forceinline__ double weight(float l) const {
+        double past;
+        const int b = bin(l, past);
+        return b < 0 ? 0.0 : sample_weight(s.octave, b, sample_exp(past, 1.0, 0.0));
+    }
+    __device__ __forceinline__ bool left_in(float l, int i) const { return !sample_before(last_l, last_i, l, i); }
+    // the base of places for a largest logit within the scan's reach
+    __device__ __forceinline__ void place_by_scan() { base = (floor((double)m * rate / kOctave) + 1.0) * kOctave; }
+    __device__ __forceinline__ void weights() const {
+        if (threadIdx.x < kOctave) s.octave[threadIdx.x] = exp2(threadIdx.x * (1.0 / kOctave));
+    }
+    // the largest of a value of each wave
+    __device__ __forceinline__ float over_waves(const float *v) const {
+        float x = v[0];
+#pragma unroll
+        for (int i = 1; i < kPickWaves; ++i) x = fmaxf(x, v[i]);
+        return x;
+    }
+    // m from the chunks' largest
+    __device__ __forceinline__ void largest() {
+        const int tid = threadIdx.x;
+        float mine = -__builtin_inff();
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
+            if (tid + k * kPickThreads < chunks) mine = fmaxf(mine, s.cmax[tid + k * kPickThreads]);
+        mine = wave_max(mine);
+        if ((tid & 63) == 0) s.tops[tid >> 6] = mine;
+        __syncthreads();
+        m = over_waves(s.tops);
+    }
+
+    // Two sums over the threads in order: what is below x and y, and the whole.
+    __device__ __forceinline__ void scan2(double &x, double &y, double &all_x, double &all_y) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const double ix = wave_scan(x), iy = wave_scan(y);
+        __syncthreads();
+        if (lane == 63) {
+            s.scan[0][wave] = ix;
+            s.scan[1][wave] = iy;
+        }
+        __syncthreads();
+        double bx = 0.0, by = 0.0;
+        all_x = all_y = 0.0;
+#pragma unroll
+        for (int i = 0; i < kPickWaves; ++i) {
+            if (i == wave) {
+                bx = all_x;
+                by = all_y;
+            }
+            all_x += s.scan[0][i];
+            all_y += s.scan[1][i];
+        }
+        x = bx + (ix - x);
+        y = by + (iy - y);
+    }
+    __device__ __forceinline__ double scan(double x, double &all) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const double ix = wave_scan(x);
+        __syncthreads();
+        if (lane == 63) s.scan[0][wave] = ix;
+        __syncthreads();
+        double bx = 0.0;
+        all = 0.0;
+#pragma unroll
+        for (int i = 0; i < kPickWaves; ++i) {
+            if (i == wave) bx = all;
+            all += s.scan[0][i];
+        }
+        return bx + (ix - x);
+    }
+
+    // The `best` (0 and above) of the last thread that has one, threads with higher ones behind
+    // those with lower; -1 where none has.  (An atomic maximum of values that differ costs
+    // a wave a loop over its lanes.)
+    __device__ __forceinline__ int last_best(int best) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const unsigned long long b = __ballot(best >= 0);
+        const int mine = b ? __builtin_amdgcn_readlane(best, 63 - __builtin_clzll(b)) : -1;
+        if (lane == 0) s.bests[wave] = mine;
+        __syncthreads();
+        int all = s.bests[0];
+#pragma unroll
+        for (int i = 1; i < kPickWaves; ++i) all = s.bests[i] > all ? s.bests[i] : all;
+        return all;
+    }
+
+    // The chunks that on(chunk) asks for, as a list in any order.
+    template <class ON>
+    __device__ __forceinline__ int ask(ON on) const {
+        const int tid = threadIdx.x, lane = tid & 63;
+        __syncthreads();
+        if (tid == 0) s.n_todo = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int c = tid; c - lane < chunks; c += kPickThreads) {
+            const bool is = c < chunks && on(c);
+            const unsigned long long b = __ballot(is);
+            int at = 0;
+            if (lane == 0 && b) at = atomicAdd(&s.n_todo, __builtin_popcountll(b));
+            at = __builtin_amdgcn_readfirstlane(at);
+            if (is) s.todo[at + __builtin_popcountll(b & ((1ull << lane) - 1))] = c;
+        }
+        __syncthreads();
+        return s.n_todo;
+    }
+    // f(token, four logits from there) of the listed chunks, each chunk by one wave, the next
+    // ones on their way; end(chunk) behind each chunk.
+    template <class F, class END>
+    __device__ __forceinline__ void each(int count, F f, END end) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int more = __builtin_ctz(chunk) - 8, subs = 1 << more;  // (chunks are 256 tokens times a power of two)
+        const int mine = count > wave ? ((count - wave - 1) / kPickWaves + 1) * subs : 0;
+        // two sets of registers, one on its way while the other is used
+        constexpr int SET = 4;
+        struct Set {
+            f32x4 v[SET];
+            int c[SET];
+        } a, b;
+        auto load = [&](Set &q, int k0) {
+#pragma unroll
+            for (int j = 0; j < SET; ++j) {
+                const int k = k0 + j < mine ? k0 + j : mine - 1;
+                q.c[j] = s.todo[wave + (k >> more) * kPickWaves];
+                q.v[j] = sample_load(src, n, (int64_t)q.c[j] * chunk + (k & (subs - 1)) * kChunk + lane * 4);
+            }
+        };
+        auto use = [&](const Set &q, int k0) {
+#pragma unroll
+            for (int j = 0; j < SET; ++j) {
+                if (k0 + j >= mine) break;
+                const int sub = (k0 + j) & (subs - 1);
+                f32x4 l;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) l[e] = sample_clean(q.v[j][e]);
+                f(q.c[j] * chunk + sub * kChunk + lane * 4, l);
+                if (sub == subs - 1) end(q.c[j]);
+            }
+        };
+        if (mine == 0) return;
+        load(a, 0);
+#pragma unroll 1
+        for (int k = 0; k < mine; k += 2 * SET) {
+            if (k + SET < mine) load(b, k + SET);
+            use(a, k);
+            if (k + SET >= mine) break;
+            if (k + 2 * SET < mine) load(a, k + 2 * SET);
+            use(b, k + SET);
+        }
+    }
+    // Those of a wave's four logits a lane that are in, to the list: one atomic for all.
+    __device__ __forceinline__ void append(int i, f32x4 l, const bool (&in)[4]) const {
+        const int lane = threadIdx.x & 63;
+        unsigned long long b[4];
+        int all = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            b[e] = __ballot(in[e]);
+            all += __builtin_popcountll(b[e]);
+        }
+        if (all == 0) return;
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&s.n_list, all);
+        at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int k = at + __builtin_popcountll(b[e] & ((1ull << lane) - 1));
+            if (in[e]) {
+                s.list_l[k] = l[e];
+                s.list_i[k] = i + e;
+            }
+            at += __builtin_popcountll(b[e]);
+        }
+    }
+    // A logit that is surely below the bin's lower end, though not by much (-inf where
+    // that is past F32): what is under it needs no place.
+    __device__ __forceinline__ float under(int bin_) const {
+        const double l = (base - kBins + bin_) / rate;
+        const float f = (float)(l - fabs(l) * 0x1p-20);
+        return fabsf(f) < 3e38f ? f : -__builtin_inff();
+    }
+
+    // The bin of the last token before which fewer than `most` tokens (by_count) or
+    // less than `most` of w lie, and what lies before the bin; the whole sum.  Bins from
+    // the highest, a thread has as many as divide them among all.  `part`: most is of the whole.
+    template <int BINS, class W>
+    __device__ __forceinline__ int pick(bool by_count, bool part, double most, W weight_of, double &base_cnt, double &base_mass,
+                                        double &whole) const {
+        constexpr int PER = (BINS + kPickThreads - 1) / kPickThreads;
+        const int tid = threadIdx.x;
+        double cnt[PER], mass[PER], all, bc = 0.0, bm = 0.0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int b = BINS - 1 - (tid * PER + j);
+            cnt[j] = b >= 0 ? s.cnt[b] : 0.0;
+            mass[j] = cnt[j] != 0.0 ? (double)s.mass[b] * weight_of(b) : 0.0;
+            bc += cnt[j];
+            bm += mass[j];
+        }
+        scan2(bc, bm, all, whole);
+        bc += base_cnt;
+        bm += base_mass;
+        const double limit = part ? most * whole : most;
+        int best = -1;
+        double kc = 0.0, km = 0.0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (cnt[j] != 0.0 && ((by_count ? bc : bm) < limit || bc == 0.0)) {
+                best = tid * PER + j;
+                kc = bc;
+                km = bm;
+            }
+            bc += cnt[j];
+            bm += mass[j];
+        }
+        const int found = last_best(best);
+        if (best >= 0 && found == best) {
+            s.base_cnt = kc;
+            s.base_mass = km;
+        }
+        __syncthreads();
+        base_cnt = s.base_cnt;
+        base_mass = s.base_mass;
+        return BINS - 1 - found;
+    }
+
+    // Of the list's n tokens those that are left in, before which lie base_cnt and
+    // base_mass: the last one that is kept becomes last_l, last_i.  Returns the sum of w
+    // up to it.
+    __device__ __forceinline__ double cut_list(int n, bool by_count, double most, double base_cnt, double base_mass) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        const float inf = __builtin_inff();
+        // 1024 stretches of the logits' bits between the least and the largest
+        float top = -inf, low = -inf;
+#pragma unroll 1
+        for (int e = tid; e < n; e += kPickThreads)
+            if (left_in(s.list_l[e], s.list_i[e])) {
+                top = fmaxf(top, s.list_l[e]);
+                low = fmaxf(low, -s.list_l[e]);
+            }
+        top = wave_max(top);
+        low = wave_max(low);
+        for (int e = tid; e < 1024; e += kPickThreads) {
+            s.mass[e] = 0;
+            s.cnt[e] = 0;
+        }
+        if (lane == 0) {
+            s.tops[wave] = top;
+            s.lows[wave] = low;
+        }
+        if (tid == 0) s.n_sort = 0;
+        __syncthreads();
+        const uint32_t lo = sample_key(-over_waves(s.lows)), span = (sample_key(over_waves(s.tops)) - lo) | 1023u;
+        const int shift = 22 - __builtin_clz(span);
+#pragma unroll 1
+        for (int e = tid; e < n; e += kPickThreads) {
+            const float l = s.list_l[e];
+            if (!left_in(l, s.list_i[e])) continue;
+            const int b = (int)((sample_key(l) - lo) >> shift);
+            atomicAdd(&s.mass[b], sample_steps(weight(l)));
+            atomicAdd(&s.cnt[b], 1u);
+        }
+        __syncthreads();
+        double some;
+        const int sub = pick<1024>(by_count, false, most, [](int) { return kStep; }, base_cnt, base_mass, some);
+        // the tokens of that stretch in order, where the list's kept ones are looked up again
+        const int count = s.cnt[sub];
+#pragma unroll 1
+        for (int e = tid; e < n; e += kPickThreads) {
+            const float l = s.list_l[e];
+            if (!left_in(l, s.list_i[e]) || (int)((sample_key(l) - lo) >> shift) != sub) continue;
+            const int at = atomicAdd(&s.n_sort, 1);
+            s.sort_l[at] = l;
+            s.sort_i[at] = s.list_i[e];
+        }
+        __syncthreads();
+        // (their places go to cnt, their weights in that order to cmass)
+#pragma unroll 1
+        for (int e = tid; e < count; e += kPickThreads) {
+            const float l = s.sort_l[e];
+            const int i = s.sort_i[e];
+            int rank = 0;
+#pragma unroll 1
+            for (int j = 0; j < count; ++j) rank += sample_before(s.sort_l[j], s.sort_i[j], l, i);
+            s.cnt[rank] = e;
+            s.cmass[rank] = weight(l);
+        }
+        __syncthreads();
+        double w[kEach], mine = 0.0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            w[k] = tid * kEach + k < count ? s.cmass[tid * kEach + k] : 0.0;
+            mine += w[k];
+        }
+        double at_mass = base_mass + scan(mine, some);
+        int best = tid == 0 ? 0 : -1;  // (the first one always)
+        double upto = base_mass + s.cmass[0];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int e = tid * kEach + k;
+            if (e < count && (by_count ? base_cnt + e : at_mass) < most) {
+                best = e;
+                upto = at_mass + w[k];
+            }
+            at_mass += w[k];
+        }
+        const int found = last_best(best);
+        if (best >= 0 && best == found) s.base_mass = upto;
+        const int at = s.cnt[found];
+        last_l = s.sort_l[at];
+        last_i = s.sort_i[at];
+        __syncthreads();
+        return s.base_mass;
+    }
+
+    // The kept sums of the list's n tokens by chunks, to `have` of chunks tid * kEach ..
+    __device__ __forceinline__ void list_sums(int n, double (&have)[kEach]) const {
+        const int tid = threadIdx.x;
+        for (int e = tid; e < kChunks; e += kPickThreads) s.mass[e] = 0;
+        __syncthreads();
+#pragma unroll 1
+        for (int e = tid; e < n; e += kPickThreads)
+            if (left_in(s.list_l[e], s.list_i[e])) {
+                const double w = weight(s.list_l[e]);
+                if (w >= min_w) atomicAdd(&s.mass[s.list_i[e] / chunk], sample_steps(w));
+            }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) have[k] += (double)s.mass[tid * kEach + k] * kStep;
+    }
+
+    // The token that u falls on, of chunks tid * kEach .. with kept sums `have`, and its
+    // share.  Tokens of bins from `steps` up to `steps_end` weigh as list_sums has them.
+    __device__ __forceinline__ void draw(int row, double u, const double (&have)[kEach], int steps, int steps_end) const {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        auto kept_w = [&](float l, int i) {
+            double past;
+            const int b = bin(l, past);
+            if (b < 0 || !left_in(l, i)) return 0.0;
+            const double w = sample_weight(s.octave, b, sample_exp(past, 1.0, 0.0));
+            return !(w >= min_w) ? 0.0 : b >= steps && b < steps_end ? (double)sample_steps(w) * kStep : w;
+        };
+        double total, mine = 0.0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) mine += have[k];
+        double before = scan(mine, total);
+        const double target = u * total * (1.0 + kNear);
+        // the last chunk with any before which no more than the target lies
+        int best = tid == 0 ? 0 : -1;
+        double rest = target;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            if (have[k] > 0.0 && before <= target) {
+                best = tid * kEach + k;
+                rest = target - before;
+            }
+            before += have[k];
+        }
+        const int found = last_best(best);
+        if (best >= 0 && best == found) s.base_mass = rest;
+        __syncthreads();
+        if (wave != 0) return;
+        double left = s.base_mass, share = 0.0;
+        const int64_t c0 = (int64_t)found * chunk;
+        int token = -1;
+        bool done = false;
+#pragma unroll 1
+        for (int64_t i = c0; i < c0 + chunk && i < n && !done; i += kChunk) {
+            const int t = (int)i + lane * 4;
+            const f32x4 v = sample_load(src, n, t);
+            double w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = kept_w(sample_clean(v[j]), t + j);
+            const double four = (w[0] + w[1]) + (w[2] + w[3]), inc = wave_scan(four);
+            double upto = inc - four, first_w = 0.0, any_w = 0.0;
+            int first = -1, any = -1;  // of the lane's four, the first that passes and the last that counts
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                upto += w[j];
+                if (w[j] > 0.0) {
+                    any = j;
+                    any_w = w[j];
+                    if (upto > left && first < 0) {
+                        first = j;
+                        first_w = w[j];
+                    }
+                }
+            }
+            const unsigned long long passed = __ballot(first >= 0), some = __ballot(any >= 0);
+            if (passed || some) {
+                const int from = passed ? __builtin_ctzll(passed) : 63 - __builtin_clzll(some);
+                token = (int)i + from * 4 + __shfl(passed ? first : any, from);
+                share = lane_of(passed ? first_w : any_w, from);
+                done = passed != 0;
+            }
+            left -= last_lane(inc);
+        }
+        if (lane == 0) {
+            p.tokens[row] = token;
+            if (p.logprob) p.logprob[row] = (float)log(share / total);
+        }
+    }
+
+    // A row without candidates, and one whose largest logit is taken: true where that is all.
+    __device__ __forceinline__ bool simple(int row, bool greedy) const {
+        const int tid = threadIdx.x;
+        if (m == -__builtin_inff()) {
+            if (tid == 0) {
+                p.tokens[row] = -1;
+                if (p.logprob) p.logprob[row] = m;
+            }
+            return true;
+        }
+        if (!greedy) return false;
+        const int all = ask([&](int c) { return s.cmax[c] == m; });
         int first = INT32_MAX;
-        x.each(has_max, [&](int i, float4 l) {
-            const int at = l.x == x.m ? i : l.y == x.m ? i + 1 : l.z == x.m ? i + 2 : l.w == x.m ? i + 3 : INT32_MAX;
-            first = at < first ? at : first;
+        each(all, [&](int i, f32x4 l) {
+#pragma unroll
+            for (int e = 3; e >= 0; --e)
+                if (l[e] == m && i + e < first) first = i + e;
         }, [](int) {});
         if (first != INT32_MAX) atomicMin(&s.found_i, first);
         __syncthreads();
@@ -228,313 +787,438 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleParams p) 
             p.tokens[row] = s.found_i;
             if (p.logprob) p.logprob[row] = 0.0f;
         }
-        return;
+        return true;
     }
-    x.flat = x.m == inf;  // only the infinite ones count
-    x.a32 = kOctave * 1.4426950408889634074 / (double)temperature;
-    float last_l = -inf;  // the last token that is kept, in the order of the cuts
-    int last_i = INT32_MAX;
-    auto left_in = [&](float l, int i) { return !SampleRow::before(last_l, last_i, l, i); };
-    if (cut_k || cut_p) {
-        const double scale = (double)(1ull << p.mass_bits);
-        // the histogram of what is left in
-        auto count_all = [&]() {
+};
+
+__global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams p) {
+    extern __shared__ __attribute__((aligned(16))) char lds_bytes[];
+    PickLds &s = *reinterpret_cast<PickLds *>(lds_bytes);
+    using Row = PickRow<kPickThreads, false>;
+    constexpr int kEach = Row::kEach;
+    const int tid = threadIdx.x, row = blockIdx.x;
+    const float inf = __builtin_inff();
+    Row x(s, p, row);
+    const SampleRules r(p, row);
+    const SamplePart *part = p.part + (int64_t)row * p.parts;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k)
+        if (tid + k * kPickThreads < p.chunks) s.cmax[tid + k * kPickThreads] = p.cmax[(int64_t)row * kChunks + tid + k * kPickThreads];
+    double part_base = 0.0;
+    if (r.cut && tid < p.parts) {
+        part_base = part[tid].used ? part[tid].base : -__builtin_inf();
+        s.low[tid] = part[tid].skipped;
+    }
+    if (tid == 0) {
+        p.rest[row].kind = kNone;
+        s.found_i = INT32_MAX;
+        s.n_list = 0;
+    }
+    x.weights();
+    x.largest();
+    if (x.simple(row, r.greedy)) return;
+    x.rate = r.rate();
+    // Whether the scan's places hold for this row: the largest logit within reach, nothing
+    // that was left out for being too low within the bins below it.
+    bool fits = fabs((double)x.m * x.rate) < kReach - kBins;
+    if (fits && r.cut)
+        for (int i = 0; i < p.parts; ++i)
+            if (s.low[i] > -inf && ((double)x.m - (double)s.low[i]) * x.rate < 2.0 * kBins) fits = false;
+    x.place_by_scan();
+    int kind = kAlone, bin = 0;
+    double most = 0.0, base_cnt = 0.0, base_mass = 0.0;
+    double have[kEach] = {};
+    if (fits && r.cut) {
+        // the parts' bins, each from its own base
+        if (tid < p.parts) {
+            const double d = x.base - part_base;
+            s.ahead[tid] = d < kBins ? (int)d : kBins;
+        }
+        __syncthreads();
+        const bool by_count = r.top_k > 0;  // (then the scan has counted only)
+        constexpr int PER = (kBins + kPickThreads - 1) / kPickThreads;
+        unsigned long long sm[PER] = {};
+        uint32_t sc[PER] = {};
+        // (eight parts' loads on their way together)
+#pragma unroll 1
+        for (int i0 = 0; i0 < p.parts; i0 += 8) {
+            uint32_t c[8][PER];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int d = i0 + i < p.parts ? s.ahead[i0 + i] : kBins;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const int b = tid + j * kPickThreads + d;
+                    c[i][j] = 0;
+                    if (b < kBins) c[i][j] = part[i0 + i].cnt[b];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < PER; ++j) sc[j] += c[i][j];
+            if (by_count) continue;
+            unsigned long long y[8][PER];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int d = i0 + i < p.parts ? s.ahead[i0 + i] : kBins;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    const int b = tid + j * kPickThreads + d;
+                    y[i][j] = 0;
+                    if (b < kBins) y[i][j] = part[i0 + i].mass[b];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < PER; ++j) sm[j] += y[i][j];
+        }
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (tid + j * kPickThreads < kBins) {
+                s.mass[tid + j * kPickThreads] = sm[j];
+                s.cnt[tid + j * kPickThreads] = sc[j];
+            }
+        __syncthreads();
+        const double unit = 1.0 / (double)(1ull << p.mass_bits), near_p = (double)r.top_p * (1.0 - kNear);
+        double whole;
+        bin = x.pick<kBins>(by_count, !by_count, by_count ? (double)r.top_k : near_p, [&](int b) { return sample_weight(s.octave, b, unit); }, base_cnt, base_mass, whole);
+        most = by_count ? (double)r.top_k : near_p * whole;
+        if (base_cnt + s.cnt[bin] <= kList) {
+            // few enough: one list of all that may be kept, cut once or twice
+            const int all = x.ask([&](int c) { return x.bin(s.cmax[c]) >= bin; });
+            const float under = x.under(bin);
+            x.each(all, [&](int i, f32x4 l) {
+                bool in[4], any = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) any |= l[e] >= under;
+                if (!__any(any)) return;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) in[e] = x.bin(l[e]) >= bin;
+                x.append(i, l, in);
+            }, [](int) {});
             __syncthreads();
-            for (int b = tid; b < kBins; b += kSampleThreads) {
+            const int n = s.n_list;
+#pragma unroll 1
+            for (int cuts = by_count && r.top_p < 1.0f ? 2 : 1, k = 0; k < cuts; ++k) {
+                const double kept = x.cut_list(n, by_count && k == 0, most, 0.0, 0.0);
+                most = near_p * kept;
+            }
+            x.min_w = (double)r.min_p * x.weight(x.m);
+            x.list_sums(n, have);
+            x.draw(row, r.u, have, 0, kBins);
+            return;
+        }
+        if (s.cnt[bin] <= kList && !(by_count && r.top_p < 1.0f)) kind = kCut;
+    } else if (fits && r.free()) {
+        // the scan's sums of chunks, each from its own base, unless one was out of reach
+        __syncthreads();
+        bool out = false;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int c = tid * kEach + k;
+            if (c >= p.chunks) continue;
+            const double cb = floor((double)s.cmax[c] * x.rate) + 1.0, at = cb - x.base + kBins;
+            if (!(at >= 0.0)) continue;
+            out |= !(fabs(cb) < kReach);
+            have[k] = sample_weight(s.octave, (int)at, p.cmass[(int64_t)row * kChunks + c]);
+        }
+        if (out) s.n_list = 1;
+        __syncthreads();
+        if (s.n_list == 0) {
+            x.draw(row, r.u, have, 0, 0);
+            return;
+        }
+    } else if (fits) {
+        kind = kBound;
+    }
+    if (tid == 0) {
+        SampleRest &o = p.rest[row];
+        o.kind = kind;
+        o.bin = kind == kCut ? bin : -1;
+        o.by_count = r.top_k > 0;
+        o.n_list = o.done = 0;
+        o.m = x.m;
+        o.most = most;
+        o.base_cnt = base_cnt;
+        o.base_mass = base_mass;
+    }
+}
+
+// All of a row's work by one workgroup.
+__device__ __forceinline__ void sample_alone(const SampleParams &p, PickLds &s, int row) {
+    using Row = PickRow<kRestThreads, true>;
+    constexpr int kPickThreads = Row::kPickThreads, kEach = Row::kEach;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float inf = __builtin_inff();
+    Row x(s, p, row);
+    const SampleRules r(p, row);
+    auto nothing = [](int) {};
+    {
+        const int all = x.ask([](int) { return true; });
+        float top = -inf;
+        x.each(all, [&](int, f32x4 l) { top = fmaxf(fmaxf(fmaxf(top, l[0]), fmaxf(l[1], l[2])), l[3]); },
+               [&](int c) {
+                   top = wave_max(top);
+                   if (lane == 0) s.cmax[c] = top;
+                   top = -inf;
+               });
+    }
+    x.weights();
+    if (tid == 0) s.found_i = INT32_MAX;
+    __syncthreads();
+    x.largest();
+    if (x.simple(row, r.greedy)) return;
+    x.flat = x.m == inf;  // only the infinite ones count
+    x.rate = r.rate();
+    const double scale = (double)(1ull << p.mass_bits), unit = 1.0 / scale;
+    double most = 0.0;
+#pragma unroll 1
+    for (int cut = r.top_k > 0 ? 0 : 1; cut < 2; ++cut) {
+        if (cut == 1 && !(r.top_p < 1.0f)) break;
+        const bool by_count = cut == 0, whole_row = cut == 1 && r.top_k == 0;
+        const double near_p = (double)r.top_p * (1.0 - kNear);
+        // the histogram of what is left in; then, as long as the bin of the last token has
+        // many, that of stretches of its logits' bits (lo .. hi)
+        int bin = -1;
+        uint32_t lo = 0, hi = 0xffffffffu, count = 0;
+        double base_cnt = 0.0, base_mass = 0.0;
+        if (by_count) most = (double)r.top_k;
+#pragma unroll 1
+        for (;;) {
+            const int shift = bin < 0 ? 0 : 22 - __builtin_clz((hi - lo) | 1023u);
+            const int all = x.ask([&](int c) { return bin < 0 ? s.cmax[c] >= x.last_l : x.bin(s.cmax[c]) >= bin; });
+            for (int b = tid; b < kBins; b += kPickThreads) {
                 s.mass[b] = 0;
                 s.cnt[b] = 0;
             }
             __syncthreads();
-            x.each([&](int c) { return s.cmax[c] >= last_l; }, [&](int i, float4 l) {
-                auto add = [&](float v, int t) {
-                    if (!x.counts(v) || !left_in(v, t)) return;
-                    const double at = x.place(v), f = floor(at);
-                    if (f < 0.0) return;
-                    atomicAdd(&s.mass[(int)f], sample_mass(at - f, scale));
-                    atomicAdd(&s.cnt[(int)f], 1u);
-                };
-                add(l.x, i);
-                add(l.y, i + 1);
-                add(l.z, i + 2);
-                add(l.w, i + 3);
-            }, [](int) {});
-            __syncthreads();
-        };
-        count_all();
-
-        // The last token, in the order of the cuts, before which fewer than `most`
-        // tokens (by_count) or less than `mass` lie; ahead: the sum of w up to it.
-        auto find = [&](bool by_count, double most, double &ahead) {
-            // thread t: bins 4095 - 4t and the three below it
-            auto pick = [&](auto weight_of, int &bin, double &base_cnt, double &base_mass) {
-                double cnt[4], mass[4], total;
-                double sc = 0.0, sm = 0.0;
+            x.each(all, [&](int i, f32x4 l) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int b = kBins - 1 - (tid * 4 + j);
-                    cnt[j] = s.cnt[b];
-                    mass[j] = cnt[j] != 0.0 ? weight_of(b) : 0.0;
-                    sc += cnt[j];
-                    sm += mass[j];
-                }
-                double bc = base_cnt + block_scan(sc, s.scan, total), bm = base_mass + block_scan(sm, s.scan2, total);
-                if (tid == 0) s.best = -1;
-                __syncthreads();
-                int best = -1;
-                double kc = 0.0, km = 0.0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (cnt[j] != 0.0 && ((by_count ? bc < most : bm < most) || bc == 0.0)) {
-                        best = tid * 4 + j;
-                        kc = bc;
-                        km = bm;
+                for (int e = 0; e < 4; ++e) {
+                    double past;
+                    int b = x.bin(l[e], past);
+                    if (b < 0 || !x.left_in(l[e], i + e)) continue;
+                    if (bin >= 0) {
+                        const uint32_t key = sample_key(l[e]);
+                        if (b != bin || key < lo || key > hi) continue;
+                        b = (int)((key - lo) >> shift);
                     }
-                    bc += cnt[j];
-                    bm += mass[j];
+                    atomicAdd(&s.mass[b], sample_mass(past, scale));
+                    atomicAdd(&s.cnt[b], 1u);
                 }
-                if (best >= 0) atomicMax(&s.best, best);
-                __syncthreads();
-                if (best >= 0 && s.best == best) {
-                    s.base_cnt = kc;
-                    s.base_mass = km;
-                }
-                __syncthreads();
-                bin = kBins - 1 - s.best;
-                base_cnt = s.base_cnt;
-                base_mass = s.base_mass;
-            };
-            double base_cnt = 0.0, base_mass = 0.0;
-            int bin;
-            const double unit = 1.0 / scale;
-            pick([&](int b) { return (double)s.mass[b] * unit * exp2((b - kAnchor) * (1.0 / kOctave)); }, bin, base_cnt, base_mass);
-            uint32_t n = s.cnt[bin];
-            const int bin0 = bin;
-            // the keys of the bin's logits, divided until few are left or all are equal
-            uint32_t lo = 0, hi = 0xffffffffu;
-            auto in_bin = [&](float l, int i) { return x.bin(l) == bin0 && sample_key(l) >= lo && sample_key(l) <= hi && left_in(l, i); };
-            auto maybe = [&](int c) { return x.bin(s.cmax[c]) >= bin0; };
+            }, nothing);
             __syncthreads();
-            while (n > kList && lo != hi) {
-                // (the histogram of the bins is built again below, where it is needed again)
-                const int shift = 32 - __builtin_clz((hi - lo) | 4095u) - 12;
-                for (int b = tid; b < kBins; b += kSampleThreads) {
-                    s.mass[b] = 0;
-                    s.cnt[b] = 0;
-                }
-                __syncthreads();
-                x.each(maybe, [&](int i, float4 l) {
-                    auto add = [&](float v, int t) {
-                        if (!in_bin(v, t)) return;
-                        const double at = x.place(v);
-                        atomicAdd(&s.mass[(sample_key(v) - lo) >> shift], sample_mass(at - floor(at), scale));
-                        atomicAdd(&s.cnt[(sample_key(v) - lo) >> shift], 1u);
-                    };
-                    add(l.x, i);
-                    add(l.y, i + 1);
-                    add(l.z, i + 2);
-                    add(l.w, i + 3);
-                }, [](int) {});
-                __syncthreads();
-                const double w0 = unit * exp2((bin0 - kAnchor) * (1.0 / kOctave));
-                pick([&](int b) { return (double)s.mass[b] * w0; }, bin, base_cnt, base_mass);
-                n = s.cnt[bin];
-                lo += (uint32_t)bin << shift;
+            // (stretches are numbered up to 1023: the bins above them are empty)
+            double whole;
+            const int found = x.pick<kBins>(by_count, bin < 0 && whole_row, bin < 0 && whole_row ? near_p : most,
+                                                           [&](int b) { return sample_weight(s.octave, bin < 0 ? b : bin, unit); }, base_cnt, base_mass, whole);
+            count = s.cnt[found];
+            if (bin < 0) {
+                if (whole_row) most = near_p * whole;
+                bin = found;
+            } else {
+                lo += (uint32_t)found << shift;
                 if (hi - lo > (1u << shift) - 1) hi = lo + ((1u << shift) - 1);
-                __syncthreads();
             }
-            if (n > kList) {
-                // equal logits: how many of them, and the number of the last one
-                const uint32_t b = lo & 0x80000000u ? lo ^ 0x80000000u : ~lo;
-                const float l = __uint_as_float(b);
-                const double w = x.weight(l);
-                double keep = by_count ? most - base_cnt : ceil((most - base_mass) / w);
-                keep = keep < 1.0 ? 1.0 : keep > n ? n : keep;
-                int mine = 0;
-                x.each(maybe, [&](int, float4 v) { mine += (v.x == l) + (v.y == l) + (v.z == l) + (v.w == l); },
-                       [&](int c) {
-                           const double sum = wave_sum((double)mine);
-                           if (lane == 0) s.cmass[c] = sum;
-                           mine = 0;
-                       });
-                __syncthreads();
-                double total;
-                const double have = tid < p.chunks && maybe(tid) ? s.cmass[tid] : 0.0;
-                const double before = block_scan(have, s.scan, total);
-                if (before < keep && before + have >= keep) {
-                    s.best = tid;
-                    s.base_cnt = keep - before;
-                }
-                __syncthreads();
-                const int c = s.best;
-                if (wave == 0) {
-                    double left = s.base_cnt;
-                    const int64_t c0 = (int64_t)c * x.chunk;
-                    for (int64_t i = c0; i < c0 + x.chunk && i < x.n && left > 0.0; i += 256) {
-                        const float4 v = x.load((int)i + lane * 4);
-                        const int is[4] = {v.x == l, v.y == l, v.z == l, v.w == l};
-                        const double all4 = is[0] + is[1] + is[2] + is[3], inc = wave_scan(all4);
-                        double at = inc - all4;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            at += is[j];
-                            if (is[j] && at == left) s.found_i = (int)i + lane * 4 + j;
-                        }
-                        left -= __shfl((float)inc, 63);
-                    }
-                }
-                __syncthreads();
-                last_l = l;
-                last_i = s.found_i;
-                ahead = base_mass + keep * w;
-                __syncthreads();
-                return bin0;
-            }
-            // the tokens of the bin in order
+            if (count <= kList || lo == hi) break;
+        }
+        const int all = x.ask([&](int c) { return x.bin(s.cmax[c]) >= bin; });
+        if (count <= kList) {
             if (tid == 0) s.n_list = 0;
             __syncthreads();
-            x.each(maybe, [&](int i, float4 l) {
-                auto add = [&](float v, int t) {
-                    if (!in_bin(v, t)) return;
-                    const int at = atomicAdd(&s.n_list, 1);
-                    s.list_l[at] = v;
-                    s.list_i[at] = t;
-                };
-                add(l.x, i);
-                add(l.y, i + 1);
-                add(l.z, i + 2);
-                add(l.w, i + 3);
-            }, [](int) {});
+            x.each(all, [&](int i, f32x4 l) {
+                bool in[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    in[e] = x.bin(l[e]) == bin && sample_key(l[e]) >= lo && sample_key(l[e]) <= hi && x.left_in(l[e], i + e);
+                x.append(i, l, in);
+            }, nothing);
             __syncthreads();
-            const int m = s.n_list;
-            if (tid < m) {
-                const float l = s.list_l[tid];
-                const int t = s.list_i[tid];
-                int rank = 0;
-                for (int j = 0; j < m; ++j) rank += SampleRow::before(s.list_l[j], s.list_i[j], l, t);
-                s.sort_l[rank] = l;
-                s.sort_i[rank] = t;
-            }
-            __syncthreads();
-            const double w = tid < m ? x.weight(s.sort_l[tid]) : 0.0;
-            double total;
-            const double at_mass = base_mass + block_scan(w, s.scan, total), at_cnt = base_cnt + tid;
-            if (tid == 0) s.best = 0;
-            __syncthreads();
-            const bool kept = tid < m && ((by_count ? at_cnt < most : at_mass < most) || at_cnt == 0.0);
-            if (kept) atomicMax(&s.best, tid);
-            __syncthreads();
-            if (tid == s.best) s.base_mass = at_mass + w;
-            last_l = s.sort_l[s.best];
-            last_i = s.sort_i[s.best];
-            __syncthreads();
-            ahead = s.base_mass;
-            return bin0;
-        };
-        double ahead = 0.0;
-        bool limited = false;
-        if (cut_k) {
-            find(true, (double)top_k, ahead);
-            limited = true;
+            most = near_p * x.cut_list(s.n_list, by_count, most, base_cnt, base_mass);
+            continue;
         }
-        if (cut_p) {
-            double whole = ahead;
-            if (limited) {
-                count_all();
-            } else {
-                double sm = 0.0;
+        // equal logits: how many of them, and the number of the last one
+        const float l = __uint_as_float(lo & 0x80000000u ? lo ^ 0x80000000u : ~lo);
+        const double w = x.weight(l);
+        double keep = by_count ? most - base_cnt : ceil((most - base_mass) / w);
+        keep = keep < 1.0 ? 1.0 : keep > count ? count : keep;
+        double same = 0.0, total, mine = 0.0;
+        for (int c = tid; c < kChunks; c += kPickThreads) s.cmass[c] = 0.0;
+        __syncthreads();
+        x.each(all, [&](int, f32x4 v) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) same += v[e] == l ? 1.0 : 0.0;
+        },
+               [&](int c) {
+                   same = wave_sum(same);
+                   if (lane == 0) s.cmass[c] = same;
+                   same = 0.0;
+               });
+        __syncthreads();
+        for (int k = 0; k < kEach; ++k) mine += s.cmass[tid * kEach + k];
+        double before = x.scan(mine, total);
+        for (int k = 0; k < kEach; ++k) {
+            const double have = s.cmass[tid * kEach + k];
+            if (before < keep && before + have >= keep) {
+                s.best = tid * kEach + k;
+                s.base_cnt = keep - before;
+            }
+            before += have;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            double left = s.base_cnt;
+            const int64_t c0 = (int64_t)s.best * x.chunk;
+#pragma unroll 1
+            for (int64_t i = c0; i < c0 + x.chunk && i < x.n && left > 0.0; i += kChunk) {
+                const f32x4 v = sample_load(x.src, x.n, i + lane * 4);
+                double is[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) is[j] = sample_clean(v[j]) == l ? 1.0 : 0.0;
+                const double four = is[0] + is[1] + is[2] + is[3], inc = wave_scan(four);
+                double at = inc - four;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int b = kBins - 1 - (tid * 4 + j);
-                    if (s.cnt[b]) sm += (double)s.mass[b] / scale * exp2((b - kAnchor) * (1.0 / kOctave));
+                    at += is[j];
+                    if (is[j] != 0.0 && at == left) s.found_i = (int)i + lane * 4 + j;
                 }
-                block_scan(sm, s.scan, whole);
-            }
-            const float kl = last_l;
-            const int ki = last_i;
-            find(false, (double)top_p * whole, ahead);
-            // (a rounding of the sums must not bring back what top-k cut off)
-            if (limited && SampleRow::before(kl, ki, last_l, last_i)) {
-                last_l = kl;
-                last_i = ki;
+                left -= last_lane(inc);
             }
         }
+        __syncthreads();
+        x.last_l = l;
+        x.last_i = s.found_i;
+        __syncthreads();
+        most = near_p * (base_mass + keep * w);
     }
-    // the kept w of each chunk
-    const double min_w = min_p > 0.0f ? (double)fminf(min_p, 1.0f) : 0.0;
-    auto kept_w = [&](float l, int i) {
-        if (!x.counts(l) || !left_in(l, i)) return 0.0;
-        const double w = x.weight(l);
-        return w >= min_w ? w : 0.0;
-    };
-    auto kept_chunk = [&](int c) { return s.cmax[c] >= last_l && s.cmax[c] > -inf; };
-    double sum = 0.0;
+    // the kept sum of each chunk
+    x.min_w = (double)r.min_p * x.weight(x.m);
+    const int all = x.ask([&](int c) { return s.cmax[c] >= x.last_l; });
+    for (int c = tid; c < kChunks; c += kPickThreads) s.cmass[c] = 0.0;
     __syncthreads();
-    x.each(kept_chunk, [&](int i, float4 l) {
-        sum += (kept_w(l.x, i) + kept_w(l.y, i + 1)) + (kept_w(l.z, i + 2) + kept_w(l.w, i + 3));
+    double sum = 0.0, have[kEach];
+    x.each(all, [&](int i, f32x4 l) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const double w = x.weight(l[e]);
+            sum += w >= x.min_w && x.left_in(l[e], i + e) ? w : 0.0;
+        }
     }, [&](int c) {
         sum = wave_sum(sum);
         if (lane == 0) s.cmass[c] = sum;
         sum = 0.0;
     });
     __syncthreads();
-    double total;
-    const double have = tid < p.chunks && kept_chunk(tid) ? s.cmass[tid] : 0.0;
-    const double before = block_scan(have, s.scan, total);
-    const double target = (double)u * total;
-    if (tid == 0) s.best = -1;
-    __syncthreads();
-    // the first chunk whose sum passes the target; where rounding leaves none, the last with any
-    if (have > 0.0 && before <= target) atomicMax(&s.best, tid);
-    __syncthreads();
-    if (tid == s.best) s.base_mass = target - before;
-    __syncthreads();
-    if (wave == 0) {
-        double left = s.base_mass;
-        const int64_t c0 = (int64_t)(s.best < 0 ? 0 : s.best) * x.chunk;
-        int token = -1;
-        float logit = 0.0f;
-        bool done = false;
-        for (int64_t i = c0; i < c0 + x.chunk && i < x.n && !done; i += 256) {
-            const int t = (int)i + lane * 4;
-            const float4 l = x.load(t);
-            const float v[4] = {l.x, l.y, l.z, l.w};
-            double w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = kept_w(v[j], t + j);
-            const double mine = (w[0] + w[1]) + (w[2] + w[3]), inc = wave_scan(mine);
-            double at = inc - mine;
-            int pick = -1, any = -1;
-#pragma unroll
-            for (int j = 3; j >= 0; --j) {
-                double upto = at;
-#pragma unroll
-                for (int k = 0; k <= j; ++k) upto += w[k];
-                if (w[j] > 0.0 && any < 0) any = j;
-                if (w[j] > 0.0 && upto > left) pick = j;
-            }
-            const unsigned long long passed = __ballot(pick >= 0), some = __ballot(any >= 0);
-            if (passed) {
-                const int from = __builtin_ctzll(passed);
-                const int j = __shfl(pick, from);
-                token = (int)i + from * 4 + j;
-                logit = __shfl(j == 0 ? v[0] : j == 1 ? v[1] : j == 2 ? v[2] : v[3], from);
-                done = true;
-            } else if (some) {  // (so far the last)
-                const int from = 63 - __builtin_clzll(some);
-                const int j = __shfl(any, from);
-                token = (int)i + from * 4 + j;
-                logit = __shfl(j == 0 ? v[0] : j == 1 ? v[1] : j == 2 ? v[2] : v[3], from);
-            }
-            left -= wave_sum(mine);
-        }
-        if (lane == 0) {
-            p.tokens[row] = token;
-            if (p.logprob) p.logprob[row] = (float)log(x.weight(logit) / total);
-        }
-    }
+    for (int k = 0; k < kEach; ++k) have[k] = s.cmass[tid * kEach + k];
+    x.draw(row, r.u, have, 0, 0);
 }
 
-static bool sample_sizes(int64_t n_vocab, int64_t n_rows) { return n_vocab >= 0 && n_rows >= 0 && n_vocab <= INT32_MAX && n_rows <= INT32_MAX; }
+__global__ __launch_bounds__(kRestThreads) void sample_rest_kernel(SampleParams p) {
+    extern __shared__ __attribute__((aligned(16))) char lds_bytes[];
+    PickLds &s = *reinterpret_cast<PickLds *>(lds_bytes);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int row = blockIdx.x / p.rest_parts, part = blockIdx.x - row * p.rest_parts;
+    const int kind = p.rest ? p.rest[row].kind : kAlone;
+    if (kind == kNone) return;
+    if (kind == kAlone) {
+        if (part == 0) sample_alone(p, s, row);
+        return;
+    }
+    using Row = PickRow<kRestThreads, false>;
+    constexpr int kPickThreads = Row::kPickThreads, kEach = Row::kEach;
+    SampleRest &o = p.rest[row];
+    Row x(s, p, row);
+    const SampleRules r(p, row);
+    const int bin = o.bin;
+    x.m = o.m;
+    x.rate = r.rate();
+    x.place_by_scan();
+#pragma unroll
+    for (int k = 0; k < kEach; ++k)
+        if (tid + k * kPickThreads < p.chunks) s.cmax[tid + k * kPickThreads] = p.cmax[(int64_t)row * kChunks + tid + k * kPickThreads];
+    x.weights();
+    if (tid == 0) s.n_list = 0;
+    __syncthreads();
+    x.min_w = (double)r.min_p * x.weight(x.m);
+    double *cmass = p.cmass + (int64_t)row * kChunks;
+    auto on = [&](int c) { return kind == kCut ? x.bin(s.cmax[c]) >= bin : x.weight(s.cmax[c]) >= x.min_w; };
+    // chunks are dealt out to the parts, so that each has its share of those that count
+    const int all = x.ask([&](int c) { return c % p.rest_parts == part && on(c); });
+    double sum = 0.0;
+    const float under = bin >= 0 ? x.under(bin) : -__builtin_inff();
+    x.each(all, [&](int i, f32x4 l) {
+        bool in[4], any = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= l[e] >= under;
+        if (!__any(any)) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            double past = 0.0;
+            const int b = x.bin(l[e], past);
+            const double w = b > bin ? sample_weight(s.octave, b, sample_exp(past, 1.0, 0.0)) : 0.0;
+            sum += w >= x.min_w ? w : 0.0;
+            in[e] = b == bin && b >= 0;
+        }
+        x.append(i, l, in);
+    }, [&](int c) {
+        sum = wave_sum(sum);
+        if (lane == 0) cmass[c] = sum;
+        sum = 0.0;
+    });
+    __syncthreads();
+    // the part's tokens of the bin to the row's; the last part to come here has them all
+    const int mine = s.n_list;
+    if (tid == 0) s.best = mine ? atomicAdd(&o.n_list, mine) : 0;
+    __syncthreads();
+    for (int e = tid; e < mine; e += kPickThreads) {
+        o.list_l[s.best + e] = s.list_l[e];
+        o.list_i[s.best + e] = s.list_i[e];
+    }
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) s.best = atomicAdd(&o.done, 1);
+    __syncthreads();
+    if (s.best != p.rest_parts - 1) return;
+    __threadfence();
+    double have[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const int c = tid * kEach + k;
+        have[k] = c < p.chunks && on(c) ? __hip_atomic_load(&cmass[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    }
+    if (kind == kCut) {
+        const int n = __hip_atomic_load(&o.n_list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int e = tid; e < n; e += kPickThreads) {
+            s.list_l[e] = __hip_atomic_load(&o.list_l[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            s.list_i[e] = __hip_atomic_load(&o.list_i[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        x.cut_list(n, o.by_count, o.most, o.base_cnt, o.base_mass);
+        x.list_sums(n, have);
+    }
+    x.draw(row, r.u, have, bin, bin + 1);
+}
+
+// How the rows are scanned: parts of them (0: not), tiles of a part.
+static void sample_split(int64_t n_vocab, int64_t n_rows, int cus, int &parts, int &tiles) {
+    parts = tiles = 0;
+    if (n_vocab > (int64_t)kChunks * kChunk || n_vocab == 0) return;
+    const int64_t all = (n_vocab + kTile - 1) / kTile;
+    int64_t want = 3 * (int64_t)cus / n_rows;
+    want = want < 1 ? 1 : want > kParts ? kParts : want;
+    if (want > all) want = all;
+    tiles = (int)((all + want - 1) / want);
+    parts = (int)((all + tiles - 1) / tiles);
+}
+// Bytes for n_rows rows and any fewer: no split has more parts in all than this.
+static size_t sample_bytes(int64_t n_vocab, int64_t n_rows, int cus) {
+    if (n_vocab > (int64_t)kChunks * kChunk || n_vocab == 0) return 0;
+    const int64_t most = n_rows * kParts, busy = n_rows > 3 * (int64_t)cus ? n_rows : 3 * (int64_t)cus;
+    return (size_t)((most < busy ? most : busy) * sizeof(SamplePart) + n_rows * (sizeof(SampleRest) + kChunks * (sizeof(float) + sizeof(double))));
+}
 
 }  // namespace q4k
 
@@ -543,34 +1227,60 @@ using namespace q4k;
 extern "C" {
 
 size_t q4k_sample_workspace_bytes(int64_t n_vocab, int64_t n_rows) {
-    (void)n_vocab;
-    (void)n_rows;
-    return 0;
+    DeviceInfo *di;
+    if (n_vocab < 0 || n_rows < 1 || n_vocab > (1 << 30) || n_rows > INT32_MAX / kParts || device_info(&di) != Q4K_OK) return 0;
+    return sample_bytes(n_vocab, n_rows, di->cus);
 }
 
 int q4k_sample(const float *src, int64_t n_vocab, int64_t n_rows, int64_t nb_src, const q4k_sample_rules *rules, int32_t *tokens, float *logprob,
                void *workspace, size_t workspace_bytes, void *stream) {
-    (void)workspace;
-    (void)workspace_bytes;
-    if (!rules || !sample_sizes(n_vocab, n_rows)) return Q4K_EINVAL;
+    if (!rules || n_vocab < 0 || n_rows < 0 || n_vocab > INT32_MAX || n_rows > INT32_MAX) return Q4K_EINVAL;
     const q4k_sample_rules &r = *rules;
     if (!aligned(src, 4) || !aligned(r.temperature, 4) || !aligned(r.top_k, 4) || !aligned(r.top_p, 4) || !aligned(r.min_p, 4) ||
         !aligned(r.uniform, 4) || !aligned(tokens, 4) || !aligned(logprob, 4))
         return Q4K_EINVAL;
     if (n_rows == 0) return Q4K_OK;
     if ((!src && n_vocab > 0) || !tokens || nb_src % 4 != 0 || (n_rows > 1 && nb_src < 4 * n_vocab)) return Q4K_EINVAL;
-    if (n_vocab > (1 << 30)) return Q4K_EUNSUPPORTED;
+    if (n_vocab > (1 << 30) || n_rows > INT32_MAX / kParts) return Q4K_EUNSUPPORTED;
     DeviceInfo *di;
     int st = device_info(&di);
     if (st != Q4K_OK) return st;
-    int chunk = 256, bits = 0;
-    while ((n_vocab + chunk - 1) / chunk > kChunks) chunk *= 2;
+    SampleParams p{};
+    p.src = reinterpret_cast<const char *>(src);
+    p.nb_src = nb_src;
+    p.n_vocab = (int)n_vocab;
+    p.n_rows = (int)n_rows;
+    p.chunk = kChunk;
+    while ((n_vocab + p.chunk - 1) / p.chunk > kChunks) p.chunk *= 2;
+    p.chunks = (int)((n_vocab + p.chunk - 1) / p.chunk);
+    int bits = 0;
     while ((int64_t)1 << bits < n_vocab) ++bits;
-    const SampleParams p{reinterpret_cast<const char *>(src), nb_src, (int)n_vocab, (int)n_rows, chunk, (int)((n_vocab + chunk - 1) / chunk),
-                         62 - bits < 44 ? 62 - bits : 44, r, tokens, logprob};
-    st = ensure_lds(di, reinterpret_cast<const void *>(&sample_kernel), (int)sizeof(SampleLds));
+    p.mass_bits = 62 - bits < 44 ? 62 - bits : 44;
+    p.r = r;
+    p.tokens = tokens;
+    p.logprob = logprob;
+    sample_split(n_vocab, n_rows, di->cus, p.parts, p.tiles);
+    st = ensure_lds(di, reinterpret_cast<const void *>(&sample_pick_kernel), (int)sizeof(PickLds));
+    if (st == Q4K_OK) st = ensure_lds(di, reinterpret_cast<const void *>(&sample_rest_kernel), (int)sizeof(PickLds));
     if (st != Q4K_OK) return st;
-    return launch(sample_kernel, dim3((unsigned)n_rows), kSampleThreads, (int)sizeof(SampleLds), stream, p);
+    Workspace ws;
+    st = ws.begin(workspace, workspace_bytes, sample_bytes(n_vocab, n_rows, di->cus), stream);
+    if (st != Q4K_OK) return st;
+    p.rest_parts = 1;
+    if (p.parts) {
+        p.cmass = (double *)ws.ptr;
+        p.part = (SamplePart *)(p.cmass + n_rows * kChunks);
+        p.rest = (SampleRest *)(p.part + n_rows * p.parts);
+        p.cmax = (float *)(p.rest + n_rows);
+        st = launch(sample_scan_kernel, dim3((unsigned)(n_rows * p.parts)), kScanThreads, 0, stream, p);
+        if (st == Q4K_OK) st = launch(sample_pick_kernel, dim3((unsigned)n_rows), kPickThreads, (int)sizeof(PickLds), stream, p);
+        // parts of 32 chunks or more, four workgroups a CU at most
+        const int64_t most = 4 * (int64_t)di->cus / n_rows;
+        p.rest_parts = p.chunks < 64 ? 1 : p.chunks < 512 ? p.chunks / 32 : kParts;
+        if (p.rest_parts > most) p.rest_parts = most < 2 ? 2 : (int)most;
+    }
+    if (st == Q4K_OK) st = launch(sample_rest_kernel, dim3((unsigned)(n_rows * p.rest_parts)), kRestThreads, (int)sizeof(PickLds), stream, p);
+    return ws.end(st, stream);
 }
 
 }  // extern "C"

@@ -188,7 +188,8 @@ size_t q4k_sample_workspace_bytes(int64_t n_vocab, int64_t n_rows);
  * The token is the first, in the order of token numbers, up to which the kept w's
  * sum exceeds uniform times their sum.  Logits of -inf and NaN are no candidates; a
  * row without any gives -1; with logits of +inf those are the candidates, alike.
- * w and its sums are 64 bits; tokens below 2^-127 of the largest w count as 0.
+ * w and its sums are 64 bits; sums within 2^-40 of a border count as equal to it,
+ * tokens below 2^-63 of the largest w as 0.
  * logprob[i] (may be NULL): the logarithm of the token's share of the kept
  * w's sum, 0 where the largest logit was taken, -inf where there is none. */
 int q4k_sample(const float *src, int64_t n_vocab, int64_t n_rows, int64_t nb_src, const q4k_sample_rules *rules,
