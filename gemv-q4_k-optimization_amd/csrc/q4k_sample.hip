@@ -8,15 +8,18 @@
 //   scan  parts of the rows, read once: the largest logit of each chunk of 256 and
 //         what the row's rules need, counts and sums of w in bins of 2^(1/24), or
 //         without cuts the sum of each chunk
-//   pick  a workgroup a row: the bin of the last token that is kept, and where the tokens
-//         from there up are few (kList) that token among them, the kept sum of each
-//         chunk, the chunk that the random number falls into and the token in it
-//   rest  where they are not, workgroups of all parts of the row again: the sums by
-//         chunks of what is above that bin and the bin's own tokens; the last of them
-//         finds the last token that is kept, and draws.  What is rare, one workgroup does
-//         from the row alone: rows out of the scan's reach, top-k and top-p both past
-//         kList, a bin of more than kList tokens (divided by the logits' bits until it
-//         has less or only equal ones, which are told apart by a count).
+//   draw  workgroups of all parts of the row find the bin of the last token that is kept
+//         from the scan's octaves and then that octave's bins, each for itself, and read
+//         the chunks that matter again: the tokens from that bin up where they are few
+//         (kList), else the sums by chunks of what is above it and the bin's own tokens.
+//         The last workgroup of a row cuts the list to the last token that is kept, sums it
+//         by chunks, and finds the chunk that the random number falls into and the token
+//         in it.  What is rare, one workgroup does from the row alone: rows out of the
+//         scan's reach, top-k and top-p both past kList, a bin of more than kList tokens
+//         (divided by the logits' bits until it has less or only equal ones, which are
+//         told apart by a count).
+// (A CU reads some 13 bytes a cycle from beyond the L2s, so that one workgroup a row would
+// take longer for a row's logits, or for whole histograms, than all else takes.)
 // Sums of bins are integers (any order gives the same), all others are 64-bit floats
 // in an order of their own: equal calls give equal bits.  A chunk whose largest
 // logit is below the cut is not read again.
@@ -32,9 +35,7 @@
 
 namespace q4k {
 
-// (Eight and four waves: what is not memory is chains of scans over the workgroup, whose
-// instructions cost each SIMD the more the more waves it has.)
-constexpr int kPickThreads = 512, kRestThreads = 256, kMostWaves = 8;
+constexpr int kDrawThreads = 512;
 constexpr int kScanThreads = 512, kScanWaves = kScanThreads / 64, kTile = kScanThreads * 8;
 constexpr int kOctave = 24, kBins = 64 * kOctave;  // what is below the last bin is never drawn
 constexpr int kChunk = 256, kChunks = 1024, kList = 1024, kParts = 16;
@@ -44,26 +45,25 @@ constexpr double kReach = 16384.0;
 // Sums nearer to a border than this part of it count as equal to it.
 constexpr double kNear = 0x1p-40;
 
+constexpr int kOctaves = kBins / kOctave;
+
 // What a part of a row was found to hold.
 struct SamplePart {
-    double base;   // bin i is place base - kBins + i
-    float skipped; // the largest logit of tiles that were too low to be placed
-    int used;      // whether some tile was not
+    double base;    // bin i is place base - kBins + i
+    float skipped;  // the largest logit of tiles that were too low to be placed
+    int used;       // whether some tile was not
+    double octave_mass[kOctaves];  // of an octave's bins, in units of its lowest one
+    uint32_t octave_cnt[kOctaves];
     unsigned long long mass[kBins];
     uint32_t cnt[kBins];
 };
 
-// What the pick leaves to the rest of a row.
-struct SampleRest {
-    int kind, bin, by_count;  // (bin: of the last token that is kept, for kCut)
-    int n_list, done;         // tokens of the bin; parts that are done
-    float m;
-    double most, base_cnt, base_mass;
-    float list_l[kList];
-    int list_i[kList];
+// What the workgroups of a row share: the list of tokens, and how many are done.
+struct SampleList {
+    int n, done;
+    float l[kList];
+    int i[kList];
 };
-// nothing; the tokens above the bin and some in it; all that min-p keeps; all of the row's work
-constexpr int kNone = 0, kCut = 1, kBound = 2, kAlone = 3;
 
 struct SampleParams {
     const char *src;
@@ -71,12 +71,12 @@ struct SampleParams {
     int n_vocab, n_rows;
     int chunk, chunks;  // tokens of a chunk (a multiple of 256), chunks of a row
     int mass_bits;      // of a token's integer weight in its bin
-    int parts, tiles;   // of a row; of a part
+    int parts, tiles;   // of a row (0: not scanned); of a part
+    int shares;         // workgroups of a row's draw
     SamplePart *part;
     float *cmax;        // [rows][kChunks]
     double *cmass;
-    SampleRest *rest;   // null: the rest does all
-    int rest_parts;
+    SampleList *list;
     q4k_sample_rules r;
     int32_t *tokens;
     float *logprob;
@@ -146,16 +146,29 @@ __device__ __forceinline__ float wave_max(float x) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
-// Four logits of a row of n; NaN and what is past the row are no candidates.
-__device__ __forceinline__ f32x4 sample_load(const float *src, int n, int64_t i) {
-    f32x4 x;
-    if (i + 4 <= n) {
-        x = load4<false>(src + i);
-    } else {
+// Four logits of a row of n from token i, read from where the row has four (no branch
+// between loads, so that all of a thread's are on their way together); sample_fix moves
+// them to their places, past the row -inf.
+__device__ __forceinline__ f32x4 sample_load(const float *src, int n, int i) {
+    if (n < 4) {
+        f32x4 x;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = i + j < n ? src[i + j] : -__builtin_inff();
+        for (int j = 0; j < 4; ++j) x[j] = j < n ? src[j] : -__builtin_inff();
+        return x;
     }
-    return x;
+    return load4<false>(src + (i < n - 4 ? i : n - 4));
+}
+__device__ __forceinline__ f32x4 sample_fix(f32x4 x, int n, int i) {
+    const int by = n < 4 ? i : i - (n - 4);
+    if (by <= 0) return x;
+    f32x4 y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        y[j] = -__builtin_inff();
+#pragma unroll
+        for (int k = j + 1; k < 4; ++k) y[j] = k - j == by ? x[k] : y[j];
+    }
+    return y;
 }
 // (zeros are equal whatever their sign)
 __device__ __forceinline__ float sample_clean(float l) { return l != l ? -__builtin_inff() : l + 0.0f; }
@@ -188,7 +201,7 @@ __device__ __forceinline__ unsigned long long sample_mass(double x, double scale
 __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams p) {
     __shared__ unsigned long long mass[kBins];
     __shared__ uint32_t cnt[kBins];
-    __shared__ double octave[kOctave];
+    __shared__ double octave[kOctave];  // the powers of 2^(1/24)
     __shared__ float tops[2][kScanWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int row = blockIdx.x / p.parts, part = blockIdx.x - row * p.parts;
@@ -199,15 +212,14 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
     // thread: tokens wave * 512 + lane * 4 and 256 past it
     const int at = wave * 2 * kChunk + lane * 4;
     f32x4 next[2];
-    next[0] = sample_load(src, p.n_vocab, beg + at);
-    next[1] = sample_load(src, p.n_vocab, beg + at + kChunk);
+    next[0] = sample_load(src, p.n_vocab, (int)beg + at);
+    next[1] = sample_load(src, p.n_vocab, (int)beg + at + kChunk);
     const SampleRules r(p, row);
     const bool cut = r.cut, by_mass = r.top_k == 0, free = r.free();  // (top-k needs counts alone)
     const double rate = r.rate(), scale = (double)(1ull << p.mass_bits);
-    if (free) {
-        if (tid < kOctave) octave[tid] = exp2(tid * (1.0 / kOctave));
-        __syncthreads();
-    }
+    if (tid < kOctave) octave[tid] = exp2(tid * (1.0 / kOctave));
+    if (part == 0 && tid == 0) p.list[row].n = p.list[row].done = 0;
+    if (free) __syncthreads();
     float *cmax = p.cmax + (int64_t)row * kChunks;
     double *cmass = p.cmass + (int64_t)row * kChunks;
     double base = 0.0;  // bins: places base - kBins .. base - 1
@@ -217,9 +229,11 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
     int par = 0;
     for (int64_t t0 = beg; t0 < end && t0 < p.n_vocab; t0 += kTile, par ^= 1) {
         f32x4 l[2] = {next[0], next[1]};
-        if (t0 + kTile < end && t0 + kTile < p.n_vocab) {
-            next[0] = sample_load(src, p.n_vocab, t0 + kTile + at);
-            next[1] = sample_load(src, p.n_vocab, t0 + kTile + at + kChunk);
+        next[0] = sample_load(src, p.n_vocab, (int)t0 + kTile + at);  // (behind the part: what is not used)
+        next[1] = sample_load(src, p.n_vocab, (int)t0 + kTile + at + kChunk);
+        if (t0 + kTile > p.n_vocab) {
+            l[0] = sample_fix(l[0], p.n_vocab, (int)t0 + at);
+            l[1] = sample_fix(l[1], p.n_vocab, (int)t0 + at + kChunk);
         }
         float top[2];
 #pragma unroll
@@ -293,9 +307,22 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
         if (by_mass) out.mass[i] = mass[b];
         out.cnt[i] = cnt[b];
     }
+    if (tid < kOctaves) {
+        double m = 0.0;
+        uint32_t c = 0;
+#pragma unroll 1
+        for (int k = 0; k < kOctave; ++k) {
+            const int i = tid * kOctave + k, b = i + off >= kBins ? i + off - kBins : i + off;
+            if (by_mass) m += (double)mass[b] * octave[k];
+            c += cnt[b];
+        }
+        out.octave_mass[tid] = m;
+        out.octave_cnt[tid] = c;
+    }
 }
 
 // ---- pick and rest: a row's token from what the scan found ----
+// (62 KB: below what a launch has to ask for)
 struct PickLds {
     unsigned long long mass[kBins];
     double octave[kOctave];  // the powers of 2^(1/24)
@@ -305,19 +332,38 @@ struct PickLds {
     float list_l[kList], sort_l[kList];
     int list_i[kList], sort_i[kList];
     int todo[kChunks];
-    double scan[2][kMostWaves];
-    float tops[kMostWaves], lows[kMostWaves];
-    int bests[kMostWaves];
+    double scan[2][kDrawThreads / 64];
+    float tops[kDrawThreads / 64], lows[kDrawThreads / 64];
+    int bests[kDrawThreads / 64];
     int n_todo, n_list, n_sort, best, found_i;
     double base_cnt, base_mass;
-    int ahead[kParts];  // bins that a part's base lies below the row's; kBins: nothing in it
+    int ahead[kParts];  // octaves that a part's base lies below the row's; kOctaves: nothing in it
     float low[kParts];
+    int bin, bin_cnt;   // of the last token that is kept
+    double whole;
 };
+
+// What workgroups of a launch hand each other: past the L2 of their own, so that no fence has to
+// write back and drop all of it (256 rows of 151936: 208 us a draw with fences, 90 without).
+template <class T>
+__device__ __forceinline__ void sample_give(T *to, T x) {
+    __hip_atomic_store(to, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <class T>
+__device__ __forceinline__ T sample_take(const T *from) {
+    return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 
 // ordered bits of a float: larger logits have larger keys
 __device__ __forceinline__ uint32_t sample_key(float l) {
     const uint32_t b = __float_as_uint(l);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+// the next float up or down (by 1 or -1), past -0
+__device__ __forceinline__ float sample_next(float l, int by) {
+    uint32_t k = sample_key(l + 0.0f) + (uint32_t)by;
+    if (k == 0x7fffffffu) k += (uint32_t)by;
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 // the order of the cuts: lower tokens of equal logits come first
 __device__ __forceinline__ bool sample_before(float l, int i, float k, int j) { return l > k || (l == k && i < j); }
@@ -484,7 +530,7 @@ struct PickRow {
             for (int j = 0; j < SET; ++j) {
                 const int k = k0 + j < mine ? k0 + j : mine - 1;
                 q.c[j] = s.todo[wave + (k >> more) * kPickWaves];
-                q.v[j] = sample_load(src, n, (int64_t)q.c[j] * chunk + (k & (subs - 1)) * kChunk + lane * 4);
+                q.v[j] = sample_load(src, n, q.c[j] * chunk + (k & (subs - 1)) * kChunk + lane * 4);
             }
         };
         auto use = [&](const Set &q, int k0) {
@@ -492,10 +538,11 @@ struct PickRow {
             for (int j = 0; j < SET; ++j) {
                 if (k0 + j >= mine) break;
                 const int sub = (k0 + j) & (subs - 1);
-                f32x4 l;
+                const int i = q.c[j] * chunk + sub * kChunk + lane * 4;
+                f32x4 l = sample_fix(q.v[j], n, i);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) l[e] = sample_clean(q.v[j][e]);
-                f(q.c[j] * chunk + sub * kChunk + lane * 4, l);
+                for (int e = 0; e < 4; ++e) l[e] = sample_clean(l[e]);
+                f(i, l);
                 if (sub == subs - 1) end(q.c[j]);
             }
         };
@@ -527,19 +574,169 @@ struct PickRow {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int k = at + __builtin_popcountll(b[e] & ((1ull << lane) - 1));
-            if (in[e]) {
+            if (in[e] && k < kList) {  // (no more are ever counted)
                 s.list_l[k] = l[e];
                 s.list_i[k] = i + e;
             }
             at += __builtin_popcountll(b[e]);
         }
     }
-    // A logit that is surely below the bin's lower end, though not by much (-inf where
-    // that is past F32): what is under it needs no place.
-    __device__ __forceinline__ float under(int bin_) const {
-        const double l = (base - kBins + bin_) / rate;
-        const float f = (float)(l - fabs(l) * 0x1p-20);
-        return fabsf(f) < 3e38f ? f : -__builtin_inff();
+    // Of the listed chunks (of 256): the logits from `least` up and below `above` to the list,
+    // the sum of w of those from `above` up to sums[chunk], where SUMS.  Four chunks of a
+    // wave at a time without a branch between them, so that their chains overlap, and four
+    // more on their way.
+    template <bool SUMS>
+    __device__ __forceinline__ void collect(int count, float least, float above, double *sums) const {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int mine = count > wave ? (count - wave - 1) / kPickWaves + 1 : 0;
+        constexpr int SET = 4;
+        struct Set {
+            f32x4 v[SET];
+            int c[SET];
+        } a, b;
+        auto load = [&](Set &q, int k0) {
+#pragma unroll
+            for (int j = 0; j < SET; ++j) {
+                const int k = k0 + j < mine ? k0 + j : mine - 1;
+                q.c[j] = __builtin_amdgcn_readfirstlane(s.todo[wave + k * kPickWaves]);
+                q.v[j] = sample_load(src, n, q.c[j] * kChunk + lane * 4);
+            }
+        };
+        auto use = [&](Set &q, int k0) {
+#pragma unroll
+            for (int j = 0; j < SET; ++j)
+                if ((q.c[j] + 1) * kChunk > n) q.v[j] = sample_fix(q.v[j], n, q.c[j] * kChunk + lane * 4);
+            if (SUMS) {
+                bool any = false;
+#pragma unroll
+                for (int j = 0; j < SET; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) any |= q.v[j][e] >= above;
+                double sum[SET] = {};
+                if (__any(any)) {
+#pragma unroll
+                    for (int j = 0; j < SET; ++j) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float l = q.v[j][e];
+                            const double t = place(l), f = floor(t);
+                            int at = (int)(f - base + kBins);
+                            at = at < 0 ? 0 : at > kBins - 1 ? kBins - 1 : at;
+                            const double w = sample_weight(s.octave, at, sample_exp(t - f, 1.0, 0.0));
+                            sum[j] += l >= above && w >= min_w ? w : 0.0;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < SET; ++j) sum[j] = wave_sum(sum[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < SET; ++j)
+                    if (lane == 0) sample_give(&sums[q.c[j]], sum[j]);  // (past the last one: that again)
+            }
+            unsigned long long in[SET][4];
+            int all = 0;
+#pragma unroll
+            for (int j = 0; j < SET; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    in[j][e] = __ballot(k0 + j < mine && q.v[j][e] >= least && q.v[j][e] < above);
+                    all += __builtin_popcountll(in[j][e]);
+                }
+            if (all == 0) return;
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&s.n_list, all);
+            at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+            for (int j = 0; j < SET; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (in[j][e] == 0) continue;
+                    const int k = at + __builtin_popcountll(in[j][e] & ((1ull << lane) - 1));
+                    if (((in[j][e] >> lane) & 1) && k < kList) {  // (no more are ever counted)
+                        s.list_l[k] = q.v[j][e] + 0.0f;
+                        s.list_i[k] = q.c[j] * kChunk + lane * 4 + e;
+                    }
+                    at += __builtin_popcountll(in[j][e]);
+                }
+        };
+        if (mine == 0) return;
+        load(a, 0);
+#pragma unroll 1
+        for (int k = 0; k < mine; k += 2 * SET) {
+            if (k + SET < mine) load(b, k + SET);
+            use(a, k);
+            if (k + SET >= mine) break;
+            if (k + 2 * SET < mine) load(a, k + 2 * SET);
+            use(b, k + SET);
+        }
+    }
+
+    // By one wave, from the scan's octaves and then one octave's bins: the bin of the last token
+    // before which fewer than `most` tokens (by_count) or less than `most` of the whole sum of w
+    // lie, its number of tokens, what lies before it, and the whole; to LDS.
+    __device__ __forceinline__ void pick_scanned(const SamplePart *part, int parts, bool by_count, double most) const {
+        const int lane = threadIdx.x & 63;
+        const double unit = 1.0 / (double)(1ull << p.mass_bits);
+        double base_cnt = 0.0, base_mass = 0.0, limit = most;
+        int octave = 0;
+#pragma unroll
+        for (int level = 0; level < 2; ++level) {
+            // lane: the octaves, then the octave's bins, from the highest
+            const int places = level == 0 ? kOctaves : kOctave;
+            double sum = 0.0, cnt = 0.0;
+            uint32_t c[kParts];
+            double m0[kParts];
+            unsigned long long m1[kParts];
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                // (read whether or not there is any, so that all loads are on their way together)
+                const int of = i < parts ? i : parts - 1, at = (level == 0 ? kOctaves - 1 - lane : octave) + s.ahead[of];
+                const int o = at < kOctaves ? at : kOctaves - 1, b = o * kOctave + kOctave - 1 - (lane < kOctave ? lane : 0);
+                c[i] = level == 0 ? part[of].octave_cnt[o] : part[of].cnt[b];
+                if (level == 0) m0[i] = part[of].octave_mass[o];
+                else m1[i] = part[of].mass[b];
+            }
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) {
+                const int at = (level == 0 ? kOctaves - 1 - lane : octave) + s.ahead[i < parts ? i : 0];
+                const bool is = i < parts && lane < places && at < kOctaves;
+                cnt += is ? c[i] : 0;
+                if (is && !by_count) sum += level == 0 ? m0[i] : (double)m1[i];
+            }
+            if (level == 0) sum = ldexp(sum * unit, -1 - lane);
+            else if (lane < kOctave) sum = sample_weight(s.octave, octave * kOctave + kOctave - 1 - lane, sum * unit);
+            const double ic = wave_scan(cnt), im = wave_scan(sum);
+            const double bc = base_cnt + (ic - cnt), bm = base_mass + (im - sum);
+            if (level == 0) {
+                const double whole = last_lane(im);
+                if (!by_count) limit = most * whole;
+                if (lane == 0) s.whole = whole;
+            }
+            const unsigned long long b = __ballot(cnt != 0.0 && ((by_count ? bc : bm) < limit || bc == 0.0));
+            const int found = 63 - __builtin_clzll(b | 1);
+            base_cnt = lane_of(bc, found);
+            base_mass = lane_of(bm, found);
+            if (level == 0) {
+                octave = kOctaves - 1 - found;
+            } else if (lane == found) {
+                s.bin = octave * kOctave + kOctave - 1 - found;
+                s.bin_cnt = (int)cnt;
+                s.base_cnt = base_cnt;
+                s.base_mass = base_mass;
+            }
+        }
+    }
+
+    // The least logit of the bins from bin_ up, so that one comparison of F32 tells (the bins'
+    // ends are steps away from their quotients by rounding only).
+    __device__ __forceinline__ float least(int bin_) const {
+        if (bin_ >= kBins) return __builtin_inff();
+        constexpr float most = 3.4028235e38f;
+        float l = (float)((base - kBins + bin_) / rate);
+        l = l != l ? -most : fminf(fmaxf(l, -most), most);
+        for (int k = 0; k < 16 && l < most && bin(l) < bin_; ++k) l = sample_next(l, 1);
+        for (int k = 0; k < 16 && l > -most && bin(sample_next(l, -1)) >= bin_; ++k) l = sample_next(l, -1);
+        return l;
     }
 
     // The bin of the last token before which fewer than `most` tokens (by_count) or
@@ -729,7 +926,7 @@ struct PickRow {
 #pragma unroll 1
         for (int64_t i = c0; i < c0 + chunk && i < n && !done; i += kChunk) {
             const int t = (int)i + lane * 4;
-            const f32x4 v = sample_load(src, n, t);
+            const f32x4 v = sample_fix(sample_load(src, n, t), n, t);
             double w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = kept_w(sample_clean(v[j]), t + j);
@@ -791,164 +988,10 @@ struct PickRow {
     }
 };
 
-__global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams p) {
-    extern __shared__ __attribute__((aligned(16))) char lds_bytes[];
-    PickLds &s = *reinterpret_cast<PickLds *>(lds_bytes);
-    using Row = PickRow<kPickThreads, false>;
-    constexpr int kEach = Row::kEach;
-    const int tid = threadIdx.x, row = blockIdx.x;
-    const float inf = __builtin_inff();
-    Row x(s, p, row);
-    const SampleRules r(p, row);
-    const SamplePart *part = p.part + (int64_t)row * p.parts;
-#pragma unroll
-    for (int k = 0; k < kEach; ++k)
-        if (tid + k * kPickThreads < p.chunks) s.cmax[tid + k * kPickThreads] = p.cmax[(int64_t)row * kChunks + tid + k * kPickThreads];
-    double part_base = 0.0;
-    if (r.cut && tid < p.parts) {
-        part_base = part[tid].used ? part[tid].base : -__builtin_inf();
-        s.low[tid] = part[tid].skipped;
-    }
-    if (tid == 0) {
-        p.rest[row].kind = kNone;
-        s.found_i = INT32_MAX;
-        s.n_list = 0;
-    }
-    x.weights();
-    x.largest();
-    if (x.simple(row, r.greedy)) return;
-    x.rate = r.rate();
-    // Whether the scan's places hold for this row: the largest logit within reach, nothing
-    // that was left out for being too low within the bins below it.
-    bool fits = fabs((double)x.m * x.rate) < kReach - kBins;
-    if (fits && r.cut)
-        for (int i = 0; i < p.parts; ++i)
-            if (s.low[i] > -inf && ((double)x.m - (double)s.low[i]) * x.rate < 2.0 * kBins) fits = false;
-    x.place_by_scan();
-    int kind = kAlone, bin = 0;
-    double most = 0.0, base_cnt = 0.0, base_mass = 0.0;
-    double have[kEach] = {};
-    if (fits && r.cut) {
-        // the parts' bins, each from its own base
-        if (tid < p.parts) {
-            const double d = x.base - part_base;
-            s.ahead[tid] = d < kBins ? (int)d : kBins;
-        }
-        __syncthreads();
-        const bool by_count = r.top_k > 0;  // (then the scan has counted only)
-        constexpr int PER = (kBins + kPickThreads - 1) / kPickThreads;
-        unsigned long long sm[PER] = {};
-        uint32_t sc[PER] = {};
-        // (eight parts' loads on their way together)
-#pragma unroll 1
-        for (int i0 = 0; i0 < p.parts; i0 += 8) {
-            uint32_t c[8][PER];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int d = i0 + i < p.parts ? s.ahead[i0 + i] : kBins;
-#pragma unroll
-                for (int j = 0; j < PER; ++j) {
-                    const int b = tid + j * kPickThreads + d;
-                    c[i][j] = 0;
-                    if (b < kBins) c[i][j] = part[i0 + i].cnt[b];
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int j = 0; j < PER; ++j) sc[j] += c[i][j];
-            if (by_count) continue;
-            unsigned long long y[8][PER];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int d = i0 + i < p.parts ? s.ahead[i0 + i] : kBins;
-#pragma unroll
-                for (int j = 0; j < PER; ++j) {
-                    const int b = tid + j * kPickThreads + d;
-                    y[i][j] = 0;
-                    if (b < kBins) y[i][j] = part[i0 + i].mass[b];
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int j = 0; j < PER; ++j) sm[j] += y[i][j];
-        }
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-            if (tid + j * kPickThreads < kBins) {
-                s.mass[tid + j * kPickThreads] = sm[j];
-                s.cnt[tid + j * kPickThreads] = sc[j];
-            }
-        __syncthreads();
-        const double unit = 1.0 / (double)(1ull << p.mass_bits), near_p = (double)r.top_p * (1.0 - kNear);
-        double whole;
-        bin = x.pick<kBins>(by_count, !by_count, by_count ? (double)r.top_k : near_p, [&](int b) { return sample_weight(s.octave, b, unit); }, base_cnt, base_mass, whole);
-        most = by_count ? (double)r.top_k : near_p * whole;
-        if (base_cnt + s.cnt[bin] <= kList) {
-            // few enough: one list of all that may be kept, cut once or twice
-            const int all = x.ask([&](int c) { return x.bin(s.cmax[c]) >= bin; });
-            const float under = x.under(bin);
-            x.each(all, [&](int i, f32x4 l) {
-                bool in[4], any = false;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) any |= l[e] >= under;
-                if (!__any(any)) return;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) in[e] = x.bin(l[e]) >= bin;
-                x.append(i, l, in);
-            }, [](int) {});
-            __syncthreads();
-            const int n = s.n_list;
-#pragma unroll 1
-            for (int cuts = by_count && r.top_p < 1.0f ? 2 : 1, k = 0; k < cuts; ++k) {
-                const double kept = x.cut_list(n, by_count && k == 0, most, 0.0, 0.0);
-                most = near_p * kept;
-            }
-            x.min_w = (double)r.min_p * x.weight(x.m);
-            x.list_sums(n, have);
-            x.draw(row, r.u, have, 0, kBins);
-            return;
-        }
-        if (s.cnt[bin] <= kList && !(by_count && r.top_p < 1.0f)) kind = kCut;
-    } else if (fits && r.free()) {
-        // the scan's sums of chunks, each from its own base, unless one was out of reach
-        __syncthreads();
-        bool out = false;
-#pragma unroll
-        for (int k = 0; k < kEach; ++k) {
-            const int c = tid * kEach + k;
-            if (c >= p.chunks) continue;
-            const double cb = floor((double)s.cmax[c] * x.rate) + 1.0, at = cb - x.base + kBins;
-            if (!(at >= 0.0)) continue;
-            out |= !(fabs(cb) < kReach);
-            have[k] = sample_weight(s.octave, (int)at, p.cmass[(int64_t)row * kChunks + c]);
-        }
-        if (out) s.n_list = 1;
-        __syncthreads();
-        if (s.n_list == 0) {
-            x.draw(row, r.u, have, 0, 0);
-            return;
-        }
-    } else if (fits) {
-        kind = kBound;
-    }
-    if (tid == 0) {
-        SampleRest &o = p.rest[row];
-        o.kind = kind;
-        o.bin = kind == kCut ? bin : -1;
-        o.by_count = r.top_k > 0;
-        o.n_list = o.done = 0;
-        o.m = x.m;
-        o.most = most;
-        o.base_cnt = base_cnt;
-        o.base_mass = base_mass;
-    }
-}
-
 // All of a row's work by one workgroup.
+template <int THREADS>
 __device__ __forceinline__ void sample_alone(const SampleParams &p, PickLds &s, int row) {
-    using Row = PickRow<kRestThreads, true>;
+    using Row = PickRow<THREADS, true>;
     constexpr int kPickThreads = Row::kPickThreads, kEach = Row::kEach;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float inf = __builtin_inff();
@@ -1012,7 +1055,7 @@ __device__ __forceinline__ void sample_alone(const SampleParams &p, PickLds &s, 
             __syncthreads();
             // (stretches are numbered up to 1023: the bins above them are empty)
             double whole;
-            const int found = x.pick<kBins>(by_count, bin < 0 && whole_row, bin < 0 && whole_row ? near_p : most,
+            const int found = x.template pick<kBins>(by_count, bin < 0 && whole_row, bin < 0 && whole_row ? near_p : most,
                                                            [&](int b) { return sample_weight(s.octave, bin < 0 ? b : bin, unit); }, base_cnt, base_mass, whole);
             count = s.cnt[found];
             if (bin < 0) {
@@ -1073,7 +1116,7 @@ __device__ __forceinline__ void sample_alone(const SampleParams &p, PickLds &s, 
             const int64_t c0 = (int64_t)s.best * x.chunk;
 #pragma unroll 1
             for (int64_t i = c0; i < c0 + x.chunk && i < x.n && left > 0.0; i += kChunk) {
-                const f32x4 v = sample_load(x.src, x.n, i + lane * 4);
+                const f32x4 v = sample_fix(sample_load(x.src, x.n, (int)i + lane * 4), x.n, (int)i + lane * 4);
                 double is[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) is[j] = sample_clean(v[j]) == l ? 1.0 : 0.0;
@@ -1116,91 +1159,154 @@ __device__ __forceinline__ void sample_alone(const SampleParams &p, PickLds &s, 
     x.draw(row, r.u, have, 0, 0);
 }
 
-__global__ __launch_bounds__(kRestThreads) void sample_rest_kernel(SampleParams p) {
+// What is read again of a row: nothing, the tokens from the bin up, those of the bin and the
+// sums above it, the sums of all that min-p keeps; or all of it, by one workgroup.
+constexpr int kNone = 0, kFew = 1, kCut = 2, kBound = 3, kAlone = 4;
+
+__global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_bytes[];
     PickLds &s = *reinterpret_cast<PickLds *>(lds_bytes);
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int row = blockIdx.x / p.rest_parts, part = blockIdx.x - row * p.rest_parts;
-    const int kind = p.rest ? p.rest[row].kind : kAlone;
-    if (kind == kNone) return;
-    if (kind == kAlone) {
-        if (part == 0) sample_alone(p, s, row);
+    using Row = PickRow<kDrawThreads, false>;
+    constexpr int kEach = Row::kEach;
+    const int tid = threadIdx.x, wave = tid >> 6;
+    const int row = blockIdx.x / p.shares, share = blockIdx.x - row * p.shares;
+    const float inf = __builtin_inff();
+    if (p.parts == 0) {
+        sample_alone<kDrawThreads>(p, s, row);
         return;
     }
-    using Row = PickRow<kRestThreads, false>;
-    constexpr int kPickThreads = Row::kPickThreads, kEach = Row::kEach;
-    SampleRest &o = p.rest[row];
     Row x(s, p, row);
     const SampleRules r(p, row);
-    const int bin = o.bin;
-    x.m = o.m;
-    x.rate = r.rate();
-    x.place_by_scan();
+    if (!r.cut && (r.greedy || r.min_p == 0.0f) && share != 0) return;
+    const SamplePart *part = p.part + (int64_t)row * p.parts;
 #pragma unroll
     for (int k = 0; k < kEach; ++k)
-        if (tid + k * kPickThreads < p.chunks) s.cmax[tid + k * kPickThreads] = p.cmax[(int64_t)row * kChunks + tid + k * kPickThreads];
+        if (tid + k * kDrawThreads < p.chunks) s.cmax[tid + k * kDrawThreads] = p.cmax[(int64_t)row * kChunks + tid + k * kDrawThreads];
+    double part_base = 0.0;
+    if (r.cut && tid < p.parts) {
+        part_base = part[tid].used ? part[tid].base : -__builtin_inf();
+        s.low[tid] = part[tid].skipped;
+    }
+    if (tid == 0) {
+        s.found_i = INT32_MAX;
+        s.n_list = 0;
+    }
     x.weights();
-    if (tid == 0) s.n_list = 0;
-    __syncthreads();
+    x.largest();
+    if (x.m == -inf || r.greedy) {
+        if (share == 0) x.simple(row, r.greedy);
+        return;
+    }
+    x.rate = r.rate();
+    // Whether the scan's places hold for this row: the largest logit within reach, nothing
+    // that was left out for being too low within the bins below it.
+    bool fits = fabs((double)x.m * x.rate) < kReach - kBins;
+    if (fits && r.cut)
+        for (int i = 0; i < p.parts; ++i)
+            if (s.low[i] > -inf && ((double)x.m - (double)s.low[i]) * x.rate < 2.0 * kBins) fits = false;
+    x.place_by_scan();
     x.min_w = (double)r.min_p * x.weight(x.m);
-    double *cmass = p.cmass + (int64_t)row * kChunks;
-    auto on = [&](int c) { return kind == kCut ? x.bin(s.cmax[c]) >= bin : x.weight(s.cmax[c]) >= x.min_w; };
-    // chunks are dealt out to the parts, so that each has its share of those that count
-    const int all = x.ask([&](int c) { return c % p.rest_parts == part && on(c); });
-    double sum = 0.0;
-    const float under = bin >= 0 ? x.under(bin) : -__builtin_inff();
-    x.each(all, [&](int i, f32x4 l) {
-        bool in[4], any = false;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) any |= l[e] >= under;
-        if (!__any(any)) return;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            double past = 0.0;
-            const int b = x.bin(l[e], past);
-            const double w = b > bin ? sample_weight(s.octave, b, sample_exp(past, 1.0, 0.0)) : 0.0;
-            sum += w >= x.min_w ? w : 0.0;
-            in[e] = b == bin && b >= 0;
+    int kind = kAlone, bin = 0;
+    double most = 0.0;
+    double have[kEach] = {};
+    if (fits && r.cut) {
+        const bool by_count = r.top_k > 0;  // (then the scan has counted only)
+        const double near_p = (double)r.top_p * (1.0 - kNear);
+        if (tid < p.parts) {
+            const double d = (x.base - part_base) / kOctave;
+            s.ahead[tid] = d < kOctaves ? (int)d : kOctaves;
         }
-        x.append(i, l, in);
-    }, [&](int c) {
-        sum = wave_sum(sum);
-        if (lane == 0) cmass[c] = sum;
-        sum = 0.0;
-    });
-    __syncthreads();
-    // the part's tokens of the bin to the row's; the last part to come here has them all
-    const int mine = s.n_list;
-    if (tid == 0) s.best = mine ? atomicAdd(&o.n_list, mine) : 0;
-    __syncthreads();
-    for (int e = tid; e < mine; e += kPickThreads) {
-        o.list_l[s.best + e] = s.list_l[e];
-        o.list_i[s.best + e] = s.list_i[e];
-    }
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) s.best = atomicAdd(&o.done, 1);
-    __syncthreads();
-    if (s.best != p.rest_parts - 1) return;
-    __threadfence();
-    double have[kEach];
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        const int c = tid * kEach + k;
-        have[k] = c < p.chunks && on(c) ? __hip_atomic_load(&cmass[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
-    }
-    if (kind == kCut) {
-        const int n = __hip_atomic_load(&o.n_list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        for (int e = tid; e < n; e += kPickThreads) {
-            s.list_l[e] = __hip_atomic_load(&o.list_l[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            s.list_i[e] = __hip_atomic_load(&o.list_i[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+        // (one wave has written what it reads)
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (wave == 0) x.pick_scanned(part, p.parts, by_count, by_count ? (double)r.top_k : near_p);
         __syncthreads();
-        x.cut_list(n, o.by_count, o.most, o.base_cnt, o.base_mass);
+        bin = s.bin;
+        most = by_count ? (double)r.top_k : near_p * s.whole;
+        if (s.base_cnt + s.bin_cnt <= kList) kind = kFew;
+        else if (s.bin_cnt <= kList && !(by_count && r.top_p < 1.0f)) kind = kCut;
+    } else if (fits && r.free()) {
+        // the scan's sums of chunks, each from its own base, unless one was out of reach
+        bool out = false;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int c = tid * kEach + k;
+            if (c >= p.chunks) continue;
+            const double cb = floor((double)s.cmax[c] * x.rate) + 1.0, at = cb - x.base + kBins;
+            if (!(at >= 0.0)) continue;
+            out |= !(fabs(cb) < kReach);
+            have[k] = sample_weight(s.octave, (int)at, p.cmass[(int64_t)row * kChunks + c]);
+        }
+        if (out) s.n_list = 1;
+        __syncthreads();
+        if (s.n_list == 0) kind = kNone;
+    } else if (fits) {
+        // (a bin below that of the least weight that min-p keeps)
+        kind = kBound;
+        bin = (int)fmax(-1.0, floor(x.place(x.m) - x.base + kBins + kOctave * log2((double)r.min_p)) - 2.0);
+    }
+    if (kind == kAlone) {
+        __syncthreads();
+        if (share == 0) sample_alone<kDrawThreads>(p, s, row);
+        return;
+    }
+    if (kind == kNone) {
+        x.draw(row, r.u, have, 0, 0);
+        return;
+    }
+    // this share's chunks of those that matter, dealt out so that each has as many
+    double *cmass = p.cmass + (int64_t)row * kChunks;
+    const double base_cnt = s.base_cnt, base_mass = s.base_mass;
+    const float above = kind == kFew ? inf : x.least(bin + 1), least = kind == kBound ? above : x.least(bin);
+    const int all = x.ask([&](int c) { return c % p.shares == share && s.cmax[c] >= least; });
+    if (kind == kFew) x.template collect<false>(all, least, above, nullptr);
+    else x.template collect<true>(all, least, above, cmass);
+    __syncthreads();
+    int n = s.n_list;
+    if (p.shares > 1) {
+        // to the row's list; the last share to come here has them all
+        SampleList &o = p.list[row];
+        if (tid == 0) s.best = n ? atomicAdd(&o.n, n) : 0;
+        __syncthreads();
+        const int at = s.best;
+        for (int e = tid; e < n && at + e < kList; e += kDrawThreads) {
+            sample_give(&o.l[at + e], s.list_l[e]);
+            sample_give(&o.i[at + e], s.list_i[e]);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) s.best = atomicAdd(&o.done, 1);
+        __syncthreads();
+        if (s.best != p.shares - 1) return;
+        n = sample_take(&o.n);
+        for (int e = tid; e < n; e += kDrawThreads) {
+            s.list_l[e] = sample_take(&o.l[e]);
+            s.list_i[e] = sample_take(&o.i[e]);
+        }
+    }
+    if (kind != kFew) {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int c = tid * kEach + k;
+            if (c < p.chunks && s.cmax[c] >= least) have[k] = sample_take(&cmass[c]);
+        }
+    }
+    __syncthreads();
+    if (kind == kFew) {
+        // all that may be kept: cut once or twice
+#pragma unroll 1
+        for (int cuts = r.top_k > 0 && r.top_p < 1.0f ? 2 : 1, k = 0; k < cuts; ++k) {
+            const double kept = x.cut_list(n, r.top_k > 0 && k == 0, most, 0.0, 0.0);
+            most = (double)r.top_p * (1.0 - kNear) * kept;
+        }
+        x.list_sums(n, have);
+    } else if (kind == kCut) {
+        x.cut_list(n, r.top_k > 0, most, base_cnt, base_mass);
         x.list_sums(n, have);
     }
-    x.draw(row, r.u, have, bin, bin + 1);
+    x.draw(row, r.u, have, kind == kFew ? 0 : bin, kind == kFew ? kBins : kind == kCut ? bin + 1 : bin);
 }
+
+static_assert(sizeof(PickLds) <= 65536, "");
 
 // How the rows are scanned: parts of them (0: not), tiles of a part.
 static void sample_split(int64_t n_vocab, int64_t n_rows, int cus, int &parts, int &tiles) {
@@ -1217,7 +1323,7 @@ static void sample_split(int64_t n_vocab, int64_t n_rows, int cus, int &parts, i
 static size_t sample_bytes(int64_t n_vocab, int64_t n_rows, int cus) {
     if (n_vocab > (int64_t)kChunks * kChunk || n_vocab == 0) return 0;
     const int64_t most = n_rows * kParts, busy = n_rows > 3 * (int64_t)cus ? n_rows : 3 * (int64_t)cus;
-    return (size_t)((most < busy ? most : busy) * sizeof(SamplePart) + n_rows * (sizeof(SampleRest) + kChunks * (sizeof(float) + sizeof(double))));
+    return (size_t)((most < busy ? most : busy) * sizeof(SamplePart) + n_rows * (sizeof(SampleList) + kChunks * (sizeof(float) + sizeof(double))));
 }
 
 }  // namespace q4k
@@ -1260,26 +1366,22 @@ int q4k_sample(const float *src, int64_t n_vocab, int64_t n_rows, int64_t nb_src
     p.tokens = tokens;
     p.logprob = logprob;
     sample_split(n_vocab, n_rows, di->cus, p.parts, p.tiles);
-    st = ensure_lds(di, reinterpret_cast<const void *>(&sample_pick_kernel), (int)sizeof(PickLds));
-    if (st == Q4K_OK) st = ensure_lds(di, reinterpret_cast<const void *>(&sample_rest_kernel), (int)sizeof(PickLds));
-    if (st != Q4K_OK) return st;
     Workspace ws;
     st = ws.begin(workspace, workspace_bytes, sample_bytes(n_vocab, n_rows, di->cus), stream);
     if (st != Q4K_OK) return st;
-    p.rest_parts = 1;
+    p.shares = 1;
     if (p.parts) {
         p.cmass = (double *)ws.ptr;
         p.part = (SamplePart *)(p.cmass + n_rows * kChunks);
-        p.rest = (SampleRest *)(p.part + n_rows * p.parts);
-        p.cmax = (float *)(p.rest + n_rows);
+        p.list = (SampleList *)(p.part + n_rows * p.parts);
+        p.cmax = (float *)(p.list + n_rows);
         st = launch(sample_scan_kernel, dim3((unsigned)(n_rows * p.parts)), kScanThreads, 0, stream, p);
-        if (st == Q4K_OK) st = launch(sample_pick_kernel, dim3((unsigned)n_rows), kPickThreads, (int)sizeof(PickLds), stream, p);
-        // parts of 32 chunks or more, four workgroups a CU at most
-        const int64_t most = 4 * (int64_t)di->cus / n_rows;
-        p.rest_parts = p.chunks < 64 ? 1 : p.chunks < 512 ? p.chunks / 32 : kParts;
-        if (p.rest_parts > most) p.rest_parts = most < 2 ? 2 : (int)most;
+        // shares of 32 chunks, four a wave, or more, at most four workgroups a CU
+        const int64_t most = 4 * (int64_t)di->cus / n_rows, want = (p.chunks + 31) / 32;
+        p.shares = (int)(want < most ? want : most < 2 ? 2 : most);
+        if (p.shares > kParts) p.shares = kParts;
     }
-    if (st == Q4K_OK) st = launch(sample_rest_kernel, dim3((unsigned)(n_rows * p.rest_parts)), kRestThreads, (int)sizeof(PickLds), stream, p);
+    if (st == Q4K_OK) st = launch(sample_draw_kernel, dim3((unsigned)(n_rows * p.shares)), kDrawThreads, (int)sizeof(PickLds), stream, p);
     return ws.end(st, stream);
 }
 
