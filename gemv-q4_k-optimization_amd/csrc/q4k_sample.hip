@@ -37,15 +37,13 @@ namespace q4k {
 
 constexpr int kDrawThreads = 512;
 constexpr int kScanThreads = 512, kScanWaves = kScanThreads / 64, kTile = kScanThreads * 8;
-constexpr int kOctave = 24, kBins = 64 * kOctave;  // what is below the last bin is never drawn
-constexpr int kChunk = 256, kChunks = 1024, kList = 1024, kParts = 16;
+constexpr int kOctave = 24, kOctaves = 64, kBins = kOctaves * kOctave;  // what is below the last bin is never drawn
+constexpr int kChunk = 256, kChunks = 1024, kList = 1024, kShort = 256, kParts = 16;
 // Rows whose a l is past this (in bins) lose bits of w and are not scanned: the pick
 // takes them by the differences from their largest logit.
 constexpr double kReach = 16384.0;
 // Sums nearer to a border than this part of it count as equal to it.
 constexpr double kNear = 0x1p-40;
-
-constexpr int kOctaves = kBins / kOctave;
 
 // What a part of a row was found to hold.
 struct SamplePart {
@@ -77,6 +75,7 @@ struct SampleParams {
     float *cmax;        // [rows][kChunks]
     double *cmass;
     SampleList *list;
+    float *pad;         // [rows][4], of rows of fewer
     q4k_sample_rules r;
     int32_t *tokens;
     float *logprob;
@@ -146,20 +145,51 @@ __device__ __forceinline__ float wave_max(float x) {
     return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
-// Four logits of a row of n from token i, read from where the row has four (no branch
-// between loads, so that all of a thread's are on their way together); sample_fix moves
-// them to their places, past the row -inf.
-__device__ __forceinline__ f32x4 sample_load(const float *src, int n, int i) {
-    if (n < 4) {
-        f32x4 x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = j < n ? src[j] : -__builtin_inff();
-        return x;
-    }
-    return load4<false>(src + (i < n - 4 ? i : n - 4));
+// Two values' largest, four values' sums: halves and quarters of the wave take one each, the
+// last lane of which ends up with its result.
+typedef uint32_t lane_pair __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float wave_max2(float x, float y) {  // lanes 31 and 63
+    const lane_pair h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    x = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    x = dpp_max<0x111, 0xf>(x);
+    x = dpp_max<0x112, 0xf>(x);
+    x = dpp_max<0x114, 0xf>(x);
+    x = dpp_max<0x118, 0xf>(x);
+    return dpp_max<0x142, 0xa>(x);
 }
+template <bool ROWS>
+__device__ __forceinline__ double half_sums(double x, double y) {
+    const unsigned long long a = __double_as_longlong(x), b = __double_as_longlong(y);
+    lane_pair lo, hi;
+    if (ROWS) {
+        lo = __builtin_amdgcn_permlane16_swap((uint32_t)a, (uint32_t)b, false, false);
+        hi = __builtin_amdgcn_permlane16_swap((uint32_t)(a >> 32), (uint32_t)(b >> 32), false, false);
+    } else {
+        lo = __builtin_amdgcn_permlane32_swap((uint32_t)a, (uint32_t)b, false, false);
+        hi = __builtin_amdgcn_permlane32_swap((uint32_t)(a >> 32), (uint32_t)(b >> 32), false, false);
+    }
+    return __longlong_as_double(((unsigned long long)hi[0] << 32) | lo[0]) + __longlong_as_double(((unsigned long long)hi[1] << 32) | lo[1]);
+}
+__device__ __forceinline__ double row_sums(double x) {
+    x += dpp64<0x111, 0xf>(x);
+    x += dpp64<0x112, 0xf>(x);
+    x += dpp64<0x114, 0xf>(x);
+    return x + dpp64<0x118, 0xf>(x);
+}
+__device__ __forceinline__ double wave_sum2(double x, double y) {  // lanes 31 and 63
+    x = row_sums(half_sums<false>(x, y));
+    return x + dpp64<0x142, 0xa>(x);
+}
+__device__ __forceinline__ double wave_sum4(double a, double b, double c, double d) {  // lanes 15, 47, 31 and 63
+    return row_sums(half_sums<true>(half_sums<false>(a, b), half_sums<false>(c, d)));
+}
+
+// Four logits of a row of n (4 or more) from token i, read from where the row has four (no
+// branch between loads, so that all of a thread's are on their way together); sample_fix moves
+// them to their places, past the row -inf.
+__device__ __forceinline__ f32x4 sample_load(const float *src, int n, int i) { return load4<false>(src + (i < n - 4 ? i : n - 4)); }
 __device__ __forceinline__ f32x4 sample_fix(f32x4 x, int n, int i) {
-    const int by = n < 4 ? i : i - (n - 4);
+    const int by = i - (n - 4);
     if (by <= 0) return x;
     f32x4 y;
 #pragma unroll
@@ -173,22 +203,32 @@ __device__ __forceinline__ f32x4 sample_fix(f32x4 x, int n, int i) {
 // (zeros are equal whatever their sign)
 __device__ __forceinline__ float sample_clean(float l) { return l != l ? -__builtin_inff() : l + 0.0f; }
 
-// scale * 2^(x / 24) + plus for 0 <= x < 1: the exponential's series (the next term is
-// 2^-48 of it).
+// The whole number nearest to t (within 2^31 of 0), and what t is past it: 1.5 * 2^52 more
+// leaves it in the last bits, two additions where floor and a conversion take 20 cycles.
+__device__ __forceinline__ int sample_place(double t, double &past) {
+    const double r = t + 0x1.8p52;
+    past = t - (r - 0x1.8p52);
+    return (int)(uint32_t)__double_as_longlong(r);
+}
+// scale * 2^(x / 24) + plus for |x| <= 1/2: the exponential's series (the next term is
+// 2^-46 of it).
 __device__ __forceinline__ double sample_exp(double x, double scale, double plus) {
     constexpr double k = 0.6931471805599453094 / kOctave;
-    double e = k * k * k * k * k * k / 720.0;
-    e = __builtin_fma(e, x, k * k * k * k * k / 120.0);
+    double e = k * k * k * k * k / 120.0;
     e = __builtin_fma(e, x, k * k * k * k / 24.0);
     e = __builtin_fma(e, x, k * k * k / 6.0);
     e = __builtin_fma(e, x, k * k / 2.0);
     e = __builtin_fma(e, x, k);
     return __builtin_fma(e * x, scale, scale + plus);
 }
-// 2^((b - kBins) / 24) times e, from the 24 powers of an octave.
+// 2^((b - kBins) / 24) times e near 1 (or any sum), from the 24 powers of an octave.
 __device__ __forceinline__ double sample_weight(const double *octave, int b, double e) {
-    const int q = b * 2731 >> 16;  // b / 24, below 8192
-    return ldexp(octave[b - q * kOctave] * e, q - kBins / kOctave);
+    const int q = b * 2731 >> 16;  // b / 24, rounded down, from -1 to 8192
+    return __longlong_as_double(__double_as_longlong(octave[b - q * kOctave] * e) + ((long long)(q - kOctaves) << 52));
+}
+__device__ __forceinline__ double sample_weight_sum(const double *octave, int b, double sum) {
+    const int q = b * 2731 >> 16;
+    return ldexp(octave[b - q * kOctave] * sum, q - kOctaves);
 }
 // as an integer of bits and one more, scale 2^bits: 2^52 more leaves it in the last bits
 __device__ __forceinline__ unsigned long long sample_mass(double x, double scale) {
@@ -236,23 +276,32 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
             l[1] = sample_fix(l[1], p.n_vocab, (int)t0 + at + kChunk);
         }
         float top[2];
+        double sum[2] = {};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            top[k] = wave_max(fmaxf(fmaxf(l[k][0], l[k][1]), fmaxf(l[k][2], l[k][3])));  // (NaN passed over)
-            const int64_t c = (t0 + at - lane * 4) / kChunk + k;
-            if (lane == 0 && c < p.chunks) cmax[c] = sample_clean(top[k]);
-            if (!free) continue;
-            const double cb = floor((double)top[k] * rate) + 1.0;
-            double sum = 0.0;
-            if (fabs(cb) < kReach) {
+        for (int k = 0; k < 2; ++k) top[k] = fmaxf(fmaxf(l[k][0], l[k][1]), fmaxf(l[k][2], l[k][3]));  // (NaN passed over)
+        const float both = wave_max2(top[0], top[1]);
+        top[0] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(both), 31));
+        top[1] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(both), 63));
+        // lanes 31 and 63 write the first and the second chunk's
+        const int c = (int)(t0 + at - lane * 4) / kChunk + (lane >> 5);
+        const bool writes = (lane & 31) == 31 && c < p.chunks;
+        if (writes) cmax[c] = sample_clean(both);
+        if (free) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const double cb = __builtin_rint((double)top[k] * rate) + 1.0;
+                if (!(fabs(cb) < kReach)) continue;
+                const int low = (int)cb - kBins;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const double t = (double)l[k][j] * rate, f = floor(t), i = f - cb + kBins;
-                    if (i >= 0.0) sum += sample_weight(octave, (int)i, sample_exp(t - f, 1.0, 0.0));
+                    double past;
+                    const int i = sample_place(fmax((double)l[k][j] * rate, cb - (kBins + 1)), past) - low;
+                    const double w = sample_weight(octave, i, sample_exp(past, 1.0, 0.0));
+                    sum[k] += i >= 0 ? w : 0.0;
                 }
-                sum = wave_sum(sum);
             }
-            if (lane == 0 && c < p.chunks) cmass[c] = sum;
+            const double sums = wave_sum2(sum[0], sum[1]);
+            if (writes) cmass[c] = sums;
         }
         if (!cut) continue;
         if (lane == 0) tops[par][wave] = fmaxf(top[0], top[1]);
@@ -266,7 +315,7 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
             continue;
         }
         if (place > kReach) continue;  // (the row's largest logit tells)
-        const double up = (floor(place / kOctave) + 1.0) * kOctave;
+        const double up = (floor(__builtin_rint(place) / kOctave) + 1.0) * kOctave;
         if (!used || up > base) {
             // bins that enter at the top, where the lowest ones were
             const int by = !used || up - base >= kBins ? kBins : (int)(up - base);
@@ -280,15 +329,17 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
             used = true;
             __syncthreads();
         }
+        const int low = (int)base - kBins;
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const double t = (double)l[k][j] * rate, f = floor(t), i = f - base + kBins;
-                if (i >= 0.0) {
-                    int b = (int)i + off;
+                double past;
+                int b = sample_place(fmax((double)l[k][j] * rate, base - (kBins + 1)), past) - low;
+                if (b >= 0) {
+                    b += off;
                     b = b >= kBins ? b - kBins : b;
-                    if (by_mass) atomicAdd(&mass[b], sample_mass(t - f, scale));
+                    if (by_mass) atomicAdd(&mass[b], sample_mass(past, scale));
                     atomicAdd(&cnt[b], 1u);
                 }
             }
@@ -395,13 +446,11 @@ struct PickRow {
           last_i(INT32_MAX) {}
 
     __device__ __forceinline__ double place(float l) const { return ALONE ? flat ? 0.0 : ((double)l - (double)m) * rate : (double)l * rate; }
-    // the bin (below 0: none), and what is past its lower end
+    // the bin (below 0: none), and what is past its middle
     __device__ __forceinline__ int bin(float l, double &past) const {
-        const double t = place(l), f = floor(t), i = f - base + kBins;
-        past = t - f;
         // (-inf: no place is, or at a rate of 0 none is a number)
-        const bool is = i >= 0.0 && (!ALONE || !flat || l == m);
-        return is ? (int)i : -1;
+        const int i = sample_place(fmax(place(l), base - (kBins + 1)), past) - ((int)base - kBins);
+        return !ALONE || !flat || l == m ? i : -1;
     }
     __device__ __forceinline__ int bin(float l) const {
         double past;
@@ -414,7 +463,7 @@ struct PickRow {
     }
     __device__ __forceinline__ bool left_in(float l, int i) const { return !sample_before(last_l, last_i, l, i); }
     // the base of places for a largest logit within the scan's reach
-    __device__ __forceinline__ void place_by_scan() { base = (floor((double)m * rate / kOctave) + 1.0) * kOctave; }
+    __device__ __forceinline__ void place_by_scan() { base = (floor(__builtin_rint((double)m * rate) / kOctave) + 1.0) * kOctave; }
     __device__ __forceinline__ void weights() const {
         if (threadIdx.x < kOctave) s.octave[threadIdx.x] = exp2(threadIdx.x * (1.0 / kOctave));
     }
@@ -589,7 +638,7 @@ struct PickRow {
     __device__ __forceinline__ void collect(int count, float least, float above, double *sums) const {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const int mine = count > wave ? (count - wave - 1) / kPickWaves + 1 : 0;
-        constexpr int SET = 4;
+        constexpr int SET = 4;  // (wave_sum4's)
         struct Set {
             f32x4 v[SET];
             int c[SET];
@@ -619,19 +668,16 @@ struct PickRow {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float l = q.v[j][e];
-                            const double t = place(l), f = floor(t);
-                            int at = (int)(f - base + kBins);
-                            at = at < 0 ? 0 : at > kBins - 1 ? kBins - 1 : at;
-                            const double w = sample_weight(s.octave, at, sample_exp(t - f, 1.0, 0.0));
+                            double past;
+                            const int at = bin(l, past);
+                            const double w = sample_weight(s.octave, at, sample_exp(past, 1.0, 0.0));
                             sum[j] += l >= above && w >= min_w ? w : 0.0;
                         }
                     }
-#pragma unroll
-                    for (int j = 0; j < SET; ++j) sum[j] = wave_sum(sum[j]);
+                    sum[0] = wave_sum4(sum[0], sum[1], sum[2], sum[3]);
                 }
-#pragma unroll
-                for (int j = 0; j < SET; ++j)
-                    if (lane == 0) sample_give(&sums[q.c[j]], sum[j]);  // (past the last one: that again)
+                // (past the last one: that again)
+                if ((lane & 15) == 15) sample_give(&sums[lane < 32 ? lane < 16 ? q.c[0] : q.c[2] : lane < 48 ? q.c[1] : q.c[3]], sum[0]);
             }
             unsigned long long in[SET][4];
             int all = 0;
@@ -704,7 +750,7 @@ struct PickRow {
                 if (is && !by_count) sum += level == 0 ? m0[i] : (double)m1[i];
             }
             if (level == 0) sum = ldexp(sum * unit, -1 - lane);
-            else if (lane < kOctave) sum = sample_weight(s.octave, octave * kOctave + kOctave - 1 - lane, sum * unit);
+            else if (lane < kOctave) sum = sample_weight_sum(s.octave, octave * kOctave + kOctave - 1 - lane, sum * unit);
             const double ic = wave_scan(cnt), im = wave_scan(sum);
             const double bc = base_cnt + (ic - cnt), bm = base_mass + (im - sum);
             if (level == 0) {
@@ -732,7 +778,7 @@ struct PickRow {
     __device__ __forceinline__ float least(int bin_) const {
         if (bin_ >= kBins) return __builtin_inff();
         constexpr float most = 3.4028235e38f;
-        float l = (float)((base - kBins + bin_) / rate);
+        float l = (float)((base - kBins + bin_ - 0.5) / rate);
         l = l != l ? -most : fminf(fmaxf(l, -most), most);
         for (int k = 0; k < 16 && l < most && bin(l) < bin_; ++k) l = sample_next(l, 1);
         for (int k = 0; k < 16 && l > -most && bin(sample_next(l, -1)) >= bin_; ++k) l = sample_next(l, -1);
@@ -783,11 +829,64 @@ struct PickRow {
         return BINS - 1 - found;
     }
 
+    // Of tokens in order, their weights in cmass (0 behind the last), their places in cnt: the last
+    // one that is kept.  Returns the sum of w up to it.
+    __device__ __forceinline__ double cut_sorted(int count, const float *list_l, const int *list_i, bool by_count, double most, double base_cnt,
+                                                 double base_mass) {
+        const int tid = threadIdx.x;
+        double w[kEach], mine = 0.0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            w[k] = tid * kEach + k < count ? s.cmass[tid * kEach + k] : 0.0;
+            mine += w[k];
+        }
+        double all, at_mass = base_mass + scan(mine, all);
+        int best = tid == 0 ? 0 : -1;  // (the first one always)
+        double upto = base_mass + s.cmass[0];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int e = tid * kEach + k;
+            if (w[k] > 0.0 && (by_count ? base_cnt + e : at_mass) < most) {
+                best = e;
+                upto = at_mass + w[k];
+            }
+            at_mass += w[k];
+        }
+        const int found = last_best(best);
+        if (best >= 0 && best == found) s.base_mass = upto;
+        const int at = s.cnt[found];
+        last_l = list_l[at];
+        last_i = list_i[at];
+        __syncthreads();
+        return s.base_mass;
+    }
+
     // Of the list's n tokens those that are left in, before which lie base_cnt and
     // base_mass: the last one that is kept becomes last_l, last_i.  Returns the sum of w
     // up to it.
     __device__ __forceinline__ double cut_list(int n, bool by_count, double most, double base_cnt, double base_mass) {
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+        const int tid = threadIdx.x;
+        double some;
+        if (n <= kShort) {
+            // every token's rank (those that are left in have keys above 0)
+            if (tid < kShort) {
+                const bool is = tid < n && left_in(s.list_l[tid], s.list_i[tid]);
+                s.mass[tid] = is ? (unsigned long long)sample_key(s.list_l[tid]) << 32 | (uint32_t)~s.list_i[tid] : 0;
+                s.cmass[tid] = 0.0;
+            }
+            __syncthreads();
+            if (tid < n && s.mass[tid]) {
+                const unsigned long long key = s.mass[tid];
+                int rank = 0;
+#pragma unroll 8
+                for (int j = 0; j < n; ++j) rank += s.mass[j] > key;
+                s.cnt[rank] = tid;
+                s.cmass[rank] = weight(s.list_l[tid]);
+            }
+            __syncthreads();
+            return cut_sorted(kShort, s.list_l, s.list_i, by_count, most, base_cnt, base_mass);
+        }
+        const int lane = tid & 63, wave = tid >> 6;
         const float inf = __builtin_inff();
         // 1024 stretches of the logits' bits between the least and the largest
         float top = -inf, low = -inf;
@@ -820,7 +919,6 @@ struct PickRow {
             atomicAdd(&s.cnt[b], 1u);
         }
         __syncthreads();
-        double some;
         const int sub = pick<1024>(by_count, false, most, [](int) { return kStep; }, base_cnt, base_mass, some);
         // the tokens of that stretch in order, where the list's kept ones are looked up again
         const int count = s.cnt[sub];
@@ -845,31 +943,7 @@ struct PickRow {
             s.cmass[rank] = weight(l);
         }
         __syncthreads();
-        double w[kEach], mine = 0.0;
-#pragma unroll
-        for (int k = 0; k < kEach; ++k) {
-            w[k] = tid * kEach + k < count ? s.cmass[tid * kEach + k] : 0.0;
-            mine += w[k];
-        }
-        double at_mass = base_mass + scan(mine, some);
-        int best = tid == 0 ? 0 : -1;  // (the first one always)
-        double upto = base_mass + s.cmass[0];
-#pragma unroll
-        for (int k = 0; k < kEach; ++k) {
-            const int e = tid * kEach + k;
-            if (e < count && (by_count ? base_cnt + e : at_mass) < most) {
-                best = e;
-                upto = at_mass + w[k];
-            }
-            at_mass += w[k];
-        }
-        const int found = last_best(best);
-        if (best >= 0 && best == found) s.base_mass = upto;
-        const int at = s.cnt[found];
-        last_l = s.sort_l[at];
-        last_i = s.sort_i[at];
-        __syncthreads();
-        return s.base_mass;
+        return cut_sorted(count, s.sort_l, s.sort_i, by_count, most, base_cnt, base_mass);
     }
 
     // The kept sums of the list's n tokens by chunks, to `have` of chunks tid * kEach ..
@@ -1231,10 +1305,10 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleParams 
         for (int k = 0; k < kEach; ++k) {
             const int c = tid * kEach + k;
             if (c >= p.chunks) continue;
-            const double cb = floor((double)s.cmax[c] * x.rate) + 1.0, at = cb - x.base + kBins;
+            const double cb = __builtin_rint((double)s.cmax[c] * x.rate) + 1.0, at = cb - x.base + kBins;
             if (!(at >= 0.0)) continue;
             out |= !(fabs(cb) < kReach);
-            have[k] = sample_weight(s.octave, (int)at, p.cmass[(int64_t)row * kChunks + c]);
+            have[k] = sample_weight_sum(s.octave, (int)at, p.cmass[(int64_t)row * kChunks + c]);
         }
         if (out) s.n_list = 1;
         __syncthreads();
@@ -1249,61 +1323,68 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleParams 
         if (share == 0) sample_alone<kDrawThreads>(p, s, row);
         return;
     }
-    if (kind == kNone) {
-        x.draw(row, r.u, have, 0, 0);
-        return;
-    }
-    // this share's chunks of those that matter, dealt out so that each has as many
-    double *cmass = p.cmass + (int64_t)row * kChunks;
-    const double base_cnt = s.base_cnt, base_mass = s.base_mass;
-    const float above = kind == kFew ? inf : x.least(bin + 1), least = kind == kBound ? above : x.least(bin);
-    const int all = x.ask([&](int c) { return c % p.shares == share && s.cmax[c] >= least; });
-    if (kind == kFew) x.template collect<false>(all, least, above, nullptr);
-    else x.template collect<true>(all, least, above, cmass);
-    __syncthreads();
-    int n = s.n_list;
-    if (p.shares > 1) {
-        // to the row's list; the last share to come here has them all
-        SampleList &o = p.list[row];
-        if (tid == 0) s.best = n ? atomicAdd(&o.n, n) : 0;
+    int steps = 0, steps_end = 0;
+    if (kind != kNone) {
+        // this share's chunks of those that matter, dealt out so that each has as many
+        double *cmass = p.cmass + (int64_t)row * kChunks;
+        const double base_cnt = s.base_cnt, base_mass = s.base_mass;
+        const float above = kind == kFew ? inf : x.least(bin + 1), least = kind == kBound ? above : x.least(bin);
+        const int all = x.ask([&](int c) { return c % p.shares == share && s.cmax[c] >= least; });
+        if (kind == kFew) x.template collect<false>(all, least, above, nullptr);
+        else x.template collect<true>(all, least, above, cmass);
         __syncthreads();
-        const int at = s.best;
-        for (int e = tid; e < n && at + e < kList; e += kDrawThreads) {
-            sample_give(&o.l[at + e], s.list_l[e]);
-            sample_give(&o.i[at + e], s.list_i[e]);
+        int n = s.n_list;
+        if (p.shares > 1) {
+            // to the row's list; the last share to come here has them all
+            SampleList &o = p.list[row];
+            if (tid == 0) s.best = n ? atomicAdd(&o.n, n) : 0;
+            __syncthreads();
+            const int at = s.best;
+            for (int e = tid; e < n && at + e < kList; e += kDrawThreads) {
+                sample_give(&o.l[at + e], s.list_l[e]);
+                sample_give(&o.i[at + e], s.list_i[e]);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (tid == 0) s.best = atomicAdd(&o.done, 1);
+            __syncthreads();
+            if (s.best != p.shares - 1) return;
+            n = sample_take(&o.n);
+            for (int e = tid; e < n; e += kDrawThreads) {
+                s.list_l[e] = sample_take(&o.l[e]);
+                s.list_i[e] = sample_take(&o.i[e]);
+            }
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (tid == 0) s.best = atomicAdd(&o.done, 1);
-        __syncthreads();
-        if (s.best != p.shares - 1) return;
-        n = sample_take(&o.n);
-        for (int e = tid; e < n; e += kDrawThreads) {
-            s.list_l[e] = sample_take(&o.l[e]);
-            s.list_i[e] = sample_take(&o.i[e]);
-        }
-    }
-    if (kind != kFew) {
+        if (kind != kFew) {
 #pragma unroll
-        for (int k = 0; k < kEach; ++k) {
-            const int c = tid * kEach + k;
-            if (c < p.chunks && s.cmax[c] >= least) have[k] = sample_take(&cmass[c]);
+            for (int k = 0; k < kEach; ++k) {
+                const int c = tid * kEach + k;
+                if (c < p.chunks && s.cmax[c] >= least) have[k] = sample_take(&cmass[c]);
+            }
         }
-    }
-    __syncthreads();
-    if (kind == kFew) {
-        // all that may be kept: cut once or twice
+        __syncthreads();
+        if (kind != kBound) {
+            // cut once or, where all that may be kept is in the list, twice
+            const bool few = kind == kFew;
 #pragma unroll 1
-        for (int cuts = r.top_k > 0 && r.top_p < 1.0f ? 2 : 1, k = 0; k < cuts; ++k) {
-            const double kept = x.cut_list(n, r.top_k > 0 && k == 0, most, 0.0, 0.0);
-            most = (double)r.top_p * (1.0 - kNear) * kept;
+            for (int cuts = few && r.top_k > 0 && r.top_p < 1.0f ? 2 : 1, k = 0; k < cuts; ++k) {
+                const double kept = x.cut_list(n, r.top_k > 0 && k == 0, most, few ? 0.0 : base_cnt, few ? 0.0 : base_mass);
+                most = (double)r.top_p * (1.0 - kNear) * kept;
+            }
+            x.list_sums(n, have);
+            steps = few ? 0 : bin;
+            steps_end = few ? kBins : bin + 1;
         }
-        x.list_sums(n, have);
-    } else if (kind == kCut) {
-        x.cut_list(n, r.top_k > 0, most, base_cnt, base_mass);
-        x.list_sums(n, have);
     }
-    x.draw(row, r.u, have, kind == kFew ? 0 : bin, kind == kFew ? kBins : kind == kCut ? bin + 1 : bin);
+    x.draw(row, r.u, have, steps, steps_end);
+}
+
+// Rows of fewer than four logits, with -inf behind them, which are no candidates.
+__global__ void sample_pad_kernel(SampleParams p) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= (int64_t)p.n_rows * 4) return;
+    const int c = (int)(i & 3);
+    p.pad[i] = c < p.n_vocab ? reinterpret_cast<const float *>(p.src + (i >> 2) * p.nb_src)[c] : -__builtin_inff();
 }
 
 static_assert(sizeof(PickLds) <= 65536, "");
@@ -1323,7 +1404,7 @@ static void sample_split(int64_t n_vocab, int64_t n_rows, int cus, int &parts, i
 static size_t sample_bytes(int64_t n_vocab, int64_t n_rows, int cus) {
     if (n_vocab > (int64_t)kChunks * kChunk || n_vocab == 0) return 0;
     const int64_t most = n_rows * kParts, busy = n_rows > 3 * (int64_t)cus ? n_rows : 3 * (int64_t)cus;
-    return (size_t)((most < busy ? most : busy) * sizeof(SamplePart) + n_rows * (sizeof(SampleList) + kChunks * (sizeof(float) + sizeof(double))));
+    return (n_vocab < 4 ? n_rows * 16 : 0) + (size_t)((most < busy ? most : busy) * sizeof(SamplePart) + n_rows * (sizeof(SampleList) + kChunks * (sizeof(float) + sizeof(double))));
 }
 
 }  // namespace q4k
@@ -1375,9 +1456,16 @@ int q4k_sample(const float *src, int64_t n_vocab, int64_t n_rows, int64_t nb_src
         p.part = (SamplePart *)(p.cmass + n_rows * kChunks);
         p.list = (SampleList *)(p.part + n_rows * p.parts);
         p.cmax = (float *)(p.list + n_rows);
-        st = launch(sample_scan_kernel, dim3((unsigned)(n_rows * p.parts)), kScanThreads, 0, stream, p);
-        // shares of 32 chunks, four a wave, or more, at most four workgroups a CU
-        const int64_t most = 4 * (int64_t)di->cus / n_rows, want = (p.chunks + 31) / 32;
+        if (n_vocab < 4) {
+            p.pad = p.cmax + n_rows * kChunks;
+            st = launch(sample_pad_kernel, dim3((unsigned)((n_rows * 4 + 255) / 256)), 256, 0, stream, p);
+            p.src = reinterpret_cast<const char *>(p.pad);
+            p.nb_src = 16;
+            p.n_vocab = 4;
+        }
+        if (st == Q4K_OK) st = launch(sample_scan_kernel, dim3((unsigned)(n_rows * p.parts)), kScanThreads, 0, stream, p);
+        // shares of 32 chunks, four a wave, or more, at most two workgroups a CU
+        const int64_t most = 2 * (int64_t)di->cus / n_rows, want = (p.chunks + 31) / 32;
         p.shares = (int)(want < most ? want : most < 2 ? 2 : most);
         if (p.shares > kParts) p.shares = kParts;
     }
