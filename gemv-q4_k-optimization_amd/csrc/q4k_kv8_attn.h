@@ -29,9 +29,18 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 struct Kv8AttnParams {
-    AttnParams a;  // rows, splits and partial results; `suf` parts only, no AttnCache
+    AttnParams a;  // rows and partial results; `suf` parts only, no AttnCache
     Kv8Cache c;
+    // Where the positions are dealt out: workgroups that share them (else 0), the number of steps
+    // before each request's and, last, of all, for the join.  (a.join stays 0: attn_emit writes dst.)
+    int shares;
+    int64_t *starts;
 };
+
+// Positions of a step of four waves; the least steps a workgroup takes (12 x 5 F16 tokens over 3001
+// positions: 1 step @@, 2 @@, 4 @@ us).
+constexpr int kKv8Step = 128, kKv8Least = 2;
+constexpr int kKv8Deal = (257 + 4 + 1) * 8;  // bytes of LDS
 
 // References move by more than 2^kKv8Lazy only; P is at most 2^kKv8Lazy.  (BF16 terms have
 // F32's range, so nothing is lost below.)
@@ -70,6 +79,7 @@ struct Kv8Cfg {
     // after that: (M, l) of four waves' rows and the rows' factors; places of 32 positions of four waves
     static constexpr int PLACES = BLOCK8 ? 0 : 4 * 32 * (16 + 8);
     static constexpr int MORE = 1024 + PLACES;
+    static constexpr int WGS = D == 256 ? 1 : D == 128 && RT == 2 ? 2 : 3;  // workgroups a CU
 };
 
 // Eight bytes as the operand of the score product.
@@ -242,7 +252,9 @@ __device__ __forceinline__ void kv8_attn_item(const Kv8AttnParams &kp, const Att
     constexpr int KJ = D / 64, VB = D / 16, VW = VB / 4;  // 16-byte pieces of a K row, bytes and dwords of a V piece
     const AttnParams &p = kp.a;
     const Kv8Cache &kv = kp.c;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // (what follows from it is worked out for each item: kept from one to the next it spills)
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
     const int row0 = tile * C::ROWS;
     const int least = attn_least<C::ROWS>(p, s, tile);
@@ -342,6 +354,7 @@ __device__ __forceinline__ void kv8_attn_item(const Kv8AttnParams &kp, const Att
         load_v();
         get_pages(t0 + 128);
     }
+    __syncthreads();  // (LDS may still be read for the item before)
     // the queries, one row tile per wave, while the first positions are on their way
     AttnRows<RT, D> w;
     attn_rows<RT, D>(p, s, row0, w);
@@ -524,45 +537,216 @@ __device__ __forceinline__ void kv8_attn_item(const Kv8AttnParams &kp, const Att
                 ls += e.y * f;
                 acc += *reinterpret_cast<const f32x4 *>(ol + (v * 16 + r) * D + ((d4 ^ r) * 4)) * f;
             }
-            attn_emit<QT>(p, s, hk, row0 + rt * 16 + r, d4 * 4, acc, M, ls);
+            if (s.slot < 0) {
+                attn_emit<QT>(p, s, hk, row0 + rt * 16 + r, d4 * 4, acc, M, ls);
+            } else if (row0 + rt * 16 + r < s.rows && d4 * 4 < p.head_dim) {
+                const int64_t at = (int64_t)s.slot * C::ROWS + rt * 16 + r;
+                if (d4 == 0) p.part_ml[at] = make_float2(M, ls);
+                *reinterpret_cast<f32x4 *>(p.part_o + at * p.head_dim + d4 * 4) = acc;
+            }
         }
     }
 }
 
+// What request r takes: its rows, tiles of them and steps.
+struct Kv8Request {
+    int t0, rows, tiles, len, steps;
+    __device__ __forceinline__ Kv8Request(const AttnParams &p, int r, int tile_rows) {
+        int t1;
+        attn_tokens(p, r, t0, t1);
+        rows = (t1 - t0) * p.group;
+        tiles = (rows + tile_rows - 1) / tile_rows;
+        len = attn_suffix(p, r);
+        steps = (len + kKv8Step - 1) / kKv8Step;
+    }
+    __device__ __forceinline__ long long all(const AttnParams &p) const { return (long long)steps * tiles * p.n_head_kv; }
+};
+__device__ __forceinline__ long long kv8_uniform(long long x) {
+    const unsigned lo = __builtin_amdgcn_readfirstlane((int)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
+    return (long long)((unsigned long long)hi << 32 | lo);
+}
+// steps of a share, of all steps
+__device__ __forceinline__ long long kv8_share(const Kv8AttnParams &kp, long long all) {
+    const long long x = (all + kp.shares - 1) / kp.shares;
+    return x < kKv8Least ? kKv8Least : x;
+}
+__device__ __forceinline__ long long kv8_wave_scan(long long x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const long long y = __shfl_up(x, d);
+        x += lane >= d ? y : 0;
+    }
+    return x;
+}
+
+// Short caches: a workgroup for each tile of rows.  Longer ones: all steps of all requests, KV heads
+// and tiles, in that order, are dealt out evenly to as many workgroups as the card holds at
+// once, whatever the requests' lengths; a tile that more than one of them works on is joined by a
+// kernel of its own.  (64 requests of 512 to 8192 positions: 232 us with splits of one length for all,
+// two a request; 183 with eight; @@ dealt out.)
 template <class C>
-__global__ __launch_bounds__(256, C::D == 256 ? 1 : 2) void kv8_attn_kernel(Kv8AttnParams kp) {
+__global__ __launch_bounds__(256, C::WGS) void kv8_attn_kernel(Kv8AttnParams kp) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnParams &p = kp.a;
-    const int item = xcd_item(blockIdx.x, p.suf_items);
-    const int tile = item % p.suf_tiles;
-    int x = item / p.suf_tiles;
-    const int hk = x % p.n_head_kv;
-    x /= p.n_head_kv;
-    const int r = x % p.n_requests, sp = x / p.n_requests;
-    int t0, t1;
-    attn_tokens(p, r, t0, t1);
-    const int len = attn_suffix(p, r);
-    AttnSpan s;
-    s.beg = sp * p.suf_len;
-    // (the first split of a request that sees nothing writes its empty rows when nothing else would)
-    if (s.beg >= len && (p.join || sp > 0)) return;
-    s.end = s.beg + p.suf_len < len ? s.beg + p.suf_len : len;
-    s.rows = (t1 - t0) * p.group;
-    s.tok0 = t0;
-    s.causal = len - (t1 - t0);
-    s.table_row = r;
-    s.slot = sp;
-    if (tile * C::ROWS >= s.rows) return;
-    kv8_attn_item<C>(kp, s, hk, tile, lds);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // where 256 requests begin and the last one ends, in steps; sums of the waves'; the request in turn
+    long long *begins = reinterpret_cast<long long *>(lds + C::LDS + C::MORE), *sums = begins + 257;
+    int &found = *reinterpret_cast<int *>(sums + 4);
+    // requests r0 .. r0 + 255, whose steps begin at `from`: returns where they end
+    auto number = [&](int r0, long long from) {
+        const long long own = r0 + tid < p.n_requests ? Kv8Request(p, r0 + tid, C::ROWS).all(p) : 0;
+        const long long inc = kv8_wave_scan(own);
+        __syncthreads();
+        if (lane == 63) sums[wave] = inc;
+        __syncthreads();
+        long long all = from;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i == wave) begins[tid] = all + inc - own;
+            all += sums[i];
+        }
+        if (tid == 0) begins[256] = all;
+        __syncthreads();
+        return kv8_uniform(all);
+    };
+    const int share = kp.shares ? xcd_item(blockIdx.x, kp.shares) : 0;
+    long long at = 0, last = 0;
+    int r0 = 0;
+    if (kp.shares) {
+        long long total = 0;
+        for (; r0 < p.n_requests; r0 += 256) {
+            const long long from = total;
+            total = number(r0, from);
+            if (share == 0 && r0 + tid < p.n_requests) kp.starts[r0 + tid] = begins[tid];
+        }
+        if (share == 0 && tid == 0) kp.starts[p.n_requests] = total;
+        const long long each = kv8_share(kp, total);
+        at = share * each;
+        last = at + each < total ? at + each : total;
+        if (at >= last) return;
+        // (the last 256 requests' numbers are there; the first ones again where there are more)
+        r0 -= 256;
+        if (r0 > 0) {
+            r0 = 0;
+            number(0, 0);
+        }
+    }
+    const long long first = at;
+    do {
+        int r, hk, tile, step = 0, n;
+        if (kp.shares) {
+            while (at >= kv8_uniform(begins[256])) {
+                r0 += 256;
+                number(r0, kv8_uniform(begins[256]));
+            }
+            if (begins[tid] <= at && at < begins[tid + 1]) found = tid;
+            __syncthreads();
+            const int in = __builtin_amdgcn_readfirstlane(found);
+            r = r0 + in;
+            const Kv8Request q(p, r, C::ROWS);
+            const int past = (int)(at - kv8_uniform(begins[in]));  // (a request's steps are below 2^31)
+            const int which = past / q.steps;
+            step = past - which * q.steps;
+            hk = which / q.tiles;
+            tile = which - hk * q.tiles;
+            n = last - at < q.steps - step ? (int)(last - at) : q.steps - step;
+        } else {
+            const int item = xcd_item(blockIdx.x, p.suf_items), x = item / p.suf_tiles;
+            tile = item - x * p.suf_tiles;
+            r = x / p.n_head_kv;
+            hk = x - r * p.n_head_kv;
+            n = kKv8Least;
+        }
+        const Kv8Request q(p, r, C::ROWS);
+        AttnSpan s;
+        s.beg = step * kKv8Step;
+        s.end = n < q.steps - step ? s.beg + n * kKv8Step : q.len;
+        s.rows = q.rows;
+        s.tok0 = q.t0;
+        s.causal = q.len - q.rows / p.group;
+        s.table_row = r;
+        s.slot = !kp.shares || n == q.steps ? -1 : 2 * share + (at > first);
+        if (tile < q.tiles) kv8_attn_item<C>(kp, s, hk, tile, lds);
+        at += n;
+    } while (at < last);
+}
+
+// Joins the parts of the tiles that several workgroups had: join_groups threads for each four
+// dimensions of a row.
+template <class QT, int TILE_ROWS>
+__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnParams kp) {
+    __shared__ f32x4 acc[256];
+    __shared__ float2 mls[256];
+    const AttnParams &p = kp.a;
+    const int q4 = p.head_dim / 4;
+    const int grp = threadIdx.x / q4, d4 = threadIdx.x - grp * q4;
+    const int sub = grp % p.join_groups, which = grp / p.join_groups;
+    const int64_t item = (int64_t)blockIdx.x * p.join_rows + which;
+    const int64_t rt = item / p.n_head;
+    const int head = (int)(item - rt * p.n_head);
+    const int64_t r = rt / p.n_q;
+    const int t = (int)(rt - r * p.n_q);
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f, M = -__builtin_inff();
+    // A part in which the row sees nothing (l of 0) adds nothing, whatever its values.
+    auto add = [&](float2 e, f32x4 x) {
+        if (e.y == 0.0f) return;
+        const float mn = fmaxf(M, e.x);
+        const float f = M == mn || l == 0.0f ? 1.0f : __builtin_amdgcn_exp2f(M - mn);
+        const float g = e.x == mn ? 1.0f : __builtin_amdgcn_exp2f(e.x - mn);
+        l = l * f + e.y * g;
+        o = o * f + x * g;
+        M = mn;
+    };
+    int64_t tok = -1;
+    if (which < p.join_rows && r < p.n_requests) {
+        const Kv8Request q(p, (int)r, TILE_ROWS);
+        const int hk = head / p.group, row = t * p.group + head - hk * p.group, tile = row / TILE_ROWS;
+        if (row < q.rows) {
+            const long long each = kv8_share(kp, kp.starts[p.n_requests]);
+            const long long beg = kp.starts[r] + ((long long)hk * q.tiles + tile) * q.steps;
+            const int b0 = (int)(beg / each), b1 = q.steps ? (int)((beg + q.steps - 1) / each) : b0;
+            // (one workgroup's own rows are where they belong; a row of no positions is nobody's)
+            if (b1 > b0 || q.steps == 0) tok = q.t0 + t;
+            constexpr int U = 4;
+            for (int i0 = sub; b1 > b0 && i0 <= b1 - b0; i0 += p.join_groups * U) {
+                float2 e[U];
+                f32x4 x[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int i = i0 + u * p.join_groups <= b1 - b0 ? i0 + u * p.join_groups : i0;
+                    const int64_t slot = 2 * (int64_t)(b0 + i) + (i == 0 && beg > b0 * each), at = slot * TILE_ROWS + row - tile * TILE_ROWS;
+                    e[u] = p.part_ml[at];
+                    x[u] = *reinterpret_cast<const f32x4 *>(p.part_o + at * p.head_dim + d4 * 4);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (i0 + u * p.join_groups <= b1 - b0) add(e[u], x[u]);
+            }
+        }
+    }
+    if (p.join_groups > 1) {
+        acc[threadIdx.x] = o;
+        mls[threadIdx.x] = make_float2(M, l);
+        __syncthreads();
+        if (sub == 0)
+            for (int i = 1; i < p.join_groups; ++i) add(mls[threadIdx.x + i * q4], acc[threadIdx.x + i * q4]);
+    }
+    if (tok < 0 || sub != 0) return;
+    QT *dst = reinterpret_cast<QT *>(p.dst + tok * p.dst_token + head * p.dst_head) + d4 * 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dst[j] = (QT)(l == 0.0f ? 0.0f : o[j] / l);
+    if (d4 == 0 && p.lse) p.lse[tok * p.n_head + head] = l == 0.0f ? -__builtin_inff() : (M + log2f(l)) * kLn2;
 }
 
 struct Kv8AttnPlan {
     Kv8AttnParams p;
     int dim, rt;  // padded head dimension, row tiles
     bool i8, block8;
-    size_t bytes;
-    int lds;
-    const void *kernel;
+    size_t bytes, start_bytes;
+    int lds, wgs;  // wgs: workgroups a CU
+    const void *kernel, *join;
 };
 // (an instantiation per type of the queries, each in a file of its own)
 void kv8_attn_f32(Kv8AttnPlan &pl);
@@ -572,7 +756,9 @@ void kv8_attn_bf16(Kv8AttnPlan &pl);
 template <class C>
 void kv8_attn_instance(Kv8AttnPlan &pl) {
     pl.kernel = reinterpret_cast<const void *>(&kv8_attn_kernel<C>);
-    pl.lds = C::LDS + C::MORE;
+    pl.join = reinterpret_cast<const void *>(&kv8_join_kernel<typename C::QT, C::ROWS>);
+    pl.lds = C::LDS + C::MORE + kKv8Deal;
+    pl.wgs = C::WGS;
 }
 template <class QT, bool I8, bool BLOCK8>
 void kv8_attn_kernel_of(Kv8AttnPlan &pl) {

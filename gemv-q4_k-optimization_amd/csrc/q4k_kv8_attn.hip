@@ -50,30 +50,26 @@ static int kv8_attn_plan(const q4k_kv8_attn_args &a, int cus, Kv8AttnPlan &pl) {
     const int64_t tiles = cdiv(rows, 16 * pl.rt);
     if (tiles > INT32_MAX / 4 / p.n_head_kv / a.n_requests) return Q4K_EUNSUPPORTED;
     const int64_t per = tiles * p.n_head_kv * a.n_requests;
-    // Splits of one length in whole steps of 128 positions.
-    int64_t len = cdiv(cdiv(a.max_len * per, 3 * (int64_t)cus), 128) * 128;
-    if (len < 256) len = 256;
-    if (len > (1 << 30)) len = 1 << 30;
-    p.suf_len = (int)len;
     p.suf_tiles = (int)tiles;
-    p.suf_splits = a.max_len > 0 ? (int)cdiv(a.max_len, len) : 1;
-    if (per * p.suf_splits > INT32_MAX / 2) return Q4K_EUNSUPPORTED;
-    p.suf_items = (int)(per * p.suf_splits);
-    p.slots = p.suf_splits;
-    p.join = p.slots > 1;
-    // (the join as in q4k_prefix_attn.hip)
-    const int groups = 256 / (p.head_dim / 4);
-    p.join_groups = 1;
-    while (p.join_groups * 4 < p.slots && p.join_groups * 2 <= groups) p.join_groups *= 2;
-    p.join_rows = groups / p.join_groups;
-    if (p.join) {
-        const int64_t all = a.n_tokens * a.n_head;
-        if (all > ((int64_t)1 << 50) / p.slots / (p.head_dim + 2)) return Q4K_EUNSUPPORTED;
-        pl.bytes = (size_t)(all * p.slots * (p.head_dim + 2) * 4);
+    a.q_type == Q4K_GGML_TYPE_F32 ? kv8_attn_f32(pl) : a.q_type == Q4K_GGML_TYPE_F16 ? kv8_attn_f16(pl) : kv8_attn_bf16(pl);
+    const int64_t steps = cdiv(a.max_len, kKv8Step), most = (int64_t)pl.wgs * cus;
+    // (the steps of one request are counted in 31 bits)
+    if (steps > INT32_MAX / p.n_head_kv / tiles) return Q4K_EUNSUPPORTED;
+    if (steps > kKv8Least) {
+        pl.p.shares = (int)(per * steps < most * kKv8Least ? cdiv(per * steps, kKv8Least) : most);
+        p.suf_items = pl.p.shares;
+        // threads for the parts of a row: half as many as there may be where lengths are alike
+        const int groups = 256 / (p.head_dim / 4);
+        p.join_groups = 1;
+        while (p.join_groups * 2 <= groups && p.join_groups * 4 * per < pl.p.shares) p.join_groups *= 2;
+        p.join_rows = groups / p.join_groups;
+        pl.start_bytes = ((size_t)a.n_requests * 8 + 8 + 15) / 16 * 16;
+        pl.bytes = pl.start_bytes + (size_t)pl.p.shares * 2 * 16 * pl.rt * (p.head_dim + 2) * 4;
+    } else {
+        p.suf_items = (int)per;
     }
     // (the join counts its rows in 31 bits, up to a workgroup's past the last one)
     if (a.n_requests * a.n_q > (INT32_MAX - 256) / a.n_head) return Q4K_EUNSUPPORTED;
-    a.q_type == Q4K_GGML_TYPE_F32 ? kv8_attn_f32(pl) : a.q_type == Q4K_GGML_TYPE_F16 ? kv8_attn_f16(pl) : kv8_attn_bf16(pl);
     return Q4K_OK;
 }
 
@@ -108,15 +104,15 @@ int q4k_kv8_attn(const q4k_kv8_attn_args *args, void *workspace, size_t workspac
     st = ws.begin(workspace, workspace_bytes, pl.bytes, stream);
     if (st != Q4K_OK) return st;
     AttnParams &p = pl.p.a;
-    p.part_o = (float *)ws.ptr;
-    p.part_ml = (float2 *)(p.part_o + (int64_t)p.n_tokens * p.n_head * p.slots * p.head_dim);
+    if (pl.p.shares) {
+        pl.p.starts = (int64_t *)ws.ptr;
+        p.part_o = (float *)((char *)ws.ptr + pl.start_bytes);
+        p.part_ml = (float2 *)(p.part_o + (int64_t)pl.p.shares * 2 * 16 * pl.rt * p.head_dim);
+    }
     st = launch((void (*)(Kv8AttnParams))pl.kernel, dim3((unsigned)p.suf_items), 256, pl.lds, stream, pl.p);
-    if (st == Q4K_OK && p.join) {
-        using Fn = void (*)(AttnParams);
-        const Fn join = args->q_type == Q4K_GGML_TYPE_F32   ? prefix_attn_join_kernel<float>
-                        : args->q_type == Q4K_GGML_TYPE_F16 ? prefix_attn_join_kernel<_Float16>
-                                                            : prefix_attn_join_kernel<__bf16>;
-        st = launch(join, dim3((unsigned)cdiv((int64_t)p.n_requests * p.n_q * p.n_head, p.join_rows)), 256, 0, stream, p);
+    if (st == Q4K_OK && pl.p.shares) {
+        const int64_t rows = (int64_t)p.n_requests * p.n_q * p.n_head;
+        st = launch((void (*)(Kv8AttnParams))pl.join, dim3((unsigned)cdiv(rows, p.join_rows)), 256, 0, stream, pl.p);
     }
     return ws.end(st, stream);
 }
