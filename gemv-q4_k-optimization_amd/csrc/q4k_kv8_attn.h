@@ -22,6 +22,7 @@
 
 #include "q4k_attn.h"
 #include "q4k_kv8.h"
+#include "q4k_scan.h"
 
 namespace q4k {
 
@@ -31,16 +32,16 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 struct Kv8AttnParams {
     AttnParams a;  // rows and partial results; `suf` parts only, no AttnCache
     Kv8Cache c;
-    // Where the positions are dealt out: workgroups that share them (else 0), the number of steps
-    // before each request's and, last, of all, for the join.  (a.join stays 0: attn_emit writes dst.)
-    int shares;
-    int64_t *starts;
+    // (a.join stays 0: attn_emit writes dst.)
+    int each;       // steps of a part of a tile's positions, where parts are of one length
+    int shares;     // workgroups that all steps are dealt out to (else 0), and the number of steps
+    double *starts; // before each request's and, last, of all, for the join
 };
 
-// Positions of a step of four waves; the least steps a workgroup takes (12 x 5 F16 tokens over 3001
-// positions: 1 step @@, 2 @@, 4 @@ us).
-constexpr int kKv8Step = 128, kKv8Least = 2;
-constexpr int kKv8Deal = (257 + 4 + 1) * 8;  // bytes of LDS
+// Positions of a step of four waves; the least steps of a part (200 positions of one request: 1 step a
+// part and a join 14.0 us, 2 11.4), the most of parts of one length.
+constexpr int kKv8Step = 128, kKv8Least = 2, kKv8Few = 4;
+constexpr int kKv8Deal = (257 + 4) * 8 + (3 * 256 + 1) * 4;  // bytes of LDS
 
 // References move by more than 2^kKv8Lazy only; P is at most 2^kKv8Lazy.  (BF16 terms have
 // F32's range, so nothing is lost below.)
@@ -79,7 +80,7 @@ struct Kv8Cfg {
     // after that: (M, l) of four waves' rows and the rows' factors; places of 32 positions of four waves
     static constexpr int PLACES = BLOCK8 ? 0 : 4 * 32 * (16 + 8);
     static constexpr int MORE = 1024 + PLACES;
-    static constexpr int WGS = D == 256 ? 1 : D == 128 && RT == 2 ? 2 : 3;  // workgroups a CU
+    static constexpr int WGS = D == 256 ? 1 : (D == 64 ? RT == 1 || (BLOCK8 && QTERMS == 1) : RT == 1 && BLOCK8 && QTERMS == 1) ? 3 : 2;  // workgroups a CU
 };
 
 // Eight bytes as the operand of the score product.
@@ -162,75 +163,75 @@ __device__ __forceinline__ void kv8_values(const uint32_t (&x)[8], Vec8<__bf16>:
     for (int d = 0; d < 4; ++d) out[d] = u[d].v;
 }
 
-// Rows row0 .. row0 + 15: of row n the dimensions (kk / 2) * 64 + g * 16 + (kk & 1) * 8 ..
-// per lane, as the score product takes them, handed to put(term, kk, vector).
-// Returns the row's factor c.
-template <class C, class PUT>
-__device__ __forceinline__ float kv8_queries(const AttnParams &p, const AttnSpan &s, int hk, int row0, PUT put) {
+// Rows row0 .. row0 + 15 of the queries: of row n the dimensions (kk / 2) * 64 + g * 16 + (kk & 1) * 8 ..
+// per lane, as the score product takes them.
+template <class C>
+struct Kv8Queries {
     using T = typename C::T;
     using QT = typename C::QT;
-    using V8 = typename Vec8<T>::type;
-    constexpr int KK = C::KK;
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const float sgn = p.scale < 0.0f ? -1.0f : 1.0f;
-    const int row = row0 + n;
-    const bool ok = row < s.rows;
-    const int t = (int)fastdiv((uint32_t)(ok ? row : 0), p.group_div);
-    const int h = hk * p.group + (ok ? row : 0) - t * p.group;
-    const QT *src = reinterpret_cast<const QT *>(p.q + (int64_t)(s.tok0 + t) * p.q_token + h * p.q_head);
-    float x[KK][8];
-    float top = 0.0f;
+    static constexpr int KK = C::KK, N = 8 * sizeof(QT) / 16;
+    union Piece {
+        u32x4 v[N];
+        QT e[8];
+    } x[KK];
+
+    __device__ __forceinline__ bool in(const AttnParams &p, const AttnSpan &s, int row0) const { return row0 + (int)(threadIdx.x & 15) < s.rows; }
+    __device__ __forceinline__ int dim(int kk) const { return (kk >> 1) * 64 + ((threadIdx.x & 63) >> 4) * 16 + (kk & 1) * 8; }
+    __device__ __forceinline__ void load(const AttnParams &p, const AttnSpan &s, int hk, int row0) {
+        const int row = in(p, s, row0) ? row0 + (int)(threadIdx.x & 15) : 0;
+        const int t = (int)fastdiv((uint32_t)row, p.group_div);
+        const int h = hk * p.group + row - t * p.group;
+        const QT *src = reinterpret_cast<const QT *>(p.q + (int64_t)(s.tok0 + t) * p.q_token + h * p.q_head);
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-        // (clamped, so that the loads need no branches)
-        const int d = (kk >> 1) * 64 + g * 16 + (kk & 1) * 8;
-        const bool in = ok && d < p.head_dim;
-        const QT *at = src + (d < p.head_dim ? d : 0);
-        if (p.q_vec) {
-            constexpr int N = 8 * sizeof(QT) / 16;
-            union {
-                u32x4 v[N];
-                QT e[8];
-            } u;
+        for (int kk = 0; kk < KK; ++kk) {
+            // (clamped, so that the loads need no branches)
+            const QT *at = src + (dim(kk) < p.head_dim ? dim(kk) : 0);
+            if (p.q_vec) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) u.v[i] = reinterpret_cast<const u32x4 *>(at)[i];
+                for (int i = 0; i < N; ++i) x[kk].v[i] = reinterpret_cast<const u32x4 *>(at)[i];
+            } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[kk][j] = (float)u.e[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[kk][j] = (float)at[j];
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[kk][j] = in ? x[kk][j] * sgn : 0.0f;
-            top = fmaxf(top, fabsf(x[kk][j]));
+                for (int j = 0; j < 8; ++j) x[kk].e[j] = at[j];
+            }
         }
     }
-    float c = fabsf(p.scale) * kLog2e, f = 1.0f;
-    if (C::QTERMS > 1) {
-        // an F32 row of any magnitude: a power of two brings its largest value to 1..2
-        top = xor_max(top);
-        int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-        e = e < -126 || e > 127 ? 0 : e > 126 ? 126 : e;
-        f = __uint_as_float((uint32_t)(127 - e) << 23);
-        c *= __uint_as_float((uint32_t)(127 + e) << 23);
-    }
+    // to put(term, kk, vector); returns the row's factor c
+    template <class PUT>
+    __device__ __forceinline__ float give(const AttnParams &p, const AttnSpan &s, int row0, PUT put) const {
+        const float sgn = p.scale < 0.0f ? -1.0f : 1.0f;
+        const bool ok = in(p, s, row0);
+        float top = 0.0f;
+        auto value = [&](int kk, int j) { return ok && dim(kk) < p.head_dim ? (float)x[kk].e[j] * sgn : 0.0f; };
+        float c = fabsf(p.scale) * kLog2e, f = 1.0f;
+        if (C::QTERMS > 1) {
+            // an F32 row of any magnitude: a power of two brings its largest value to 1..2
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-        V8 v[C::QTERMS];
+            for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            T t8[C::QTERMS];
-            split_terms<T, C::QTERMS>(x[kk][j] * f, t8);
-#pragma unroll
-            for (int i = 0; i < C::QTERMS; ++i) v[i][j] = t8[i];
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(value(kk, j)));
+            top = xor_max(top);
+            int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+            e = e < -126 || e > 127 ? 0 : e > 126 ? 126 : e;
+            f = __uint_as_float((uint32_t)(127 - e) << 23);
+            c *= __uint_as_float((uint32_t)(127 + e) << 23);
         }
 #pragma unroll
-        for (int i = 0; i < C::QTERMS; ++i) put(i, kk, v[i]);
+        for (int kk = 0; kk < KK; ++kk) {
+            typename Vec8<T>::type v[C::QTERMS];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                T t8[C::QTERMS];
+                split_terms<T, C::QTERMS>(value(kk, j) * f, t8);
+#pragma unroll
+                for (int i = 0; i < C::QTERMS; ++i) v[i][j] = t8[i];
+            }
+#pragma unroll
+            for (int i = 0; i < C::QTERMS; ++i) put(i, kk, v[i]);
+        }
+        // (above zero, so that c * -inf of an unseen position stays -inf at a scale of 0)
+        return fmaxf(c, 1e-37f);
     }
-    // (above zero, so that c * -inf of an unseen position stays -inf at a scale of 0)
-    return fmaxf(c, 1e-37f);
-}
+};
 
 // Some byte of e4m3 that is NaN (0x7f, 0xff): zeroed, and told.
 __device__ __forceinline__ bool kv8_nan(uint32_t &w) {
@@ -347,6 +348,9 @@ __device__ __forceinline__ void kv8_attn_item(const Kv8AttnParams &kp, const Att
             }
         }
     };
+    // the queries, one row tile per wave, then the first positions
+    Kv8Queries<C> own;
+    if (wave < RT) own.load(p, s, hk, row0 + wave * 16);
     int t0 = s.beg + wave * 32;
     if (t0 < s.end) {
         get_pages(t0);
@@ -355,13 +359,12 @@ __device__ __forceinline__ void kv8_attn_item(const Kv8AttnParams &kp, const Att
         get_pages(t0 + 128);
     }
     __syncthreads();  // (LDS may still be read for the item before)
-    // the queries, one row tile per wave, while the first positions are on their way
     AttnRows<RT, D> w;
     attn_rows<RT, D>(p, s, row0, w);
     V8 q[C::QLDS ? 1 : RT][QTERMS][KK];
     float *cs = reinterpret_cast<float *>(more);
     if (wave < RT) {
-        const float c = kv8_queries<C>(p, s, hk, row0 + wave * 16, [&](int i, int kk, V8 v) {
+        const float c = own.give(p, s, row0 + wave * 16, [&](int i, int kk, V8 v) {
             *reinterpret_cast<V8 *>(lds + ((wave * QTERMS + i) * KK + kk) * 1024 + lane * 16) = v;
         });
         if (g == 0) cs[wave * 16 + n] = c;
@@ -549,58 +552,55 @@ __device__ __forceinline__ void kv8_attn_item(const Kv8AttnParams &kp, const Att
 }
 
 // What request r takes: its rows, tiles of them and steps.
+template <int TILE_ROWS>
 struct Kv8Request {
-    int t0, rows, tiles, len, steps;
-    __device__ __forceinline__ Kv8Request(const AttnParams &p, int r, int tile_rows) {
-        int t1;
+    int t0, t1, len;
+    __device__ __forceinline__ Kv8Request(int first, int end, int n) : t0(first), t1(end), len(n) {}
+    __device__ __forceinline__ Kv8Request(const AttnParams &p, int r) {
         attn_tokens(p, r, t0, t1);
-        rows = (t1 - t0) * p.group;
-        tiles = (rows + tile_rows - 1) / tile_rows;
         len = attn_suffix(p, r);
-        steps = (len + kKv8Step - 1) / kKv8Step;
     }
-    __device__ __forceinline__ long long all(const AttnParams &p) const { return (long long)steps * tiles * p.n_head_kv; }
+    __device__ __forceinline__ int rows(const AttnParams &p) const { return (t1 - t0) * p.group; }
+    __device__ __forceinline__ int tiles(const AttnParams &p) const { return (rows(p) + TILE_ROWS - 1) / TILE_ROWS; }
+    __device__ __forceinline__ int steps() const { return (len + kKv8Step - 1) / kKv8Step; }
+    // (below 2^31)
+    __device__ __forceinline__ int all(const AttnParams &p) const { return steps() * tiles(p) * p.n_head_kv; }
 };
-__device__ __forceinline__ long long kv8_uniform(long long x) {
-    const unsigned lo = __builtin_amdgcn_readfirstlane((int)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
-    return (long long)((unsigned long long)hi << 32 | lo);
-}
+// Steps are counted in whole numbers below 2^53, held in 64-bit floats: quotients are 15 instructions
+// instead of 150, and exact once rounded down.
+__device__ __forceinline__ double kv8_quotient(double x, double y) { return floor(x / y); }
 // steps of a share, of all steps
-__device__ __forceinline__ long long kv8_share(const Kv8AttnParams &kp, long long all) {
-    const long long x = (all + kp.shares - 1) / kp.shares;
-    return x < kKv8Least ? kKv8Least : x;
-}
-__device__ __forceinline__ long long kv8_wave_scan(long long x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const long long y = __shfl_up(x, d);
-        x += lane >= d ? y : 0;
-    }
-    return x;
+__device__ __forceinline__ double kv8_share(const Kv8AttnParams &kp, double all) {
+    return fmax(kv8_quotient(all + (kp.shares - 1), kp.shares), kKv8Least);
 }
 
-// Short caches: a workgroup for each tile of rows.  Longer ones: all steps of all requests, KV heads
-// and tiles, in that order, are dealt out evenly to as many workgroups as the card holds at
-// once, whatever the requests' lengths; a tile that more than one of them works on is joined by a
-// kernel of its own.  (64 requests of 512 to 8192 positions: 232 us with splits of one length for all,
-// two a request; 183 with eight; @@ dealt out.)
+// Parts of one length, where they are of a few steps; else all steps of all requests, KV heads and
+// tiles, in that order, dealt out evenly to as many workgroups as the card holds at once, whatever
+// the requests' lengths.  Tiles of several parts are joined by a kernel of its own.  (64 requests of
+// 512 to 8192 positions: 232 us with two parts of one length a request, 183 with eight, 151 dealt out;
+// 12 x 5 F16 tokens over up to 3001 positions: 16.2 us with parts of three steps, 21.7 dealt out, which
+// has to count all lengths first, and to wait for a second tile's first positions.)
 template <class C>
 __global__ __launch_bounds__(256, C::WGS) void kv8_attn_kernel(Kv8AttnParams kp) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnParams &p = kp.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // where 256 requests begin and the last one ends, in steps; sums of the waves'; the request in turn
-    long long *begins = reinterpret_cast<long long *>(lds + C::LDS + C::MORE), *sums = begins + 257;
-    int &found = *reinterpret_cast<int *>(sums + 4);
+    using Request = Kv8Request<C::ROWS>;
+    // 256 requests: where they begin in steps, and the last one ends; what they take
+    double *begins = reinterpret_cast<double *>(lds + C::LDS + C::MORE), *sums = begins + 257;
+    int *tokens = reinterpret_cast<int *>(sums + 4), *ends = tokens + 256, *lens = ends + 256, &found = lens[256];
     // requests r0 .. r0 + 255, whose steps begin at `from`: returns where they end
-    auto number = [&](int r0, long long from) {
-        const long long own = r0 + tid < p.n_requests ? Kv8Request(p, r0 + tid, C::ROWS).all(p) : 0;
-        const long long inc = kv8_wave_scan(own);
+    auto number = [&](int r0, double from) {
+        Request q(0, 0, 0);
+        if (r0 + tid < p.n_requests) q = Request(p, r0 + tid);
+        const double own = q.all(p), inc = wave_scan(own);
         __syncthreads();
+        tokens[tid] = q.t0;
+        ends[tid] = q.t1;
+        lens[tid] = q.len;
         if (lane == 63) sums[wave] = inc;
         __syncthreads();
-        long long all = from;
+        double all = from;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (i == wave) begins[tid] = all + inc - own;
@@ -608,22 +608,21 @@ __global__ __launch_bounds__(256, C::WGS) void kv8_attn_kernel(Kv8AttnParams kp)
         }
         if (tid == 0) begins[256] = all;
         __syncthreads();
-        return kv8_uniform(all);
+        return lane_of(all, 0);
     };
     const int share = kp.shares ? xcd_item(blockIdx.x, kp.shares) : 0;
-    long long at = 0, last = 0;
+    double at = 0, last = 0;
     int r0 = 0;
     if (kp.shares) {
-        long long total = 0;
+        double total = 0;
         for (; r0 < p.n_requests; r0 += 256) {
-            const long long from = total;
-            total = number(r0, from);
+            total = number(r0, total);
             if (share == 0 && r0 + tid < p.n_requests) kp.starts[r0 + tid] = begins[tid];
         }
         if (share == 0 && tid == 0) kp.starts[p.n_requests] = total;
-        const long long each = kv8_share(kp, total);
-        at = share * each;
-        last = at + each < total ? at + each : total;
+        const double each = kv8_share(kp, total);
+        at = lane_of(share * each, 0);
+        last = lane_of(fmin(at + each, total), 0);
         if (at >= last) return;
         // (the last 256 requests' numbers are there; the first ones again where there are more)
         r0 -= 256;
@@ -632,42 +631,51 @@ __global__ __launch_bounds__(256, C::WGS) void kv8_attn_kernel(Kv8AttnParams kp)
             number(0, 0);
         }
     }
-    const long long first = at;
+    const double first = at;
     do {
-        int r, hk, tile, step = 0, n;
+        int r, hk, tile, step, n, slot;
+        Request q(0, 0, 0);
         if (kp.shares) {
-            while (at >= kv8_uniform(begins[256])) {
+            while (at >= lane_of(begins[256], 0)) {
                 r0 += 256;
-                number(r0, kv8_uniform(begins[256]));
+                number(r0, lane_of(begins[256], 0));
             }
             if (begins[tid] <= at && at < begins[tid + 1]) found = tid;
             __syncthreads();
             const int in = __builtin_amdgcn_readfirstlane(found);
             r = r0 + in;
-            const Kv8Request q(p, r, C::ROWS);
-            const int past = (int)(at - kv8_uniform(begins[in]));  // (a request's steps are below 2^31)
-            const int which = past / q.steps;
-            step = past - which * q.steps;
-            hk = which / q.tiles;
-            tile = which - hk * q.tiles;
-            n = last - at < q.steps - step ? (int)(last - at) : q.steps - step;
+            q = Request(__builtin_amdgcn_readfirstlane(tokens[in]), __builtin_amdgcn_readfirstlane(ends[in]), __builtin_amdgcn_readfirstlane(lens[in]));
+            const int past = (int)(at - lane_of(begins[in], 0));
+            const int which = past / q.steps();
+            step = past - which * q.steps();
+            hk = which / q.tiles(p);
+            tile = which - hk * q.tiles(p);
+            n = (int)fmin(last - at, q.steps() - step);
+            slot = 2 * share + (at > first);
         } else {
-            const int item = xcd_item(blockIdx.x, p.suf_items), x = item / p.suf_tiles;
+            // part (slowest), request, KV head, tile
+            const int item = xcd_item(blockIdx.x, p.suf_items);
+            int x = item / p.suf_tiles;
             tile = item - x * p.suf_tiles;
-            r = x / p.n_head_kv;
-            hk = x - r * p.n_head_kv;
-            n = kKv8Least;
+            hk = x % p.n_head_kv;
+            x /= p.n_head_kv;
+            r = x % p.n_requests;
+            step = x / p.n_requests * kp.each;
+            n = kp.each;
+            slot = item;
+            q = Request(p, r);
+            // (the first part of a request that sees nothing writes its empty rows)
+            if (step > 0 && step >= q.steps()) return;
         }
-        const Kv8Request q(p, r, C::ROWS);
         AttnSpan s;
         s.beg = step * kKv8Step;
-        s.end = n < q.steps - step ? s.beg + n * kKv8Step : q.len;
-        s.rows = q.rows;
+        s.end = n < q.steps() - step ? s.beg + n * kKv8Step : q.len;
+        s.rows = q.rows(p);
         s.tok0 = q.t0;
-        s.causal = q.len - q.rows / p.group;
+        s.causal = q.len - (q.t1 - q.t0);
         s.table_row = r;
-        s.slot = !kp.shares || n == q.steps ? -1 : 2 * share + (at > first);
-        if (tile < q.tiles) kv8_attn_item<C>(kp, s, hk, tile, lds);
+        s.slot = step == 0 && n >= q.steps() ? -1 : slot;
+        if (tile < q.tiles(p)) kv8_attn_item<C>(kp, s, hk, tile, lds);
         at += n;
     } while (at < last);
 }
@@ -701,28 +709,42 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnParams kp) {
     };
     int64_t tok = -1;
     if (which < p.join_rows && r < p.n_requests) {
-        const Kv8Request q(p, (int)r, TILE_ROWS);
+        const Kv8Request<TILE_ROWS> q(p, (int)r);
         const int hk = head / p.group, row = t * p.group + head - hk * p.group, tile = row / TILE_ROWS;
-        if (row < q.rows) {
-            const long long each = kv8_share(kp, kp.starts[p.n_requests]);
-            const long long beg = kp.starts[r] + ((long long)hk * q.tiles + tile) * q.steps;
-            const int b0 = (int)(beg / each), b1 = q.steps ? (int)((beg + q.steps - 1) / each) : b0;
-            // (one workgroup's own rows are where they belong; a row of no positions is nobody's)
-            if (b1 > b0 || q.steps == 0) tok = q.t0 + t;
+        if (row < q.rows(p)) {
+            // the number of parts, and where they are; none to join where one workgroup had all
+            int parts, first = 0;
+            int64_t slot0, stride;
+            if (kp.shares) {
+                const double each = kv8_share(kp, kp.starts[p.n_requests]);
+                const double beg = kp.starts[r] + (double)((hk * q.tiles(p) + tile) * q.steps());
+                const int b0 = (int)kv8_quotient(beg, each);
+                parts = q.len ? (int)kv8_quotient(beg + (q.steps() - 1), each) - b0 + 1 : 0;
+                first = beg > b0 * each;
+                slot0 = 2 * (int64_t)b0;
+                stride = 2;
+            } else {
+                parts = (q.steps() + kp.each - 1) / kp.each;
+                stride = (int64_t)p.n_requests * p.n_head_kv * p.suf_tiles;
+                slot0 = (r * p.n_head_kv + hk) * p.suf_tiles + tile;
+            }
+            // (a request of no positions was dealt out to nobody)
+            if (parts > 1 || (parts == 0 && kp.shares)) tok = q.t0 + t;
+            if (parts <= 1) parts = 0;
             constexpr int U = 4;
-            for (int i0 = sub; b1 > b0 && i0 <= b1 - b0; i0 += p.join_groups * U) {
+            for (int i0 = sub; i0 < parts; i0 += p.join_groups * U) {
                 float2 e[U];
                 f32x4 x[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const int i = i0 + u * p.join_groups <= b1 - b0 ? i0 + u * p.join_groups : i0;
-                    const int64_t slot = 2 * (int64_t)(b0 + i) + (i == 0 && beg > b0 * each), at = slot * TILE_ROWS + row - tile * TILE_ROWS;
+                    const int i = i0 + u * p.join_groups < parts ? i0 + u * p.join_groups : i0;
+                    const int64_t slot = slot0 + i * stride + (i == 0 ? first : 0), at = slot * TILE_ROWS + row - tile * TILE_ROWS;
                     e[u] = p.part_ml[at];
                     x[u] = *reinterpret_cast<const f32x4 *>(p.part_o + at * p.head_dim + d4 * 4);
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u)
-                    if (i0 + u * p.join_groups <= b1 - b0) add(e[u], x[u]);
+                    if (i0 + u * p.join_groups < parts) add(e[u], x[u]);
             }
         }
     }
@@ -745,6 +767,7 @@ struct Kv8AttnPlan {
     int dim, rt;  // padded head dimension, row tiles
     bool i8, block8;
     size_t bytes, start_bytes;
+    int64_t slots;  // of parts that are joined
     int lds, wgs;  // wgs: workgroups a CU
     const void *kernel, *join;
 };

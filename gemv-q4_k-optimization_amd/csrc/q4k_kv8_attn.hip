@@ -55,19 +55,29 @@ static int kv8_attn_plan(const q4k_kv8_attn_args &a, int cus, Kv8AttnPlan &pl) {
     const int64_t steps = cdiv(a.max_len, kKv8Step), most = (int64_t)pl.wgs * cus;
     // (the steps of one request are counted in 31 bits)
     if (steps > INT32_MAX / p.n_head_kv / tiles) return Q4K_EUNSUPPORTED;
-    if (steps > kKv8Least) {
-        pl.p.shares = (int)(per * steps < most * kKv8Least ? cdiv(per * steps, kKv8Least) : most);
-        p.suf_items = pl.p.shares;
+    int64_t each = cdiv(per * steps, most);
+    if (each < kKv8Least) each = kKv8Least;
+    int64_t slots = 0;  // of parts
+    if (each > kKv8Few) {
+        pl.p.shares = (int)most;
+        pl.start_bytes = ((size_t)a.n_requests * 8 + 8 + 15) / 16 * 16;
+        slots = 2 * most;
+        p.suf_items = (int)most;
+    } else {
+        pl.p.each = (int)each;
+        const int64_t parts = steps > each ? cdiv(steps, each) : 1;
+        p.suf_items = (int)(per * parts);
+        if (parts > 1) slots = p.suf_items;
+    }
+    if (slots) {
         // threads for the parts of a row: half as many as there may be where lengths are alike
         const int groups = 256 / (p.head_dim / 4);
         p.join_groups = 1;
-        while (p.join_groups * 2 <= groups && p.join_groups * 4 * per < pl.p.shares) p.join_groups *= 2;
+        while (p.join_groups * 2 <= groups && p.join_groups * 4 * per < p.suf_items) p.join_groups *= 2;
         p.join_rows = groups / p.join_groups;
-        pl.start_bytes = ((size_t)a.n_requests * 8 + 8 + 15) / 16 * 16;
-        pl.bytes = pl.start_bytes + (size_t)pl.p.shares * 2 * 16 * pl.rt * (p.head_dim + 2) * 4;
-    } else {
-        p.suf_items = (int)per;
+        pl.bytes = pl.start_bytes + (size_t)slots * 16 * pl.rt * (p.head_dim + 2) * 4;
     }
+    pl.slots = slots;
     // (the join counts its rows in 31 bits, up to a workgroup's past the last one)
     if (a.n_requests * a.n_q > (INT32_MAX - 256) / a.n_head) return Q4K_EUNSUPPORTED;
     return Q4K_OK;
@@ -104,13 +114,11 @@ int q4k_kv8_attn(const q4k_kv8_attn_args *args, void *workspace, size_t workspac
     st = ws.begin(workspace, workspace_bytes, pl.bytes, stream);
     if (st != Q4K_OK) return st;
     AttnParams &p = pl.p.a;
-    if (pl.p.shares) {
-        pl.p.starts = (int64_t *)ws.ptr;
-        p.part_o = (float *)((char *)ws.ptr + pl.start_bytes);
-        p.part_ml = (float2 *)(p.part_o + (int64_t)pl.p.shares * 2 * 16 * pl.rt * p.head_dim);
-    }
+    pl.p.starts = (double *)ws.ptr;
+    p.part_o = (float *)((char *)ws.ptr + pl.start_bytes);
+    p.part_ml = (float2 *)(p.part_o + pl.slots * 16 * pl.rt * p.head_dim);
     st = launch((void (*)(Kv8AttnParams))pl.kernel, dim3((unsigned)p.suf_items), 256, pl.lds, stream, pl.p);
-    if (st == Q4K_OK && pl.p.shares) {
+    if (st == Q4K_OK && pl.slots) {
         const int64_t rows = (int64_t)p.n_requests * p.n_q * p.n_head;
         st = launch((void (*)(Kv8AttnParams))pl.join, dim3((unsigned)cdiv(rows, p.join_rows)), 256, 0, stream, pl.p);
     }
