@@ -9,6 +9,9 @@
 // moves between lanes but the sum of squares, and works out the cosines of its
 // token once for all its heads: lane i those of pair i, from pos * freq in turns in
 // 64 bits, less the whole quarter turns before it is rounded.
+//
+// Many tokens are bound by memory: 4096 tokens of 64 + 8 heads of 128 with norms, F32 to BF16,
+// 226 MB, take 46 us, 4.9 TB/s (a large copy: 5.2).  One token takes 4.2 us, a launch's own time.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -31,34 +34,37 @@ struct RopeParams {
     const float *factors;
     int n_q, n_head;  // heads of the queries, of both
     int n_tokens, chunks, per;  // heads' rounds of a wave, waves of a token
-    int head_dim, n_rot, neox;
+    int head_dim, n_rot;
+    bool past;  // results go past the caches
     float eps, magnitude;
     double turns[Q4K_ROPE_MAX_HEAD_DIM / 2];  // of a pair per position
 };
 
 template <int W, class T>
-__device__ __forceinline__ void rope_load(const char *p, float *x) {
-    typedef T vec __attribute__((ext_vector_type(W)));
-    const vec v = *reinterpret_cast<const vec *>(p);
-#pragma unroll
-    for (int j = 0; j < W; ++j) x[j] = (float)v[j];
-}
-template <>
-__device__ __forceinline__ void rope_load<1, float>(const char *p, float *x) { x[0] = *reinterpret_cast<const float *>(p); }
-template <>
-__device__ __forceinline__ void rope_load<1, _Float16>(const char *p, float *x) { x[0] = (float)*reinterpret_cast<const _Float16 *>(p); }
-template <>
-__device__ __forceinline__ void rope_load<1, __bf16>(const char *p, float *x) { x[0] = (float)*reinterpret_cast<const __bf16 *>(p); }
+struct RopeVec {
+    typedef T type __attribute__((ext_vector_type(W)));
+    typedef __attribute__((address_space(1))) type global;
+};
+template <class T>
+struct RopeVec<1, T> {
+    typedef T type;
+    typedef __attribute__((address_space(1))) T global;
+};
 template <int W, class T>
-__device__ __forceinline__ void rope_store(char *p, const float *x) {
-    if constexpr (W == 1) {
-        *reinterpret_cast<T *>(p) = (T)x[0];
-    } else {
-        typedef T vec __attribute__((ext_vector_type(W)));
-        vec v;
+__device__ __forceinline__ void rope_store(char *p, const float *x, bool past) {
+    union {
+        T e[W];
+        typename RopeVec<W, T>::type v;
+    } u;
 #pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = (T)x[j];
-        *reinterpret_cast<vec *>(p) = v;
+    for (int j = 0; j < W; ++j) u.e[j] = (T)x[j];
+    auto *to = (typename RopeVec<W, T>::global *)p;
+    if (past) {
+        __builtin_nontemporal_store(u.v, to);
+    } else {
+        asm volatile("");  // (on both sides, or the compiler makes the two stores one, of this kind)
+        *to = u.v;
+        asm volatile("");
     }
 }
 
@@ -77,9 +83,17 @@ __device__ __forceinline__ float2 rope_angle(double turns) {
     }
 }
 
+// The values in scalar registers: a choice between two parts' else becomes each lane's own load
+// of what it chose, round by round.  (What comes out are addresses of no known memory: loads and stores
+// say that theirs is global.  4096 x 72 heads: 59.8 us, 51.2 so).
+__device__ __forceinline__ RopePart rope_scalars(RopePart r) {
+    asm("" : "+s"(r.src), "+s"(r.dst), "+s"(r.src_token), "+s"(r.src_head), "+s"(r.dst_token), "+s"(r.dst_head));
+    return r;
+}
+
 // W: pairs of a unit (a lane's two pieces of W values), NU: units of a lane; LANES:
 // lanes of a head, a power of two.
-template <int W, int NU, int LANES, class S, class D>
+template <int W, int NU, int LANES, bool NEOX, class S, class D>
 __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
     constexpr int HEADS = 64 / LANES;  // of a wave's round
     __shared__ float2 table[4][Q4K_ROPE_MAX_HEAD_DIM / 2];
@@ -87,6 +101,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
     const int item = blockIdx.x * 4 + wave;
     const int tok = item / p.chunks, chunk = item - tok * p.chunks;
     const bool there = tok < p.n_tokens;
+    const RopePart q = rope_scalars(p.q), k = rope_scalars(p.k);
     const int sub = lane % LANES;
     const int half = p.n_rot / 2;
 
@@ -99,7 +114,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
         const int i = (sub + u * LANES) * W;  // pairs before this unit
         in[u] = 2 * i < p.head_dim;
         pair[u] = i;
-        if (p.neox && i < half) {
+        if (NEOX && i < half) {
             at[u][0] = i;
             at[u][1] = half + i;
         } else {
@@ -107,26 +122,26 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
             at[u][1] = 2 * i + W;
         }
     }
-    auto load = [&](int round, float (&x)[NU][2 * W]) {
+    // (as they are in memory: a conversion would wait for them; where there is nothing: the row's first
+    // values, or the first row's)
+    union Pieces {
+        typename RopeVec<W, S>::type v[2];
+        S e[2 * W];
+    } pieces[NU];
+    auto load = [&](int round) {
         const int head = round * HEADS + lane / LANES;
-        const bool isq = head < p.n_q, ok = there && head < p.n_head;
-        const RopePart &r = isq ? p.q : p.k;
-        const char *row = r.src + (ok ? tok * r.src_token + (isq ? head : head - p.n_q) * r.src_head : 0);
+        const bool ok = there && head < p.n_head, isq = head < p.n_q || (!ok && p.n_q > 0);
+        const char *row = isq ? q.src : k.src;
+        if (ok) row += isq ? tok * q.src_token + head * q.src_head : tok * k.src_token + (head - p.n_q) * k.src_head;
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            if (ok && in[u]) {
-                rope_load<W, S>(row + at[u][0] * sizeof(S), x[u]);
-                rope_load<W, S>(row + at[u][1] * sizeof(S), x[u] + W);
-            } else {
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
-                for (int j = 0; j < 2 * W; ++j) x[u][j] = 0.0f;
-            }
-        }
+            for (int i = 0; i < 2; ++i)
+                pieces[u].v[i] = *(const typename RopeVec<W, S>::global *)(row + (in[u] ? at[u][i] : 0) * sizeof(S));
     };
     int round = chunk * p.per;
     const int rounds = (p.n_head + HEADS - 1) / HEADS, end = round + p.per < rounds ? round + p.per : rounds;
-    float x[NU][2 * W];
-    load(round, x);
+    load(round);
     const int pos = there ? p.pos[tok] : 0;
     for (int i = lane; i < half; i += 64) {
         double t = (double)pos * p.turns[i];
@@ -157,9 +172,13 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
                 cs[u][j].y *= p.magnitude;
             }
         }
-    for (; round < end; ++round) {
-        float xn[NU][2 * W];
-        if (round + 1 < end) load(round + 1, xn);
+    // (a second round on its way beside the one in hand: 52.6 us)
+    for (;;) {
+        float x[NU][2 * W];
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int j = 0; j < 2 * W; ++j) x[u][j] = in[u] ? (float)pieces[u].e[j] : 0.0f;
         const int head = round * HEADS + lane / LANES;
         const bool isq = head < p.n_q;
         if (norms) {
@@ -170,17 +189,16 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
                 for (int j = 0; j < 2 * W; ++j) sum = __builtin_fmaf(x[u][j], x[u][j], sum);
 #pragma unroll
             for (int o = LANES / 2; o > 0; o /= 2) sum += __shfl_xor(sum, o);
-            const float r = 1.0f / sqrtf(sum / (float)p.head_dim + p.eps);
+            // (rows without a norm: times 1)
             const bool have = isq ? p.q.norm != nullptr : p.k.norm != nullptr;
+            const float r = have ? 1.0f / sqrtf(sum / (float)p.head_dim + p.eps) : 1.0f;
 #pragma unroll
             for (int u = 0; u < NU; ++u)
 #pragma unroll
-                for (int j = 0; j < 2 * W; ++j)
-                    if (have) x[u][j] = x[u][j] * r * (isq ? w[0][u][j] : w[1][u][j]);
+                for (int j = 0; j < 2 * W; ++j) x[u][j] = x[u][j] * r * (isq ? w[0][u][j] : w[1][u][j]);
         }
-        const RopePart &part = isq ? p.q : p.k;
         if (there && head < p.n_head) {
-            char *row = part.dst + tok * part.dst_token + (isq ? head : head - p.n_q) * part.dst_head;
+            char *row = isq ? q.dst + tok * q.dst_token + head * q.dst_head : k.dst + tok * k.dst_token + (head - p.n_q) * k.dst_head;
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
                 if (!in[u]) continue;
@@ -189,29 +207,21 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeParams p) {
                 for (int j = 0; j < W; ++j) {
                     // pair j: (j, W + j) of halves, (2j, 2j + 1) of neighbours; where
                     // nothing turns either way is the same
-                    const float na = x[u][2 * j], nb = x[u][2 * j + 1], ha = x[u][j], hb = x[u][W + j];
-                    const float a = p.neox ? ha : na, b = p.neox ? hb : nb;
+                    const int i0 = NEOX ? j : 2 * j, i1 = NEOX ? W + j : 2 * j + 1;
+                    const float a = x[u][i0], b = x[u][i1];
                     const float2 t = cs[u][j];
-                    const float ra = a * t.x - b * t.y, rb = a * t.y + b * t.x;
-                    if (p.neox) {
-                        y[j] = ra;
-                        y[W + j] = rb;
-                    } else {
-                        y[2 * j] = ra;
-                        y[2 * j + 1] = rb;
-                    }
+                    y[i0] = a * t.x - b * t.y;
+                    y[i1] = a * t.y + b * t.x;
                 }
                 if (pair[u] >= half)
 #pragma unroll
                     for (int j = 0; j < 2 * W; ++j) y[j] = x[u][j];
-                rope_store<W, D>(row + at[u][0] * sizeof(D), y);
-                rope_store<W, D>(row + at[u][1] * sizeof(D), y + W);
+                rope_store<W, D>(row + at[u][0] * sizeof(D), y, p.past);
+                rope_store<W, D>(row + at[u][1] * sizeof(D), y + W, p.past);
             }
         }
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-            for (int j = 0; j < 2 * W; ++j) x[u][j] = xn[u][j];
+        if (++round >= end) break;
+        load(round);
     }
 }
 
@@ -239,19 +249,27 @@ static bool rope_rows_vec(const q4k_rope_rows &r) {
 }
 
 using RopeFn = void (*)(RopeParams);
-template <class S, class D>
+template <bool NEOX, class S, class D>
 static RopeFn rope_fn(int dim, bool vec, int &lanes) {
     if (vec) {
         const int units = (dim + 7) / 8;
         lanes = units <= 8 ? 8 : units <= 16 ? 16 : 32;
-        return lanes == 8 ? rope_kernel<4, 1, 8, S, D> : lanes == 16 ? rope_kernel<4, 1, 16, S, D> : rope_kernel<4, 1, 32, S, D>;
+        return lanes == 8 ? rope_kernel<4, 1, 8, NEOX, S, D> : lanes == 16 ? rope_kernel<4, 1, 16, NEOX, S, D> : rope_kernel<4, 1, 32, NEOX, S, D>;
     }
     lanes = 64;
-    return dim <= 128 ? rope_kernel<1, 1, 64, S, D> : rope_kernel<1, 2, 64, S, D>;
+    return dim <= 128 ? rope_kernel<1, 1, 64, NEOX, S, D> : rope_kernel<1, 2, 64, NEOX, S, D>;
+}
+template <bool NEOX>
+static RopeFn rope_fn(int src_type, int dst_type, int dim, bool vec, int &lanes) {
+    if (src_type == Q4K_GGML_TYPE_F32)
+        return dst_type == Q4K_GGML_TYPE_F32   ? rope_fn<NEOX, float, float>(dim, vec, lanes)
+               : dst_type == Q4K_GGML_TYPE_F16 ? rope_fn<NEOX, float, _Float16>(dim, vec, lanes)
+                                               : rope_fn<NEOX, float, __bf16>(dim, vec, lanes);
+    return src_type == Q4K_GGML_TYPE_F16 ? rope_fn<NEOX, _Float16, _Float16>(dim, vec, lanes) : rope_fn<NEOX, __bf16, __bf16>(dim, vec, lanes);
 }
 
 // One launch over the queries' and the keys' rows where their types agree.
-static int rope_launch(RopeParams &p, const q4k_rope_rows *q, const q4k_rope_rows *k, int cus, void *stream) {
+static int rope_launch(RopeParams &p, const q4k_rope_rows *q, const q4k_rope_rows *k, bool neox, int cus, void *stream) {
     auto part = [](const q4k_rope_rows *r) {
         return r ? RopePart{(const char *)r->src, (char *)r->dst, r->norm, r->nb_src_token, r->nb_src_head, r->nb_dst_token, r->nb_dst_head}
                  : RopePart{};
@@ -264,14 +282,9 @@ static int rope_launch(RopeParams &p, const q4k_rope_rows *q, const q4k_rope_row
     const bool vec = (!q || rope_rows_vec(*q)) && (!k || rope_rows_vec(*k)) && p.n_rot % 8 == 0 && p.head_dim % 8 == 0;
     const q4k_rope_rows &any = q ? *q : *k;
     int lanes;
-    RopeFn fn;
-    if (any.src_type == Q4K_GGML_TYPE_F32)
-        fn = any.dst_type == Q4K_GGML_TYPE_F32   ? rope_fn<float, float>(p.head_dim, vec, lanes)
-             : any.dst_type == Q4K_GGML_TYPE_F16 ? rope_fn<float, _Float16>(p.head_dim, vec, lanes)
-                                                 : rope_fn<float, __bf16>(p.head_dim, vec, lanes);
-    else
-        fn = any.src_type == Q4K_GGML_TYPE_F16 ? rope_fn<_Float16, _Float16>(p.head_dim, vec, lanes)
-                                               : rope_fn<__bf16, __bf16>(p.head_dim, vec, lanes);
+    const RopeFn fn = neox ? rope_fn<true>(any.src_type, any.dst_type, p.head_dim, vec, lanes) : rope_fn<false>(any.src_type, any.dst_type, p.head_dim, vec, lanes);
+    // (kStreamFloats: 4096 x 72 heads of 128 to BF16, 75 MB, 52.8 us into the caches, 46.0 past them)
+    p.past = p.n_tokens * (int64_t)p.n_head * p.head_dim * rope_size(any.dst_type) >= kStreamFloats * 4;
     // A round of a wave's heads each where tokens are few; the more rounds of a token
     // the fewer times its cosines are worked out, while 16 waves a CU remain.
     const int heads = 64 / lanes;
@@ -317,7 +330,7 @@ extern "C" int q4k_rope(const q4k_rope_args *args, void *stream) {
     p.n_tokens = (int)a.n_tokens;
     p.head_dim = a.head_dim;
     p.n_rot = a.n_rot;
-    p.neox = a.mode == Q4K_ROPE_NEOX;
+    const bool neox = a.mode == Q4K_ROPE_NEOX;
     p.eps = a.eps;
     double m = a.attn_factor, lo = 0.0, hi = 0.0;
     constexpr double two_pi = 6.283185307179586476925;
@@ -341,8 +354,8 @@ extern "C" int q4k_rope(const q4k_rope_args *args, void *stream) {
         p.turns[i] = f * s;
     }
     if (q && k && (q->src_type != k->src_type || q->dst_type != k->dst_type)) {
-        st = rope_launch(p, q, nullptr, di->cus, stream);
-        return st == Q4K_OK ? rope_launch(p, nullptr, k, di->cus, stream) : st;
+        st = rope_launch(p, q, nullptr, neox, di->cus, stream);
+        return st == Q4K_OK ? rope_launch(p, nullptr, k, neox, di->cus, stream) : st;
     }
-    return rope_launch(p, q, k, di->cus, stream);
+    return rope_launch(p, q, k, neox, di->cus, stream);
 }
