@@ -797,13 +797,14 @@ class Rope:
 
 def _rope_rows(x, out, norm, tokens, dim, device, what):
     st, es = _float_type(x, what)
-    dt, ds = _float_type(out, what)
-    if x.dim() != 3 or x.shape[0] != tokens or x.shape[2] != dim or x.get_device() != device or (x.stride(2) != 1 and dim > 1):
+    dt, ds = (st, es) if out.dtype is x.dtype else _float_type(out, what)
+    shape, strides, to = x.shape, x.stride(), out.stride()
+    if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or x.get_device() != device or (strides[2] != 1 and dim > 1):
         raise ValueError(f"{what}: [{tokens}, heads, {dim}] with contiguous dimensions on device {device} expected")
-    if out.shape != x.shape or out.get_device() != device or (out.stride(2) != 1 and dim > 1):
+    if out.shape != shape or out.get_device() != device or (to[2] != 1 and dim > 1):
         raise ValueError(f"{what}_out: shape and device of {what} with contiguous dimensions expected")
-    return q4k_rope_rows(x.data_ptr(), out.data_ptr(), st, dt, x.shape[1], x.stride(0) * es, x.stride(1) * es, out.stride(0) * ds,
-                         out.stride(1) * ds, norm)
+    return ctypes.pointer(q4k_rope_rows(x.data_ptr(), out.data_ptr(), st, dt, shape[1], strides[0] * es, strides[1] * es, to[0] * ds,
+                                        to[1] * ds, norm))
 
 
 def rope(r: Rope, q, k, pos, q_out=None, k_out=None, stream=None):
@@ -823,11 +824,11 @@ def rope(r: Rope, q, k, pos, q_out=None, k_out=None, stream=None):
     if q is not None:
         if q_out is None:
             q_out = _new(q.shape, q.dtype, q.device, stream)
-        args.q = ctypes.pointer(_rope_rows(q, q_out, r.q_norm, n, r.head_dim, dev, "q"))
+        args.q = _rope_rows(q, q_out, r.q_norm, n, r.head_dim, dev, "q")
     if k is not None:
         if k_out is None:
             k_out = _new(k.shape, k.dtype, k.device, stream)
-        args.k = ctypes.pointer(_rope_rows(k, k_out, r.k_norm, n, r.head_dim, dev, "k"))
+        args.k = _rope_rows(k, k_out, r.k_norm, n, r.head_dim, dev, "k")
     _on_device("q4k_rope", dev, ctypes.byref(args), _stream_of(stream, dev))
     return q_out, k_out
 
@@ -906,11 +907,12 @@ def _kv8_rows(name, pages, k, v, lens, max_len, n_q, q_start, stream):
         if x is None:
             at.append((None, 0, 0))
             continue
-        if x.shape != shape or x.dtype is not some.dtype or x.get_device() != dev or x.stride(2) != 1:
+        strides = x.stride()
+        if x.shape != shape or x.dtype is not some.dtype or x.get_device() != dev or strides[2] != 1:
             raise ValueError(f"k, v: {some.dtype} {list(shape)} with contiguous dimensions on device {dev} expected")
-        at.append((x.data_ptr(), x.stride(0) * es, x.stride(1) * es))
-    (kp, *ks), (vp, *vs) = at
-    args = q4k_kv8_rows(pages._of(requests), t, n, requests, n_q, start, lens, max_len, kp, vp, *ks, *vs)
+        at.append((x.data_ptr(), strides[0] * es, strides[1] * es))
+    (kp, kt, kh), (vp, vt, vh) = at
+    args = q4k_kv8_rows(pages._of(requests), t, n, requests, n_q, start, lens, max_len, kp, vp, kt, kh, vt, vh)
     _on_device(name, dev, ctypes.byref(args), _stream_of(stream, dev))
 
 
@@ -932,19 +934,21 @@ def kv8_load(pages: KV8Pages, k, v, lens, max_len, n_q=None, q_start=None, strea
 
 def _kv8_attn_args(q, pages, lens, max_len, n_q, q_start, scale, out, lse):
     dev = pages.device
-    if q.dim() != 3 or q.shape[2] != pages.dim or q.get_device() != dev or (q.stride(2) != 1 and pages.dim > 1):
+    shape, strides = q.shape, q.stride()
+    if len(shape) != 3 or shape[2] != pages.dim or q.get_device() != dev or (strides[2] != 1 and pages.dim > 1):
         raise ValueError("q: [tokens, heads, head_dim] with contiguous dimensions, of the cache's head_dim and device expected")
-    n, heads, dim = q.shape
+    n, heads, dim = shape
     t, es = _float_type(q, "q")
     requests, n_q, start, lens = _kv8_requests(n, n_q, q_start, lens, dev)
     if out is None:
         out = q
-    elif out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev or (out.stride(2) != 1 and dim > 1):
+    to = out.stride()
+    if out.shape != shape or out.dtype is not q.dtype or out.get_device() != dev or (to[2] != 1 and dim > 1):
         raise ValueError("out: shape, type and device of q with contiguous dimensions expected")
     if lse is not None:
         lse = _lse(lse, n, heads, dev)
     return q4k_kv8_attn_args(pages._of(requests), t, heads, dim ** -0.5 if scale is None else scale, n, requests, n_q, start, lens, max_len,
-                             q.data_ptr(), q.stride(0) * es, q.stride(1) * es, out.data_ptr(), out.stride(0) * es, out.stride(1) * es, lse)
+                             q.data_ptr(), strides[0] * es, strides[1] * es, out.data_ptr(), to[0] * es, to[1] * es, lse)
 
 
 def _lse(lse, n, heads, device):
