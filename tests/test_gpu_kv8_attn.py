@@ -294,3 +294,59 @@ def test_kv8_attention_a_step_with_rope_and_store(Q, gpu):
             out = Q.kv8_attention(q, pages, lens, most, n_q=max(n), q_start=start)
             want, _, tol, _ = _step.attention8(q, spans, plain, lens.tolist(), D ** -0.5)
             _batch.assert_close(out, want, tol, f"step {step}")
+
+
+@pytest.mark.parametrize("qt,kv", TYPES)
+@pytest.mark.parametrize("B,nq,H,hk,D,most,page,block", [
+    (40, 1, 8, 8, 64, 1300, 32, 16), (300, 1, 8, 8, 32, 300, 20, 4), (600, 2, 4, 4, 16, 290, 16, 16), (9, 1, 16, 8, 256, 1900, 64, 64), (20, 20, 16, 4, 128, 1200, 48, 12)])
+def test_kv8_attention_dealt_out(Q, gpu, qt, kv, B, nq, H, hk, D, most, page, block):
+    """Enough positions for every workgroup to take steps of several requests and heads,
+    of more requests than a workgroup counts at once; requests of none and of one."""
+    lens = [(i * 7919 + 13) % (most + 1) for i in range(B)]
+    lens[0], lens[1], lens[B - 1], lens[B // 2] = 0, 1, most, 0
+    Case(gpu, B, nq, H, hk, D, most, page, block, qt, kv, seed=B + D, lens=lens).check(Q)
+
+
+@pytest.mark.parametrize("lens", [[0] * 64, [0] * 63 + [4000], [4000] + [1] * 63, [128] * 64, [129] * 64])
+def test_kv8_attention_dealt_out_of_one_request(Q, gpu, lens):
+    """Bounds far past the lengths: all of the work in one request, or in none."""
+    case = Case(gpu, 64, 1, 8, 2, 64, 4000, 64, 32, BF16, E4M3, seed=3, lens=lens)
+    out, _ = case.check(Q)
+    assert torch.equal(out, case.run(Q)[0])
+
+
+def test_kv8_attention_dealt_out_ragged_in_a_graph(Q, gpu):
+    """Requests of their own numbers of tokens, with rows of none before, between and behind them,
+    replayed with other lengths."""
+    B, most = 48, 1500
+    spans, at = [], 3
+    for i in range(B):
+        spans.append((at, at + (0, 1, 5, 2)[i % 4]))
+        at = spans[-1][1]
+    case = Case(gpu, B, 5, 16, 8, 64, most, 32, 8, F16, I8, seed=5, spans=spans, lens=[0] * B)
+    pages = Q.KV8Pages(*case.t, table=case.table)
+    q = torch.cat([case.q, case.q[:4]])
+    lens = torch.tensor([0] * B, dtype=torch.int32, device=gpu)
+    full = torch.randint(1, most, (B,), generator=torch.Generator().manual_seed(1)).int()
+    for t, s in zip(case.t[:2], case.t[2:]):
+        t.view(torch.uint8).copy_(torch.randint(0, 120, t.shape, device=gpu, generator=case.g).to(torch.uint8))
+        s.copy_(torch.rand(s.shape, device=gpu, generator=case.g) * 0.01)
+    ws = Q.kv8_attention_workspace(q, pages, lens, most, n_q=5, q_start=case.q_start)
+    out, lse = torch.full_like(q, 3.0), torch.full(q.shape[:2], 4.0, device=gpu)
+    call = dict(n_q=5, q_start=case.q_start, scale=case.scale, out=out, lse=lse, workspace=ws)
+    Q.kv8_attention(q, pages, lens, most, **call)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        Q.kv8_attention(q, pages, lens, most, **call)
+    for i in range(4):
+        lens.copy_((full * (i + 1) // 4).to(gpu))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = Q.kv8_attention(q, pages, lens, most, **dict(call, out=torch.full_like(q, 3.0), lse=None, workspace=None))
+        assert torch.equal(out, eager)
+        n = case.q.shape[0]
+        assert (out[:3] == 3).all() and (out[n:] == 3).all() and (lse[:3] == 4).all() and (lse[n:] == 4).all()
+        want, wl, tol, tl = _step.attention8(case.q, spans, _step.Cache8(*case.t, case.table), lens.tolist(), case.scale)
+        _batch.assert_close(out[3:n], want[3:], tol[3:], "out")
+        _batch.assert_close(lse[3:n], wl[3:], tl[3:], "lse")

@@ -179,3 +179,49 @@ def test_sample_many_rows_after_the_rules_of_the_logits(Q, gpu):
     assert int(tokens[7]) == -1
     bit = (mask.gather(1, (ok // 32)[:, None])[:, 0] >> (ok % 32)) & 1
     assert ((bit == 1) | (tokens < 0)).all()
+
+
+@pytest.mark.parametrize("V,spread", [(128256, 2.0), (151936, 0.2), (262144, 4.0), (262145, 2.0), (300001, 0.05)])
+def test_sample_large_vocabularies(Q, gpu, V, spread):
+    """Cuts that keep few tokens and many, two of them past what a list holds, bounds
+    alone; rows of more tokens than a scan numbers."""
+    rules = [(1.0, 5000, 1.0, 0.0), (1.0, 5000, 0.9, 0.0), (0.8, 0, 0.99, 0.0), (1.2, 0, 0.9, 0.02), (1.0, 0, 1.0, 0.3), (1.0, 0, 1.0, 1e-4), (1.0, 0, 1.0, 1.0),
+             (0.7, 40, 0.95, 0.05), (0.7, 200, 0.8, 0.0), (1.0, 1024, 1.0, 0.0), (1.0, 1025, 0.5, 0.0), (0.05, 0, 0.5, 0.0), (50.0, 3, 0.5, 0.1), (1.0, 0, 1.0, 0.0)]
+    x, u = logits(gpu, len(rules), V, V, spread)
+    t, k, p, m = (list(c) for c in zip(*rules))
+    check(Q, x, u, t, k, p, m)
+    # what a mask leaves, by the lowest value instead of infinities: a range of 2^128
+    x[:, torch.arange(V, device=gpu) % 50 != 3] = torch.finfo(torch.float32).min
+    check(Q, x, u, t, k, p, m)
+
+
+def test_sample_logits_out_of_a_scans_reach(Q, gpu):
+    """a l past what the bins number, of the largest logit, of parts alone and of all."""
+    V = 60000
+    rules = [(1.0, 0, 1.0, 0.0), (1.0, 50, 0.9, 0.0), (1.0, 0, 0.9, 0.0), (1.0, 0, 1.0, 0.1), (1.0, 2000, 1.0, 0.0), (1.0, 1, 1.0, 0.0)]
+    t, k, p, m = (list(c) for c in zip(*rules))
+    for seed, f in enumerate((lambda x: x + 4000.0, lambda x: x - 1e5, lambda x: x * 1e4, lambda x: torch.where(x < 0, x - 1e6, x), lambda x: x * 1e-30)):
+        x, u = logits(gpu, len(rules), V, seed, 1.0)
+        check(Q, f(x), u, t, k, p, m)
+        check(Q, f(x), u, [1e-4] * len(rules), k, p, m)
+
+
+def test_sample_calls_at_once_and_again(Q, gpu):
+    """Equal bits whatever runs beside a call, each with a workspace of its own."""
+    n, V = 40, 50257
+    x, u = logits(gpu, n, V, 12)
+    rules = dict(temperature=torch.full((n,), 0.9, device=gpu), top_k=torch.tensor([0, 50] * 20, dtype=torch.int32, device=gpu),
+                 top_p=torch.tensor([0.9] * 30 + [1.0] * 10, device=gpu), min_p=torch.tensor([0.0] * 35 + [0.01] * 5, device=gpu))
+    u = torch.tensor(u, device=gpu)
+    want, lp = Q.sample(x, u, logprob=torch.empty(n, device=gpu), **rules)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    spaces = [Q.sample_workspace(x) for _ in streams]
+    got = []
+    for i in range(12):
+        s = streams[i % 3]
+        with torch.cuda.stream(s):
+            got.append(Q.sample(x, u, logprob=torch.empty(n, device=gpu), workspace=spaces[i % 3], **rules))
+    torch.cuda.synchronize()
+    for tokens, l in got:
+        assert torch.equal(tokens, want) and torch.equal(l, lp)
