@@ -23,6 +23,12 @@
 // Sums of bins are integers (any order gives the same), all others are 64-bit floats
 // in an order of their own: equal calls give equal bits.  A chunk whose largest
 // logit is below the cut is not read again.
+//
+// Bound by: 256 rows of 151936 (156 MB) 55 us of scan, of which the reads alone take 30 and the
+// 64-bit arithmetic as long, beside them in part; 74 us of draw, one workgroup a CU for its
+// registers (two, at 128 of them, spill: 122 us for both kernels at mixed rules, 124 so, and 33 against
+// 35 us for 8 rows).  Few rows: chains of round trips (1 x 32768: 6 + 19 us).  In three launches, with
+// one that finds the bins alone: 174 us and 25.
 #include <hip/hip_runtime.h>
 
 #include "../../include/q4k_step.h"
@@ -1312,8 +1318,9 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleParams 
         const int all = x.ask([&](int c) { return c % p.shares == share && s.cmax[c] >= least; });
         if (kind == kFew) x.template collect<false>(all, least, above, nullptr);
         else x.template collect<true>(all, least, above, cmass);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the sums are where the others will look)
         __syncthreads();
-        int n = s.n_list;
+        int n = s.n_list < kList ? s.n_list : kList;  // (no more are ever counted)
         if (p.shares > 1) {
             // to the row's list; the last share to come here has them all
             SampleList &o = p.list[row];
@@ -1330,6 +1337,7 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleParams 
             __syncthreads();
             if (s.best != p.shares - 1) return;
             n = sample_take(&o.n);
+            n = n < kList ? n : kList;
             for (int e = tid; e < n; e += kDrawThreads) {
                 s.list_l[e] = sample_take(&o.l[e]);
                 s.list_i[e] = sample_take(&o.i[e]);
@@ -1369,7 +1377,8 @@ __global__ void sample_pad_kernel(SampleParams p) {
 
 static_assert(sizeof(PickLds) <= 65536, "");
 
-// How the rows are scanned: parts of them (0: not), tiles of a part.
+// How the rows are scanned: parts of them (0: not), tiles of a part.  Three workgroups a CU are there
+// at once (256 rows of 151936: 123 us for the call, with eight 119; with top-p alone 155 and 158).
 static void sample_split(int64_t n_vocab, int64_t n_rows, int cus, int &parts, int &tiles) {
     parts = tiles = 0;
     if (n_vocab > (int64_t)kChunks * kChunk || n_vocab == 0) return;
@@ -1444,9 +1453,10 @@ int q4k_sample(const float *src, int64_t n_vocab, int64_t n_rows, int64_t nb_src
             p.n_vocab = 4;
         }
         if (st == Q4K_OK) st = launch(sample_scan_kernel, dim3((unsigned)(n_rows * p.parts)), kScanThreads, 0, stream, p);
-        // shares of 32 chunks, four a wave, or more, at most two workgroups a CU
+        // Shares of 32 chunks, four a wave, or more, up to two workgroups a CU (256 rows of 151936, mixed rules:
+        // one a row 142 us, two 134, four 151; all with top-p alone 147, 170 and 203).
         const int64_t most = 2 * (int64_t)di->cus / n_rows, want = (p.chunks + 31) / 32;
-        p.shares = (int)(want < most ? want : most < 2 ? 2 : most);
+        p.shares = (int)(want < most ? want : most < 1 ? 1 : most);
         if (p.shares > kParts) p.shares = kParts;
     }
     if (st == Q4K_OK) st = launch(sample_draw_kernel, dim3((unsigned)(n_rows * p.shares)), kDrawThreads, (int)sizeof(PickLds), stream, p);

@@ -225,3 +225,9 @@ def test_sample_calls_at_once_and_again(Q, gpu):
     torch.cuda.synchronize()
     for tokens, l in got:
         assert torch.equal(tokens, want) and torch.equal(l, lp)
+
+
+def test_sample_more_rows_than_workgroups_at_once(Q, gpu):
+    n, V = 600, 20000
+    x, u = logits(gpu, n, V, 14, 1.5)
+    check(Q, x, u, [0.9, 1.0, 0.0] * 200, [0, 40, 3000, 0, 0, 0] * 100, [0.95, 1.0, 0.9, 0.5, 1.0, 1.0] * 100, [0.0, 0.0, 0.0, 0.0, 0.2, 0.0] * 100)
