@@ -513,19 +513,22 @@ __device__ __forceinline__ void kv8_attn_item(const Kv8AttnParams &kp, const Att
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const float sum = xor_sum(w.l[rt]);
+        const int left = s.rows - row0 - rt * 16, rows = left < 16 ? left : 16;
         __syncthreads();
-        if (g == 0) ml[wave * 16 + n] = make_float2(kv8_ref(w.m[rt], w.c[rt]), sum);
+        if (n < rows) {
+            if (g == 0) ml[wave * 16 + n] = make_float2(kv8_ref(w.m[rt], w.c[rt]), sum);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int x = 0; x < VW; ++x) {
-                f32x4 y;
+                for (int x = 0; x < VW; ++x) {
+                    f32x4 y;
 #pragma unroll
-                for (int d = 0; d < 4; ++d) y[d] = w.o[rt][x * 4 + d][j];
-                *reinterpret_cast<f32x4 *>(ol + (wave * 16 + n) * D + ((((g * 4 + j) * VW + x) ^ n) * 4)) = y;
-            }
+                    for (int d = 0; d < 4; ++d) y[d] = w.o[rt][x * 4 + d][j];
+                    *reinterpret_cast<f32x4 *>(ol + (wave * 16 + n) * D + ((((g * 4 + j) * VW + x) ^ n) * 4)) = y;
+                }
+        }
         __syncthreads();
-        for (int x = tid; x < 16 * Q4; x += 256) {
+        for (int x = tid; x < rows * Q4; x += 256) {
             const int r = x / Q4, d4 = x % Q4;
             float M = -__builtin_inff();
 #pragma unroll
@@ -542,7 +545,7 @@ __device__ __forceinline__ void kv8_attn_item(const Kv8AttnParams &kp, const Att
             }
             if (s.slot < 0) {
                 attn_emit<QT>(p, s, hk, row0 + rt * 16 + r, d4 * 4, acc, M, ls);
-            } else if (row0 + rt * 16 + r < s.rows && d4 * 4 < p.head_dim) {
+            } else if (d4 * 4 < p.head_dim) {
                 const int64_t at = (int64_t)s.slot * C::ROWS + rt * 16 + r;
                 if (d4 == 0) p.part_ml[at] = make_float2(M, ls);
                 *reinterpret_cast<f32x4 *>(p.part_o + at * p.head_dim + d4 * 4) = acc;
