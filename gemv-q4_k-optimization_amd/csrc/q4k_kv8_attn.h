@@ -572,6 +572,20 @@ struct Kv8Request {
 // Steps are counted in whole numbers below 2^53, held in 64-bit floats: quotients are 15 instructions
 // instead of 150, and exact once rounded down.
 __device__ __forceinline__ double kv8_quotient(double x, double y) { return floor(x / y); }
+// Steps `step` and up of a request, n of them at most, whose partial results go to `slot` unless these
+// are all.
+template <int TILE_ROWS>
+__device__ __forceinline__ AttnSpan kv8_span(const AttnParams &p, const Kv8Request<TILE_ROWS> &q, int r, int step, int n, int slot) {
+    AttnSpan s;
+    s.beg = step * kKv8Step;
+    s.end = n < q.steps() - step ? s.beg + n * kKv8Step : q.len;
+    s.rows = q.rows(p);
+    s.tok0 = q.t0;
+    s.causal = q.len - (q.t1 - q.t0);
+    s.table_row = r;
+    s.slot = step == 0 && n >= q.steps() ? -1 : slot;
+    return s;
+}
 // steps of a share, of all steps
 __device__ __forceinline__ double kv8_share(const Kv8AttnParams &kp, double all) {
     return fmax(kv8_quotient(all + (kp.shares - 1), kp.shares), kKv8Least);
@@ -583,8 +597,25 @@ __device__ __forceinline__ double kv8_share(const Kv8AttnParams &kp, double all)
 // 512 to 8192 positions: 232 us with two parts of one length a request, 183 with eight, 151 dealt out;
 // 12 x 5 F16 tokens over up to 3001 positions: 16.2 us with parts of three steps, 21.7 dealt out, which
 // has to count all lengths first, and to wait for a second tile's first positions.)
+// (two kernels: in one, each keeps the other's arguments in registers)
 template <class C>
 __global__ __launch_bounds__(256, C::WGS) void kv8_attn_kernel(Kv8AttnParams kp) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const AttnParams &p = kp.a;
+    // part (slowest), request, KV head, tile
+    const int item = xcd_item(blockIdx.x, p.suf_items);
+    int x = item / p.suf_tiles;
+    const int tile = item - x * p.suf_tiles, hk = x % p.n_head_kv;
+    x /= p.n_head_kv;
+    const int r = x % p.n_requests, step = x / p.n_requests * kp.each;
+    const Kv8Request<C::ROWS> q(p, r);
+    // (the first part of a request that sees nothing writes its empty rows)
+    if (tile >= q.tiles(p) || (step > 0 && step >= q.steps())) return;
+    kv8_attn_item<C>(kp, kv8_span(p, q, r, step, kp.each, item), hk, tile, lds);
+}
+
+template <class C>
+__global__ __launch_bounds__(256, C::WGS) void kv8_attn_dealt_kernel(Kv8AttnParams kp) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const AttnParams &p = kp.a;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -613,74 +644,39 @@ __global__ __launch_bounds__(256, C::WGS) void kv8_attn_kernel(Kv8AttnParams kp)
         __syncthreads();
         return lane_of(all, 0);
     };
-    const int share = kp.shares ? xcd_item(blockIdx.x, kp.shares) : 0;
-    double at = 0, last = 0;
+    const int share = xcd_item(blockIdx.x, kp.shares);
+    double total = 0;
     int r0 = 0;
-    if (kp.shares) {
-        double total = 0;
-        for (; r0 < p.n_requests; r0 += 256) {
-            total = number(r0, total);
-            if (share == 0 && r0 + tid < p.n_requests) kp.starts[r0 + tid] = begins[tid];
-        }
-        if (share == 0 && tid == 0) kp.starts[p.n_requests] = total;
-        const double each = kv8_share(kp, total);
-        at = lane_of(share * each, 0);
-        last = lane_of(fmin(at + each, total), 0);
-        if (at >= last) return;
-        // (the last 256 requests' numbers are there; the first ones again where there are more)
-        r0 -= 256;
-        if (r0 > 0) {
-            r0 = 0;
-            number(0, 0);
-        }
+    for (; r0 < p.n_requests; r0 += 256) {
+        total = number(r0, total);
+        if (share == 0 && r0 + tid < p.n_requests) kp.starts[r0 + tid] = begins[tid];
     }
-    const double first = at;
-    do {
-        int r, hk, tile, step, n, slot;
-        Request q(0, 0, 0);
-        if (kp.shares) {
-            while (at >= lane_of(begins[256], 0)) {
-                r0 += 256;
-                number(r0, lane_of(begins[256], 0));
-            }
-            if (begins[tid] <= at && at < begins[tid + 1]) found = tid;
-            __syncthreads();
-            const int in = __builtin_amdgcn_readfirstlane(found);
-            r = r0 + in;
-            q = Request(__builtin_amdgcn_readfirstlane(tokens[in]), __builtin_amdgcn_readfirstlane(ends[in]), __builtin_amdgcn_readfirstlane(lens[in]));
-            const int past = (int)(at - lane_of(begins[in], 0));
-            const int which = past / q.steps();
-            step = past - which * q.steps();
-            hk = which / q.tiles(p);
-            tile = which - hk * q.tiles(p);
-            n = (int)fmin(last - at, q.steps() - step);
-            slot = 2 * share + (at > first);
-        } else {
-            // part (slowest), request, KV head, tile
-            const int item = xcd_item(blockIdx.x, p.suf_items);
-            int x = item / p.suf_tiles;
-            tile = item - x * p.suf_tiles;
-            hk = x % p.n_head_kv;
-            x /= p.n_head_kv;
-            r = x % p.n_requests;
-            step = x / p.n_requests * kp.each;
-            n = kp.each;
-            slot = item;
-            q = Request(p, r);
-            // (the first part of a request that sees nothing writes its empty rows)
-            if (step > 0 && step >= q.steps()) return;
+    if (share == 0 && tid == 0) kp.starts[p.n_requests] = total;
+    const double each = kv8_share(kp, total);
+    const double first = lane_of(share * each, 0), last = lane_of(fmin(first + each, total), 0);
+    if (first >= last) return;
+    // (the last 256 requests' numbers are there; the first ones again where there are more)
+    r0 -= 256;
+    if (r0 > 0) {
+        r0 = 0;
+        number(0, 0);
+    }
+    for (double at = first; at < last;) {
+        while (at >= lane_of(begins[256], 0)) {
+            r0 += 256;
+            number(r0, lane_of(begins[256], 0));
         }
-        AttnSpan s;
-        s.beg = step * kKv8Step;
-        s.end = n < q.steps() - step ? s.beg + n * kKv8Step : q.len;
-        s.rows = q.rows(p);
-        s.tok0 = q.t0;
-        s.causal = q.len - (q.t1 - q.t0);
-        s.table_row = r;
-        s.slot = step == 0 && n >= q.steps() ? -1 : slot;
-        if (tile < q.tiles(p)) kv8_attn_item<C>(kp, s, hk, tile, lds);
+        if (begins[tid] <= at && at < begins[tid + 1]) found = tid;
+        __syncthreads();
+        const int in = __builtin_amdgcn_readfirstlane(found);
+        const Request q(__builtin_amdgcn_readfirstlane(tokens[in]), __builtin_amdgcn_readfirstlane(ends[in]), __builtin_amdgcn_readfirstlane(lens[in]));
+        const int past = (int)(at - lane_of(begins[in], 0));
+        const int which = past / q.steps(), step = past - which * q.steps();
+        const int hk = which / q.tiles(p), tile = which - hk * q.tiles(p);
+        const int n = (int)fmin(last - at, q.steps() - step);
+        kv8_attn_item<C>(kp, kv8_span(p, q, r0 + in, step, n, 2 * share + (at > first)), hk, tile, lds);
         at += n;
-    } while (at < last);
+    }
 }
 
 // Joins the parts of the tiles that several workgroups had: join_groups threads for each four
@@ -772,7 +768,7 @@ struct Kv8AttnPlan {
     size_t bytes, start_bytes;
     int64_t slots;  // of parts that are joined
     int lds, wgs;  // wgs: workgroups a CU
-    const void *kernel, *join;
+    const void *kernel, *dealt, *join;
 };
 // (an instantiation per type of the queries, each in a file of its own)
 void kv8_attn_f32(Kv8AttnPlan &pl);
@@ -782,8 +778,9 @@ void kv8_attn_bf16(Kv8AttnPlan &pl);
 template <class C>
 void kv8_attn_instance(Kv8AttnPlan &pl) {
     pl.kernel = reinterpret_cast<const void *>(&kv8_attn_kernel<C>);
+    pl.dealt = reinterpret_cast<const void *>(&kv8_attn_dealt_kernel<C>);
     pl.join = reinterpret_cast<const void *>(&kv8_join_kernel<typename C::QT, C::ROWS>);
-    pl.lds = C::LDS + C::MORE + kKv8Deal;
+    pl.lds = C::LDS + C::MORE;
     pl.wgs = C::WGS;
 }
 template <class QT, bool I8, bool BLOCK8>

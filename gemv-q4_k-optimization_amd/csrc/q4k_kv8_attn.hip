@@ -60,6 +60,8 @@ static int kv8_attn_plan(const q4k_kv8_attn_args &a, int cus, Kv8AttnPlan &pl) {
     int64_t slots = 0;  // of parts
     if (each > kKv8Few) {
         pl.p.shares = (int)most;
+        pl.kernel = pl.dealt;
+        pl.lds += kKv8Deal;
         pl.start_bytes = ((size_t)a.n_requests * 8 + 8 + 15) / 16 * 16;
         slots = 2 * most;
         p.suf_items = (int)most;
