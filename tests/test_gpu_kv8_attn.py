@@ -350,3 +350,16 @@ def test_kv8_attention_dealt_out_ragged_in_a_graph(Q, gpu):
         want, wl, tol, tl = _step.attention8(case.q, spans, _step.Cache8(*case.t, case.table), lens.tolist(), case.scale)
         _batch.assert_close(out[3:n], want[3:], tol[3:], "out")
         _batch.assert_close(lse[3:n], wl[3:], tl[3:], "lse")
+
+
+def test_kv8_attention_more_steps_than_are_counted(Q, gpu):
+    """(host checks alone: no workspace is named for what a call would refuse)"""
+    k = torch.zeros(64, device=gpu)
+    lens = torch.zeros(1, dtype=torch.int32, device=gpu)
+    args = Q.q4k_kv8_attn_args()
+    pages = Q.q4k_kv8_pages(Q.TYPE_I8, 300, 16, 1 << 30, k.data_ptr(), k.data_ptr(), 1, 1 << 30, 16, 16, 16, 16, 16, 16, k.data_ptr(), k.data_ptr(), 4, 4, 4, None, 0, 1)
+    import ctypes
+    for heads, some in ((300, False), (100, True)):
+        pages.n_head_kv = heads
+        args = Q.q4k_kv8_attn_args(ctypes.pointer(pages), Q.GGML_TYPE_F32, heads, 1.0, 1, 1, 1, None, lens.data_ptr(), 1 << 30, k.data_ptr(), 64, 64, k.data_ptr(), 64, 64, None)
+        assert (Q.lib().q4k_kv8_attn_workspace_bytes(ctypes.byref(args)) > 0) == some
