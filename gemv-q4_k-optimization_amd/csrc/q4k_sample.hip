@@ -816,30 +816,50 @@ struct PickRow {
     }
 
     // Of tokens in order, their weights in cmass (0 behind the last), their places in cnt: the last
-    // one that is kept.  Returns the sum of w up to it.
+    // one that is kept; where `then` is 0 or above, of what was kept the last one before which less
+    // than that part of it lies.  Returns the sum of w up to it.
     __device__ __forceinline__ double cut_sorted(int count, const float *list_l, const int *list_i, bool by_count, double most, double base_cnt,
-                                                 double base_mass) {
+                                                 double base_mass, double then) {
         const int tid = threadIdx.x;
-        double w[kEach], mine = 0.0;
+        double w[kEach], before[kEach], mine = 0.0;
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
             w[k] = tid * kEach + k < count ? s.cmass[tid * kEach + k] : 0.0;
             mine += w[k];
         }
         double all, at_mass = base_mass + scan(mine, all);
-        int best = tid == 0 ? 0 : -1;  // (the first one always)
-        double upto = base_mass + s.cmass[0];
+        const double first = base_mass + s.cmass[0];
+        int found, best = tid == 0 ? 0 : -1;  // (the first one always)
+        double upto = first;
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
             const int e = tid * kEach + k;
-            if (w[k] > 0.0 && (by_count ? base_cnt + e : at_mass) < most) {
-                best = e;
-                upto = at_mass + w[k];
-            }
+            before[k] = at_mass;
             at_mass += w[k];
+            if (w[k] > 0.0 && (by_count ? base_cnt + e : before[k]) < most) {
+                best = e;
+                upto = at_mass;
+            }
         }
-        const int found = last_best(best);
+        found = last_best(best);
         if (best >= 0 && best == found) s.base_mass = upto;
+        if (then >= 0.0) {
+            __syncthreads();
+            const double limit = then * s.base_mass;
+            const int last = found;
+            best = tid == 0 ? 0 : -1;
+            upto = first;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const int e = tid * kEach + k;
+                if (w[k] > 0.0 && e <= last && before[k] < limit) {
+                    best = e;
+                    upto = before[k] + w[k];
+                }
+            }
+            found = last_best(best);
+            if (best >= 0 && best == found) s.base_mass = upto;
+        }
         const int at = s.cnt[found];
         last_l = list_l[at];
         last_i = list_i[at];
@@ -849,8 +869,8 @@ struct PickRow {
 
     // Of the list's n tokens those that are left in, before which lie base_cnt and
     // base_mass: the last one that is kept becomes last_l, last_i.  Returns the sum of w
-    // up to it.
-    __device__ __forceinline__ double cut_list(int n, bool by_count, double most, double base_cnt, double base_mass) {
+    // up to it.  `then` as above, of kShort tokens at most.
+    __device__ __forceinline__ double cut_list(int n, bool by_count, double most, double base_cnt, double base_mass, double then = -1.0) {
         const int tid = threadIdx.x;
         double some;
         if (n <= kShort) {
@@ -870,7 +890,7 @@ struct PickRow {
                 s.cmass[rank] = weight(s.list_l[tid]);
             }
             __syncthreads();
-            return cut_sorted(kShort, s.list_l, s.list_i, by_count, most, base_cnt, base_mass);
+            return cut_sorted(kShort, s.list_l, s.list_i, by_count, most, base_cnt, base_mass, then);
         }
         const int lane = tid & 63, wave = tid >> 6;
         const float inf = __builtin_inff();
@@ -929,7 +949,7 @@ struct PickRow {
             s.cmass[rank] = weight(l);
         }
         __syncthreads();
-        return cut_sorted(count, s.sort_l, s.sort_i, by_count, most, base_cnt, base_mass);
+        return cut_sorted(count, s.sort_l, s.sort_i, by_count, most, base_cnt, base_mass, -1.0);
     }
 
     // The kept sums of the list's n tokens by chunks, to `have` of chunks tid * kEach ..
@@ -1352,12 +1372,13 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleParams 
         }
         __syncthreads();
         if (kind != kBound) {
-            // cut once or, where all that may be kept is in the list, twice
-            const bool few = kind == kFew;
+            // cut once or, where all that may be kept is in the list, twice (at once in a short one)
+            const bool few = kind == kFew, both = few && r.top_k > 0 && r.top_p < 1.0f;
+            const double near_p = (double)r.top_p * (1.0 - kNear);
 #pragma unroll 1
-            for (int cuts = few && r.top_k > 0 && r.top_p < 1.0f ? 2 : 1, k = 0; k < cuts; ++k) {
-                const double kept = x.cut_list(n, r.top_k > 0 && k == 0, most, few ? 0.0 : base_cnt, few ? 0.0 : base_mass);
-                most = (double)r.top_p * (1.0 - kNear) * kept;
+            for (int cuts = both && n > kShort ? 2 : 1, k = 0; k < cuts; ++k) {
+                const double kept = x.cut_list(n, r.top_k > 0 && k == 0, most, few ? 0.0 : base_cnt, few ? 0.0 : base_mass, both && n <= kShort ? near_p : -1.0);
+                most = near_p * kept;
             }
             x.list_sums(n, have);
             steps = few ? 0 : bin;
