@@ -72,10 +72,12 @@ static int kv8_attn_plan(const q4k_kv8_attn_args &a, int cus, Kv8AttnPlan &pl) {
         if (parts > 1) slots = p.suf_items;
     }
     if (slots) {
-        // threads for the parts of a row: half as many as there may be where lengths are alike
+        // Threads for the parts of a row, so that each reads its up to four at once (dealt out: of a request
+        // twice as long as the others).
         const int groups = 256 / (p.head_dim / 4);
+        const int64_t parts = pl.p.shares ? 2 * most / per + 1 : slots / per;
         p.join_groups = 1;
-        while (p.join_groups * 2 <= groups && p.join_groups * 4 * per < p.suf_items) p.join_groups *= 2;
+        while (p.join_groups * 2 <= groups && p.join_groups * 4 < parts) p.join_groups *= 2;
         p.join_rows = groups / p.join_groups;
         pl.bytes = pl.start_bytes + (size_t)slots * 16 * pl.rt * (p.head_dim + 2) * 4;
     }
