@@ -121,8 +121,8 @@ class Cache8:
 
 
 # ------------------------------------------------ attention over caches of 8 bits ----
-#: what a probability times its value's scale keeps: terms of BF16, three, two and one
-PROBABILITY = {torch.float32: 2.0 ** -23, torch.float16: 2.0 ** -15, torch.bfloat16: 2.0 ** -8}
+#: what a probability times its value's scale keeps: terms of BF16, three and two
+PROBABILITY = {torch.float32: 2.0 ** -23, torch.float16: 2.0 ** -15, torch.bfloat16: 2.0 ** -15}
 
 
 def attention8(q, spans, cache, lens, scale):
