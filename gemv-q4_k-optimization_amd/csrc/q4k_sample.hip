@@ -25,9 +25,9 @@
 // logit is below the cut is not read again.
 //
 // Bound by: 256 rows of 151936 (156 MB) 55 us of scan, of which the reads alone take 30 and the
-// 64-bit arithmetic as long, beside them in part; 74 us of draw, one workgroup a CU for its
-// registers (two, at 128 of them, spill: 122 us for both kernels at mixed rules, 124 so, and 33 against
-// 35 us for 8 rows).  Few rows: chains of round trips (1 x 32768: 6 + 19 us).  In three launches, with
+// 64-bit arithmetic as long, beside them in part; 76 us of draw, one workgroup a CU for its
+// registers (two, at 128 of them, spill: 8 rows 35 us for both kernels instead of 33).
+// Few rows: chains of round trips (1 x 32768: 6 + 17 us).  In three launches, with
 // one that finds the bins alone: 174 us and 25.
 #include <hip/hip_runtime.h>
 
@@ -1474,9 +1474,10 @@ int q4k_sample(const float *src, int64_t n_vocab, int64_t n_rows, int64_t nb_src
             p.n_vocab = 4;
         }
         if (st == Q4K_OK) st = launch(sample_scan_kernel, dim3((unsigned)(n_rows * p.parts)), kScanThreads, 0, stream, p);
-        // Shares of 32 chunks, four a wave, or more, up to two workgroups a CU (256 rows of 151936, mixed rules:
-        // one a row 142 us, two 134, four 151; all with top-p alone 147, 170 and 203).
-        const int64_t most = 2 * (int64_t)di->cus / n_rows, want = (p.chunks + 31) / 32;
+        // Shares of 32 chunks, four a wave, or more, as many as there are at once, one a CU (256 rows of 151936:
+        // one a row 131 us with top-p alone and 64 with all cuts, two 155 and 82, which were better only
+        // where every row has rules of its own, 122 against 128).
+        const int64_t most = (int64_t)di->cus / n_rows, want = (p.chunks + 31) / 32;
         p.shares = (int)(want < most ? want : most < 1 ? 1 : most);
         if (p.shares > kParts) p.shares = kParts;
     }
