@@ -18,6 +18,11 @@
 //      which belongs to tile dt of the output
 // A lane's eight positions share a page and, where blocks are multiples of eight
 // tokens, a scale.
+//
+// Long caches are bound by memory: 64 requests of 512 to 8192 positions, 8 heads of 128 e4m3, 680 MB,
+// BF16 queries of 64 heads, 147 us, 4.6 TB/s, what large reads reach here.  16 of them with F32 queries,
+// 175 MB of int8, 48 us and 6 us of join, of which 8 us pass before the first step (lengths counted, page,
+// first positions); two steps on their way a wave: 51 us.  One request of 200: 9 us, a chain.
 #pragma once
 
 #include "q4k_attn.h"
@@ -39,7 +44,8 @@ struct Kv8AttnParams {
 };
 
 // Positions of a step of four waves; the least steps of a part (200 positions of one request: 1 step a
-// part and a join 14.0 us, 2 11.4), the most of parts of one length.
+// part and a join 14.0 us, 2 11.4), the most of parts of one length (at 3 steps those are faster,
+// 16.2 us against 21.7 for 12 x 5 tokens over up to 3001 positions; at 16 the others, 53.5 against 58).
 constexpr int kKv8Step = 128, kKv8Least = 2, kKv8Few = 4;
 constexpr int kKv8Deal = (257 + 4) * 8 + (3 * 256 + 1) * 4;  // bytes of LDS
 
@@ -81,7 +87,9 @@ struct Kv8Cfg {
     // after that: (M, l) of four waves' rows and the rows' factors; places of 32 positions of four waves
     static constexpr int PLACES = BLOCK8 ? 0 : 4 * 32 * (16 + 8);
     static constexpr int MORE = 1024 + PLACES;
-    static constexpr int WGS = D == 256 ? 1 : (D == 64 ? RT == 1 || (BLOCK8 && QTERMS == 1) : RT == 1 && BLOCK8 && QTERMS == 1) ? 3 : 2;  // workgroups a CU
+    // Workgroups a CU: as many as spill nothing or little (F32 queries of 128 dimensions in three, 52 bytes
+    // a lane: 16 requests 59.4 us, in two 53.5).
+    static constexpr int WGS = D == 256 ? 1 : (D == 64 ? RT == 1 || (BLOCK8 && QTERMS == 1) : RT == 1 && BLOCK8 && QTERMS == 1) ? 3 : 2;
 };
 
 // Eight bytes as the operand of the score product.
