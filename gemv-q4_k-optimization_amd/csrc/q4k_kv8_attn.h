@@ -26,6 +26,7 @@
 #pragma once
 
 #include "q4k_attn.h"
+#include "q4k_join.h"
 #include "q4k_kv8.h"
 #include "q4k_scan.h"
 
@@ -691,14 +692,13 @@ __global__ __launch_bounds__(256, C::WGS) void kv8_attn_dealt_kernel(Kv8AttnPara
 // Joins the parts of the tiles that several workgroups had: join_groups threads for each four
 // dimensions of a row.
 template <class QT, int TILE_ROWS>
-__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnParams kp) {
-    __shared__ f32x4 acc[256];
-    __shared__ float2 mls[256];
+__global__ __launch_bounds__(kJoinThreads) void kv8_join_kernel(Kv8AttnParams kp) {
+    __shared__ f32x4 acc[kJoinThreads];
+    __shared__ float2 mls[kJoinThreads];
     const AttnParams &p = kp.a;
-    const int q4 = p.head_dim / 4;
-    const int grp = threadIdx.x / q4, d4 = threadIdx.x - grp * q4;
-    const int sub = grp % p.join_groups, which = grp / p.join_groups;
-    const int64_t item = (int64_t)blockIdx.x * p.join_rows + which;
+    const JoinThread me(threadIdx.x, p.head_dim, p.join_groups, p.join_rows);
+    const int d4 = me.d4, sub = me.sub;
+    const int64_t item = (int64_t)blockIdx.x * p.join_rows + me.which;
     const int64_t rt = item / p.n_head;
     const int head = (int)(item - rt * p.n_head);
     const int64_t r = rt / p.n_q;
@@ -716,7 +716,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnParams kp) {
         M = mn;
     };
     int64_t tok = -1;
-    if (which < p.join_rows && r < p.n_requests) {
+    if (me.there && r < p.n_requests) {
         const Kv8Request<TILE_ROWS> q(p, (int)r);
         const int hk = head / p.group, row = t * p.group + head - hk * p.group, tile = row / TILE_ROWS;
         if (row < q.rows(p)) {
@@ -760,10 +760,13 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnParams kp) {
         acc[threadIdx.x] = o;
         mls[threadIdx.x] = make_float2(M, l);
         __syncthreads();
-        if (sub == 0)
-            for (int i = 1; i < p.join_groups; ++i) add(mls[threadIdx.x + i * q4], acc[threadIdx.x + i * q4]);
+        if (me.collects())
+            for (int i = 1; i < p.join_groups; ++i) {
+                const int at = JoinThread::place(threadIdx.x, p.head_dim, i);
+                add(mls[at], acc[at]);
+            }
     }
-    if (tok < 0 || sub != 0) return;
+    if (tok < 0 || !me.collects()) return;
     QT *dst = reinterpret_cast<QT *>(p.dst + tok * p.dst_token + head * p.dst_head) + d4 * 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) dst[j] = (QT)(l == 0.0f ? 0.0f : o[j] / l);

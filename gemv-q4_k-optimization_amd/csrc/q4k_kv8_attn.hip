@@ -72,13 +72,10 @@ static int kv8_attn_plan(const q4k_kv8_attn_args &a, int cus, Kv8AttnPlan &pl) {
         if (parts > 1) slots = p.suf_items;
     }
     if (slots) {
-        // Threads for the parts of a row, so that each reads its up to four at once (dealt out: of a request
-        // twice as long as the others).
-        const int groups = 256 / (p.head_dim / 4);
-        const int64_t parts = pl.p.shares ? 2 * most / per + 1 : slots / per;
-        p.join_groups = 1;
-        while (p.join_groups * 2 <= groups && p.join_groups * 4 < parts) p.join_groups *= 2;
-        p.join_rows = groups / p.join_groups;
+        // (parts of a row; dealt out: of a request twice as long as the others)
+        const JoinSplit join = join_split(p.head_dim, pl.p.shares ? 2 * most / per + 1 : slots / per);
+        p.join_groups = join.groups;
+        p.join_rows = join.rows;
         pl.bytes = pl.start_bytes + (size_t)slots * 16 * pl.rt * (p.head_dim + 2) * 4;
     }
     pl.slots = slots;
