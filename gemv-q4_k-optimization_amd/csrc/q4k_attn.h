@@ -19,6 +19,7 @@
 
 #include "q4k_batch.h"
 #include "q4k_device.h"
+#include "q4k_join.h"
 
 namespace q4k {
 
@@ -846,13 +847,12 @@ __global__ __launch_bounds__(256, CP::D == 256 ? 1 : 2) void prefix_attn_kernel(
 // split with a running reference, so that nothing waits for a first pass over the
 // references.
 template <class QT>
-__global__ __launch_bounds__(256) void prefix_attn_join_kernel(AttnParams p) {
-    __shared__ f32x4 acc[256];
-    __shared__ float2 mls[256];
-    const int q4 = p.head_dim / 4;
-    const int grp = threadIdx.x / q4, d4 = threadIdx.x - grp * q4;
-    const int sub = grp % p.join_groups, which = grp / p.join_groups;
-    const int item = blockIdx.x * p.join_rows + which;
+__global__ __launch_bounds__(kJoinThreads) void prefix_attn_join_kernel(AttnParams p) {
+    __shared__ f32x4 acc[kJoinThreads];
+    __shared__ float2 mls[kJoinThreads];
+    const JoinThread me(threadIdx.x, p.head_dim, p.join_groups, p.join_rows);
+    const int d4 = me.d4, sub = me.sub;
+    const int item = blockIdx.x * p.join_rows + me.which;
     const int rt = item / p.n_head, head = item - rt * p.n_head;
     const int r = rt / p.n_q, t = rt - r * p.n_q;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -868,7 +868,7 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(AttnParams p) {
         M = mn;
     };
     int tok = -1;
-    if (which < p.join_rows && r < p.n_requests) {
+    if (me.there && r < p.n_requests) {
         int t0, t1;
         attn_tokens(p, r, t0, t1);
         if (t0 + t < t1) tok = t0 + t;
@@ -896,10 +896,13 @@ __global__ __launch_bounds__(256) void prefix_attn_join_kernel(AttnParams p) {
         acc[threadIdx.x] = o;
         mls[threadIdx.x] = make_float2(M, l);
         __syncthreads();
-        if (sub == 0)
-            for (int i = 1; i < p.join_groups; ++i) add(mls[threadIdx.x + i * q4], acc[threadIdx.x + i * q4]);
+        if (me.collects())
+            for (int i = 1; i < p.join_groups; ++i) {
+                const int at = JoinThread::place(threadIdx.x, p.head_dim, i);
+                add(mls[at], acc[at]);
+            }
     }
-    if (tok < 0 || sub != 0) return;
+    if (tok < 0 || !me.collects()) return;
     QT *dst = reinterpret_cast<QT *>(p.dst + tok * p.dst_token + head * p.dst_head) + d4 * 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) dst[j] = (QT)(l == 0.0f ? 0.0f : o[j] / l);

@@ -149,10 +149,9 @@ static int attn_plan(const q4k_prefix_attn_args &a, int cus, AttnPlan &pl) {
     p.join = p.slots > 1 || (a.n_prefix > 0 && a.q_start);
     // the join: four splits or so to a group of lanes, more rows to a workgroup where
     // that leaves groups (4096 rows of 2 splits: 8.5 us with a workgroup each)
-    const int groups = 256 / (a.head_dim / 4);
-    p.join_groups = 1;
-    while (p.join_groups * 4 < p.slots && p.join_groups * 2 <= groups) p.join_groups *= 2;
-    p.join_rows = groups / p.join_groups;
+    const JoinSplit join = join_split(a.head_dim, p.slots);
+    p.join_groups = join.groups;
+    p.join_rows = join.rows;
     if (p.join) {
         const int64_t rows = a.n_tokens * a.n_head;
         if (rows > ((int64_t)1 << 50) / p.slots / (a.head_dim + 2)) return Q4K_EUNSUPPORTED;

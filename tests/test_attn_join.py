@@ -4,6 +4,8 @@ threads, and no thread reads LDS past the workgroup's own."""
 import os
 import subprocess
 
+import pytest
+
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gemv-q4_k-optimization_amd", "csrc")
 
 PROGRAM = r"""
@@ -45,3 +47,15 @@ def test_join_threads_stay_within_their_row(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-I", CSRC, str(tmp_path / "join.cpp"), "-o", exe], check=True)
     r = subprocess.run([exe], stdout=subprocess.PIPE, text=True, timeout=60)
     assert r.returncode == 0 and int(r.stdout.split()[0]) > 1000, r.stdout
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [8, 48, 80, 96, 112, 200])
+def test_joined_rows_where_threads_are_left_over(Q, gpu, D):
+    """Many parts of few rows, of head dimensions that 256 threads do not divide among."""
+    import test_gpu_kv8_attn as eight
+    import test_gpu_prefix_attn as sixteen
+    for prefix, suffix, lens in ((3000, 0, None), (900, 700, [700, 3, 0])):
+        sixteen.Case(gpu, 3, 1, 3, 1, D, prefix, suffix, 32, lens=lens, seed=D).check(Q)
+    if D % 16 == 0:
+        eight.Case(gpu, 3, 1, 3, 1, D, 3000, 64, 32, lens=[3000, 700, 1], seed=D).check(Q)
