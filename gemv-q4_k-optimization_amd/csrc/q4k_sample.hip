@@ -1311,8 +1311,9 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleParams 
         for (int k = 0; k < kEach; ++k) {
             const int c = tid * kEach + k;
             if (c >= p.chunks) continue;
+            // (cb: one past the bin of the chunk's largest logit, which has to be numbered itself)
             const double cb = __builtin_rint((double)s.cmax[c] * x.rate) + 1.0, at = cb - x.base + kBins;
-            if (!(at >= 0.0)) continue;
+            if (!(at >= 1.0)) continue;
             out |= !(fabs(cb) < kReach);
             have[k] = sample_weight_sum(s.octave, (int)at, p.cmass[(int64_t)row * kChunks + c]);
         }
