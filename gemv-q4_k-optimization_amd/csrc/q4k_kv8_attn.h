@@ -395,7 +395,7 @@ __device__ __forceinline__ void kv8_attn_item(const Kv8AttnParams &kp, const Att
         const bool ok = ok_next;
         const uint32_t there = there_next;
         // positions that some row does not see, or that are not there
-        const bool careful = t0 + 32 > least || (C::BLOCK8 ? !__all(ok) : there != 0xffffffffu);
+        const bool differ = t0 + 32 > least, careful = differ || (C::BLOCK8 ? !__all(ok) : there != 0xffffffffu);
 #pragma unroll
         for (int e = 0; e < (C::BLOCK8 ? 1 : 8); ++e) vs[e] = vs_next[e];
         f32x4 sx[RT][2];
@@ -435,7 +435,8 @@ __device__ __forceinline__ void kv8_attn_item(const Kv8AttnParams &kp, const Att
 #pragma unroll
                     for (int x = 0; x < VW; ++x) {
                         if (!here) vf[e][x] = 0;
-                        fine = !kv8_nan(vf[e][x]) && fine;
+                        // (what is there and every row sees stays: the products take it to all of them)
+                        if (differ) fine = !kv8_nan(vf[e][x]) && fine;
                     }
                 }
             }
