@@ -214,16 +214,18 @@ struct Kv8Queries {
         auto value = [&](int kk, int j) { return ok && dim(kk) < p.head_dim ? (float)x[kk].e[j] * sgn : 0.0f; };
         float c = fabsf(p.scale) * kLog2e, f = 1.0f;
         if (C::QTERMS > 1) {
-            // an F32 row of any magnitude: a power of two brings its largest value to 1..2
+            // An F32 row of any magnitude: a power of two brings its largest value to 2^14..2^15, near the
+            // end of F16's range.  The second term's smallest step, 2^-24, leaves each value its 22
+            // bits down to 2^-17 of the row's largest (brought to 1..2, one at 2^-10 of it would keep 15).
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(value(kk, j)));
             top = xor_max(top);
             int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-            e = e < -126 || e > 127 ? 0 : e > 126 ? 126 : e;
-            f = __uint_as_float((uint32_t)(127 - e) << 23);
-            c *= __uint_as_float((uint32_t)(127 + e) << 23);
+            e = e > 127 ? 14 : e < -112 ? -112 : e;  // (not finite: as it is)
+            f = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+            c *= __uint_as_float((uint32_t)(127 + e - 14) << 23);
         }
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) {

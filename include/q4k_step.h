@@ -157,9 +157,9 @@ size_t q4k_kv8_attn_workspace_bytes(const q4k_kv8_attn_args *args);
  * are left as they are.  Scores, the softmax's maximum and sum and the output sum
  * are F32.  Bytes enter the matrix cores exactly, as F16 (keys; BF16 with BF16
  * queries) and BF16 (values), scales are applied in F32; queries of F32 enter as
- * two F16 values (22 bits), probabilities times their value's scale as three BF16
- * values with F32 queries and two with queries of 16 bits.  Scales of values below
- * 2^100.  dst and lse must not overlap what is read.  max_len / 128 times the KV heads
+ * two F16 values (22 bits, or 2^-39 of the head's largest value), probabilities times
+ * their value's scale as three BF16 values with F32 queries and two with queries of
+ * 16 bits.  Scales of keys below 2^96, of values below 2^100.  dst and lse must not overlap what is read.  max_len / 128 times the KV heads
  * times a request's tiles of 16 rows stays below 2^31, else Q4K_EUNSUPPORTED. */
 int q4k_kv8_attn(const q4k_kv8_attn_args *args, void *workspace, size_t workspace_bytes, void *stream);
 
