@@ -363,7 +363,10 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
 struct PickLds {
     unsigned long long mass[kBins];
     double octave[kOctave];  // the powers of 2^(1/24)
-    double cmass[kChunks];
+    union {
+        double cmass[kChunks];
+        unsigned long long rest[kChunks];  // of a list's sums
+    };
     uint32_t cnt[kBins];
     float cmax[kChunks];
     float list_l[kList], sort_l[kList];
@@ -404,10 +407,14 @@ __device__ __forceinline__ float sample_next(float l, int by) {
 }
 // the order of the cuts: lower tokens of equal logits come first
 __device__ __forceinline__ bool sample_before(float l, int i, float k, int j) { return l > k || (l == k && i < j); }
-// A list's weights are taken in steps of 2^-42 (the row's largest is above 1/2): sums of a
-// thousand in any order are the same.
-__device__ __forceinline__ unsigned long long sample_steps(double w) { return (unsigned long long)(w * 0x1p42 + 0.5); }
-constexpr double kStep = 0x1p-42;
+// A list's weights (up to 1, the row's largest above 1/2) as whole numbers, so that sums of a thousand
+// in any order are the same: steps of 2^-53 and, of what these leave, of 2^-106, in which
+// a weight of 2^-63 has 43 bits.
+constexpr double kStep = 0x1p-53;
+__device__ __forceinline__ unsigned long long sample_steps(double w) { return (unsigned long long)(w * 0x1p53); }
+__device__ __forceinline__ unsigned long long sample_rest(double w, unsigned long long steps) {
+    return (unsigned long long)((w * 0x1p53 - (double)steps) * 0x1p53);
+}
 
 // (Loops over chunks and cuts are kept rolled: the code runs once for a row, and waits
 // for its own instructions too.)
@@ -955,29 +962,30 @@ struct PickRow {
     // The kept sums of the list's n tokens by chunks, to `have` of chunks tid * kEach ..
     __device__ __forceinline__ void list_sums(int n, double (&have)[kEach]) const {
         const int tid = threadIdx.x;
-        for (int e = tid; e < kChunks; e += kPickThreads) s.mass[e] = 0;
+        for (int e = tid; e < kChunks; e += kPickThreads) s.mass[e] = s.rest[e] = 0;
         __syncthreads();
 #pragma unroll 1
         for (int e = tid; e < n; e += kPickThreads)
             if (left_in(s.list_l[e], s.list_i[e])) {
                 const double w = weight(s.list_l[e]);
-                if (w >= min_w) atomicAdd(&s.mass[s.list_i[e] / chunk], sample_steps(w));
+                if (w >= min_w) {
+                    const unsigned long long steps = sample_steps(w);
+                    atomicAdd(&s.mass[s.list_i[e] / chunk], steps);
+                    atomicAdd(&s.rest[s.list_i[e] / chunk], sample_rest(w, steps));
+                }
             }
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kEach; ++k) have[k] += (double)s.mass[tid * kEach + k] * kStep;
+        for (int k = 0; k < kEach; ++k) have[k] += (double)s.mass[tid * kEach + k] * kStep + (double)s.rest[tid * kEach + k] * (kStep * kStep);
     }
 
     // The token that u falls on, of chunks tid * kEach .. with kept sums `have`, and its
-    // share.  Tokens of bins from `steps` up to `steps_end` weigh as list_sums has them.
-    __device__ __forceinline__ void draw(int row, double u, const double (&have)[kEach], int steps, int steps_end) const {
+    // share.
+    __device__ __forceinline__ void draw(int row, double u, const double (&have)[kEach]) const {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         auto kept_w = [&](float l, int i) {
-            double past;
-            const int b = bin(l, past);
-            if (b < 0 || !left_in(l, i)) return 0.0;
-            const double w = sample_weight(s.octave, b, sample_exp(past, 1.0, 0.0));
-            return !(w >= min_w) ? 0.0 : b >= steps && b < steps_end ? (double)sample_steps(w) * kStep : w;
+            const double w = weight(l);
+            return left_in(l, i) && w >= min_w ? w : 0.0;
         };
         double total, mine = 0.0;
 #pragma unroll
@@ -1236,7 +1244,7 @@ __device__ __forceinline__ void sample_alone(const SampleParams &p, PickLds &s, 
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kEach; ++k) have[k] = s.cmass[tid * kEach + k];
-    x.draw(row, r.u, have, 0, 0);
+    x.draw(row, r.u, have);
 }
 
 // What is read again of a row: nothing, the tokens from the bin up, those of the bin and the
@@ -1330,7 +1338,6 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleParams 
         if (share == 0) sample_alone<kDrawThreads>(p, s, row);
         return;
     }
-    int steps = 0, steps_end = 0;
     if (kind != kNone) {
         // this share's chunks of those that matter, dealt out so that each has as many
         double *cmass = p.cmass + (int64_t)row * kChunks;
@@ -1382,11 +1389,9 @@ __global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleParams 
                 most = near_p * kept;
             }
             x.list_sums(n, have);
-            steps = few ? 0 : bin;
-            steps_end = few ? kBins : bin + 1;
         }
     }
-    x.draw(row, r.u, have, steps, steps_end);
+    x.draw(row, r.u, have);
 }
 
 // Rows of fewer than four logits, with -inf behind them, which are no candidates.

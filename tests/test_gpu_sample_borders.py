@@ -34,3 +34,68 @@ def test_sample_of_a_first_chunk_at_the_end_of_the_bins(Q, gpu, T, chunks):
                     total = (chunks - 1) * 256
                     want = torch.where(got == 0, w * math.log(2), 0.0) - math.log(total)
                     assert ((lp - want).abs() <= 2.0 ** -24 * want.abs() + 1e-10).all()
+
+
+def drawn(x, t, u, kept):
+    """(token, log-probability, margin) of a row for each random number of u (all F32 values, in 64 bits):
+    weights of the kept tokens in their order, sums without a rounding of their own; the margin is how far from
+    u times the whole sum, in parts of it, the nearest token's sum lies."""
+    w = [math.exp((float(x[i]) - float(x.max())) / t) for i in kept]
+    upto, total = [], math.fsum(w)
+    for i in range(len(w)):
+        upto.append(math.fsum(w[:i + 1]))
+    out = []
+    for v in u:
+        border = v * total
+        n = next(i for i, s in enumerate(upto) if s > border)
+        margin = min((abs(s - border) / border for s in upto[:-1]), default=1.0) if border else 1.0
+        out.append((kept[n], math.log(w[n] / total), margin))
+    return out
+
+
+def check(Q, gpu, x, t, u, kept, k=0, p=1.0, m=0.0):
+    """Each random number of u on the row x, but for those nearer than 2^-38 of it to a border."""
+    n = len(u)
+    t, p, m = (float(torch.tensor(v, dtype=torch.float32)) for v in (t, p, m))
+    u = torch.tensor(u, dtype=torch.float32).tolist()
+    full = lambda v, d=torch.float32: torch.full((n,), v, dtype=d, device=gpu)  # noqa: E731
+    lp = full(7.0)
+    got, _ = Q.sample(x.to(gpu).repeat(n, 1), torch.tensor(u, device=gpu), temperature=full(t), top_k=full(k, torch.int32), top_p=full(p), min_p=full(m), logprob=lp)
+    tested = 0
+    for i, (token, w, margin) in enumerate(drawn(x, t, u, kept)):
+        if margin < 2.0 ** -38:
+            continue
+        tested += 1
+        assert int(got[i]) == token, (i, u[i], int(got[i]), token, margin)
+        assert abs(float(lp[i]) - w) <= 2.0 ** -24 * abs(w) + 1e-10, (i, float(lp[i]), w)
+    assert tested * 2 > n
+
+
+def test_sample_draws_what_a_cut_keeps_however_little_it_weighs(Q, gpu):
+    x = torch.tensor([-4.0, 0.0])
+    check(Q, gpu, x, 0.1, [0.0, 1e-30, 0.5], [0, 1], k=2)
+    check(Q, gpu, torch.cat([x, torch.full((300,), -8.0)]), 0.1, [0.0, 1e-30, 1e-18, 0.5], [0, 1], k=2)
+    check(Q, gpu, torch.cat([x, x - 0.01]), 0.1, [0.0, 0.5, 0.99], [0, 1, 3], k=3)
+
+
+@pytest.mark.parametrize("n", [3, 200, 256, 257, 600, 1024])
+@pytest.mark.parametrize("deep", [10, 30, 45])
+def test_sample_small_weights_of_a_list_add_up(Q, gpu, n, deep):
+    """n - 1 tokens of about 2^-deep each, and behind them one of 1, kept by top-k, by top-k and top-p (all of
+    them: the part is 1 - 2^-24 of a sum that lacks less), or by min-p too: random numbers that fall among the small ones."""
+    g = torch.Generator().manual_seed(n + deep)
+    for V in (2048, 40000):
+        x = torch.full((V,), -200.0)
+        at = torch.sort(torch.randperm(1024, generator=g)[:n - 1])[0]
+        x[at] = -(deep - 1.5 * torch.rand(n - 1, generator=g)) * math.log(2)
+        last = int(torch.randint(1280, V, (1,), generator=g))
+        x[last] = 0.0
+        kept = [*at.tolist(), last]
+        small = math.fsum(math.exp(float(x[i])) for i in at.tolist())
+        u = [0.0] + [small * v / (1 + small) for v in (1e-6, 1e-3, 0.1, 0.25, 0.5, 0.77, 0.9, 0.999, 1.3, 100.0)] + [0.7]
+        u = [v for v in u if v < 1]
+        check(Q, gpu, x, 1.0, u, kept, k=n)
+        if n > 3:
+            check(Q, gpu, x, 1.0, u, kept, k=n, m=2.0 ** -62)
+            if deep > 30:
+                check(Q, gpu, x, 1.0, u, [last], k=n, p=1 - 2.0 ** -24)
