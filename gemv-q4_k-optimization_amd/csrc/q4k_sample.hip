@@ -501,8 +501,8 @@ struct PickRow {
             all_x += s.scan[0][i];
             all_y += s.scan[1][i];
         }
-        x = bx + (ix - x);
-        y = by + (iy - y);
+        x = bx + wave_before(ix);
+        y = by + wave_before(iy);
     }
     __device__ __forceinline__ double scan(double x, double &all) const {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -517,7 +517,7 @@ struct PickRow {
             if (i == wave) bx = all;
             all += s.scan[0][i];
         }
-        return bx + (ix - x);
+        return bx + wave_before(ix);
     }
 
     // The `best` (0 and above) of the last thread that has one, threads with higher ones behind
@@ -745,7 +745,7 @@ struct PickRow {
             if (level == 0) sum = ldexp(sum * unit, -1 - lane);
             else if (lane < kOctave) sum = sample_weight_sum(s.octave, octave * kOctave + kOctave - 1 - lane, sum * unit);
             const double ic = wave_scan(cnt), im = wave_scan(sum);
-            const double bc = base_cnt + (ic - cnt), bm = base_mass + (im - sum);
+            const double bc = base_cnt + wave_before(ic), bm = base_mass + wave_before(im);
             if (level == 0) {
                 const double whole = last_lane(im);
                 if (!by_count) limit = most * whole;
@@ -1019,7 +1019,7 @@ struct PickRow {
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = kept_w(sample_clean(v[j]), t + j);
             const double four = (w[0] + w[1]) + (w[2] + w[3]), inc = wave_scan(four);
-            double upto = inc - four, first_w = 0.0, any_w = 0.0;
+            double upto = wave_before(inc), first_w = 0.0, any_w = 0.0;
             int first = -1, any = -1;  // of the lane's four, the first that passes and the last that counts
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -1209,7 +1209,7 @@ __device__ __forceinline__ void sample_alone(const SampleParams &p, PickLds &s, 
 #pragma unroll
                 for (int j = 0; j < 4; ++j) is[j] = sample_clean(v[j]) == l ? 1.0 : 0.0;
                 const double four = is[0] + is[1] + is[2] + is[3], inc = wave_scan(four);
-                double at = inc - four;
+                double at = wave_before(inc);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     at += is[j];

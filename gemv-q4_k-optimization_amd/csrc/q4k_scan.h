@@ -21,6 +21,9 @@ __device__ __forceinline__ double wave_scan(double x) {  // inclusive
     x += dpp64<0x143, 0xc>(x);  // of row 1 to rows 2 and 3
     return x;
 }
+// What lies before each lane, from an inclusive scan: the lane before's, 0 in the first.  (Less the
+// lane's own it would lose what is 2^-53 of that.)
+__device__ __forceinline__ double wave_before(double inclusive) { return dpp64<0x138, 0xf>(inclusive); }  // wave_shr:1
 __device__ __forceinline__ double lane_of(double x, int lane) {
     const unsigned long long b = __double_as_longlong(x);
     const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);

@@ -79,7 +79,7 @@ def test_sample_draws_what_a_cut_keeps_however_little_it_weighs(Q, gpu):
 
 
 @pytest.mark.parametrize("n", [3, 200, 256, 257, 600, 1024])
-@pytest.mark.parametrize("deep", [10, 30, 45])
+@pytest.mark.parametrize("deep", [10, 30, 45, 60])
 def test_sample_small_weights_of_a_list_add_up(Q, gpu, n, deep):
     """n - 1 tokens of about 2^-deep each, and behind them one of 1, kept by top-k, by top-k and top-p (all of
     them: the part is 1 - 2^-24 of a sum that lacks less), or by min-p too: random numbers that fall among the small ones."""
@@ -99,3 +99,45 @@ def test_sample_small_weights_of_a_list_add_up(Q, gpu, n, deep):
             check(Q, gpu, x, 1.0, u, kept, k=n, m=2.0 ** -62)
             if deep > 30:
                 check(Q, gpu, x, 1.0, u, [last], k=n, p=1 - 2.0 ** -24)
+
+
+@pytest.mark.parametrize("rules", [dict(), dict(k=300), dict(m=2.0 ** -62), dict(k=40)])
+@pytest.mark.parametrize("V,seed", [(256, 0), (3000, 1), (40000, 2), (300001, 3)])
+def test_sample_small_weights_before_a_large_one(Q, gpu, V, seed, rules):
+    """Tokens of 2^-50 to 2^-62 around and right before one of 1, by twos and fours of a lane, in other
+    lanes, chunks and stretches: random numbers that fall on each of them."""
+    g = torch.Generator().manual_seed(seed)
+    last = V - 3
+    x = torch.full((V,), -float("inf"))
+    at = sorted({*range(last - 9, last), last + 1, *(int(V * torch.rand(1, generator=g)) for _ in range(24))} - {last})
+    x[at] = -(50 + 12 * torch.rand(len(at), generator=g)) * math.log(2)
+    x[last] = 0.0
+    kept = sorted([*at, last])
+    total = math.fsum(math.exp(float(x[i])) for i in kept)
+    u, upto = [0.0], 0.0
+    for i in kept[:kept.index(last)]:
+        w = math.exp(float(x[i]))
+        u += [(upto + w * v) / total for v in (0.01, 0.5, 0.99)]
+        upto += w
+    u += [upto * 1.01 / total, 0.5]
+    check(Q, gpu, x, 1.0, u, kept, **rules)
+
+
+def test_sample_of_a_large_weight_between_small_ones_by_chunks(Q, gpu):
+    """Whole chunks of small weights, then one of 1 in a chunk of its own; thousands of tokens."""
+    g = torch.Generator().manual_seed(9)
+    for V, deep in ((40000, 55), (151936, 58)):
+        x = -(deep + 4 * torch.rand(V, generator=g)) * math.log(2)
+        last = V * 3 // 4
+        x[last] = 0.0
+        w = torch.exp(x.double())
+        upto = torch.cumsum(w[:last], 0)
+        total = float(w.sum())
+        at = [1, 200, 255, 256, 3000, 10000, last - 1]
+        u = torch.tensor([float(upto[i] - w[i] * 0.5) / total for i in at])
+        for kw in (dict(), dict(min_p=torch.full((len(at),), 2.0 ** -63, device=gpu))):
+            lp = torch.empty(len(at), device=gpu)
+            got, _ = Q.sample(x.to(gpu).repeat(len(at), 1), u.to(gpu), logprob=lp, **kw)
+            assert got.tolist() == at
+            want = (x[at].double() - math.log(total)).to(gpu)
+            assert ((lp - want).abs() <= 2.0 ** -24 * want.abs() + 1e-10).all()
