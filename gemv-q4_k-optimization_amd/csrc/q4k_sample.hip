@@ -45,6 +45,7 @@ namespace q4k {
 constexpr int kDrawThreads = 512;
 constexpr int kScanThreads = 512, kScanWaves = kScanThreads / 64, kTile = kScanThreads * 8;
 constexpr int kOctave = 24, kOctaves = 64, kBins = kOctaves * kOctave;  // what is below the last bin is never drawn
+constexpr int kMassBits = 44;  // of a token's integer weight in its bin (of up to 2^18, what a scan numbers)
 constexpr int kChunk = 256, kChunks = 1024, kList = 1024, kShort = 256, kParts = 16;
 // Rows whose a l is past this (in bins) lose bits of w and are not scanned: the pick
 // takes them by the differences from their largest logit.
@@ -75,7 +76,7 @@ struct SampleParams {
     int64_t nb_src;
     int n_vocab, n_rows;
     int chunk, chunks;  // tokens of a chunk (a multiple of 256), chunks of a row
-    int mass_bits;      // of a token's integer weight in its bin
+    int past_bits;      // sample_past's
     int parts, tiles;   // of a row (0: not scanned); of a part
     int shares;         // workgroups of a row's draw
     SamplePart *part;
@@ -220,6 +221,11 @@ __device__ __forceinline__ double sample_weight_sum(const double *octave, int b,
 __device__ __forceinline__ unsigned long long sample_mass(double x, double scale) {
     return __double_as_longlong(sample_exp(x, scale, 0x1p52)) & 0xfffffffffffffull;
 }
+// What it is past 1, within 2^-6.1 of it, as an integer with a sign: of 2^30 tokens it leaves room
+// for 39 bits, where the whole weight would for 33.
+__device__ __forceinline__ unsigned long long sample_past(double x, double scale) {
+    return (unsigned long long)(__double_as_longlong(sample_exp(x, scale, 0x1.8p52 - scale)) - __double_as_longlong(0x1.8p52));
+}
 
 // ---- scan: parts of the rows ----
 // Tiles of 4096 logits, eight a thread, the next one on its way.  The bins are a ring
@@ -242,7 +248,7 @@ __global__ __launch_bounds__(kScanThreads) void sample_scan_kernel(SampleParams 
     next[1] = sample_load(src, p.n_vocab, (int)beg + at + kChunk);
     const SampleRules r(p, row);
     const bool cut = r.cut, by_mass = r.top_k == 0, free = r.free();  // (top-k needs counts alone)
-    const double rate = r.rate(), scale = (double)(1ull << p.mass_bits);
+    const double rate = r.rate(), scale = (double)(1ull << kMassBits);
     if (tid < kOctave) octave[tid] = exp2(tid * (1.0 / kOctave));
     if (part == 0 && tid == 0) p.list[row].n = p.list[row].done = 0;
     if (free) __syncthreads();
@@ -715,7 +721,7 @@ struct PickRow {
     // lie, its number of tokens, what lies before it, and the whole; to LDS.
     __device__ __forceinline__ void pick_scanned(const SamplePart *part, int parts, bool by_count, double most) const {
         const int lane = threadIdx.x & 63;
-        const double unit = 1.0 / (double)(1ull << p.mass_bits);
+        const double unit = 1.0 / (double)(1ull << kMassBits);
         double base_cnt = 0.0, base_mass = 0.0, limit = most;
         int octave = 0;
 #pragma unroll
@@ -780,9 +786,10 @@ struct PickRow {
 
     // The bin of the last token before which fewer than `most` tokens (by_count) or
     // less than `most` of w lie, and what lies before the bin; the whole sum.  Bins from
-    // the highest, a thread has as many as divide them among all.  `part`: most is of the whole.
+    // the highest, a thread has as many as divide them among all; mass_of(bin): the sum of w of one that
+    // is not empty.  `part`: most is of the whole.
     template <int BINS, class W>
-    __device__ __forceinline__ int pick(bool by_count, bool part, double most, W weight_of, double &base_cnt, double &base_mass,
+    __device__ __forceinline__ int pick(bool by_count, bool part, double most, W mass_of, double &base_cnt, double &base_mass,
                                         double &whole) const {
         constexpr int PER = (BINS + kPickThreads - 1) / kPickThreads;
         const int tid = threadIdx.x;
@@ -791,7 +798,7 @@ struct PickRow {
         for (int j = 0; j < PER; ++j) {
             const int b = BINS - 1 - (tid * PER + j);
             cnt[j] = b >= 0 ? s.cnt[b] : 0.0;
-            mass[j] = cnt[j] != 0.0 ? (double)s.mass[b] * weight_of(b) : 0.0;
+            mass[j] = cnt[j] != 0.0 ? mass_of(b) : 0.0;
             bc += cnt[j];
             bm += mass[j];
         }
@@ -932,7 +939,7 @@ struct PickRow {
             atomicAdd(&s.cnt[b], 1u);
         }
         __syncthreads();
-        const int sub = pick<1024>(by_count, false, most, [](int) { return kStep; }, base_cnt, base_mass, some);
+        const int sub = pick<1024>(by_count, false, most, [&](int b) { return (double)s.mass[b] * kStep; }, base_cnt, base_mass, some);
         // the tokens of that stretch in order, where the list's kept ones are looked up again
         const int count = s.cnt[sub];
 #pragma unroll 1
@@ -1103,7 +1110,7 @@ __device__ __forceinline__ void sample_alone(const SampleParams &p, PickLds &s, 
     if (x.simple(row, r.greedy)) return;
     x.flat = x.m == inf;  // only the infinite ones count
     x.rate = r.rate();
-    const double scale = (double)(1ull << p.mass_bits), unit = 1.0 / scale;
+    const double scale = (double)(1ull << p.past_bits), unit = 1.0 / scale;
     double most = 0.0;
 #pragma unroll 1
     for (int cut = r.top_k > 0 ? 0 : 1; cut < 2; ++cut) {
@@ -1136,7 +1143,7 @@ __device__ __forceinline__ void sample_alone(const SampleParams &p, PickLds &s, 
                         if (b != bin || key < lo || key > hi) continue;
                         b = (int)((key - lo) >> shift);
                     }
-                    atomicAdd(&s.mass[b], sample_mass(past, scale));
+                    atomicAdd(&s.mass[b], sample_past(past, scale));
                     atomicAdd(&s.cnt[b], 1u);
                 }
             }, nothing);
@@ -1144,7 +1151,10 @@ __device__ __forceinline__ void sample_alone(const SampleParams &p, PickLds &s, 
             // (stretches are numbered up to 1023: the bins above them are empty)
             double whole;
             const int found = x.template pick<kBins>(by_count, bin < 0 && whole_row, bin < 0 && whole_row ? near_p : most,
-                                                           [&](int b) { return sample_weight(s.octave, bin < 0 ? b : bin, unit); }, base_cnt, base_mass, whole);
+                                                           [&](int b) {
+                                                               const double sum = (double)s.cnt[b] + (double)(long long)s.mass[b] * unit;
+                                                               return sample_weight(s.octave, bin < 0 ? b : bin, sum);
+                                                           }, base_cnt, base_mass, whole);
             count = s.cnt[found];
             if (bin < 0) {
                 if (whole_row) most = near_p * whole;
@@ -1458,7 +1468,7 @@ int q4k_sample(const float *src, int64_t n_vocab, int64_t n_rows, int64_t nb_src
     p.chunks = (int)((n_vocab + p.chunk - 1) / p.chunk);
     int bits = 0;
     while ((int64_t)1 << bits < n_vocab) ++bits;
-    p.mass_bits = 62 - bits < 44 ? 62 - bits : 44;
+    p.past_bits = 69 - bits < kMassBits ? 69 - bits : kMassBits;
     p.r = r;
     p.tokens = tokens;
     p.logprob = logprob;

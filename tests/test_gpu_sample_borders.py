@@ -141,3 +141,22 @@ def test_sample_of_a_large_weight_between_small_ones_by_chunks(Q, gpu):
             assert got.tolist() == at
             want = (x[at].double() - math.log(total)).to(gpu)
             assert ((lp - want).abs() <= 2.0 ** -24 * want.abs() + 1e-10).all()
+
+
+@pytest.mark.parametrize("d,p", [(1.1291229724884033, 0.5224581956863403), (1.2371230125427246, 0.591297447681427)])
+def test_sample_top_p_over_a_hundred_million_tokens(Q, gpu, d, p):
+    """One token of 1 and 2^27 - 1 alike of w = exp(-d), where p times the whole sum lies 4 to 5 parts in
+    10000 of w past a token's sum (2^-39 of the sum): the last token that is kept, by a random number
+    whose token changes with it.  Sums within 2^-40 of a border may count as equal to it: 1.1 in 10000 here."""
+    V = 1 << 27
+    w = math.exp(-d)
+    places = (p * (1 + (V - 1) * w) - 1) / w
+    assert 3e-4 < places % 1 < 6e-4
+    kept = 1 + (math.floor(places) + 1) * w
+    u = next(v for v in (1 - i * 2.0 ** -24 for i in range(1, 200)) if 0.3 < (v * kept - 1) / w % 1 < 0.7)
+    x = torch.full((1, V), -d, device=gpu)
+    x[0, 0] = 0.0
+    lp = torch.empty(1, device=gpu)
+    got, _ = Q.sample(x, torch.tensor([u], device=gpu), top_p=torch.tensor([p], device=gpu), logprob=lp)
+    assert int(got) == math.floor((u * kept - 1) / w) + 1
+    assert abs(float(lp) - math.log(w / kept)) <= 2.0 ** -24 * 30 + 1e-10
