@@ -2,7 +2,7 @@
 // values into pages of 8 bits with a scale for each block of tokens and head, and
 // back.
 //
-//   store   s' = max(s if the block holds earlier tokens, max |x| / top)
+//   store   s' = max(s if the block holds earlier tokens, max |x| / top), 1 where that is 0 and some |x| infinite
 //           q = rne(x / s') for new tokens; earlier ones rne(q s / s') where s' > s
 //   load    x = q s
 //
@@ -146,7 +146,23 @@ __global__ __launch_bounds__(THREADS) void kv8_store_kernel(Kv8RowsParams p) {
 #pragma unroll
         for (int i = 0; i < THREADS / 64; ++i) top = fmaxf(top, tops[i]);
     }
-    const float s = fmaxf(top / Kv8Scale<I8>::top, was);
+    float s = fmaxf(top / Kv8Scale<I8>::top, was);
+    if (s == 0.0f) {
+        // Nothing to take a scale from: 1 where there is an infinity, so that it reads back as the largest
+        // of its sign.
+        bool inf = false;
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) inf |= __builtin_isinf(xs[i][e]);
+        for (int at = HELD * per + sub; on && at < end - beg; at += per) {
+            float y[4];
+            kv8_row4<T>(row_of(at), y);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) inf |= __builtin_isinf(y[e]);
+        }
+        if (__syncthreads_or(inf)) s = 1.0f;
+    }
     const Kv8Scale<I8> by(s);
     const bool grows = !(s <= was);
     auto put = [&](int position, const float (&y)[4]) {

@@ -116,13 +116,13 @@ typedef struct q4k_kv8_rows {
  * largest magnitude of its new tokens / 127 (E4M3: / 448), or stays what it is
  * where the block holds earlier tokens of the request and their scale is larger;
  * where it grows, the earlier tokens are rounded again from the values that they
- * stood for (in F32).  Values are the nearest to x / scale, ties to even (worked out exactly);
- * infinities and values that are not finite take no part in the magnitude and
- * become the largest of their sign, NaN 0.  Tokens at positions below 0 or in
- * pages out of range are left out, bytes of positions that no new or earlier
- * token of the block has stay as they are.  Two requests' new tokens must not fall
- * into one block, nor a block of one hold earlier tokens of another that is
- * read meanwhile. */
+ * stood for (in F32).  Values are the nearest to x / scale, ties to even (worked out
+ * exactly).  Infinities and NaN take no part in the magnitude; infinities become the
+ * largest of their sign (of a scale of 1 where the block's would be 0), NaN 0.
+ * Tokens at positions below 0 or in pages out of range are left out, bytes of
+ * positions that no new or earlier token of the block has stay as they are.  Two
+ * requests' new tokens must not fall into one block, nor a block of one hold earlier
+ * tokens of another that is read meanwhile. */
 int q4k_kv8_store(const q4k_kv8_rows *rows, void *stream);
 
 /* Reads each request's last tokens as the values they stand for, rounded to
