@@ -435,13 +435,17 @@ __device__ __forceinline__ void kv8_attn_item(const Kv8AttnParams &kp, const Att
                     if (!here || t0 + u >= w.limit[rt]) sx[rt][e >> 2][e & 3] = -__builtin_inff();
                 if (!C::I8) {
 #pragma unroll
-                    for (int x = 0; x < VW; ++x) {
+                    for (int x = 0; x < VW; ++x)
                         if (!here) vf[e][x] = 0;
-                        // (what is there and every row sees stays: the products take it to all of them)
-                        if (differ) fine = !kv8_nan(vf[e][x]) && fine;
-                    }
                 }
             }
+        }
+        // (where rows see the same, the products take what is there to all of them)
+        if (!C::I8 && differ) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int x = 0; x < VW; ++x) fine = !kv8_nan(vf[e][x]) && fine;
         }
         // new references when some row passes its old one by 2^kKv8Lazy (-inf: always)
         float top[RT];
