@@ -31,8 +31,13 @@ __device__ __forceinline__ void store4(float *p, f32x4 x) {
     else *v = x;
 }
 
+// A launch has fewer than 2^32 threads.  (The runtime refuses more, and leaves an error that
+// the next call of anyone on this thread may report as its own.)
+constexpr bool launches(int64_t workgroups, int threads) { return workgroups <= (int64_t)UINT32_MAX / threads; }
+
 template <class P>
 int launch(void (*fn)(P), dim3 grid, int threads, int lds, void *stream, const P &p) {
+    if (!launches(grid.x, threads)) return Q4K_EUNSUPPORTED;
     void *args[] = {const_cast<P *>(&p)};
     const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(fn), grid, dim3((unsigned)threads), args,
                                          (size_t)lds, (hipStream_t)stream);

@@ -81,6 +81,7 @@ static int kv8_attn_plan(const q4k_kv8_attn_args &a, int cus, Kv8AttnPlan &pl) {
     pl.slots = slots;
     // (the join counts its rows in 31 bits, up to a workgroup's past the last one)
     if (a.n_requests * a.n_q > (INT32_MAX - 256) / a.n_head) return Q4K_EUNSUPPORTED;
+    if (!launches(p.suf_items, 256) || (slots && !launches(cdiv(a.n_requests * a.n_q * a.n_head, p.join_rows), kJoinThreads))) return Q4K_EUNSUPPORTED;
     return Q4K_OK;
 }
 

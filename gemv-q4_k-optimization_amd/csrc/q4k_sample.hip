@@ -1441,7 +1441,7 @@ extern "C" {
 
 size_t q4k_sample_workspace_bytes(int64_t n_vocab, int64_t n_rows) {
     DeviceInfo *di;
-    if (n_vocab < 0 || n_rows < 1 || n_vocab > (1 << 30) || n_rows > INT32_MAX / kParts || device_info(&di) != Q4K_OK) return 0;
+    if (n_vocab < 0 || n_rows < 1 || n_vocab > (1 << 30) || !launches(n_rows, kDrawThreads) || device_info(&di) != Q4K_OK) return 0;
     return sample_bytes(n_vocab, n_rows, di->cus);
 }
 
@@ -1454,7 +1454,7 @@ int q4k_sample(const float *src, int64_t n_vocab, int64_t n_rows, int64_t nb_src
         return Q4K_EINVAL;
     if (n_rows == 0) return Q4K_OK;
     if ((!src && n_vocab > 0) || !tokens || nb_src % 4 != 0 || (n_rows > 1 && nb_src < 4 * n_vocab)) return Q4K_EINVAL;
-    if (n_vocab > (1 << 30) || n_rows > INT32_MAX / kParts) return Q4K_EUNSUPPORTED;
+    if (n_vocab > (1 << 30) || !launches(n_rows, kDrawThreads)) return Q4K_EUNSUPPORTED;
     DeviceInfo *di;
     int st = device_info(&di);
     if (st != Q4K_OK) return st;

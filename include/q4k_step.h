@@ -18,6 +18,9 @@
  * of a captured graph, entries out of range are ignored as each call states.
  * Equal calls give equal bits.  A workspace needs no initial contents and may be
  * used by any call that the stream orders after the last one, by one at a time.
+ * A call that would take 2^32 threads and more in a launch (64 a token of q4k_rope,
+ * 512 a row of q4k_sample, one for eight values that n_requests times n_q tokens
+ * would have in q4k_kv8_load) is refused with Q4K_EUNSUPPORTED as a whole.
  */
 #ifndef Q4K_STEP_H
 #define Q4K_STEP_H
