@@ -243,6 +243,16 @@ static bool kv8_row_ok(const void *p, int64_t token, int64_t head, int es, const
     return aligned(p, es) && ((token | head) & (es - 1)) == 0 && (c.n_head_kv == 1 || head >= (int64_t)es * c.head_dim);
 }
 
+// Rows of `bytes` that one step of a stride apart do not overlap, where there is more than one: what
+// workgroups write at once.
+static bool kv8_apart(int64_t stride, int64_t n, int64_t bytes) { return n <= 1 || stride >= bytes || stride <= -bytes; }
+static bool kv8_writable(const q4k_kv8_pages &c) {
+    const int64_t blocks = c.page_size / c.block;
+    return kv8_apart(c.nb_k_page, c.n_pages, c.head_dim) && kv8_apart(c.nb_k_token, c.page_size, c.head_dim) && kv8_apart(c.nb_k_head, c.n_head_kv, c.head_dim) &&
+           kv8_apart(c.nb_v_page, c.n_pages, c.head_dim) && kv8_apart(c.nb_v_token, c.page_size, c.head_dim) && kv8_apart(c.nb_v_head, c.n_head_kv, c.head_dim) &&
+           kv8_apart(c.nb_s_page, c.n_pages, 4) && kv8_apart(c.nb_s_block, blocks, 4) && kv8_apart(c.nb_s_head, c.n_head_kv, 4);
+}
+
 static int kv8_rows_check(const q4k_kv8_rows *rows, bool store, bool &empty) {
     if (!rows || !rows->pages) return Q4K_EINVAL;
     const q4k_kv8_rows &a = *rows;
@@ -256,6 +266,7 @@ static int kv8_rows_check(const q4k_kv8_rows *rows, bool store, bool &empty) {
     if (!kv8_row_ok(a.k, a.nb_k_token, a.nb_k_head, es, c) || !kv8_row_ok(a.v, a.nb_v_token, a.nb_v_head, es, c)) return Q4K_EINVAL;
     if (!kv8_pages_ok(c, a.max_len, a.n_requests)) return Q4K_EINVAL;
     if (!kv8_pages_vec(c)) return Q4K_EUNSUPPORTED;
+    if (store && !kv8_writable(c)) return Q4K_EINVAL;
     empty = !a.k && !a.v;
     return Q4K_OK;
 }

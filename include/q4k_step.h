@@ -125,7 +125,8 @@ typedef struct q4k_kv8_rows {
  * Tokens at positions below 0 or in pages out of range are left out, bytes of
  * positions that no new or earlier token of the block has stay as they are.  Two
  * requests' new tokens must not fall into one block, nor a block of one hold earlier
- * tokens of another that is read meanwhile. */
+ * tokens of another that is read meanwhile.  Pages, tokens, heads and scales that overlap
+ * (a stride of 0, say, which q4k_kv8_load and q4k_kv8_attn take) are Q4K_EINVAL. */
 int q4k_kv8_store(const q4k_kv8_rows *rows, void *stream);
 
 /* Reads each request's last tokens as the values they stand for, rounded to
