@@ -10,8 +10,8 @@
 // over its rows for the magnitude, held in registers for the rounding.
 //
 // Bound by chains of round trips (lengths, page, rows and scale, stores): one token of 16 requests 4.4 us
-// to store, 4.4 to load, a launch's own time; 8 x 512 BF16 tokens of 8 heads of 128 to e4m3, 25 MB, 13.5 us,
-// 5.6 of which are the rounding's vector work, and back, 25 MB, 7.4 us.
+// to store, 4.4 to load, a launch's own time; 8 x 512 BF16 tokens of 8 heads of 128 to e4m3, 25 MB, 13.1 to 13.5 us,
+// 5.6 of which are the rounding's vector work, and back, 25 MB, 7.4 to 7.8 us.
 #include "q4k_kv8.h"
 
 namespace q4k {

@@ -23,6 +23,9 @@
 // BF16 queries of 64 heads, 147 us, 4.6 TB/s, what large reads reach here.  16 of them with F32 queries,
 // 175 MB of int8, 48 us and 6 us of join, of which 8 us pass before the first step (lengths counted, page,
 // first positions); two steps on their way a wave: 51 us.  One request of 200: 9 us, a chain.
+// Prompts are bound by arithmetic, of which a tile of 32 rows does all that its request has, also what lies behind its
+// causal bound, and every tile converts every byte again: the first 2048 tokens of 32/8 heads of 128, BF16 on e4m3,
+// 218 us, 158 TFLOP/s of what the rows see, the second 2048 339 us, 304.
 #pragma once
 
 #include "q4k_attn.h"
@@ -45,8 +48,10 @@ struct Kv8AttnParams {
 };
 
 // Positions of a step of four waves; the least steps of a part (200 positions of one request: 1 step a
-// part and a join 14.0 us, 2 11.4), the most of parts of one length (at 3 steps those are faster,
-// 16.2 us against 21.7 for 12 x 5 tokens over up to 3001 positions; at 16 the others, 53.5 against 58).
+// part and a join 14.0 us, 2 11.4), the most of parts of one length.  Parts against steps dealt out, us, BF16 on
+// e4m3: 2 steps 17.0 and 26.0 (16 requests), 3 steps 23.1 and 26.8 (16), 26.5 and 28.8 (64), 4 steps 26.6 and 29.6; 6 steps
+// 34.2 and 33.1 (16), 41.8 and 32.7 (64), 11 steps 60.5 and 53.1.  (Blocks of 12 tokens and 12 x 5 queries gain by parts
+// up to 12 steps, 39.3 against 42.1, which this leaves.)
 constexpr int kKv8Step = 128, kKv8Least = 2, kKv8Few = 4;
 constexpr int kKv8Deal = (257 + 4) * 8 + (3 * 256 + 1) * 4;  // bytes of LDS
 

@@ -129,8 +129,8 @@ typedef struct q4k_kv8_rows {
  * (a stride of 0, say, which q4k_kv8_load and q4k_kv8_attn take) are Q4K_EINVAL. */
 int q4k_kv8_store(const q4k_kv8_rows *rows, void *stream);
 
-/* Reads each request's last tokens as the values they stand for, rounded to
- * `type`: zeros at positions below 0 and in pages out of range.  Rows of no
+/* Reads each request's last tokens as the values they stand for (byte times scale in
+ * F32, then rounded to `type`): zeros at positions below 0 and in pages out of range.  Rows of no
  * request stay as they are.  k or v may be NULL. */
 int q4k_kv8_load(const q4k_kv8_rows *rows, void *stream);
 
@@ -193,8 +193,8 @@ size_t q4k_sample_workspace_bytes(int64_t n_vocab, int64_t n_rows);
  * The token is the first, in the order of token numbers, up to which the kept w's
  * sum exceeds uniform times their sum.  Logits of -inf and NaN are no candidates; a
  * row without any gives -1; with logits of +inf those are the candidates, alike.
- * w and its sums are 64 bits; sums within 2^-40 of a border count as equal to it,
- * tokens below 2^-63 of the largest w as 0.
+ * w and its sums are 64 bits; sums within 2^-40 of a border (of its own value) count as
+ * equal to it, tokens below 2^-63 of the largest w as 0.
  * logprob[i] (may be NULL): the logarithm of the token's share of the kept
  * w's sum, 0 where the largest logit was taken, -inf where there is none. */
 int q4k_sample(const float *src, int64_t n_vocab, int64_t n_rows, int64_t nb_src, const q4k_sample_rules *rules,
