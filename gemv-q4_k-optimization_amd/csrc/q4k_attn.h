@@ -247,12 +247,15 @@ __device__ __forceinline__ float attn_queries(const AttnParams &p, const AttnSpa
     }
     float c = fabsf(p.scale) * kLog2e, f = 1.0f;
     if (TERMS > 1) {
-        // an F32 row of any magnitude: a power of two brings its largest value to 1..2
+        // An F32 row of any magnitude: a power of two brings its largest value to 1..2, in F16 to 2^14..2^15,
+        // near the end of its range, where the second term's smallest step, 2^-24, leaves each value its 22
+        // bits down to 2^-17 of the largest.
+        constexpr int UP = __is_same(T, _Float16) ? 14 : 0;
         top = xor_max(top);
         int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-        e = e < -126 || e > 127 ? 0 : e > 126 ? 126 : e;
-        f = __uint_as_float((uint32_t)(127 - e) << 23);
-        c *= __uint_as_float((uint32_t)(127 + e) << 23);
+        e = e > 127 ? UP : e < UP - 126 ? UP - 126 : e > UP + 126 ? UP + 126 : e;  // (not finite: as it is)
+        f = __uint_as_float((uint32_t)(127 + UP - e) << 23);
+        c *= __uint_as_float((uint32_t)(127 + e - UP) << 23);
     }
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
