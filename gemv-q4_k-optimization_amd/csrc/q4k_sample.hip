@@ -989,8 +989,7 @@ struct PickRow {
         for (int k = 0; k < kEach; ++k) have[k] += (double)s.mass[tid * kEach + k] * kStep + (double)s.rest[tid * kEach + k] * (kStep * kStep);
     }
 
-    // The token that u falls on, of chunks tid * kEach .. with kept sums `have`, and its
-    // share.
+    // The token that u falls on, of chunks tid * kEach .. with kept sums `have`, and its share.
     __device__ __forceinline__ void draw(int row, double u, const double (&have)[kEach]) const {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
         auto kept_w = [&](float l, int i) {

@@ -129,8 +129,8 @@ size_t q4k_prefix_attn_workspace_bytes(const q4k_prefix_attn_args *args);
  * lengths, have no effect on it whatever they hold.  Scores, the softmax's
  * maximum and sum and the output sum are F32.  With q_type F32 the queries and
  * probabilities enter the matrix cores as sums of two (F16) or three (BF16)
- * values of kv_type (a query's: 22 or 24 bits, with F16 at most to 2^-39 of its
- * head's largest value), with q_type kv_type as one rounded value.  Tokens of no
+ * values of kv_type (a query's to 22 or 24 bits, or with F16 to 2^-39 of the head's
+ * largest value), with q_type kv_type as one rounded value.  Tokens of no
  * request (before, between and behind those that q_start names, or past n_q of a
  * request) are left as they are.  dst and lse must not overlap what is read.  Up
  * to 2^30 positions a part. */
